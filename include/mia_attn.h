@@ -58,6 +58,7 @@ enum mia_dtype {
   MIA_DTYPE_I32 = 4,
   MIA_DTYPE_I64 = 5,
   MIA_DTYPE_U32 = 6,
+  MIA_DTYPE_I8 = 7,
 };
 
 /* How a new K/V row is quantised into an FP8 cache.  The reference uses two
@@ -79,7 +80,8 @@ const char *mia_last_error(void);
 /* sizeof() of each argument struct, so bindings can check their layout.
  * which: 0 kv_write, 1 gather, 2 mask, 3 decode, 4 prefill, 5 slot_mapping,
  * 6 packed_k, 7 swa_trim, 8 scatter_rows, 9 stage, 10 qkv_epilogue,
- * 11 row_norm.  Returns 0 for an unknown index. */
+ * 11 row_norm, 12 skinny_linear, 13 quant_kv, 14 cross, 15 shared_prefix.
+ * Returns 0 for an unknown index. */
 size_t mia_args_size(int which);
 
 /* ------------------------------------------------------------------------ */
@@ -649,6 +651,151 @@ typedef struct {
 } mia_skinny_linear_args;
 
 int mia_skinny_linear(const mia_skinny_linear_args *args, mia_stream_t stream);
+
+/* ------------------------------------------------------------------------ */
+/* K/V rows quantised to 8 bits in the paged cache with one fp32 scale per   */
+/* (token, kv head), and read back (no counterpart in the reference, whose   */
+/* FP8 caches have one static scale per layer or head).                      */
+/* Write: row x[0..d) of token t and head h, amax = max |x|, goes to slot    */
+/*   slots[t]: scale = fl32(amax / Q), code = rn(x * Q / amax), Q = 127      */
+/*   (int8, ties to even) or 448 (e4m3fn).  A row of zeros has scale 0; a    */
+/*   row with a NaN or infinity scale NaN and zero codes; where Q * scale    */
+/*   would overflow fp32, scale is the next smaller number.                  */
+/* Read: row t = fl(code * scale) in the row dtype.                          */
+/* Slots outside [0, num_blocks * block_size) are skipped (write) or give    */
+/* zeros (read).  The slots of one write must differ.  head_dim <= 512.      */
+/* ------------------------------------------------------------------------ */
+typedef struct {
+  void *k;             /* rows: read by the write, written by the read */
+  void *v;
+  int32_t row_dtype;   /* BF16, F16 or F32 */
+  int32_t code_dtype;  /* I8 or FP8_E4M3FN */
+  int64_t k_stride[3]; /* token, head, dim (elements) */
+  int64_t v_stride[3];
+  const void *slots; /* [num_tokens] */
+  int32_t slot_dtype; /* I32, I64 or U32 */
+  int32_t _pad0;
+  int64_t num_tokens;
+  void *k_cache;
+  void *v_cache;
+  int64_t k_cache_stride[4]; /* block, head, token, dim */
+  int64_t v_cache_stride[4];
+  float *k_scales;
+  float *v_scales;
+  int64_t k_scale_stride[3]; /* block, head, token */
+  int64_t v_scale_stride[3];
+  int32_t num_blocks;
+  int32_t block_size;
+  int32_t num_kv_heads;
+  int32_t head_dim;
+} mia_quant_kv_args;
+
+int mia_quant_kv_write(const mia_quant_kv_args *args, mia_stream_t stream);
+int mia_quant_kv_read(const mia_quant_kv_args *args, mia_stream_t stream);
+
+/* ------------------------------------------------------------------------ */
+/* Cross attention: query tokens of each sequence over all keys of the       */
+/* sequence's encoder (no causal mask).  No counterpart in the reference.    */
+/* Sequence i has query tokens [cu_seqlens_q[i], cu_seqlens_q[i+1]) (one     */
+/* each, token i, if cu_seqlens_q is NULL; at most max_seqlen_q are          */
+/* computed) and keys [0, key_lens[i]) in the cache through block_table row  */
+/* i, or, with block_table NULL, in "block" i of a dense [num_seqs, head,    */
+/* block_size, d] tensor.  key_lens are clamped to what the table holds.     */
+/* Rows of a sequence without keys give 0; rows of no sequence are left as   */
+/* they were.                                                                */
+/* Caches: bf16; e4m3fn with per-head factors k_dequant / v_dequant (NULL =  */
+/* 1) or with the per-token scales of mia_quant_kv_write; int8 with those.   */
+/* head_dim: a multiple of 8 (8-bit caches: 16) up to 128.  With a table,    */
+/* block_size is a multiple of 16.                                           */
+/* ------------------------------------------------------------------------ */
+typedef struct {
+  const void *q; /* bf16 */
+  int64_t q_stride[3]; /* token, hq, d */
+  void *out;           /* bf16 */
+  int64_t out_stride[3];
+  int32_t num_tokens; /* rows of q and out */
+  int32_t num_seqs;
+  const int32_t *cu_seqlens_q; /* device, [num_seqs + 1], or NULL */
+  int32_t max_seqlen_q;
+  int32_t num_q_heads;
+  int32_t num_kv_heads;
+  int32_t head_dim;
+  const void *k_cache;
+  const void *v_cache;
+  int32_t cache_dtype; /* BF16, FP8_E4M3FN or I8 */
+  int32_t num_blocks;
+  int64_t k_cache_stride[4]; /* block, head, token, dim */
+  int64_t v_cache_stride[4];
+  int32_t block_size;
+  int32_t blocks_per_seq;
+  const int32_t *block_table; /* device, or NULL */
+  int64_t bt_stride[2];       /* seq, j */
+  const int32_t *key_lens;    /* device, [num_seqs] */
+  const float *k_scales;      /* per token and head, or NULL */
+  const float *v_scales;
+  int64_t k_scale_stride[3]; /* block, head, token */
+  int64_t v_scale_stride[3];
+  const float *k_dequant; /* [Hkv] or NULL */
+  const float *v_dequant;
+  float softmax_scale;
+  int32_t _pad0;
+  void *workspace; /* mia_cross_workspace_bytes(), 256-byte aligned */
+  size_t workspace_bytes;
+} mia_cross_args;
+
+size_t mia_cross_workspace_bytes(const mia_cross_args *args);
+int mia_cross_attention(const mia_cross_args *args, mia_stream_t stream);
+
+/* ------------------------------------------------------------------------ */
+/* Decode attention of a batch that shares a long prefix (no counterpart in  */
+/* the reference, whose decode reads the prefix once per row).               */
+/* Every row sees the keys [0, prefix_len) of prefix_table; row (b, s) also  */
+/* sees its own keys [0, seq_lens[b] - S + 1 + s) of block_table row b,      */
+/* which hold the S active tokens last (already written).  One softmax over  */
+/* both, and the sink logit in the denominator.  Rows without keys give 0.   */
+/* prefix_len is one int32 on the device; lengths are clamped to what the    */
+/* tables hold.  Caches as for mia_cross_attention.                          */
+/* ------------------------------------------------------------------------ */
+typedef struct {
+  const void *q; /* bf16 */
+  int64_t q_stride[4]; /* b, s, hq, d */
+  void *out;           /* bf16 */
+  int64_t out_stride[4];
+  int32_t batch;
+  int32_t s_active;
+  int32_t num_q_heads;
+  int32_t num_kv_heads;
+  int32_t head_dim;
+  int32_t cache_dtype; /* BF16, FP8_E4M3FN or I8 */
+  const void *k_cache;
+  const void *v_cache;
+  int64_t k_cache_stride[4]; /* block, head, token, dim */
+  int64_t v_cache_stride[4];
+  int32_t num_blocks;
+  int32_t block_size;
+  const int32_t *prefix_table; /* device, [prefix_blocks] */
+  int64_t prefix_stride;
+  const int32_t *prefix_len; /* device, [1] */
+  const int32_t *block_table; /* device */
+  int64_t bt_stride[2];       /* b, j */
+  const int32_t *seq_lens;    /* device, [batch] */
+  int32_t prefix_blocks;
+  int32_t blocks_per_seq;
+  const float *k_scales; /* per token and head, or NULL */
+  const float *v_scales;
+  int64_t k_scale_stride[3]; /* block, head, token */
+  int64_t v_scale_stride[3];
+  const float *k_dequant; /* [Hkv] or NULL */
+  const float *v_dequant;
+  const float *sink; /* [Hq] or NULL */
+  float softmax_scale;
+  int32_t _pad0;
+  void *workspace; /* mia_shared_prefix_workspace_bytes(), 256-byte aligned */
+  size_t workspace_bytes;
+} mia_shared_prefix_args;
+
+size_t mia_shared_prefix_workspace_bytes(const mia_shared_prefix_args *args);
+int mia_shared_prefix_attention(const mia_shared_prefix_args *args, mia_stream_t stream);
 
 #ifdef __cplusplus
 }

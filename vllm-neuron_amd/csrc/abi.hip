@@ -38,6 +38,57 @@ static bool aligned(const void *p, size_t a) {
   return ((uintptr_t)p % a) == 0;
 }
 
+// What cross and shared-prefix attention ask of their heads, rows and cache.
+template <typename A>
+static int check_span(const A &a, const int64_t *q_rows, const int64_t *out_rows, int n_rows,
+                      int64_t rows, bool paged) {
+  MIA_REQUIRE(a.num_q_heads > 0 && a.num_kv_heads > 0 && a.num_q_heads % a.num_kv_heads == 0,
+              MIA_ERR_VALUE, "GQA requires q_heads divisible by kv_heads");
+  MIA_REQUIRE(a.cache_dtype == MIA_DTYPE_BF16 || a.cache_dtype == MIA_DTYPE_FP8_E4M3FN ||
+                  a.cache_dtype == MIA_DTYPE_I8,
+              MIA_ERR_NOT_IMPLEMENTED, "span attention: cache dtype must be bf16, fp8 or int8");
+  const bool bf = a.cache_dtype == MIA_DTYPE_BF16;
+  MIA_REQUIRE(a.head_dim > 0 && a.head_dim <= 128 && a.head_dim % (bf ? 8 : 16) == 0,
+              MIA_ERR_NOT_IMPLEMENTED,
+              "span attention: head_dim must be a multiple of 8 (8-bit caches: 16) up to 128");
+  MIA_REQUIRE(!a.k_scales == !a.v_scales, MIA_ERR_VALUE,
+              "span attention: per-token scales of K and V go together");
+  MIA_REQUIRE(!(bf && a.k_scales), MIA_ERR_VALUE,
+              "span attention: a bf16 cache has no per-token scales");
+  MIA_REQUIRE(a.cache_dtype != MIA_DTYPE_I8 || a.k_scales, MIA_ERR_VALUE,
+              "span attention: an int8 cache needs per-token scales");
+  MIA_REQUIRE(a.num_blocks > 0 && a.block_size > 0 && a.blocks_per_seq > 0, MIA_ERR_VALUE,
+              "span attention: empty cache or table");
+  MIA_REQUIRE(!paged || a.block_size % 16 == 0, MIA_ERR_NOT_IMPLEMENTED,
+              "span attention: block_size must be a multiple of 16");
+  MIA_REQUIRE((int64_t)a.blocks_per_seq * a.block_size < (1ll << 30), MIA_ERR_VALUE,
+              "span attention: context beyond 2^30 tokens");
+  MIA_REQUIRE(rows * a.num_q_heads < (1ll << 30), MIA_ERR_VALUE,
+              "span attention: query tokens * heads beyond 2^30");
+  const int64_t eb = bf ? 2 : 1;
+  for (int i = 0; i < 2; ++i) {
+    const void *c = i ? a.v_cache : a.k_cache;
+    const int64_t *s = i ? a.v_cache_stride : a.k_cache_stride;
+    MIA_REQUIRE(s[3] == 1 && aligned(c, 16) && s[0] * eb % 16 == 0 && s[1] * eb % 16 == 0 &&
+                    s[2] * eb % 16 == 0,
+                MIA_ERR_VALUE,
+                "span attention: cache head_dim must be contiguous and its rows 16-byte aligned");
+    MIA_REQUIRE(s[2] >= 0 && s[2] * eb < (1ll << 27), MIA_ERR_VALUE,
+                "span attention: cache token stride out of range");
+  }
+  MIA_REQUIRE(aligned(a.q, 16) && q_rows[n_rows] == 1, MIA_ERR_VALUE,
+              "span attention: q rows must be contiguous and 16-byte aligned");
+  MIA_REQUIRE(aligned(a.out, 8) && out_rows[n_rows] == 1, MIA_ERR_VALUE,
+              "span attention: out rows must be contiguous and 8-byte aligned");
+  for (int i = 0; i < n_rows; ++i) {
+    MIA_REQUIRE(q_rows[i] % 8 == 0, MIA_ERR_VALUE,
+                "span attention: q rows must be contiguous and 16-byte aligned");
+    MIA_REQUIRE(out_rows[i] % 4 == 0, MIA_ERR_VALUE,
+                "span attention: out rows must be contiguous and 8-byte aligned");
+  }
+  return MIA_OK;
+}
+
 extern "C" {
 
 int mia_abi_version(void) { return MIA_ABI_VERSION; }
@@ -59,6 +110,9 @@ size_t mia_args_size(int which) {
     case 10: return sizeof(mia_qkv_epilogue_args);
     case 11: return sizeof(mia_row_norm_args);
     case 12: return sizeof(mia_skinny_linear_args);
+    case 13: return sizeof(mia_quant_kv_args);
+    case 14: return sizeof(mia_cross_args);
+    case 15: return sizeof(mia_shared_prefix_args);
     default: return 0;
   }
 }
@@ -624,6 +678,99 @@ int mia_scatter_rows(const mia_scatter_rows_args *a, mia_stream_t stream) {
   MIA_REQUIRE(a->num_rows >= 0 && a->head_dim > 0, MIA_ERR_VALUE,
               "scatter_rows: bad geometry");
   return mia::launch_scatter_rows(*a, (hipStream_t)stream);
+}
+
+static int quant_kv(const mia_quant_kv_args *a, bool write, mia_stream_t stream) {
+  mia::g_last_error.clear();
+  MIA_REQUIRE(a, MIA_ERR_VALUE, "quant_kv: null args");
+  MIA_REQUIRE(a->num_tokens >= 0, MIA_ERR_VALUE, "quant_kv: num_tokens < 0");
+  if (a->num_tokens == 0) return MIA_OK;
+  MIA_REQUIRE(a->k && a->v && a->slots && a->k_cache && a->v_cache && a->k_scales && a->v_scales,
+              MIA_ERR_VALUE, "quant_kv: null tensor pointer");
+  MIA_REQUIRE(a->row_dtype == MIA_DTYPE_BF16 || a->row_dtype == MIA_DTYPE_F16 ||
+                  a->row_dtype == MIA_DTYPE_F32,
+              MIA_ERR_NOT_IMPLEMENTED, "quant_kv: row dtype must be bf16/f16/f32");
+  MIA_REQUIRE(a->code_dtype == MIA_DTYPE_I8 || a->code_dtype == MIA_DTYPE_FP8_E4M3FN,
+              MIA_ERR_NOT_IMPLEMENTED, "quant_kv: cache dtype must be int8 or fp8 e4m3fn");
+  MIA_REQUIRE(a->slot_dtype == MIA_DTYPE_I32 || a->slot_dtype == MIA_DTYPE_I64 ||
+                  a->slot_dtype == MIA_DTYPE_U32,
+              MIA_ERR_VALUE, "quant_kv: slot dtype must be int32/int64/uint32");
+  MIA_REQUIRE(a->num_blocks > 0 && a->block_size > 0 && a->num_kv_heads > 0 && a->head_dim > 0,
+              MIA_ERR_VALUE, "quant_kv: bad cache geometry");
+  MIA_REQUIRE(a->head_dim <= 512, MIA_ERR_NOT_IMPLEMENTED, "quant_kv: head_dim above 512");
+  MIA_REQUIRE(a->num_tokens < (1ll << 31) / a->num_kv_heads, MIA_ERR_VALUE,
+              "quant_kv: num_tokens * kv_heads beyond 2^31");
+  return mia::launch_quant_kv(*a, write, (hipStream_t)stream);
+}
+
+int mia_quant_kv_write(const mia_quant_kv_args *a, mia_stream_t stream) {
+  return quant_kv(a, true, stream);
+}
+
+int mia_quant_kv_read(const mia_quant_kv_args *a, mia_stream_t stream) {
+  return quant_kv(a, false, stream);
+}
+
+static int validate_cross(const mia_cross_args *a) {
+  MIA_REQUIRE(a, MIA_ERR_VALUE, "cross_attention: null args");
+  MIA_REQUIRE(a->num_tokens >= 0 && a->num_seqs >= 0, MIA_ERR_VALUE, "cross_attention: bad shape");
+  if (a->num_tokens == 0 || a->num_seqs == 0) return MIA_OK;
+  MIA_REQUIRE(a->q && a->out && a->k_cache && a->v_cache && a->key_lens, MIA_ERR_VALUE,
+              "cross_attention: null tensor pointer");
+  MIA_REQUIRE(!a->cu_seqlens_q || a->max_seqlen_q > 0, MIA_ERR_VALUE,
+              "cross_attention: max_seqlen_q must be positive");
+  MIA_REQUIRE(a->block_table || (a->num_blocks >= a->num_seqs && a->blocks_per_seq == 1),
+              MIA_ERR_VALUE, "cross_attention: dense keys need one block per sequence");
+  return check_span(*a, a->q_stride, a->out_stride, 2, a->num_tokens, a->block_table != nullptr);
+}
+
+size_t mia_cross_workspace_bytes(const mia_cross_args *a) {
+  mia::g_last_error.clear();
+  if (validate_cross(a) || a->num_tokens == 0 || a->num_seqs == 0) return 0;
+  return mia::cross_workspace(*a);
+}
+
+int mia_cross_attention(const mia_cross_args *a, mia_stream_t stream) {
+  mia::g_last_error.clear();
+  const int rc = validate_cross(a);
+  if (rc) return rc;
+  if (a->num_tokens == 0 || a->num_seqs == 0) return MIA_OK;
+  MIA_REQUIRE(a->workspace && aligned(a->workspace, 256) &&
+                  a->workspace_bytes >= mia::cross_workspace(*a),
+              MIA_ERR_VALUE, "cross_attention: workspace missing, unaligned or too small");
+  return mia::launch_cross(*a, (hipStream_t)stream);
+}
+
+static int validate_shared_prefix(const mia_shared_prefix_args *a) {
+  MIA_REQUIRE(a, MIA_ERR_VALUE, "shared_prefix: null args");
+  MIA_REQUIRE(a->batch >= 0 && a->s_active > 0, MIA_ERR_VALUE, "shared_prefix: bad shape");
+  if (a->batch == 0) return MIA_OK;
+  MIA_REQUIRE(a->q && a->out && a->k_cache && a->v_cache && a->prefix_table && a->prefix_len &&
+                  a->block_table && a->seq_lens,
+              MIA_ERR_VALUE, "shared_prefix: null tensor pointer");
+  MIA_REQUIRE(a->s_active <= 64, MIA_ERR_NOT_IMPLEMENTED,
+              "shared_prefix: at most 64 active tokens per row");
+  MIA_REQUIRE(a->prefix_blocks > 0 &&
+                  (int64_t)a->prefix_blocks * a->block_size < (1ll << 30),
+              MIA_ERR_VALUE, "shared_prefix: empty prefix table or prefix beyond 2^30 tokens");
+  return check_span(*a, a->q_stride, a->out_stride, 3, (int64_t)a->batch * a->s_active, true);
+}
+
+size_t mia_shared_prefix_workspace_bytes(const mia_shared_prefix_args *a) {
+  mia::g_last_error.clear();
+  if (validate_shared_prefix(a) || a->batch == 0) return 0;
+  return mia::shared_prefix_workspace(*a);
+}
+
+int mia_shared_prefix_attention(const mia_shared_prefix_args *a, mia_stream_t stream) {
+  mia::g_last_error.clear();
+  const int rc = validate_shared_prefix(a);
+  if (rc) return rc;
+  if (a->batch == 0) return MIA_OK;
+  MIA_REQUIRE(a->workspace && aligned(a->workspace, 256) &&
+                  a->workspace_bytes >= mia::shared_prefix_workspace(*a),
+              MIA_ERR_VALUE, "shared_prefix: workspace missing, unaligned or too small");
+  return mia::launch_shared_prefix(*a, (hipStream_t)stream);
 }
 
 }  // extern "C"

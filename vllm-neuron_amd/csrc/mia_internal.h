@@ -33,6 +33,11 @@ int launch_stage_rows(const mia_stage_args &a, hipStream_t s);
 int launch_qkv_epilogue(const mia_qkv_epilogue_args &a, hipStream_t s);
 int launch_row_norm(const mia_row_norm_args &a, hipStream_t s);
 int launch_skinny_linear(const mia_skinny_linear_args &a, hipStream_t s);
+int launch_quant_kv(const mia_quant_kv_args &a, bool write, hipStream_t s);
+size_t cross_workspace(const mia_cross_args &a);
+int launch_cross(const mia_cross_args &a, hipStream_t s);
+size_t shared_prefix_workspace(const mia_shared_prefix_args &a);
+int launch_shared_prefix(const mia_shared_prefix_args &a, hipStream_t s);
 
 // Paged decode: split-K plan shared by the workspace query and the launch.
 struct DecodePlan {

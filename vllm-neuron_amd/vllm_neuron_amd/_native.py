@@ -27,6 +27,7 @@ DTYPE_FP8_E4M3FN = 3
 DTYPE_I32 = 4
 DTYPE_I64 = 5
 DTYPE_U32 = 6
+DTYPE_I8 = 7
 
 QUANT_NONE = 0
 QUANT_MUL_BF16 = 1
@@ -40,6 +41,7 @@ _TORCH_TO_MIA = {
     torch.float8_e4m3fn: DTYPE_FP8_E4M3FN,
     torch.int32: DTYPE_I32,
     torch.int64: DTYPE_I64,
+    torch.int8: DTYPE_I8,
 }
 if hasattr(torch, "uint32"):
     _TORCH_TO_MIA[torch.uint32] = DTYPE_U32
@@ -207,11 +209,56 @@ class SkinnyLinearArgs(ctypes.Structure):
     ]
 
 
+class QuantKvArgs(ctypes.Structure):
+    _fields_ = [
+        ("k", c_vp), ("v", c_vp), ("row_dtype", c_i32), ("code_dtype", c_i32),
+        ("k_stride", c_i64 * 3), ("v_stride", c_i64 * 3), ("slots", c_vp),
+        ("slot_dtype", c_i32), ("_pad0", c_i32), ("num_tokens", c_i64),
+        ("k_cache", c_vp), ("v_cache", c_vp),
+        ("k_cache_stride", c_i64 * 4), ("v_cache_stride", c_i64 * 4),
+        ("k_scales", c_vp), ("v_scales", c_vp),
+        ("k_scale_stride", c_i64 * 3), ("v_scale_stride", c_i64 * 3),
+        ("num_blocks", c_i32), ("block_size", c_i32), ("num_kv_heads", c_i32),
+        ("head_dim", c_i32),
+    ]
+
+
+class CrossArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", c_vp), ("q_stride", c_i64 * 3), ("out", c_vp), ("out_stride", c_i64 * 3),
+        ("num_tokens", c_i32), ("num_seqs", c_i32), ("cu_seqlens_q", c_vp),
+        ("max_seqlen_q", c_i32), ("num_q_heads", c_i32), ("num_kv_heads", c_i32),
+        ("head_dim", c_i32), ("k_cache", c_vp), ("v_cache", c_vp), ("cache_dtype", c_i32),
+        ("num_blocks", c_i32), ("k_cache_stride", c_i64 * 4), ("v_cache_stride", c_i64 * 4),
+        ("block_size", c_i32), ("blocks_per_seq", c_i32), ("block_table", c_vp),
+        ("bt_stride", c_i64 * 2), ("key_lens", c_vp), ("k_scales", c_vp), ("v_scales", c_vp),
+        ("k_scale_stride", c_i64 * 3), ("v_scale_stride", c_i64 * 3),
+        ("k_dequant", c_vp), ("v_dequant", c_vp), ("softmax_scale", c_f32), ("_pad0", c_i32),
+        ("workspace", c_vp), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class SharedPrefixArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", c_vp), ("q_stride", c_i64 * 4), ("out", c_vp), ("out_stride", c_i64 * 4),
+        ("batch", c_i32), ("s_active", c_i32), ("num_q_heads", c_i32), ("num_kv_heads", c_i32),
+        ("head_dim", c_i32), ("cache_dtype", c_i32), ("k_cache", c_vp), ("v_cache", c_vp),
+        ("k_cache_stride", c_i64 * 4), ("v_cache_stride", c_i64 * 4),
+        ("num_blocks", c_i32), ("block_size", c_i32), ("prefix_table", c_vp),
+        ("prefix_stride", c_i64), ("prefix_len", c_vp), ("block_table", c_vp),
+        ("bt_stride", c_i64 * 2), ("seq_lens", c_vp), ("prefix_blocks", c_i32),
+        ("blocks_per_seq", c_i32), ("k_scales", c_vp), ("v_scales", c_vp),
+        ("k_scale_stride", c_i64 * 3), ("v_scale_stride", c_i64 * 3),
+        ("k_dequant", c_vp), ("v_dequant", c_vp), ("sink", c_vp), ("softmax_scale", c_f32),
+        ("_pad0", c_i32), ("workspace", c_vp), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
 
 ARGS_STRUCTS = {
     0: KvWriteArgs, 1: GatherArgs, 2: MaskArgs, 3: DecodeArgs, 4: PrefillArgs,
     5: SlotMappingArgs, 6: PackedKArgs, 7: SwaTrimArgs, 8: ScatterRowsArgs, 9: StageArgs,
-    10: QkvEpilogueArgs, 11: RowNormArgs, 12: SkinnyLinearArgs,
+    10: QkvEpilogueArgs, 11: RowNormArgs, 12: SkinnyLinearArgs, 13: QuantKvArgs,
+    14: CrossArgs, 15: SharedPrefixArgs,
 }
 
 # Exported symbols (must match include/mia_attn.h).
@@ -222,6 +269,8 @@ EXPORTS = [
     "mia_slot_mapping_host", "mia_remap_null_block", "mia_swa_trim",
     "mia_packed_k_convert", "mia_scatter_rows", "mia_stage_rows", "mia_qkv_epilogue",
     "mia_row_norm", "mia_skinny_linear", "mia_paged_decode_noalloc",
+    "mia_quant_kv_write", "mia_quant_kv_read", "mia_cross_workspace_bytes",
+    "mia_cross_attention", "mia_shared_prefix_workspace_bytes", "mia_shared_prefix_attention",
 ]
 
 # Static scratch capacity of mia_paged_decode_noalloc (include/mia_attn.h).
@@ -244,7 +293,10 @@ def _declare(lib: ctypes.CDLL) -> None:
                      ("mia_swa_trim", SwaTrimArgs), ("mia_packed_k_convert", PackedKArgs),
                      ("mia_scatter_rows", ScatterRowsArgs), ("mia_stage_rows", StageArgs),
                      ("mia_qkv_epilogue", QkvEpilogueArgs), ("mia_row_norm", RowNormArgs),
-                     ("mia_skinny_linear", SkinnyLinearArgs)):
+                     ("mia_skinny_linear", SkinnyLinearArgs),
+                     ("mia_quant_kv_write", QuantKvArgs), ("mia_quant_kv_read", QuantKvArgs),
+                     ("mia_cross_attention", CrossArgs),
+                     ("mia_shared_prefix_attention", SharedPrefixArgs)):
         fn = getattr(lib, name)
         fn.argtypes = [P(st), c_vp]
         fn.restype = c_i32
@@ -252,6 +304,10 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.mia_decode_workspace_bytes.restype = ctypes.c_size_t
     lib.mia_prefill_workspace_bytes.argtypes = [P(PrefillArgs)]
     lib.mia_prefill_workspace_bytes.restype = ctypes.c_size_t
+    lib.mia_cross_workspace_bytes.argtypes = [P(CrossArgs)]
+    lib.mia_cross_workspace_bytes.restype = ctypes.c_size_t
+    lib.mia_shared_prefix_workspace_bytes.argtypes = [P(SharedPrefixArgs)]
+    lib.mia_shared_prefix_workspace_bytes.restype = ctypes.c_size_t
     lib.mia_slot_mapping_host.argtypes = [P(SlotMappingArgs)]
     lib.mia_slot_mapping_host.restype = c_i32
     lib.mia_remap_null_block.argtypes = [c_vp, c_vp, c_i64, c_i32, c_vp]
@@ -326,6 +382,27 @@ def stream_ptr(device: torch.device) -> int:
     # Stream object around it: ~2 us of a launch's host time)
     return torch._C._cuda_getCurrentRawStream(
         torch.cuda.current_device() if device.index is None else device.index)
+
+
+class _Here:
+    """A guard that does nothing (a context of contextlib costs ~1 us)."""
+
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return None
+
+
+_HERE = _Here()
+
+
+def on_device(device: torch.device):
+    """Guard for a launch on ``device``, a no-op where it is the current one:
+    a kernel goes to the current device, whatever its stream's is."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _HERE
+    return torch.cuda.device(device)
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

@@ -553,9 +553,130 @@ def skinny_linear(x, w, norm: bool = False, gamma=None, eps: float = 0.0,
     return _skinny_linear(x, w, bool(norm), gamma, float(eps), int(dim_actual))
 
 
+# ---------------------------------------------------------------------------
+# quantised cache
+# ---------------------------------------------------------------------------
+@custom_op("mia::quant_kv_write", mutates_args=("k_cache", "v_cache", "k_scales", "v_scales"))
+def _quant_kv_write(k: Tensor, v: Tensor, slots: Tensor, k_cache: Tensor, v_cache: Tensor,
+                    k_scales: Tensor, v_scales: Tensor) -> None:
+    K.quant_kv_write(k, v, slots, k_cache, v_cache, k_scales, v_scales)
+
+
+@_quant_kv_write.register_fake
+def _(k, v, slots, k_cache, v_cache, k_scales, v_scales):
+    return None
+
+
+def quant_kv_write(k, v, slots, k_cache, v_cache, k_scales, v_scales) -> None:
+    if _plain(k, v, slots, k_cache, v_cache, k_scales, v_scales):
+        K.quant_kv_write(k, v, slots, k_cache, v_cache, k_scales, v_scales)
+        _written(k_cache, v_cache, k_scales, v_scales)
+        return
+    _quant_kv_write(k, v, slots, k_cache, v_cache, k_scales, v_scales)
+
+
+@custom_op("mia::quant_kv_read", mutates_args=())
+def _quant_kv_read(k_cache: Tensor, v_cache: Tensor, k_scales: Tensor, v_scales: Tensor,
+                   slots: Tensor, dtype: torch.dtype) -> Tuple[Tensor, Tensor]:
+    return K.quant_kv_read(k_cache, v_cache, k_scales, v_scales, slots, dtype)
+
+
+@_quant_kv_read.register_fake
+def _(k_cache, v_cache, k_scales, v_scales, slots, dtype):
+    shape = (slots.shape[0], k_cache.shape[1], k_cache.shape[3])
+    return k_cache.new_empty(shape, dtype=dtype), k_cache.new_empty(shape, dtype=dtype)
+
+
+def quant_kv_read(k_cache, v_cache, k_scales, v_scales, slots,
+                  dtype=torch.bfloat16) -> Tuple[Tensor, Tensor]:
+    if _plain(k_cache, v_cache, k_scales, v_scales, slots):
+        return K.quant_kv_read(k_cache, v_cache, k_scales, v_scales, slots, dtype)
+    return _quant_kv_read(k_cache, v_cache, k_scales, v_scales, slots, dtype)
+
+
+# ---------------------------------------------------------------------------
+# attention over key spans of another length
+# ---------------------------------------------------------------------------
+@custom_op("mia::cross_attention", mutates_args=("out", "workspace"))
+def _cross_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, key_lens: Tensor, out: Tensor,
+                     block_table: Optional[Tensor], cu_seqlens_q: Optional[Tensor],
+                     k_scales: Optional[Tensor], v_scales: Optional[Tensor],
+                     k_dequant: Optional[Tensor], v_dequant: Optional[Tensor],
+                     workspace: Optional[Tensor], max_seqlen_q: int,
+                     softmax_scale: float) -> None:
+    K.cross_attention(q, k_cache, v_cache, key_lens, out, softmax_scale=softmax_scale,
+                      block_table=block_table, cu_seqlens_q=cu_seqlens_q,
+                      max_seqlen_q=max_seqlen_q, k_scales=k_scales, v_scales=v_scales,
+                      k_dequant=k_dequant, v_dequant=v_dequant, workspace=workspace)
+
+
+@_cross_attention.register_fake
+def _(q, k_cache, v_cache, key_lens, out, block_table, cu_seqlens_q, k_scales, v_scales,
+      k_dequant, v_dequant, workspace, max_seqlen_q, softmax_scale):
+    return None
+
+
+def cross_attention(q, k_cache, v_cache, key_lens, *, softmax_scale: float, block_table=None,
+                    cu_seqlens_q=None, max_seqlen_q: int = 0, k_scales=None, v_scales=None,
+                    k_dequant=None, v_dequant=None, out=None, workspace=None) -> Tensor:
+    if out is None:
+        out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+    if _plain(q, k_cache, v_cache, key_lens, out, block_table, cu_seqlens_q, k_scales, v_scales,
+              k_dequant, v_dequant, workspace):
+        K.cross_attention(q, k_cache, v_cache, key_lens, out, softmax_scale=float(softmax_scale),
+                          block_table=block_table, cu_seqlens_q=cu_seqlens_q,
+                          max_seqlen_q=int(max_seqlen_q), k_scales=k_scales, v_scales=v_scales,
+                          k_dequant=k_dequant, v_dequant=v_dequant, workspace=workspace)
+        _written(out, workspace)
+        return out
+    _cross_attention(q, k_cache, v_cache, key_lens, out, block_table, cu_seqlens_q, k_scales,
+                     v_scales, k_dequant, v_dequant, workspace, int(max_seqlen_q),
+                     float(softmax_scale))
+    return out
+
+
+@custom_op("mia::shared_prefix_attention", mutates_args=("out", "workspace"))
+def _shared_prefix_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, prefix_table: Tensor,
+                             prefix_len: Tensor, block_table: Tensor, seq_lens: Tensor,
+                             out: Tensor, sink: Optional[Tensor], k_scales: Optional[Tensor],
+                             v_scales: Optional[Tensor], k_dequant: Optional[Tensor],
+                             v_dequant: Optional[Tensor], workspace: Optional[Tensor],
+                             softmax_scale: float) -> None:
+    K.shared_prefix_attention(q, k_cache, v_cache, prefix_table, prefix_len, block_table,
+                              seq_lens, out, softmax_scale=softmax_scale, sink=sink,
+                              k_scales=k_scales, v_scales=v_scales, k_dequant=k_dequant,
+                              v_dequant=v_dequant, workspace=workspace)
+
+
+@_shared_prefix_attention.register_fake
+def _(q, k_cache, v_cache, prefix_table, prefix_len, block_table, seq_lens, out, sink, k_scales,
+      v_scales, k_dequant, v_dequant, workspace, softmax_scale):
+    return None
+
+
+def shared_prefix_attention(q, k_cache, v_cache, prefix_table, prefix_len, block_table, seq_lens,
+                            *, softmax_scale: float, sink=None, k_scales=None, v_scales=None,
+                            k_dequant=None, v_dequant=None, out=None, workspace=None) -> Tensor:
+    if out is None:
+        out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+    if _plain(q, k_cache, v_cache, prefix_table, prefix_len, block_table, seq_lens, out, sink,
+              k_scales, v_scales, k_dequant, v_dequant, workspace):
+        K.shared_prefix_attention(q, k_cache, v_cache, prefix_table, prefix_len, block_table,
+                                  seq_lens, out, softmax_scale=float(softmax_scale), sink=sink,
+                                  k_scales=k_scales, v_scales=v_scales, k_dequant=k_dequant,
+                                  v_dequant=v_dequant, workspace=workspace)
+        _written(out, workspace)
+        return out
+    _shared_prefix_attention(q, k_cache, v_cache, prefix_table, prefix_len, block_table, seq_lens,
+                             out, sink, k_scales, v_scales, k_dequant, v_dequant, workspace,
+                             float(softmax_scale))
+    return out
+
+
 OPS: List[str] = [
     "kv_write", "gather_kv", "packed_k_convert", "scatter_rows", "stage_rows", "decode_mask",
     "slot_mapping", "remap_null_block", "swa_trim", "paged_decode", "paged_decode_write",
     "paged_prefill",
     "qkv_epilogue", "row_norm", "skinny_linear",
+    "quant_kv_write", "quant_kv_read", "cross_attention", "shared_prefix_attention",
 ]
