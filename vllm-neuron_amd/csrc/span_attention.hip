@@ -5,21 +5,33 @@
 //
 // Mathematics.  Every row of a (sequence, kv head) sees every key of its
 // span: out = sum_k exp(s_k - m) v_k / sum_k exp(s_k - m), s_k = scale q.k_k,
-// accumulated over 64-key tiles with a running maximum m and sum l in fp32.
-// Spans of the same row are joined by their (m, l, o).  Codes of a quantised
-// cache are exact in bf16, so they go to the MFMA as they are: the scale of a
-// key multiplies its score, the scale of its value the probability.
+// accumulated tile by tile with a running maximum m and sum l in fp32.  Spans
+// of the same row are joined by their (m, l, o).  Codes of a quantised cache
+// are exact in bf16, so they go to the MFMA as they are: the scale of a key
+// multiplies its score, the scale of its value the probability.
 //
 // Rows.  The query rows of one kv head are packed GQA-first: row r = pos * G
-// + g is query token `pos` and q head h * G + g.  A segment is (sequence, kv
-// head, tile of 128 rows); its keys are walked in 64-key tiles.
+// + g is query token `pos` and q head h * G + g.
 //
-// Work split.  The tiles of all segments are laid end to end and cut into
-// equal shares, one per workgroup (two workgroups per CU), whatever the
-// lengths: each workgroup computes its share from the lengths on the device
-// (a block scan), so a captured call follows its tensors.  A share begins and
-// ends inside a segment; pieces of cut segments go to the workspace as fp32
-// (o, m, l) and a second kernel joins them.
+// Two forms of a tile, chosen by the rows that share a span (list.thin):
+//   tall  a workgroup takes 128 rows, 32 per wave; 64-key tiles of K and V go
+//         through LDS and serve all four waves (v_mfma_f32_32x32x16_bf16).
+//         Bound by the MFMAs and exponentials.
+//   thin  at most 16 or 32 rows: each wave streams 32-key tiles of its own, K
+//         straight into MFMA operands, V through a piece of LDS of the wave
+//         (v_mfma_f32_16x16x32_bf16).  Bound by HBM.
+// Both compute S^T = K Q^T and O^T = V^T P^T, so a lane holds scores of one
+// row, and its probabilities are the second product's operand as they are.
+//
+// Work split.  The tiles of all segments ((sequence, kv head, row tile)) of
+// a form are laid end to end and cut into equal shares, one per workgroup
+// (tall) or wave (thin), whatever the lengths: every workgroup computes its
+// share from the lengths on the device (a block scan), so a captured call
+// follows its tensors.  A share begins and ends inside a segment; pieces of
+// cut segments go to the workspace as fp32 (o, m, l) and a second kernel joins
+// them.  A call with both forms (shared prefix) gives them workgroups in
+// proportion to their tiles' costs, side by side in one launch: the prefix's
+// products run beside the own spans' HBM streams.
 #include <algorithm>
 
 #include "mia_device.h"
@@ -32,16 +44,22 @@ typedef float f32x16_t __attribute__((ext_vector_type(16)));
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4_t lds_s16x4_t;
 typedef __attribute__((address_space(3))) uint8_t lds_u8_t;
+typedef __attribute__((address_space(3))) u32x4_t lds_u32x4_t;
+typedef __attribute__((address_space(3))) f32x4_t lds_f32x4_t;
+typedef __attribute__((address_space(3))) float lds_f32_t;
 
 constexpr int kThreads = 256;
-constexpr int kRows = 128;  // query rows per segment (4 waves x 32)
-constexpr int kKT = 64;     // keys per tile
+constexpr int kWaves = 4;
+constexpr int kRows = 128;    // query rows of a tall segment (4 waves x 32)
+constexpr int kTallKeys = 64;  // keys per tall tile
+constexpr int kThinKeys = 32;  // keys per thin tile
 
 enum CacheKind { kBf16 = 0, kFp8 = 1, kI8 = 2 };
 
 // One list of sequences and their key spans.
 struct SpanList {
   int n;              // sequences
+  int thin;           // form of its tiles
   const int32_t *cu;  // [n + 1] first query tokens, or NULL: tok_per each
   int tok_per;
   int tok_max;        // query tokens of a sequence at most
@@ -50,7 +68,6 @@ struct SpanList {
   int len_cap;        // keys the table (or the dense rows) can hold
   const int32_t *bt;  // block table, or NULL: block = sequence
   int64_t bt_s, bt_j;
-  int cost;           // cost of a tile in the work split
   int part_rows;      // rows of a partial
   int64_t part0;      // first partial row
 };
@@ -73,11 +90,24 @@ struct SpanParams {
   FastDiv bs_div;
   float scale_log2;
   SpanList list[2];
-  int join;  // every piece goes to the workspace (rows have several spans)
-  int *hdr;
+  int join;        // every piece goes to the workspace (rows have several spans)
+  float cost[2];   // time of a tall tile per workgroup, of a thin one per wave
+  int least[2];    // tiles of a share at least
+  int *hdr;        // see plan()
   float *part_o;   // [partial row][D]
-  float *part_ml;  // [partial row][2]
+  float2 *part_ml; // [partial row]
 };
+
+// The launch's parameters (the first kernel argument) read anew from the
+// kernel's argument segment: what a piece's start or end needs is not kept in
+// scalar registers through the tile loops (kept, the 128-wide kernels
+// spilled over 100 of them to scratch).
+MIA_DEV const SpanParams &fresh() {
+  auto *k = (const __attribute__((address_space(4))) SpanParams *)
+      __builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(k));
+  return *(const SpanParams *)k;
+}
 
 MIA_DEV int list_len(const SpanList &l, int i) {
   return max(0, min(l.len[i] - l.len_sub, l.len_cap));
@@ -94,137 +124,222 @@ MIA_DEV int2 list_tokens(const SpanList &l, int i, int num_tokens) {
   }
   return make_int2(a, min(b - a, l.tok_max));
 }
-MIA_DEV int row_tiles(int rows) { return (rows + kRows - 1) / kRows; }
-
-// Cost of sequence u of the joined lists.
-MIA_DEV int64_t seq_cost(const SpanParams &p, int u) {
-  const int li = u < p.list[0].n ? 0 : 1;
-  const SpanList &l = p.list[li];
-  const int i = li ? u - p.list[0].n : u;
-  const int tiles = (list_len(l, i) + kKT - 1) / kKT;
-  if (tiles == 0) return 0;
-  const int rt = row_tiles(list_tokens(l, i, p.num_tokens).y * p.G);
-  return (int64_t)tiles * rt * p.Hkv * l.cost;
+MIA_DEV int row_tiles(const SpanList &l, int rows) {
+  return l.thin ? (rows > 0) : (rows + kRows - 1) / kRows;
+}
+MIA_DEV int key_tiles(const SpanList &l, int len) {
+  return l.thin ? (len + kThinKeys - 1) / kThinKeys : (len + kTallKeys - 1) / kTallKeys;
 }
 
-// Workgroup whose share [floor(w N / W), floor((w + 1) N / W)) holds cost
-// coordinate x: the largest w with floor(w N / W) <= x.
-MIA_DEV int wg_of(int64_t x, int64_t n, int w) { return (int)(((x + 1) * w - 1) / n); }
+// N tiles cut into W shares: the first `rem` hold base + 1, the others base.
+struct Cut {
+  int base, rem;
+};
+MIA_DEV int cut_start(Cut c, int w) { return w * c.base + min(w, c.rem); }
+MIA_DEV int cut_of(Cut c, int x) {  // the share that holds tile x
+  const int head = c.rem * (c.base + 1);
+  return x < head ? x / (c.base + 1) : c.rem + (x - head) / c.base;
+}
 
-// Where a workgroup's share starts, found by the plan.
+// Workspace header.  Joined calls: [0..3] the cuts of both forms, [8 + u] the
+// first tile of joined sequence u in its form's stream.  Cross attention: 8
+// ints per share: pieces of the cut segment that starts in it (0: none), its
+// first query token, rows, row tile, head.
+constexpr int kHdr = 8;
+
+// Where a share starts.
 struct Share {
-  int64_t n;        // total cost
-  int w_eff, w;     // workgroups with work, this one's number
-  int64_t x0, x1;   // its cost range
-  int u;            // first sequence with a tile at or past x0
-  int64_t base;     // cost before that sequence
+  Cut cut;
+  int w;       // number of the share
+  int x0, x1;  // its tiles
+  int u;       // sequence of tile x0
+  int xu;      // first tile of that sequence
 };
 
-MIA_DEV int64_t read64(int64_t x) {
-  return (int64_t)(((uint64_t)(uint32_t)readfirstlane((int)(x >> 32)) << 32) |
-                   (uint32_t)readfirstlane((int)x));
+struct PlanLds {
+  int tot[2][kWaves];
+  int seq[kWaves], first[kWaves];
+  int empty;
+};
+
+MIA_DEV int wave_scan(int x, int lane) {  // inclusive
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int y = __shfl_up(x, o, 64);
+    if (lane >= o) x += y;
+  }
+  return x;
 }
 
-// Block scan of the sequences' costs (each thread sums a contiguous run) and
-// this workgroup's share.  scan: int64 [kThreads + 1] and found: int64 [4] in
-// LDS.  With `hdr` the partials of every segment of the joined lists are
-// listed there: hdr[2 g] = first partial, hdr[2 g + 1] = how many.
-MIA_DEV bool plan_share(const SpanParams &p, int64_t *scan, int64_t *found, Share &sh) {
+// Rows of sequences without any key (cross attention): zeros.
+MIA_DEV void zero_empty(const SpanParams &p) {
+  const SpanList &l = p.list[1];
+  for (int i = blockIdx.x; i < l.n; i += gridDim.x) {
+    if (list_len(l, i) > 0) continue;
+    const int2 tk = list_tokens(l, i, p.num_tokens);
+    const int c8 = p.d / 8, hq = p.Hkv * p.G;
+    const int per_tok = hq * c8;
+    for (int t = tk.x; t < tk.x + tk.y; ++t)
+      for (int k = threadIdx.x; k < per_tok; k += kThreads) {
+        const int h = k / c8, c = k - h * c8;
+        const int b = (int)fdiv((uint32_t)t, p.s_div);
+        uint16_t *op = p.out + (int64_t)b * p.os_b + (int64_t)(t - b * p.S) * p.os_s +
+                       (int64_t)h * p.os_h + c * 8;
+        *reinterpret_cast<u32x2_t *>(op) = u32x2_t{0u, 0u};
+        *reinterpret_cast<u32x2_t *>(op + 4) = u32x2_t{0u, 0u};
+      }
+  }
+}
+
+// The plan of a launch, in every workgroup: a block scan of the sequences'
+// tiles (each thread a contiguous run of the joined lists), the workgroups of
+// each form, and this workgroup's (tall) or wave's (thin) share.  Returns 0
+// for a tall share, 1 for a thin one, -1 for none; uniform in the workgroup
+// (a thin wave without tiles has x0 == x1).
+MIA_DEV int plan(const SpanParams &p, PlanLds &lds, Share &sh) {
   const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = readfirstlane(tid >> 6);
   const int n_seq = p.list[0].n + p.list[1].n;
   const int per = (n_seq + kThreads - 1) / kThreads;
   const int u0 = min(tid * per, n_seq), u1 = min(u0 + per, n_seq);
-  int64_t sum = 0;
-  for (int u = u0; u < u1; ++u) sum += seq_cost(p, u);
-  // exclusive scan over the threads
-  scan[tid] = sum;
-  __syncthreads();
-  for (int o = 1; o < kThreads; o <<= 1) {
-    const int64_t v = tid >= o ? scan[tid - o] : 0;
-    __syncthreads();
-    scan[tid] += v;
-    __syncthreads();
+  auto tiles_of = [&](int u, int &thin, bool &empty) {
+    const int li = u < p.list[0].n ? 0 : 1;
+    const SpanList &l = p.list[li];
+    const int i = li ? u - p.list[0].n : u;
+    thin = l.thin;
+    const int len = list_len(l, i);
+    const int rows = list_tokens(l, i, p.num_tokens).y * p.G;
+    empty = len == 0 && rows > 0;
+    return key_tiles(l, len) * row_tiles(l, rows) * p.Hkv;
+  };
+  int sum[2] = {0, 0};
+  bool zero = false;
+  for (int u = u0; u < u1; ++u) {
+    int thin;
+    bool e;
+    const int n = tiles_of(u, thin, e);
+    sum[0] += thin ? 0 : n;
+    sum[1] += thin ? n : 0;
+    zero |= e && u % (int)gridDim.x == (int)blockIdx.x;
   }
-  const int64_t n = read64(scan[kThreads - 1]);
-  const int64_t base = scan[tid] - sum;
-  sh.n = n;
-  // shares of at least two of the dearest tiles, so that every workgroup
-  // between a segment's first and last has a piece of it
-  const int64_t least = 2 * max(p.list[0].cost, p.list[1].cost);
+  int inc[2];
+#pragma unroll
+  for (int f = 0; f < 2; ++f) {
+    inc[f] = wave_scan(sum[f], lane);
+    if (lane == 63) lds.tot[f][wave] = inc[f];
+  }
+  if (tid == 0) lds.empty = 0;
+  __syncthreads();
+  if (zero && !p.join) lds.empty = 1;
+  int n[2], base[2];
+#pragma unroll
+  for (int f = 0; f < 2; ++f) {
+    n[f] = 0;
+    base[f] = inc[f] - sum[f];
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      base[f] += w < wave ? lds.tot[f][w] : 0;
+      n[f] += lds.tot[f][w];
+    }
+    n[f] = readfirstlane(n[f]);
+  }
+  // workgroups of each form: in proportion to the costs, whole multiples of
+  // the 8 XCDs where there are enough
   const int grid = gridDim.x;
-  int w_eff = n == 0 ? 0 : (int)min((int64_t)grid, max((int64_t)1, n / least));
-  // workgroups go round-robin over the 8 XCDs: neighbouring shares (the row
-  // tiles of one head over the same keys) stay on one XCD's L2
-  int w = blockIdx.x;
-  if (w_eff >= 8) {
-    w_eff &= ~7;
-    w = (int)(blockIdx.x % 8) * (w_eff / 8) + blockIdx.x / 8;
-    if ((int)(blockIdx.x / 8) >= w_eff / 8) w = w_eff;
+  int wt = (n[0] + p.least[0] - 1) / p.least[0];
+  int ws = (n[1] + kWaves * p.least[1] - 1) / (kWaves * p.least[1]);
+  if (wt + ws > grid) {
+    const float a = (float)n[0] * p.cost[0], b = (float)n[1] * p.cost[1];
+    const int share = (int)((float)grid * (a / (a + b)) + 0.5f);
+    wt = n[0] == 0 ? 0 : n[1] == 0 ? grid : min(max(share, 1), grid - 1);
+    if (wt > 8 && wt < grid) wt &= ~7;
+    ws = n[1] == 0 ? 0 : grid - wt;
+  } else if (wt > 8) {
+    wt &= ~7;
   }
-  sh.w_eff = w_eff;
-  sh.w = w;
+  const int wv = ws * kWaves;
+  Cut cut[2];
+  cut[0].base = wt ? n[0] / wt : 0;
+  cut[0].rem = n[0] - cut[0].base * wt;
+  cut[1].base = wv ? n[1] / wv : 0;
+  cut[1].rem = n[1] - cut[1].base * wv;
   if (p.join) {
-    // every segment's partials (also those without any), by the workgroup of
-    // its sequence
-    int64_t x = base;
-    for (int u = u0; u < u1; ++u) {
-      const int li = u < p.list[0].n ? 0 : 1;
-      const SpanList &l = p.list[li];
-      const int i = li ? u - p.list[0].n : u;
-      const int tiles = (list_len(l, i) + kKT - 1) / kKT;
-      const int rt = row_tiles(list_tokens(l, i, p.num_tokens).y * p.G);
-      const int segs = rt * p.Hkv;
-      const int g0 = li ? row_tiles(p.num_tokens * p.G) * p.Hkv * p.list[0].n + i * segs : 0;
-      const int g_in = li ? i * segs : 0;  // segment number inside its list
-      if (u % grid == (int)blockIdx.x) {
-        for (int s = 0; s < segs; ++s) {
-          const int64_t xs = x + (int64_t)s * tiles * l.cost;
-          int first = 0, cnt = 0;
-          if (tiles > 0) {
-            first = wg_of(xs, n, w_eff);
-            cnt = wg_of(xs + (int64_t)(tiles - 1) * l.cost, n, w_eff) - first + 1;
-          }
-          p.hdr[2 * (g0 + s)] = g_in + s + first;
-          p.hdr[2 * (g0 + s) + 1] = cnt;
-        }
+    if (blockIdx.x == 0) {
+      if (tid == 0) {
+        p.hdr[0] = cut[0].base, p.hdr[1] = cut[0].rem;
+        p.hdr[2] = cut[1].base, p.hdr[3] = cut[1].rem;
       }
-      x += (int64_t)tiles * segs * l.cost;
+      int x[2] = {base[0], base[1]};
+      for (int u = u0; u < u1; ++u) {
+        int thin;
+        bool e;
+        const int c = tiles_of(u, thin, e);
+        p.hdr[kHdr + u] = thin ? x[1] : x[0];
+        x[0] += thin ? 0 : c;
+        x[1] += thin ? c : 0;
+      }
     }
-  } else if (tid == 0 && w < grid) {
-    // the cut segment that starts in this share, if any, fills it in later
-    if (w < w_eff) p.hdr[8 * w] = 0;
-    else p.hdr[8 * blockIdx.x] = 0;
   }
-  if (w >= w_eff) return false;
-  sh.x0 = w * n / w_eff;
-  sh.x1 = (int64_t)(w + 1) * n / w_eff;
-  if (base <= sh.x0 && sh.x0 < base + sum) {
-    int64_t x = base;
-    for (int u = u0; u < u1; ++u) {
-      const int64_t c = seq_cost(p, u);
-      if (sh.x0 < x + c) {
-        found[0] = u;
-        found[1] = x;
-        break;
+  const int b = blockIdx.x;
+  const int form = b < wt ? 0 : b < wt + ws ? 1 : -1;
+  int w;
+  if (form == 0) {
+    // workgroups go round-robin over the 8 XCDs: neighbouring shares (the row
+    // tiles of one head over the same keys) stay on one XCD's L2
+    w = wt >= 8 && wt % 8 == 0 ? (b % 8) * (wt / 8) + b / 8 : b;
+  } else {
+    w = (b - wt) * kWaves;
+  }
+  if (!p.join && lane == 0) {
+    // (one form only) no cut segment starts in a share unless it says so: the
+    // header is cleared by the thread that may set it
+    if (p.list[1].thin) p.hdr[kHdr * (b * kWaves + wave)] = 0;
+    else if (wave == 0) p.hdr[kHdr * (form == 0 ? w : b)] = 0;
+  }
+  const int f = form == 1 ? 1 : 0;
+  const int shares = form == 1 ? kWaves : 1;
+#pragma unroll
+  for (int k = 0; k < kWaves; ++k) {
+    if (form < 0 || k >= shares) break;
+    const int x = cut_start(cut[f], w + k);
+    if (x < n[f] && base[f] <= x && x < base[f] + sum[f]) {
+      int xu = base[f];
+      for (int u = u0; u < u1; ++u) {
+        int thin;
+        bool e;
+        const int c = tiles_of(u, thin, e);
+        if (thin != f) continue;
+        if (x < xu + c) {
+          lds.seq[k] = u;
+          lds.first[k] = xu;
+          break;
+        }
+        xu += c;
       }
-      x += c;
     }
   }
   __syncthreads();
-  sh.u = readfirstlane((int)found[0]);
-  sh.base = read64(found[1]);
-  return true;
+  if (lds.empty) zero_empty(p);
+  if (form < 0) return -1;
+  const int k = form == 1 ? wave : 0;
+  sh.cut = cut[f];
+  sh.w = w + k;
+  sh.x0 = cut_start(cut[f], sh.w);
+  sh.x1 = cut_start(cut[f], sh.w + 1);
+  sh.u = readfirstlane(lds.seq[k]);
+  sh.xu = readfirstlane(lds.first[k]);
+  return form;
 }
 
-// A position in the stream of tiles: segment and tile (all wave-uniform).
+// A position in a stream of tiles (wave-uniform).
 struct Pos {
-  int li, i;        // list, sequence
-  int tok0, rows;   // first query token, rows (tokens x G)
-  int len, tiles;   // keys, tiles
-  int rt_n, rt, h;  // row tiles, this one, kv head
-  int t;            // tile
-  int64_t x;        // cost coordinate of the tile
-  bool ok;          // inside the share
+  int li, i;          // list, sequence
+  int tok0, rows;     // first query token, rows (tokens x G)
+  int len, tiles;     // keys, tiles
+  int rt_n, rt, h;    // row tiles, this one, kv head
+  int t;              // tile
+  int left;           // tiles of the share from here on
 };
 
 MIA_DEV void load_seq(const SpanParams &p, Pos &c) {
@@ -233,19 +348,39 @@ MIA_DEV void load_seq(const SpanParams &p, Pos &c) {
   c.tok0 = readfirstlane(tk.x);
   c.rows = readfirstlane(tk.y * p.G);
   c.len = readfirstlane(list_len(l, c.i));
-  c.tiles = (c.len + kKT - 1) / kKT;
-  c.rt_n = row_tiles(c.rows);
+  c.tiles = key_tiles(l, c.len);
+  c.rt_n = row_tiles(l, c.rows);
 }
 
-// The first sequence at or after (li, i) with a tile and a row; clears ok
-// past the last.
-MIA_DEV void skip_empty(const SpanParams &p, Pos &c) {
+MIA_DEV Pos first_pos(const SpanParams &p, const Share &sh) {
+  Pos c;
+  c.li = sh.u < p.list[0].n ? 0 : 1;
+  c.i = c.li ? sh.u - p.list[0].n : sh.u;
+  load_seq(p, c);
+  const int k = sh.x0 - sh.xu;  // tile of the sequence
+  const int seg = k / c.tiles;
+  c.t = k - seg * c.tiles;
+  c.h = seg / c.rt_n;
+  c.rt = seg - c.h * c.rt_n;
+  c.left = sh.x1 - sh.x0;
+  return c;
+}
+
+// To the next tile of the share (left > 1), over sequences without tiles and
+// lists of the other form.
+MIA_DEV void advance(const SpanParams &p, Pos &c) {
+  --c.left;
+  if (++c.t < c.tiles) return;
+  c.t = 0;
+  if (++c.rt < c.rt_n) return;
+  c.rt = 0;
+  if (++c.h < p.Hkv) return;
+  c.h = 0;
+  const int form = p.list[c.li].thin;
+  ++c.i;
   while (true) {
-    if (c.i >= p.list[c.li].n) {
-      if (c.li == 1) {
-        c.ok = false;
-        return;
-      }
+    if (c.i >= p.list[c.li].n || p.list[c.li].thin != form) {
+      if (c.li == 1) return;  // not reached while tiles are left
       c.li = 1;
       c.i = 0;
       continue;
@@ -256,220 +391,245 @@ MIA_DEV void skip_empty(const SpanParams &p, Pos &c) {
   }
 }
 
-MIA_DEV Pos first_pos(const SpanParams &p, const Share &sh) {
-  Pos c;
-  c.ok = true;
-  c.li = sh.u < p.list[0].n ? 0 : 1;
-  c.i = c.li ? sh.u - p.list[0].n : sh.u;
-  load_seq(p, c);
-  const int cost = p.list[c.li].cost;
-  const int64_t k = (sh.x0 - sh.base + cost - 1) / cost;  // tile of the sequence
-  const int seg = (int)(k / c.tiles);
-  c.t = (int)(k - (int64_t)seg * c.tiles);
-  c.x = sh.base + k * cost;
-  c.h = seg / c.rt_n;
-  c.rt = seg - c.h * c.rt_n;
-  if (c.h >= p.Hkv) {  // x0 lies behind the start of the sequence's last tile
-    ++c.i;
-    c.h = c.rt = c.t = 0;
-    skip_empty(p, c);
-  }
-  if (c.x >= sh.x1) c.ok = false;
-  return c;
-}
-
-MIA_DEV void advance(const SpanParams &p, const Share &sh, Pos &c) {
-  c.x += p.list[c.li].cost;
-  if (c.x >= sh.x1) {
-    c.ok = false;
-    return;
-  }
-  if (++c.t < c.tiles) return;
-  c.t = 0;
-  if (++c.rt < c.rt_n) return;
-  c.rt = 0;
-  if (++c.h < p.Hkv) return;
-  c.h = 0;
-  ++c.i;
-  skip_empty(p, c);
-}
-
-MIA_DEV bool same_segment(const Pos &a, const Pos &b) {
-  return a.li == b.li && a.i == b.i && a.h == b.h && a.rt == b.rt;
-}
-
 template <int D>
 MIA_DEV constexpr int k_swz(int row) { return D == 128 ? row & 15 : (row >> 1) & 7; }
 template <int D>
 MIA_DEV constexpr int v_swz(int row) { return D == 128 ? (row & 3) << 2 : (row & 2) << 1; }
 
-// 16 bytes of codes -> two 16-byte chunks of bf16 (exact).
+// 8 codes (two dwords) -> 8 bf16 (exact).
 template <int CT>
-MIA_DEV void widen(u32x4_t w, u32x4_t (&out)[2]) {
+MIA_DEV u32x4_t widen8(uint32_t a, uint32_t b) {
+  u32x4_t o;
   if constexpr (CT == kFp8) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      out[i >> 1][(i & 1) * 2] = __builtin_bit_cast(
-          uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[i], 1.0f, false));
-      out[i >> 1][(i & 1) * 2 + 1] = __builtin_bit_cast(
-          uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[i], 1.0f, true));
-    }
+    o[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, false));
+    o[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, true));
+    o[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, false));
+    o[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, true));
   } else {
+    // bytes + 128 as unsigned, converted one by one
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      // bytes + 128 as unsigned, converted one by one
-      const uint32_t u = w[i] ^ 0x80808080u;
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t u = (i ? b : a) ^ 0x80808080u;
       const float f0 = (float)(u & 0xffu) - 128.f, f1 = (float)((u >> 8) & 0xffu) - 128.f;
       const float f2 = (float)((u >> 16) & 0xffu) - 128.f, f3 = (float)(u >> 24) - 128.f;
-      out[i >> 1][(i & 1) * 2] = pack2_bf16(f0, f1);
-      out[i >> 1][(i & 1) * 2 + 1] = pack2_bf16(f2, f3);
+      o[2 * i] = pack2_bf16(f0, f1);
+      o[2 * i + 1] = pack2_bf16(f2, f3);
     }
   }
+  return o;
 }
 
-MIA_DEV float row_max2(float x) {  // over the lanes l and l ^ 32 of a row
+// over the lanes l and l ^ 32
+MIA_DEV float max32(float x) {
   const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x),
                                                    false, false);
   return fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
 }
-MIA_DEV float row_sum2(float x) {
+MIA_DEV float sum32(float x) {
   const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x),
                                                    false, false);
   return __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
 }
+// over the lanes l and l ^ 16
+MIA_DEV float max16(float x) {
+  const auto sw = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x),
+                                                   false, false);
+  return fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+}
+MIA_DEV float sum16(float x) {
+  const auto sw = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x),
+                                                   false, false);
+  return __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
+}
 
-// Address of token t's row of head h (t = b * S + s).
+// Offset of token t (t = b * S + s).
 MIA_DEV int64_t tok_off(const SpanParams &p, int t, int64_t sb, int64_t ss) {
   const int b = (int)fdiv((uint32_t)t, p.s_div);
   return (int64_t)b * sb + (int64_t)(t - b * p.S) * ss;
 }
 
-// Rows of sequences without any key (cross attention): zeros.
-MIA_DEV void zero_empty(const SpanParams &p) {
-  const SpanList &l = p.list[1];
-  for (int i = blockIdx.x; i < l.n; i += gridDim.x) {
-    if (list_len(l, i) > 0) continue;
-    const int2 tk = list_tokens(l, i, p.num_tokens);
-    const int c8 = p.d / 8, hq = p.Hkv * p.G;
-    for (int64_t k = threadIdx.x; k < (int64_t)tk.y * hq * c8; k += kThreads) {
-      const int c = (int)(k % c8);
-      const int h = (int)(k / c8 % hq);
-      const int t = tk.x + (int)(k / ((int64_t)c8 * hq));
-      uint16_t *op = p.out + tok_off(p, t, p.os_b, p.os_s) + (int64_t)h * p.os_h + c * 8;
-      *reinterpret_cast<u32x2_t *>(op) = u32x2_t{0u, 0u};
-      *reinterpret_cast<u32x2_t *>(op + 4) = u32x2_t{0u, 0u};
+// The 16-key group of key k0 (k0 % 16 == 0, clamped into the span): its block
+// and the byte offsets of its first row in K and V.
+struct Group {
+  int k16;           // first key
+  int blk, off;
+};
+MIA_DEV Group key_group(const SpanParams &p, const Pos &c, int k0) {
+  const SpanList &l = p.list[c.li];
+  Group g;
+  g.k16 = min(k0, (c.len - 1) & ~15);
+  if (l.bt) {
+    const int bj = (int)fdiv((uint32_t)g.k16, p.bs_div);
+    const int blk = l.bt[(int64_t)c.i * l.bt_s + (int64_t)bj * l.bt_j];
+    g.blk = readfirstlane(min(max(blk, 0), p.nb - 1));
+    g.off = g.k16 - bj * p.bs;
+  } else {
+    g.blk = c.i;
+    g.off = g.k16;
+  }
+  return g;
+}
+MIA_DEV const uint8_t *k_row(const SpanParams &p, const Pos &c, const Group &g) {
+  return p.k_cache + (int64_t)g.blk * p.kc_blk + (int64_t)c.h * p.kc_h + (int64_t)g.off * p.kc_t;
+}
+MIA_DEV const uint8_t *v_row(const SpanParams &p, const Pos &c, const Group &g) {
+  return p.v_cache + (int64_t)g.blk * p.vc_blk + (int64_t)c.h * p.vc_h + (int64_t)g.off * p.vc_t;
+}
+MIA_DEV const float *k_scale(const SpanParams &p, const Pos &c, const Group &g) {
+  return p.k_sc + (int64_t)g.blk * p.ks_blk + (int64_t)c.h * p.ks_h + (int64_t)g.off * p.ks_t;
+}
+MIA_DEV const float *v_scale(const SpanParams &p, const Pos &c, const Group &g) {
+  return p.v_sc + (int64_t)g.blk * p.vs_blk + (int64_t)c.h * p.vs_h + (int64_t)g.off * p.vs_t;
+}
+
+// log2(e) x softmax scale x per-head scale of K: its magnitude; a negative
+// factor goes to q (sign bits), so that the largest product is the largest
+// score.
+MIA_DEV float score_factor(const SpanParams &p, int h, uint32_t &neg) {
+  float c1 = p.scale_log2;
+  if (p.k_deq) c1 *= p.k_deq[h];
+  neg = c1 < 0.f ? 0x80008000u : 0u;
+  const float c2 = fabsf(c1);
+  return c2 == 0.f ? 1e-37f : c2;  // masked scores (-inf) stay masked
+}
+
+// Partial row (or none: < 0) of row `rloc` of the piece [t0, c.t] of c's
+// segment in share sh.w, and the header of a cut segment.
+MIA_DEV int64_t piece_slot(const SpanParams &p, const Share &sh, const Pos &c, int t0,
+                           bool writer) {
+  const SpanList &ls = p.list[c.li];
+  int64_t slot;
+  if (p.join) {
+    const int segs = c.rt_n * p.Hkv;
+    slot = (int64_t)(c.li ? c.i * segs : 0) + c.h * c.rt_n + c.rt + sh.w;
+  } else {
+    slot = 2 * sh.w + (t0 == 0 ? 1 : 0);
+    if (t0 == 0 && writer) {
+      int *hd = p.hdr + kHdr * sh.w;
+      hd[1] = c.tok0;
+      hd[2] = c.rows;
+      hd[3] = c.rt;
+      hd[4] = c.h;
+      // the last tile of the segment lies tiles - 1 - t behind the share's last
+      hd[0] = cut_of(sh.cut, sh.x1 - 1 + c.tiles - 1 - c.t) - sh.w + 1;
     }
   }
+  return ls.part0 + slot * ls.part_rows;
+}
+
+// ---------------------------------------------------------------------------
+// tall form
+// ---------------------------------------------------------------------------
+template <int D, int CT, bool SC>
+struct TallLds {
+  static constexpr int TILEB = kTallKeys * D * 2;
+  uint8_t kv[2][2][TILEB];                       // [stage][K, V]
+  float sc[2][2][SC ? kTallKeys : 4];            // [stage][K, V]
+};
+
+// One 16-byte-per-lane copy HBM -> LDS: lane data lands at lds_dst + 16 *
+// lane; inactive lanes leave theirs.  Inline assembly, so that the compiler
+// adds no waits before reads of the other stage; the wait for the copies is
+// explicit.  M0 (the LDS base of the copy) is saved and restored around it.
+MIA_DEV void copy16(const uint8_t *src, uint32_t lds_dst) {
+  const uint32_t m0 = readfirstlane((int)lds_dst);
+  uint32_t saved;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_mov_b32 m0, %1\n\t"
+      "global_load_lds_dwordx4 %2, off\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(saved)
+      : "s"(m0), "v"(src)
+      : "memory");
 }
 
 template <int D, int CT, bool SC>
-__global__ __launch_bounds__(kThreads, 2) void span_kernel(SpanParams p) {
-  static_assert(D == 64 || D == 128, "tile widths");
-  static_assert(CT != kBf16 || !SC, "bf16 caches have no per-key scales");
+MIA_DEV void tall_body(const Share &sh, TallLds<D, CT, SC> &lds) {
+  constexpr bool DMA = CT == kBf16;    // else through registers, widened
   constexpr int EB = CT == kBf16 ? 2 : 1;
   constexpr int CE = 16 / EB;          // elements per 16-byte load
   constexpr int LPR = D / CE;          // lanes per key row
   constexpr int RPW = 64 / LPR;        // key rows per wave and load
-  constexpr int RP = 4 * RPW;          // key rows per load of the workgroup
-  constexpr int NP = kKT / RP;         // loads per thread and tile (K, V each)
+  constexpr int RP = kWaves * RPW;     // key rows per load of the workgroup
+  constexpr int NP = kTallKeys / RP;   // loads per thread and tile (K, V each)
   static_assert(RPW <= 16, "a wave's rows of a load lie in one 16-key group");
   constexpr int ROWB = D * 2;
-  constexpr int TILEB = kKT * ROWB;
+  constexpr int TILEB = kTallKeys * ROWB;
   constexpr int KSTEPS = D / 16;
   constexpr int DBLK = D / 32;
-
-  __shared__ __attribute__((aligned(1024))) uint8_t kv_lds[2][2][TILEB];
-  __shared__ __attribute__((aligned(16))) float sc_lds[2][2][SC ? kKT : 4];
-  __shared__ int64_t found[2];
-
-  if (!p.join) zero_empty(p);
-  Share sh;
-  if (!plan_share(p, reinterpret_cast<int64_t *>(&kv_lds[0][0][0]), found, sh)) return;
-  __syncthreads();  // the scan's memory becomes tiles
 
   const int tid = threadIdx.x;
   const int wave = readfirstlane(tid >> 6);
   const int lane = tid & 63;
   const int half = lane >> 5;
   const int rl = lane & 31;
-  lds_u8_t *const base = (lds_u8_t *)&kv_lds[0][0][0];
+  lds_u8_t *const base = (lds_u8_t *)&lds.kv[0][0][0];
+  lds_f32_t *const scb = (lds_f32_t *)&lds.sc[0][0][0];
 
   // ---- loads of a tile: thread -> key row j * RP + lrow, chunk lc
   const int lrow = wave * RPW + lane / LPR;
   const int lc = lane % LPR;
   const int g16 = (wave * RPW) & ~15;  // 16-key group of load 0
-  const bool ch_ok = lc * CE < p.d;
-  u32x4_t kr[NP], vr[NP];
-  float sr[NP];
-  auto load_tile = [&](const Pos &c) {
-    const SpanList &l = p.list[c.li];
-    const int kt = c.t * kKT;
+  const int d_used = fresh().d;
+  const bool ch_ok = lc * CE < d_used;
+  constexpr int NR = DMA ? 1 : NP;
+  u32x4_t kr[NR], vr[NR];
+  float sr[NR];
+  auto load_tile = [&](const Pos &c, int buf) {
+    const SpanParams &p = fresh();
+    const int kt = c.t * kTallKeys;
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
       // the group's block is wave-uniform; rows past the span read its last
       // key (in bounds) and are masked or cleared later
-      const int k16 = min(kt + j * RP + g16, (c.len - 1) & ~15);
-      int blk, off;
-      if (l.bt) {
-        const int bj = (int)fdiv((uint32_t)k16, p.bs_div);
-        blk = l.bt[(int64_t)c.i * l.bt_s + (int64_t)bj * l.bt_j];
-        blk = readfirstlane(min(max(blk, 0), p.nb - 1));
-        off = k16 - bj * p.bs;
+      const Group g = key_group(p, c, kt + j * RP + g16);
+      const int row = j * RP + lrow;
+      const int rr = min(kt + row, c.len - 1) - g.k16;
+      const uint8_t *kb = k_row(p, c, g), *vb = v_row(p, c, g);
+      if constexpr (DMA) {
+        const uint32_t dst = (uint32_t)(uintptr_t)base + (buf * 2) * TILEB +
+                             (j * RP + wave * RPW) * ROWB;
+        // the lane's slot of the copy is chunk lc of its row in LDS: it reads
+        // the chunk that the swizzle puts there
+        const int kc = lc ^ k_swz<D>(row), vc = lc ^ v_swz<D>(row);
+        if (kc * CE < d_used) copy16(kb + rr * (int)p.kc_t + kc * 16, dst);
+        if (vc * CE < d_used) copy16(vb + rr * (int)p.vc_t + vc * 16, dst + TILEB);
       } else {
-        blk = c.i;
-        off = k16;
-      }
-      const int rr = min(kt + j * RP + lrow, c.len - 1) - k16;
-      const uint8_t *kb = p.k_cache + (int64_t)blk * p.kc_blk + (int64_t)c.h * p.kc_h +
-                          (int64_t)off * p.kc_t;
-      const uint8_t *vb = p.v_cache + (int64_t)blk * p.vc_blk + (int64_t)c.h * p.vc_h +
-                          (int64_t)off * p.vc_t;
-      kr[j] = u32x4_t{0u, 0u, 0u, 0u};
-      vr[j] = u32x4_t{0u, 0u, 0u, 0u};
-      if (ch_ok) {
-        kr[j] = *reinterpret_cast<const u32x4_t *>(kb + rr * (int)p.kc_t + lc * 16);
-        vr[j] = *reinterpret_cast<const u32x4_t *>(vb + rr * (int)p.vc_t + lc * 16);
-      }
-      if constexpr (SC) {
-        const float *ks = p.k_sc + (int64_t)blk * p.ks_blk + (int64_t)c.h * p.ks_h +
-                          (int64_t)off * p.ks_t;
-        const float *vs = p.v_sc + (int64_t)blk * p.vs_blk + (int64_t)c.h * p.vs_h +
-                          (int64_t)off * p.vs_t;
-        sr[j] = 0.f;
-        if (lc < 2) sr[j] = lc ? vs[rr * p.vs_t] : ks[rr * p.ks_t];
+        kr[j] = u32x4_t{0u, 0u, 0u, 0u};
+        vr[j] = u32x4_t{0u, 0u, 0u, 0u};
+        if (ch_ok) {
+          kr[j] = *reinterpret_cast<const u32x4_t *>(kb + rr * (int)p.kc_t + lc * 16);
+          vr[j] = *reinterpret_cast<const u32x4_t *>(vb + rr * (int)p.vc_t + lc * 16);
+        }
+        if constexpr (SC) {
+          const float *ks = k_scale(p, c, g), *vs = v_scale(p, c, g);
+          sr[j] = 0.f;
+          if (lc < 2) sr[j] = lc ? vs[rr * p.vs_t] : ks[rr * p.ks_t];
+        }
       }
     }
   };
+  // 8-bit caches: the loaded tile widened into stage buf
   auto store_tile = [&](const Pos &c, int buf) {
-    const int kt = c.t * kKT;
+    const int kt = c.t * kTallKeys;
     lds_u8_t *const kb = base + (buf * 2) * TILEB;
     lds_u8_t *const vb = base + (buf * 2 + 1) * TILEB;
 #pragma unroll
-    for (int j = 0; j < NP; ++j) {
+    for (int j = 0; j < NR; ++j) {
       const int row = j * RP + lrow;
       // values past the span are cleared: 0 * NaN would reach the sums
       const bool in = kt + row < c.len;
       const u32x4_t v = in ? vr[j] : u32x4_t{0u, 0u, 0u, 0u};
-      if constexpr (CT == kBf16) {
-        *(__attribute__((address_space(3))) u32x4_t *)(kb + row * ROWB +
-                                                       ((lc ^ k_swz<D>(row)) << 4)) = kr[j];
-        *(__attribute__((address_space(3))) u32x4_t *)(vb + row * ROWB +
-                                                       ((lc ^ v_swz<D>(row)) << 4)) = v;
-      } else {
-        u32x4_t w[2];
-        widen<CT>(kr[j], w);
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
-          *(__attribute__((address_space(3))) u32x4_t *)(
-              kb + row * ROWB + (((2 * lc + x) ^ k_swz<D>(row)) << 4)) = w[x];
-        widen<CT>(v, w);
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-          *(__attribute__((address_space(3))) u32x4_t *)(
-              vb + row * ROWB + (((2 * lc + x) ^ v_swz<D>(row)) << 4)) = w[x];
+      for (int x = 0; x < 2; ++x) {
+        *(lds_u32x4_t *)(kb + row * ROWB + (((2 * lc + x) ^ k_swz<D>(row)) << 4)) =
+            widen8<CT>(kr[j][2 * x], kr[j][2 * x + 1]);
+        *(lds_u32x4_t *)(vb + row * ROWB + (((2 * lc + x) ^ v_swz<D>(row)) << 4)) =
+            widen8<CT>(v[2 * x], v[2 * x + 1]);
       }
       if constexpr (SC) {
-        if (lc < 2) sc_lds[buf][lc][row] = in ? sr[j] : 0.f;
+        if (lc < 2) scb[(buf * 2 + lc) * kTallKeys + row] = in ? sr[j] : 0.f;
       }
     }
   };
@@ -478,20 +638,18 @@ __global__ __launch_bounds__(kThreads, 2) void span_kernel(SpanParams p) {
   bf16x8_t qf[KSTEPS];
   f32x16_t acc[DBLK];
   float m_run = -INFINITY, l_run = 0.f;
-  float c2 = 0.f;  // log2(e) x softmax scale x per-head scale of K
+  float c2 = 0.f;
+  bool live = false;  // the wave has rows
   auto begin_piece = [&](const Pos &c) {
+    const SpanParams &p = fresh();
     const int r = c.rt * kRows + wave * 32 + rl;
+    live = c.rt * kRows + wave * 32 < c.rows;
     const bool ok = r < c.rows;
     const int pos = (int)fdiv((uint32_t)(ok ? r : 0), p.g_div);
     const int hq = c.h * p.G + (ok ? r - pos * p.G : 0);
     const uint16_t *qp = p.q + tok_off(p, c.tok0 + pos, p.qs_b, p.qs_s) + (int64_t)hq * p.qs_h;
-    float c1 = p.scale_log2;
-    if (p.k_deq) c1 *= p.k_deq[c.h];
-    // a negative factor goes to q, so that the largest product is the
-    // largest score
-    const uint32_t neg = c1 < 0.f ? 0x80008000u : 0u;
-    c2 = fabsf(c1);
-    if (c2 == 0.f) c2 = 1e-37f;  // masked scores (-inf) stay masked
+    uint32_t neg;
+    c2 = score_factor(p, c.h, neg);
 #pragma unroll
     for (int ks = 0; ks < KSTEPS; ++ks) {
       u32x4_t w = {0u, 0u, 0u, 0u};
@@ -511,6 +669,8 @@ __global__ __launch_bounds__(kThreads, 2) void span_kernel(SpanParams p) {
     l_run = 0.f;
   };
 
+  // transposed reads of V: within a 16-lane group, result lane k gets element
+  // k % 4 of the 8 bytes read by lane 4j + k/4
   const int tr_k = lane & 15;
   const int tr_col = ((lane >> 4) & 1) * 16 + 4 * (tr_k & 3);
   const int tr_row = half * 4 + (tr_k >> 2);
@@ -518,6 +678,8 @@ __global__ __launch_bounds__(kThreads, 2) void span_kernel(SpanParams p) {
   auto compute = [&](const Pos &c, int buf) {
     const lds_u8_t *kb = base + (buf * 2) * TILEB;
     const lds_u8_t *vb = base + (buf * 2 + 1) * TILEB;
+    const lds_f32_t *ksb = scb + (buf * 2) * kTallKeys;
+    const lds_f32_t *vsb = ksb + kTallKeys;
     // S^T = K . Q^T: lane = row rl, value e of block b: key b*32 + (e/4)*8 +
     // half*4 + e%4
     f32x16_t s[2];
@@ -528,8 +690,8 @@ __global__ __launch_bounds__(kThreads, 2) void span_kernel(SpanParams p) {
 #pragma unroll
       for (int ks = 0; ks < KSTEPS; ++ks) {
         const int row = b * 32 + rl;
-        const u32x4_t kf = *(const __attribute__((address_space(3))) u32x4_t *)(
-            kb + row * ROWB + (((ks * 2 + half) ^ k_swz<D>(row)) << 4));
+        const u32x4_t kf =
+            *(const lds_u32x4_t *)(kb + row * ROWB + (((ks * 2 + half) ^ k_swz<D>(row)) << 4));
         s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, kf), qf[ks],
                                                        s[b], 0, 0, 0);
       }
@@ -539,13 +701,12 @@ __global__ __launch_bounds__(kThreads, 2) void span_kernel(SpanParams p) {
       for (int b = 0; b < 2; ++b)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          const f32x4_t ks4 =
-              *reinterpret_cast<const f32x4_t *>(&sc_lds[buf][0][b * 32 + g * 8 + half * 4]);
+          const f32x4_t ks4 = *(const lds_f32x4_t *)(ksb + b * 32 + g * 8 + half * 4);
 #pragma unroll
           for (int i = 0; i < 4; ++i) s[b][g * 4 + i] *= ks4[i];
         }
     }
-    const int left = c.len - c.t * kKT - half * 4;
+    const int left = c.len - c.t * kTallKeys - half * 4;
     if (c.t == c.tiles - 1) {
 #pragma unroll
       for (int b = 0; b < 2; ++b)
@@ -556,14 +717,41 @@ __global__ __launch_bounds__(kThreads, 2) void span_kernel(SpanParams p) {
     // online softmax; the maximum moves only when a score passes it by more
     // than 8 (log2 units): probabilities stay below 2^8, the accumulators are
     // rescaled on few tiles
-    float mx = -INFINITY;
+    uint32_t pk[2][8];
+    auto exps = [&]() {
+      const float nm = m_run == -INFINITY ? 0.f : -m_run;
+      float ps[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+      for (int b = 0; b < 2; ++b)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[b][e]);
-    mx = row_max2(mx) * c2;
-    const bool bump = mx > m_run + 8.f || (m_run == -INFINITY && mx > -INFINITY);
-    if (__builtin_amdgcn_ballot_w64(bump)) {
+        for (int g = 0; g < 4; ++g) {
+          float pr[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            pr[i] = __builtin_amdgcn_exp2f(fmaf(s[b][g * 4 + i], c2, nm));
+            ps[i] += pr[i];
+          }
+          if constexpr (SC) {
+            const f32x4_t vs4 = *(const lds_f32x4_t *)(vsb + b * 32 + g * 8 + half * 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) pr[i] *= vs4[i];
+          }
+          // probabilities rounded to bf16 for the MFMA (half a step, 2^-8 of
+          // each); their sum keeps the unrounded ones
+          pk[b][g * 2] = pack2_bf16(pr[0], pr[1]);
+          pk[b][g * 2 + 1] = pack2_bf16(pr[2], pr[3]);
+        }
+      return (ps[0] + ps[1]) + (ps[2] + ps[3]);
+    };
+    auto raise = [&]() {  // moves the maximum where it must; true if it did
+      float mx = -INFINITY;
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[b][e]);
+      mx = max32(mx) * c2;
+      const bool bump = mx > m_run + 8.f || (m_run == -INFINITY && mx > -INFINITY);
+      if (!__builtin_amdgcn_ballot_w64(bump)) return false;
       const float m_new = bump ? mx : m_run;
       const float alpha = m_run == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
       m_run = m_new;
@@ -572,32 +760,15 @@ __global__ __launch_bounds__(kThreads, 2) void span_kernel(SpanParams p) {
       for (int i = 0; i < DBLK; ++i)
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[i][e] *= alpha;
-    }
-    const float nm = m_run == -INFINITY ? 0.f : -m_run;
-    uint32_t pk[2][8];
-    float ps[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        float pr[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          pr[i] = __builtin_amdgcn_exp2f(fmaf(s[b][g * 4 + i], c2, nm));
-          ps[i] += pr[i];
-        }
-        if constexpr (SC) {
-          const f32x4_t vs4 =
-              *reinterpret_cast<const f32x4_t *>(&sc_lds[buf][1][b * 32 + g * 8 + half * 4]);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) pr[i] *= vs4[i];
-        }
-        // probabilities rounded to bf16 for the MFMA (half a step, 2^-9);
-        // their sum keeps the unrounded ones
-        pk[b][g * 2] = pack2_bf16(pr[0], pr[1]);
-        pk[b][g * 2 + 1] = pack2_bf16(pr[2], pr[3]);
-      }
-    l_run += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+      return true;
+    };
+    // A half sum below 2^8 proves that no score passed the maximum by more
+    // than 8, so most tiles need no maximum; a row without one yet does
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(m_run == -INFINITY) != 0, 0)) raise();
+    float psum = exps();
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(psum < 256.f)) != 0, 0))
+      if (raise()) psum = exps();
+    l_run += psum;
     // O^T += V^T . P^T
 #pragma unroll
     for (int k2 = 0; k2 < 4; ++k2) {
@@ -625,12 +796,11 @@ __global__ __launch_bounds__(kThreads, 2) void span_kernel(SpanParams p) {
   // ---- end of a piece: final rows, or a partial.  t0: its first tile, c:
   // its last
   auto end_piece = [&](const Pos &c, int t0) {
-    const float l = row_sum2(l_run);
+    const SpanParams &p = fresh();
+    const float l = sum32(l_run);
     const int rloc = wave * 32 + rl;
     const int r = c.rt * kRows + rloc;
-    const bool whole = t0 == 0 && c.t == c.tiles - 1;
-    const SpanList &ls = p.list[c.li];
-    if (!p.join && whole) {
+    if (!p.join && t0 == 0 && c.t == c.tiles - 1) {
       if (r >= c.rows) return;
       const int pos = (int)fdiv((uint32_t)r, p.g_div);
       uint16_t *op = p.out + tok_off(p, c.tok0 + pos, p.os_b, p.os_s) +
@@ -642,33 +812,15 @@ __global__ __launch_bounds__(kThreads, 2) void span_kernel(SpanParams p) {
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const int d0 = i * 32 + g * 8 + half * 4;
-          if (d0 < p.d) {
-            const u32x2_t w = {pack2_bf16(acc[i][g * 4] * inv, acc[i][g * 4 + 1] * inv),
-                               pack2_bf16(acc[i][g * 4 + 2] * inv, acc[i][g * 4 + 3] * inv)};
-            *reinterpret_cast<u32x2_t *>(op + d0) = w;
-          }
+          if (d0 < p.d)
+            *reinterpret_cast<u32x2_t *>(op + d0) =
+                u32x2_t{pack2_bf16(acc[i][g * 4] * inv, acc[i][g * 4 + 1] * inv),
+                        pack2_bf16(acc[i][g * 4 + 2] * inv, acc[i][g * 4 + 3] * inv)};
         }
       return;
     }
-    int64_t slot;
-    if (p.join) {
-      const int segs = c.rt_n * p.Hkv;
-      slot = (int64_t)(c.li ? c.i * segs : 0) + c.h * c.rt_n + c.rt + sh.w;
-    } else {
-      slot = 2 * sh.w + (t0 == 0 ? 1 : 0);
-      if (t0 == 0 && tid == 0) {
-        const int cost = ls.cost;
-        int *hd = p.hdr + 8 * sh.w;
-        const int64_t x_last = c.x + (int64_t)(c.tiles - 1 - c.t) * cost;
-        hd[1] = c.tok0;
-        hd[2] = c.rows;
-        hd[3] = c.rt;
-        hd[4] = c.h;
-        hd[0] = wg_of(x_last, sh.n, sh.w_eff) - sh.w + 1;
-      }
-    }
-    if (r >= c.rows || rloc >= ls.part_rows) return;
-    const int64_t pr = ls.part0 + slot * ls.part_rows + rloc;
+    const int64_t pr = piece_slot(p, sh, c, t0, tid == 0) + rloc;
+    if (r >= c.rows || rloc >= p.list[c.li].part_rows) return;
     float *po = p.part_o + pr * D;
 #pragma unroll
     for (int i = 0; i < DBLK; ++i)
@@ -676,41 +828,448 @@ __global__ __launch_bounds__(kThreads, 2) void span_kernel(SpanParams p) {
       for (int g = 0; g < 4; ++g)
         *reinterpret_cast<f32x4_t *>(po + i * 32 + g * 8 + half * 4) =
             f32x4_t{acc[i][g * 4], acc[i][g * 4 + 1], acc[i][g * 4 + 2], acc[i][g * 4 + 3]};
-    if (half == 0) {
-      p.part_ml[2 * pr] = m_run;
-      p.part_ml[2 * pr + 1] = l;
+    if (half == 0) p.part_ml[pr] = make_float2(m_run, l);
+  };
+
+  // ---- the stream
+  if (sh.x0 >= sh.x1) return;
+  Pos cur = first_pos(fresh(), sh);
+  Pos nxt = cur;
+  int buf = 0, t0 = cur.t;
+  if constexpr (DMA) {
+    if (d_used < D) {  // channels past d: zero in both stages, never written again
+      for (int o = tid * 16; o < 4 * TILEB; o += kThreads * 16)
+        *(lds_u32x4_t *)(base + o) = u32x4_t{0u, 0u, 0u, 0u};
+      __syncthreads();
+    }
+    load_tile(cur, 0);
+    begin_piece(cur);
+    while (true) {
+      // own copies of tile `cur` have landed; the barrier makes every
+      // thread's visible and the other stage free
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      const bool more = cur.left > 1;
+      if (more) {
+        advance(fresh(), nxt);
+        load_tile(nxt, buf ^ 1);
+      }
+      const int left = cur.len - cur.t * kTallKeys;
+      if (left < kTallKeys) {
+        // values past the span are cleared: 0 * NaN would reach the sums
+        lds_u8_t *const vb = base + (buf * 2 + 1) * TILEB;
+        for (int o = left * ROWB + tid * 16; o < TILEB; o += kThreads * 16)
+          *(lds_u32x4_t *)(vb + o) = u32x4_t{0u, 0u, 0u, 0u};
+        __syncthreads();
+      }
+      if (live) compute(cur, buf);
+      const bool ends = !more || nxt.t == 0;
+      if (ends) {
+        end_piece(cur, t0);
+        if (!more) return;
+        begin_piece(nxt);
+        t0 = 0;
+      }
+      cur = nxt;
+      buf ^= 1;
+    }
+  } else {
+    load_tile(cur, 0);
+    begin_piece(cur);
+    store_tile(cur, 0);
+    bool more = cur.left > 1;
+    if (more) {
+      advance(fresh(), nxt);
+      load_tile(nxt, 0);
+    }
+    __syncthreads();
+    while (true) {
+      if (live) compute(cur, buf);
+      if (!more || nxt.t == 0) {
+        end_piece(cur, t0);
+        if (!more) return;
+        begin_piece(nxt);
+        t0 = 0;
+      }
+      store_tile(nxt, buf ^ 1);
+      cur = nxt;
+      more = cur.left > 1;
+      if (more) {
+        advance(fresh(), nxt);
+        load_tile(nxt, 0);
+      }
+      __syncthreads();
+      buf ^= 1;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// thin form
+// ---------------------------------------------------------------------------
+template <int D, bool SC>
+struct ThinLds {
+  uint8_t v[kWaves][kThinKeys * D * 2];
+  float sc[kWaves][SC ? 2 * kThinKeys : 4];
+};
+
+// NC groups of 16 columns (rows of the segment).
+template <int D, int CT, bool SC, int NC>
+MIA_DEV void thin_body(const Share &sh, ThinLds<D, SC> &lds) {
+  constexpr int EB = CT == kBf16 ? 2 : 1;
+  constexpr int KSTEPS = D / 32;
+  constexpr int VE = 16 / EB;          // V elements per 16-byte load
+  constexpr int DS = D / VE;           // lanes per V row
+  constexpr int TL = 64 / DS;          // V rows per load
+  constexpr int NV = kThinKeys / TL;   // V loads per tile
+  static_assert(TL <= 16, "a V load's rows lie in one 16-key group");
+  // K: bf16 k-step ks of lane group kg holds channels 32 ks + 8 kg; 8-bit
+  // k-steps 2u and 2u + 1 channels 64 u + 16 kg and + 8 (one 16-byte load)
+  constexpr int NK = CT == kBf16 ? KSTEPS : KSTEPS / 2;  // K loads per 16 keys
+  constexpr int ROWB = D * 2;
+  constexpr int VNCH = D / 8;
+  constexpr int DB16 = D / 16;
+
+  const int wave = readfirstlane((int)threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  const int col = lane & 15;
+  const int kg = lane >> 4;
+  lds_u8_t *const vw = (lds_u8_t *)&lds.v[wave][0];
+  lds_f32_t *const sw = (lds_f32_t *)&lds.sc[wave][0];
+
+  const int d_used = fresh().d;
+  auto k_chan = [](int j, int g) { return CT == kBf16 ? j * 32 + g * 8 : j * 64 + g * 16; };
+  const int vds = lane % DS, vtl = lane / DS;
+
+  u32x4_t kr[2][NK], vr[NV];
+  float sr = 0.f;
+  struct Groups {
+    Group g[2];
+  };
+  auto groups = [&](const Pos &c) {
+    const SpanParams &p = fresh();
+    Groups x;
+    x.g[0] = key_group(p, c, c.t * kThinKeys);
+    x.g[1] = key_group(p, c, c.t * kThinKeys + 16);
+    return x;
+  };
+  // rows past the span read its last key (in bounds) and are masked or
+  // cleared later
+  auto load_k = [&](const Pos &c, const Groups &gs) {
+    const SpanParams &p = fresh();
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const Group &g = gs.g[b];
+      const int rr = min(c.t * kThinKeys + b * 16 + col, c.len - 1) - g.k16;
+      const uint8_t *a = k_row(p, c, g) + rr * (int)p.kc_t;
+#pragma unroll
+      for (int j = 0; j < NK; ++j) {
+        kr[b][j] = u32x4_t{0u, 0u, 0u, 0u};
+        if (k_chan(j, kg) < d_used)
+          kr[b][j] = *reinterpret_cast<const u32x4_t *>(a + k_chan(j, kg) * EB);
+      }
+    }
+  };
+  auto load_v = [&](const Pos &c, const Groups &gs) {
+    const SpanParams &p = fresh();
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const Group &g = gs.g[j * TL / 16];
+      const int rr = min(c.t * kThinKeys + j * TL + vtl, c.len - 1) - g.k16;
+      vr[j] = u32x4_t{0u, 0u, 0u, 0u};
+      if (vds * VE < d_used)
+        vr[j] = *reinterpret_cast<const u32x4_t *>(v_row(p, c, g) + rr * (int)p.vc_t + vds * 16);
+    }
+  };
+  // lane l: scale of key l (K), of key l - 32 (V)
+  auto load_s = [&](const Pos &c, const Groups &gs) {
+    if constexpr (SC) {
+      const SpanParams &p = fresh();
+      const int k = lane & 31;
+      const Group &g = gs.g[0], &g1 = gs.g[1];
+      const bool hi = k >= 16;
+      const int rr = min(c.t * kThinKeys + k, c.len - 1) - (hi ? g1.k16 : g.k16);
+      const float *ks = hi ? k_scale(p, c, g1) : k_scale(p, c, g);
+      const float *vs = hi ? v_scale(p, c, g1) : v_scale(p, c, g);
+      sr = lane < 32 ? ks[rr * p.ks_t] : vs[rr * p.vs_t];
+      if (c.t * kThinKeys + k >= c.len) sr = 0.f;
     }
   };
 
-  // ---- the stream: tile n is computed while tile n + 1 is in LDS's other
-  // buffer or in flight
-  Pos cur = first_pos(p, sh);
-  if (!cur.ok) return;
-  load_tile(cur);
+  // ---- state of the current piece
+  bf16x8_t qf[NC][KSTEPS];
+  f32x4_t acc[NC][DB16];
+  float m_run[NC], l_run[NC];
+  float c2 = 0.f;
+  auto begin_piece = [&](const Pos &c) {
+    const SpanParams &p = fresh();
+    uint32_t neg;
+    c2 = score_factor(p, c.h, neg);
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+      const int r = n * 16 + col;
+      const bool ok = r < c.rows;
+      const int pos = (int)fdiv((uint32_t)(ok ? r : 0), p.g_div);
+      const int hq = c.h * p.G + (ok ? r - pos * p.G : 0);
+      const uint16_t *qp = p.q + tok_off(p, c.tok0 + pos, p.qs_b, p.qs_s) + (int64_t)hq * p.qs_h;
+#pragma unroll
+      for (int ks = 0; ks < KSTEPS; ++ks) {
+        const int d0 = CT == kBf16 ? k_chan(ks, kg) : k_chan(ks >> 1, kg) + (ks & 1) * 8;
+        u32x4_t w = {0u, 0u, 0u, 0u};
+        if (ok && d0 < p.d) {
+          w = *reinterpret_cast<const u32x4_t *>(qp + d0);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[i] ^= neg;
+        }
+        qf[n][ks] = __builtin_bit_cast(bf16x8_t, w);
+      }
+#pragma unroll
+      for (int i = 0; i < DB16; ++i) acc[n][i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      m_run[n] = -INFINITY;
+      l_run[n] = 0.f;
+    }
+  };
+
+  // V^T operand of 16 channels: k index j of lane group kg is key 4 kg + j
+  // (j < 4), 16 + 4 kg + j - 4 (else), the keys whose scores the lane holds;
+  // source lane s of a 16-lane group addresses key 4 kg + s/4, channels 4 (s%4)
+  const int tr_s = lane & 15;
+  const int tr_row = 4 * kg + (tr_s >> 2);
+  const int tr_x = tr_row & (VNCH - 1);
+
+  // S^T of the tile; frees the K registers
+  f32x4_t s[NC][2];
+  auto scores = [&]() {
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+#pragma unroll
+      for (int n = 0; n < NC; ++n) s[n][b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < KSTEPS; ++ks) {
+        u32x4_t w;
+        if constexpr (CT == kBf16) w = kr[b][ks];
+        else w = widen8<CT>(kr[b][ks >> 1][(ks & 1) * 2], kr[b][ks >> 1][(ks & 1) * 2 + 1]);
+#pragma unroll
+        for (int n = 0; n < NC; ++n)
+          s[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, w),
+                                                            qf[n][ks], s[n][b], 0, 0, 0);
+      }
+    }
+  };
+  auto store_v = [&](const Pos &c) {
+    const int left = c.len - c.t * kThinKeys;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int t = j * TL + vtl;
+      // values past the span are cleared: 0 * NaN would reach the sums
+      const u32x4_t v = t < left ? vr[j] : u32x4_t{0u, 0u, 0u, 0u};
+      if constexpr (CT == kBf16) {
+        *(lds_u32x4_t *)(vw + t * ROWB + ((vds ^ (t & (VNCH - 1))) << 4)) = v;
+      } else {
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          *(lds_u32x4_t *)(vw + t * ROWB + (((2 * vds + x) ^ (t & (VNCH - 1))) << 4)) =
+              widen8<CT>(v[2 * x], v[2 * x + 1]);
+      }
+    }
+  };
+  u32x4_t pk[NC];
+  auto softmax = [&](const Pos &c) {
+    f32x4_t ks4[2], vs4[2];
+    if constexpr (SC) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        ks4[b] = *(const lds_f32x4_t *)(sw + b * 16 + kg * 4);
+        vs4[b] = *(const lds_f32x4_t *)(sw + 32 + b * 16 + kg * 4);
+      }
+    }
+    const int left = c.len - c.t * kThinKeys - kg * 4;
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float x = s[n][b][i];
+          if constexpr (SC) x *= ks4[b][i];
+          x = b * 16 + i < left ? x : -INFINITY;
+          s[n][b][i] = x;
+          mx = fmaxf(mx, x);
+        }
+      mx = max32(max16(mx)) * c2;
+      const bool bump = mx > m_run[n] + 8.f || (m_run[n] == -INFINITY && mx > -INFINITY);
+      if (__builtin_amdgcn_ballot_w64(bump)) {
+        const float m_new = bump ? mx : m_run[n];
+        const float alpha =
+            m_run[n] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run[n] - m_new);
+        m_run[n] = m_new;
+        l_run[n] *= alpha;
+#pragma unroll
+        for (int i = 0; i < DB16; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[n][i][e] *= alpha;
+      }
+      const float nm = m_run[n] == -INFINITY ? 0.f : -m_run[n];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        float pr[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          pr[i] = __builtin_amdgcn_exp2f(fmaf(s[n][b][i], c2, nm));
+          l_run[n] += pr[i];
+          if constexpr (SC) pr[i] *= vs4[b][i];
+        }
+        // rounded to bf16 for the MFMA; the sum keeps the unrounded ones
+        pk[n][2 * b] = pack2_bf16(pr[0], pr[1]);
+        pk[n][2 * b + 1] = pack2_bf16(pr[2], pr[3]);
+      }
+    }
+  };
+  auto values = [&]() {
+#pragma unroll
+    for (int blk = 0; blk < DB16; ++blk) {
+      const uint32_t off = tr_row * ROWB + (((blk * 2 + ((tr_s >> 1) & 1)) ^ tr_x) << 4) +
+                           ((tr_s & 1) << 3);
+      // row + 16 has the same swizzle (VNCH divides 16)
+      const u32x2_t t0 = __builtin_bit_cast(
+          u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t *)(vw + off)));
+      const u32x2_t t1 = __builtin_bit_cast(
+          u32x2_t,
+          __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t *)(vw + off + 16 * ROWB)));
+      const u32x4_t v = {t0[0], t0[1], t1[0], t1[1]};
+#pragma unroll
+      for (int n = 0; n < NC; ++n)
+        acc[n][blk] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+            __builtin_bit_cast(bf16x8_t, v), __builtin_bit_cast(bf16x8_t, pk[n]), acc[n][blk], 0,
+            0, 0);
+    }
+  };
+  auto end_piece = [&](const Pos &c, int t0) {
+    const SpanParams &p = fresh();
+    const bool whole = !p.join && t0 == 0 && c.t == c.tiles - 1;
+    const int64_t pr0 = whole ? 0 : piece_slot(p, sh, c, t0, lane == 0);
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+      const float l = sum32(sum16(l_run[n]));
+      const int r = n * 16 + col;
+      if (r >= c.rows) continue;
+      if (whole) {
+        const int pos = (int)fdiv((uint32_t)r, p.g_div);
+        uint16_t *op = p.out + tok_off(p, c.tok0 + pos, p.os_b, p.os_s) +
+                       (int64_t)(c.h * p.G + r - pos * p.G) * p.os_h;
+        float inv = l == 0.f ? 0.f : 1.f / l;
+        if (p.v_deq) inv *= p.v_deq[c.h];
+#pragma unroll
+        for (int i = 0; i < DB16; ++i) {
+          const int d0 = i * 16 + kg * 4;
+          if (d0 < p.d)
+            *reinterpret_cast<u32x2_t *>(op + d0) =
+                u32x2_t{pack2_bf16(acc[n][i][0] * inv, acc[n][i][1] * inv),
+                        pack2_bf16(acc[n][i][2] * inv, acc[n][i][3] * inv)};
+        }
+      } else if (r < p.list[c.li].part_rows) {
+        float *po = p.part_o + (pr0 + r) * D;
+#pragma unroll
+        for (int i = 0; i < DB16; ++i)
+          *reinterpret_cast<f32x4_t *>(po + i * 16 + kg * 4) = acc[n][i];
+        if (kg == 0) p.part_ml[pr0 + r] = make_float2(m_run[n], l);
+      }
+    }
+  };
+
+  // ---- the stream: K (V) of the next tile is issued once this tile's
+  // product (copy to LDS) has freed the registers
+  if (sh.x0 >= sh.x1) return;
+  Pos cur = first_pos(fresh(), sh);
+  Groups gs = groups(cur);
+  load_k(cur, gs);
+  load_s(cur, gs);
+  load_v(cur, gs);
   begin_piece(cur);
-  store_tile(cur, 0);
-  Pos nxt = cur;
-  advance(p, sh, nxt);
-  if (nxt.ok) load_tile(nxt);
-  __syncthreads();
-  int buf = 0, t0 = cur.t;
+  int t0 = cur.t;
   while (true) {
-    compute(cur, buf);
-    if (!nxt.ok) {
-      end_piece(cur, t0);
-      return;
+    const bool more = cur.left > 1;
+    Pos nxt = cur;
+    if (more) {
+      advance(fresh(), nxt);
+      gs = groups(nxt);
     }
-    if (!same_segment(cur, nxt)) {
+    scores();
+    if constexpr (SC) sw[lane] = sr;
+    if (more) {
+      load_k(nxt, gs);
+      load_s(nxt, gs);
+    }
+    softmax(cur);
+    store_v(cur);
+    if (more) load_v(nxt, gs);
+    values();
+    if (!more || nxt.t == 0) {
       end_piece(cur, t0);
+      if (!more) return;
       begin_piece(nxt);
-      t0 = nxt.t;
+      t0 = 0;
     }
-    store_tile(nxt, buf ^ 1);
     cur = nxt;
-    advance(p, sh, nxt);
-    if (nxt.ok) load_tile(nxt);
-    __syncthreads();
-    buf ^= 1;
+  }
+}
+
+template <int D, int CT, bool SC, int NC>
+__global__ __launch_bounds__(kThreads, 2) void span_kernel(SpanParams p) {
+  static_assert(D == 64 || D == 128, "tile widths");
+  static_assert(CT != kBf16 || !SC, "bf16 caches have no per-key scales");
+  __shared__ union __attribute__((aligned(1024))) {
+    TallLds<D, CT, SC> tall;
+    ThinLds<D, SC> thin;
+  } lds;
+  __shared__ PlanLds plan_lds;
+  Share sh;
+  const int form = plan(fresh(), plan_lds, sh);
+  if (form == 0) tall_body<D, CT, SC>(sh, lds.tall);
+  else if (form == 1) thin_body<D, CT, SC, NC>(sh, lds.thin);
+}
+
+// Weighted sum of the n pieces of a row (partial row prow(j)) by the D / 4
+// lanes of the row, four channels each: the lanes take a piece's (m, l) each,
+// then all of them every piece's o.
+template <int LPR, typename F>
+MIA_DEV void sum_pieces(const SpanParams &p, int n, F prow, int c, int D, float &m, float &l,
+                        f32x4_t &o) {
+  for (int k0 = 0; k0 < n; k0 += LPR) {
+    const int cnt = min(LPR, n - k0);
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (c < cnt) ml = p.part_ml[prow(k0 + c)];
+    float mc = ml.x;
+#pragma unroll
+    for (int x = 1; x < LPR; x <<= 1) mc = fmaxf(mc, __shfl_xor(mc, x, 64));
+    const float m_new = fmaxf(m, mc);
+    const float mm = m_new == -INFINITY ? 0.f : m_new;
+    const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mm);
+    m = m_new;
+    const float w = c < cnt ? __builtin_amdgcn_exp2f(ml.x - mm) : 0.f;
+    float ls = c < cnt ? w * ml.y : 0.f;
+#pragma unroll
+    for (int x = 1; x < LPR; x <<= 1) ls += __shfl_xor(ls, x, 64);
+    l = l * alpha + ls;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] *= alpha;
+    for (int j = 0; j < cnt; j += 4) {
+      f32x4_t v[4];
+      float wj[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        v[u] = *reinterpret_cast<const f32x4_t *>(p.part_o + prow(k0 + min(j + u, cnt - 1)) * D +
+                                                  c * 4);
+        wj[u] = __shfl(w, min(j + u, LPR - 1), LPR);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (j + u >= cnt) break;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] += wj[u] * v[u][i];
+      }
+    }
   }
 }
 
@@ -719,32 +1278,21 @@ __global__ __launch_bounds__(kThreads, 2) void span_kernel(SpanParams p) {
 template <int D>
 __global__ __launch_bounds__(256) void span_merge_kernel(SpanParams p) {
   const int w = blockIdx.x;
-  const int *hd = p.hdr + 8 * w;
+  const int *hd = p.hdr + kHdr * w;
   const int n = hd[0];
   if (n == 0) return;
   constexpr int LPR = D / 4;
-  constexpr int RPB = 256 / LPR;
   const int c = threadIdx.x % LPR;
   const SpanList &l = p.list[1];
-  const int rloc = blockIdx.y * RPB + threadIdx.x / LPR;
+  const int rloc = blockIdx.y * (256 / LPR) + threadIdx.x / LPR;
   const int r = hd[3] * kRows + rloc;
-  if (r >= hd[2] || rloc >= l.part_rows) return;
+  if (r >= hd[2] || rloc >= l.part_rows) return;  // whole groups of LPR lanes leave
   auto prow = [&](int j) {
     return l.part0 + (int64_t)(j == 0 ? 2 * w + 1 : 2 * (w + j)) * l.part_rows + rloc;
   };
-  float m = -INFINITY;
-  for (int j = 0; j < n; ++j) m = fmaxf(m, p.part_ml[2 * prow(j)]);
-  const float mm = m == -INFINITY ? 0.f : m;
+  float m = -INFINITY, ls = 0.f;
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-  float ls = 0.f;
-  for (int j = 0; j < n; ++j) {
-    const int64_t pr = prow(j);
-    const float wgt = __builtin_amdgcn_exp2f(p.part_ml[2 * pr] - mm);
-    ls += wgt * p.part_ml[2 * pr + 1];
-    const f32x4_t v = *reinterpret_cast<const f32x4_t *>(p.part_o + pr * D + c * 4);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] += wgt * v[i];
-  }
+  sum_pieces<LPR>(p, n, prow, c, D, m, ls, o);
   float inv = ls == 0.f ? 0.f : 1.f / ls;
   const int h = hd[4];
   if (p.v_deq) inv *= p.v_deq[h];
@@ -760,51 +1308,45 @@ __global__ __launch_bounds__(256) void span_merge_kernel(SpanParams p) {
 // new tokens that not every row of its sequence sees (the last S - 1 keys,
 // row s sees s of them) and the sink.  D / 4 lanes per row.
 template <int D, int CT, bool SC>
-__global__ __launch_bounds__(256) void span_join_kernel(SpanParams p) {
+__global__ __launch_bounds__(256) void span_join_kernel(SpanParams p, FastDiv hq_div) {
   constexpr int LPR = D / 4;
   const int c = threadIdx.x % LPR;
-  const int64_t row = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
-  const int Hq = p.Hkv * p.G;
-  if (row >= (int64_t)p.num_tokens * Hq) return;  // whole groups of LPR lanes leave
-  const int t = (int)(row / Hq);
-  const int hq = (int)(row - (int64_t)t * Hq);
+  const int row = blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
+  if (row >= p.num_tokens * (int)hq_div.d) return;  // whole groups of LPR lanes leave
+  const int t = (int)fdiv((uint32_t)row, hq_div);
+  const int hq = row - t * (int)hq_div.d;
   const int h = (int)fdiv((uint32_t)hq, p.g_div);
   const int g = hq - h * p.G;
   const int b = (int)fdiv((uint32_t)t, p.s_div);
   const int s = t - b * p.S;
+  // first partial row and pieces of the row in list li, sequence i, its row r
+  auto pieces = [&](int li, int i, int r, int rows, int64_t &first) {
+    const SpanList &l = p.list[li];
+    const int tiles = key_tiles(l, list_len(l, i));
+    first = 0;
+    if (tiles == 0) return 0;
+    const int rt_n = row_tiles(l, rows), rt = l.thin ? 0 : r / kRows;
+    const int in = h * rt_n + rt;  // segment of the sequence
+    const Cut cut = {p.hdr[2 * l.thin], p.hdr[2 * l.thin + 1]};
+    const int x = p.hdr[kHdr + (li ? p.list[0].n + i : i)] + in * tiles;
+    const int w = cut_of(cut, x);
+    first = l.part0 + ((int64_t)i * rt_n * p.Hkv + in + w) * l.part_rows + (r - rt * kRows);
+    return cut_of(cut, x + tiles - 1) - w + 1;
+  };
   const SpanList &l0 = p.list[0], &l1 = p.list[1];
-  const int rt0 = row_tiles(p.num_tokens * p.G), rt1 = row_tiles(p.S * p.G);
-  const int r0 = t * p.G + g, r1 = s * p.G + g;
-  const int seg0 = h * rt0 + r0 / kRows;
-  const int seg1 = rt0 * p.Hkv * l0.n + (b * p.Hkv + h) * rt1 + r1 / kRows;
-  int n0 = 0;
-  int64_t f0 = 0;
-  if (l0.n) {
-    f0 = l0.part0 + (int64_t)p.hdr[2 * seg0] * l0.part_rows + r0 % kRows;
-    n0 = p.hdr[2 * seg0 + 1];
-  }
-  const int64_t f1 = l1.part0 + (int64_t)p.hdr[2 * seg1] * l1.part_rows + r1 % kRows;
-  const int n1 = p.hdr[2 * seg1 + 1];
+  int64_t f0, f1;
+  const int n0 = pieces(0, 0, t * p.G + g, p.num_tokens * p.G, f0);
+  const int n1 = pieces(1, b, s * p.G + g, p.S * p.G, f1);
   auto prow = [&](int j) {
     return j < n0 ? f0 + (int64_t)j * l0.part_rows : f1 + (int64_t)(j - n0) * l1.part_rows;
   };
-  const int n = n0 + n1;
-  float m = -INFINITY;
-  for (int j = c; j < n; j += LPR) m = fmaxf(m, p.part_ml[2 * prow(j)]);
-#pragma unroll
-  for (int o = 1; o < LPR; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-  if (p.sink) m = fmaxf(m, p.sink[hq] * kLog2e);
-  float mm = m == -INFINITY ? 0.f : m;
+  float m = -INFINITY, ls = 0.f;
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-  float ls = p.sink ? __builtin_amdgcn_exp2f(p.sink[hq] * kLog2e - mm) : 0.f;
-  for (int j = 0; j < n; ++j) {
-    const int64_t pr = prow(j);
-    const float wgt = __builtin_amdgcn_exp2f(p.part_ml[2 * pr] - mm);
-    ls += wgt * p.part_ml[2 * pr + 1];
-    const f32x4_t v = *reinterpret_cast<const f32x4_t *>(p.part_o + pr * D + c * 4);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] += wgt * v[i];
+  if (p.sink) {
+    m = p.sink[hq] * kLog2e;
+    ls = 1.f;
   }
+  sum_pieces<LPR>(p, n0 + n1, prow, c, D, m, ls, o);
   // the keys between the span that all rows see and row s's own last key
   if (s > 0) {
     const int common = list_len(l1, b);
@@ -891,32 +1433,35 @@ int64_t up(int64_t x, int64_t a) { return (x + a - 1) / a * a; }
 struct Layout {
   int grid;
   size_t hdr, ml, o, total;  // byte offsets and size
-  int64_t part_rows;
 };
 
-// Sizes of a call's workspace; fills the lists' partial regions.
+// Launch size and workspace of a call; fills the lists' forms and partials.
 Layout span_layout(SpanParams &p, int D) {
   Layout w;
   w.grid = 2 * cu_count();
-  int64_t rows = 0, hdr = 0;
-  if (p.join) {
-    for (int li = 0; li < 2; ++li) {
-      SpanList &l = p.list[li];
-      const int64_t seq_rows = (li ? (int64_t)p.S : (int64_t)p.num_tokens) * p.G;
-      const int64_t segs = (seq_rows + kRows - 1) / kRows * p.Hkv * l.n;
-      l.part_rows = (int)std::min<int64_t>(kRows, seq_rows);
-      l.part0 = rows;
-      rows += (segs + w.grid) * l.part_rows;
-      hdr += segs * 2;
+  int64_t rows = 0, hdr = kHdr;
+  for (int li = 0; li < 2; ++li) {
+    SpanList &l = p.list[li];
+    if (l.n == 0) {
+      l.thin = p.list[1].thin;
+      continue;
     }
-  } else {
-    SpanList &l = p.list[1];
-    l.part_rows = (int)std::min<int64_t>(kRows, (int64_t)l.tok_max * p.G);
-    l.part0 = 0;
-    rows = (int64_t)2 * w.grid * l.part_rows;
-    hdr = (int64_t)8 * w.grid;
+    const int64_t seq_rows = (int64_t)l.tok_max * p.G;
+    l.thin = seq_rows <= 32;
+    const int64_t units = (int64_t)w.grid * (l.thin ? kWaves : 1);
+    l.part_rows = (int)std::min<int64_t>(kRows, seq_rows);
+    l.part0 = rows;
+    if (p.join) {
+      const int64_t segs = (seq_rows + kRows - 1) / kRows * p.Hkv * l.n;
+      rows += (segs + units) * l.part_rows;
+      hdr += l.n;
+    } else {
+      rows += 2 * units * l.part_rows;
+      hdr += units * kHdr;
+    }
   }
-  w.part_rows = rows;
+  p.cost[0] = 1.0f, p.cost[1] = 0.6f;
+  p.least[0] = 2, p.least[1] = 2;
   w.hdr = 0;
   w.ml = (size_t)up(hdr * 4, 256);
   w.o = w.ml + (size_t)up(rows * 8, 256);
@@ -926,7 +1471,7 @@ Layout span_layout(SpanParams &p, int D) {
 
 void bind_workspace(SpanParams &p, const Layout &w, void *ws) {
   p.hdr = (int *)((uint8_t *)ws + w.hdr);
-  p.part_ml = (float *)((uint8_t *)ws + w.ml);
+  p.part_ml = (float2 *)((uint8_t *)ws + w.ml);
   p.part_o = (float *)((uint8_t *)ws + w.o);
 }
 
@@ -966,7 +1511,6 @@ SpanParams cross_params(const mia_cross_args &a) {
   l.len = a.key_lens;
   l.len_cap = a.block_table ? a.blocks_per_seq * a.block_size : a.block_size;
   l.bt = a.block_table, l.bt_s = a.bt_stride[0], l.bt_j = a.bt_stride[1];
-  l.cost = 1;
   return p;
 }
 
@@ -985,24 +1529,26 @@ SpanParams prefix_params(const mia_shared_prefix_args &a) {
   l0.len = a.prefix_len;
   l0.len_cap = a.prefix_blocks * a.block_size;
   l0.bt = a.prefix_table, l0.bt_j = a.prefix_stride;
-  l0.cost = 1;
   l1.n = a.batch;
   l1.tok_per = l1.tok_max = a.s_active;
   l1.len = a.seq_lens;
   l1.len_sub = a.s_active - 1;
   l1.len_cap = a.blocks_per_seq * a.block_size;
   l1.bt = a.block_table, l1.bt_s = a.bt_stride[0], l1.bt_j = a.bt_stride[1];
-  l1.cost = 1;
   return p;
 }
 
 template <int D, int CT, bool SC>
 void launch_span(const SpanParams &p, int grid, hipStream_t s) {
-  span_kernel<D, CT, SC><<<grid, kThreads, 0, s>>>(p);
+  const int cols = std::max(p.list[0].thin && p.list[0].n ? p.list[0].part_rows : 0,
+                            p.list[1].thin ? p.list[1].part_rows : 0);
+  if (cols <= 16) span_kernel<D, CT, SC, 1><<<grid, kThreads, 0, s>>>(p);
+  else span_kernel<D, CT, SC, 2><<<grid, kThreads, 0, s>>>(p);
   if (p.join) {
-    const int64_t rows = (int64_t)p.num_tokens * p.Hkv * p.G;
+    const int hq = p.Hkv * p.G;
     constexpr int RPB = 256 / (D / 4);
-    span_join_kernel<D, CT, SC><<<(unsigned)((rows + RPB - 1) / RPB), 256, 0, s>>>(p);
+    span_join_kernel<D, CT, SC>
+        <<<(p.num_tokens * hq + RPB - 1) / RPB, 256, 0, s>>>(p, make_fastdiv(hq));
   }
 }
 
@@ -1016,7 +1562,8 @@ void launch_width(const SpanParams &p, int cache_dtype, int grid, hipStream_t s)
   if (!p.join) {
     constexpr int RPB = 256 / (D / 4);
     const SpanList &l = p.list[1];
-    span_merge_kernel<D><<<dim3(grid, (l.part_rows + RPB - 1) / RPB), 256, 0, s>>>(p);
+    const int units = grid * (l.thin ? kWaves : 1);
+    span_merge_kernel<D><<<dim3(units, (l.part_rows + RPB - 1) / RPB), 256, 0, s>>>(p);
   }
 }
 
