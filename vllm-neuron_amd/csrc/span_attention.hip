@@ -109,15 +109,21 @@ MIA_DEV const SpanParams &fresh() {
   return *(const SpanParams *)k;
 }
 
+// Lengths and tables through the scalar cache: nothing writes them while the
+// kernel runs, which the compiler cannot know of a plain pointer.
+MIA_DEV int scalar_load(const int32_t *p, int64_t i) {
+  return ((const __attribute__((address_space(4))) int32_t *)(uintptr_t)p)[i];
+}
+
 MIA_DEV int list_len(const SpanList &l, int i) {
-  return max(0, min(l.len[i] - l.len_sub, l.len_cap));
+  return max(0, min(scalar_load(l.len, i) - l.len_sub, l.len_cap));
 }
 // first query token and token count of sequence i
 MIA_DEV int2 list_tokens(const SpanList &l, int i, int num_tokens) {
   int a, b;
   if (l.cu) {
-    a = min(max(l.cu[i], 0), num_tokens);
-    b = min(max(l.cu[i + 1], a), num_tokens);
+    a = min(max(scalar_load(l.cu, i), 0), num_tokens);
+    b = min(max(scalar_load(l.cu, i + 1), a), num_tokens);
   } else {
     a = min(i * l.tok_per, num_tokens);
     b = min(a + l.tok_per, num_tokens);
@@ -448,39 +454,57 @@ MIA_DEV int64_t tok_off(const SpanParams &p, int t, int64_t sb, int64_t ss) {
   return (int64_t)b * sb + (int64_t)(t - b * p.S) * ss;
 }
 
-// The 16-key group of key k0 (k0 % 16 == 0, clamped into the span): its block
-// and the byte offsets of its first row in K and V.
-struct Group {
-  int k16;           // first key
-  int blk, off;
-};
-MIA_DEV Group key_group(const SpanParams &p, const Pos &c, int k0) {
-  const SpanList &l = p.list[c.li];
-  Group g;
-  g.k16 = min(k0, (c.len - 1) & ~15);
-  if (l.bt) {
-    const int bj = (int)fdiv((uint32_t)g.k16, p.bs_div);
-    const int blk = l.bt[(int64_t)c.i * l.bt_s + (int64_t)bj * l.bt_j];
-    g.blk = readfirstlane(min(max(blk, 0), p.nb - 1));
-    g.off = g.k16 - bj * p.bs;
-  } else {
-    g.blk = c.i;
-    g.off = g.k16;
+// Where a segment's keys lie (wave-uniform): its table row and the first byte
+// of its head in K and V.
+struct Keys {
+  const int32_t *bt;  // NULL: dense, block = sequence
+  int64_t bt_j;
+  const uint8_t *k, *v;
+  int64_t k_blk, v_blk;
+  int k_t, v_t;
+  int seq, len, nb, bs;
+  FastDiv bs_div;
+
+  MIA_DEV void set(const SpanParams &p, const Pos &c) {
+    const SpanList &l = p.list[c.li];
+    bt = l.bt ? l.bt + (int64_t)c.i * l.bt_s : nullptr;
+    bt_j = l.bt_j;
+    k = p.k_cache + (int64_t)c.h * p.kc_h;
+    v = p.v_cache + (int64_t)c.h * p.vc_h;
+    k_blk = p.kc_blk, v_blk = p.vc_blk;
+    k_t = (int)p.kc_t, v_t = (int)p.vc_t;
+    seq = c.i, len = c.len, nb = p.nb, bs = p.bs;
+    bs_div = p.bs_div;
   }
-  return g;
-}
-MIA_DEV const uint8_t *k_row(const SpanParams &p, const Pos &c, const Group &g) {
-  return p.k_cache + (int64_t)g.blk * p.kc_blk + (int64_t)c.h * p.kc_h + (int64_t)g.off * p.kc_t;
-}
-MIA_DEV const uint8_t *v_row(const SpanParams &p, const Pos &c, const Group &g) {
-  return p.v_cache + (int64_t)g.blk * p.vc_blk + (int64_t)c.h * p.vc_h + (int64_t)g.off * p.vc_t;
-}
-MIA_DEV const float *k_scale(const SpanParams &p, const Pos &c, const Group &g) {
-  return p.k_sc + (int64_t)g.blk * p.ks_blk + (int64_t)c.h * p.ks_h + (int64_t)g.off * p.ks_t;
-}
-MIA_DEV const float *v_scale(const SpanParams &p, const Pos &c, const Group &g) {
-  return p.v_sc + (int64_t)g.blk * p.vs_blk + (int64_t)c.h * p.vs_h + (int64_t)g.off * p.vs_t;
-}
+  // The 16-key group of key k0 (k0 % 16 == 0), clamped into the span: its
+  // first key and, loaded ahead of its use, its table entry.
+  MIA_DEV int first(int k0) const { return min(k0, (len - 1) & ~15); }
+  MIA_DEV int entry(int k0) const {
+    return bt ? scalar_load(bt, (int64_t)fdiv((uint32_t)first(k0), bs_div) * bt_j) : seq;
+  }
+};
+
+// A 16-key group: block and first key inside it.
+struct Group {
+  int k16, blk, off;
+  MIA_DEV void set(const Keys &s, int k0, int entry) {
+    k16 = s.first(k0);
+    blk = s.bt ? min(max(entry, 0), s.nb - 1) : s.seq;
+    off = s.bt ? k16 - (int)fdiv((uint32_t)k16, s.bs_div) * s.bs : k16;
+  }
+  MIA_DEV const uint8_t *k(const Keys &s) const {
+    return s.k + (int64_t)blk * s.k_blk + (int64_t)off * s.k_t;
+  }
+  MIA_DEV const uint8_t *v(const Keys &s) const {
+    return s.v + (int64_t)blk * s.v_blk + (int64_t)off * s.v_t;
+  }
+  MIA_DEV const float *ks(const SpanParams &p, int h) const {
+    return p.k_sc + (int64_t)blk * p.ks_blk + (int64_t)h * p.ks_h + (int64_t)off * p.ks_t;
+  }
+  MIA_DEV const float *vs(const SpanParams &p, int h) const {
+    return p.v_sc + (int64_t)blk * p.vs_blk + (int64_t)h * p.vs_h + (int64_t)off * p.vs_t;
+  }
+};
 
 // log2(e) x softmax scale x per-head scale of K: its magnitude; a negative
 // factor goes to q (sign bits), so that the largest product is the largest
@@ -576,39 +600,57 @@ MIA_DEV void tall_body(const Share &sh, TallLds<D, CT, SC> &lds) {
   constexpr int NR = DMA ? 1 : NP;
   u32x4_t kr[NR], vr[NR];
   float sr[NR];
+  // table entries of this wave's 16-key groups of a tile, loaded one tile ahead
+  Keys ks_;
+  int ent[NP];
+  auto load_entries = [&](int t) {
+#pragma unroll
+    for (int j = 0; j < NP; ++j) ent[j] = ks_.entry(t * kTallKeys + j * RP + g16);
+  };
   auto load_tile = [&](const Pos &c, int buf) {
-    const SpanParams &p = fresh();
     const int kt = c.t * kTallKeys;
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
-      // the group's block is wave-uniform; rows past the span read its last
-      // key (in bounds) and are masked or cleared later
-      const Group g = key_group(p, c, kt + j * RP + g16);
+      // rows past the span read its last key (in bounds) and are masked or
+      // cleared later
+      Group g;
+      g.set(ks_, kt + j * RP + g16, ent[j]);
       const int row = j * RP + lrow;
-      const int rr = min(kt + row, c.len - 1) - g.k16;
-      const uint8_t *kb = k_row(p, c, g), *vb = v_row(p, c, g);
+      const int rr = min(kt + row, ks_.len - 1) - g.k16;
+      const uint8_t *kb = g.k(ks_), *vb = g.v(ks_);
       if constexpr (DMA) {
         const uint32_t dst = (uint32_t)(uintptr_t)base + (buf * 2) * TILEB +
                              (j * RP + wave * RPW) * ROWB;
         // the lane's slot of the copy is chunk lc of its row in LDS: it reads
         // the chunk that the swizzle puts there
         const int kc = lc ^ k_swz<D>(row), vc = lc ^ v_swz<D>(row);
-        if (kc * CE < d_used) copy16(kb + rr * (int)p.kc_t + kc * 16, dst);
-        if (vc * CE < d_used) copy16(vb + rr * (int)p.vc_t + vc * 16, dst + TILEB);
+        if (kc * CE < d_used) copy16(kb + rr * ks_.k_t + kc * 16, dst);
+        if (vc * CE < d_used) copy16(vb + rr * ks_.v_t + vc * 16, dst + TILEB);
       } else {
         kr[j] = u32x4_t{0u, 0u, 0u, 0u};
         vr[j] = u32x4_t{0u, 0u, 0u, 0u};
         if (ch_ok) {
-          kr[j] = *reinterpret_cast<const u32x4_t *>(kb + rr * (int)p.kc_t + lc * 16);
-          vr[j] = *reinterpret_cast<const u32x4_t *>(vb + rr * (int)p.vc_t + lc * 16);
+          kr[j] = *reinterpret_cast<const u32x4_t *>(kb + rr * ks_.k_t + lc * 16);
+          vr[j] = *reinterpret_cast<const u32x4_t *>(vb + rr * ks_.v_t + lc * 16);
         }
         if constexpr (SC) {
-          const float *ks = k_scale(p, c, g), *vs = v_scale(p, c, g);
+          const SpanParams &p = fresh();
+          const float *ks = g.ks(p, c.h), *vs = g.vs(p, c.h);
           sr[j] = 0.f;
           if (lc < 2) sr[j] = lc ? vs[rr * p.vs_t] : ks[rr * p.ks_t];
         }
       }
     }
+  };
+  // the tile at c (its entries are loaded, or c starts a segment) and the
+  // entries of the one behind it
+  auto fetch = [&](const Pos &c, int buf, bool anew) {
+    if (anew) {
+      ks_.set(fresh(), c);
+      load_entries(c.t);
+    }
+    load_tile(c, buf);
+    if (c.t + 1 < c.tiles) load_entries(c.t + 1);
   };
   // 8-bit caches: the loaded tile widened into stage buf
   auto store_tile = [&](const Pos &c, int buf) {
@@ -842,7 +884,7 @@ MIA_DEV void tall_body(const Share &sh, TallLds<D, CT, SC> &lds) {
         *(lds_u32x4_t *)(base + o) = u32x4_t{0u, 0u, 0u, 0u};
       __syncthreads();
     }
-    load_tile(cur, 0);
+    fetch(cur, 0, true);
     begin_piece(cur);
     while (true) {
       // own copies of tile `cur` have landed; the barrier makes every
@@ -852,7 +894,7 @@ MIA_DEV void tall_body(const Share &sh, TallLds<D, CT, SC> &lds) {
       const bool more = cur.left > 1;
       if (more) {
         advance(fresh(), nxt);
-        load_tile(nxt, buf ^ 1);
+        fetch(nxt, buf ^ 1, nxt.t == 0);
       }
       const int left = cur.len - cur.t * kTallKeys;
       if (left < kTallKeys) {
@@ -874,13 +916,13 @@ MIA_DEV void tall_body(const Share &sh, TallLds<D, CT, SC> &lds) {
       buf ^= 1;
     }
   } else {
-    load_tile(cur, 0);
+    fetch(cur, 0, true);
     begin_piece(cur);
     store_tile(cur, 0);
     bool more = cur.left > 1;
     if (more) {
       advance(fresh(), nxt);
-      load_tile(nxt, 0);
+      fetch(nxt, 0, nxt.t == 0);
     }
     __syncthreads();
     while (true) {
@@ -896,7 +938,7 @@ MIA_DEV void tall_body(const Share &sh, TallLds<D, CT, SC> &lds) {
       more = cur.left > 1;
       if (more) {
         advance(fresh(), nxt);
-        load_tile(nxt, 0);
+        fetch(nxt, 0, nxt.t == 0);
       }
       __syncthreads();
       buf ^= 1;
@@ -943,25 +985,31 @@ MIA_DEV void thin_body(const Share &sh, ThinLds<D, SC> &lds) {
 
   u32x4_t kr[2][NK], vr[NV];
   float sr = 0.f;
-  struct Groups {
-    Group g[2];
+  Keys ks_;
+  Group g[2];
+  int ent[2];  // table entries of a tile, loaded one tile ahead
+  auto load_entries = [&](int t) {
+    ent[0] = ks_.entry(t * kThinKeys);
+    ent[1] = ks_.entry(t * kThinKeys + 16);
   };
-  auto groups = [&](const Pos &c) {
-    const SpanParams &p = fresh();
-    Groups x;
-    x.g[0] = key_group(p, c, c.t * kThinKeys);
-    x.g[1] = key_group(p, c, c.t * kThinKeys + 16);
-    return x;
+  // the groups of the tile at c (its entries are loaded, or c starts a
+  // segment), and the entries of the one behind it
+  auto locate = [&](const Pos &c, bool anew) {
+    if (anew) {
+      ks_.set(fresh(), c);
+      load_entries(c.t);
+    }
+    g[0].set(ks_, c.t * kThinKeys, ent[0]);
+    g[1].set(ks_, c.t * kThinKeys + 16, ent[1]);
+    if (c.t + 1 < c.tiles) load_entries(c.t + 1);
   };
   // rows past the span read its last key (in bounds) and are masked or
   // cleared later
-  auto load_k = [&](const Pos &c, const Groups &gs) {
-    const SpanParams &p = fresh();
+  auto load_k = [&](const Pos &c) {
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
-      const Group &g = gs.g[b];
-      const int rr = min(c.t * kThinKeys + b * 16 + col, c.len - 1) - g.k16;
-      const uint8_t *a = k_row(p, c, g) + rr * (int)p.kc_t;
+      const int rr = min(c.t * kThinKeys + b * 16 + col, ks_.len - 1) - g[b].k16;
+      const uint8_t *a = g[b].k(ks_) + rr * ks_.k_t;
 #pragma unroll
       for (int j = 0; j < NK; ++j) {
         kr[b][j] = u32x4_t{0u, 0u, 0u, 0u};
@@ -970,29 +1018,27 @@ MIA_DEV void thin_body(const Share &sh, ThinLds<D, SC> &lds) {
       }
     }
   };
-  auto load_v = [&](const Pos &c, const Groups &gs) {
-    const SpanParams &p = fresh();
+  auto load_v = [&](const Pos &c) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const Group &g = gs.g[j * TL / 16];
-      const int rr = min(c.t * kThinKeys + j * TL + vtl, c.len - 1) - g.k16;
+      const Group &x = g[j * TL / 16];
+      const int rr = min(c.t * kThinKeys + j * TL + vtl, ks_.len - 1) - x.k16;
       vr[j] = u32x4_t{0u, 0u, 0u, 0u};
       if (vds * VE < d_used)
-        vr[j] = *reinterpret_cast<const u32x4_t *>(v_row(p, c, g) + rr * (int)p.vc_t + vds * 16);
+        vr[j] = *reinterpret_cast<const u32x4_t *>(x.v(ks_) + rr * ks_.v_t + vds * 16);
     }
   };
   // lane l: scale of key l (K), of key l - 32 (V)
-  auto load_s = [&](const Pos &c, const Groups &gs) {
+  auto load_s = [&](const Pos &c) {
     if constexpr (SC) {
       const SpanParams &p = fresh();
       const int k = lane & 31;
-      const Group &g = gs.g[0], &g1 = gs.g[1];
       const bool hi = k >= 16;
-      const int rr = min(c.t * kThinKeys + k, c.len - 1) - (hi ? g1.k16 : g.k16);
-      const float *ks = hi ? k_scale(p, c, g1) : k_scale(p, c, g);
-      const float *vs = hi ? v_scale(p, c, g1) : v_scale(p, c, g);
+      const int rr = min(c.t * kThinKeys + k, ks_.len - 1) - (hi ? g[1].k16 : g[0].k16);
+      const float *ks = hi ? g[1].ks(p, c.h) : g[0].ks(p, c.h);
+      const float *vs = hi ? g[1].vs(p, c.h) : g[0].vs(p, c.h);
       sr = lane < 32 ? ks[rr * p.ks_t] : vs[rr * p.vs_t];
-      if (c.t * kThinKeys + k >= c.len) sr = 0.f;
+      if (c.t * kThinKeys + k >= ks_.len) sr = 0.f;
     }
   };
 
@@ -1182,10 +1228,10 @@ MIA_DEV void thin_body(const Share &sh, ThinLds<D, SC> &lds) {
   // product (copy to LDS) has freed the registers
   if (sh.x0 >= sh.x1) return;
   Pos cur = first_pos(fresh(), sh);
-  Groups gs = groups(cur);
-  load_k(cur, gs);
-  load_s(cur, gs);
-  load_v(cur, gs);
+  locate(cur, true);
+  load_k(cur);
+  load_s(cur);
+  load_v(cur);
   begin_piece(cur);
   int t0 = cur.t;
   while (true) {
@@ -1193,17 +1239,17 @@ MIA_DEV void thin_body(const Share &sh, ThinLds<D, SC> &lds) {
     Pos nxt = cur;
     if (more) {
       advance(fresh(), nxt);
-      gs = groups(nxt);
+      locate(nxt, nxt.t == 0);
     }
     scores();
     if constexpr (SC) sw[lane] = sr;
     if (more) {
-      load_k(nxt, gs);
-      load_s(nxt, gs);
+      load_k(nxt);
+      load_s(nxt);
     }
     softmax(cur);
     store_v(cur);
-    if (more) load_v(nxt, gs);
+    if (more) load_v(nxt);
     values();
     if (!more || nxt.t == 0) {
       end_piece(cur, t0);
@@ -1230,53 +1276,65 @@ __global__ __launch_bounds__(kThreads, 2) void span_kernel(SpanParams p) {
   else if (form == 1) thin_body<D, CT, SC, NC>(sh, lds.thin);
 }
 
-// Weighted sum of the n pieces of a row (partial row prow(j)) by the D / 4
-// lanes of the row, four channels each: the lanes take a piece's (m, l) each,
-// then all of them every piece's o.
-template <int LPR, typename F>
-MIA_DEV void sum_pieces(const SpanParams &p, int n, F prow, int c, int D, float &m, float &l,
-                        f32x4_t &o) {
-  for (int k0 = 0; k0 < n; k0 += LPR) {
-    const int cnt = min(LPR, n - k0);
-    float2 ml = make_float2(-INFINITY, 0.f);
-    if (c < cnt) ml = p.part_ml[prow(k0 + c)];
-    float mc = ml.x;
+// A row is joined by GR groups of D / 4 lanes, four channels a lane.
+template <int D, int GR>
+struct JoinLds {
+  f32x4_t o[256 / (D / 4)][D / 4];
+  float2 ml[256 / (D / 4)];
+};
+
+MIA_DEV void add_piece(float &m, float &l, f32x4_t &o, float m1, float l1, const f32x4_t &o1) {
+  const float m2 = fmaxf(m, m1);
+  const float mm = m2 == -INFINITY ? 0.f : m2;
+  const float a = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mm);
+  const float b = m1 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m1 - mm);
+  m = m2;
+  l = l * a + l1 * b;
 #pragma unroll
-    for (int x = 1; x < LPR; x <<= 1) mc = fmaxf(mc, __shfl_xor(mc, x, 64));
-    const float m_new = fmaxf(m, mc);
-    const float mm = m_new == -INFINITY ? 0.f : m_new;
-    const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mm);
-    m = m_new;
-    const float w = c < cnt ? __builtin_amdgcn_exp2f(ml.x - mm) : 0.f;
-    float ls = c < cnt ? w * ml.y : 0.f;
+  for (int i = 0; i < 4; ++i) o[i] = o[i] * a + o1[i] * b;
+}
+
+// The row's n pieces (partial row prow(j)): group g adds g, g + GR, ... to its
+// (m, l, o), four loads in flight.
+template <int D, int GR, typename F>
+MIA_DEV void sum_pieces(const SpanParams &p, int n, F prow, float &m, float &l, f32x4_t &o) {
+  constexpr int LPR = D / 4;
+  const int g = threadIdx.x / LPR % GR, c = threadIdx.x % LPR;
+  for (int j = g; j < n; j += 4 * GR) {
+    float2 ml[4];
+    f32x4_t v[4];
 #pragma unroll
-    for (int x = 1; x < LPR; x <<= 1) ls += __shfl_xor(ls, x, 64);
-    l = l * alpha + ls;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] *= alpha;
-    for (int j = 0; j < cnt; j += 4) {
-      f32x4_t v[4];
-      float wj[4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        v[u] = *reinterpret_cast<const f32x4_t *>(p.part_o + prow(k0 + min(j + u, cnt - 1)) * D +
-                                                  c * 4);
-        wj[u] = __shfl(w, min(j + u, LPR - 1), LPR);
-      }
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        if (j + u >= cnt) break;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] += wj[u] * v[u][i];
-      }
+    for (int u = 0; u < 4; ++u) {
+      const int64_t r = prow(min(j + u * GR, n - 1));
+      ml[u] = p.part_ml[r];
+      v[u] = *reinterpret_cast<const f32x4_t *>(p.part_o + r * D + c * 4);
     }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (j + u * GR < n) add_piece(m, l, o, ml[u].x, ml[u].y, v[u]);
   }
+}
+
+// The groups of a row added through LDS (every thread of the workgroup calls
+// this); group 0 has the result.
+template <int D, int GR>
+MIA_DEV void sum_groups(JoinLds<D, GR> &lds, float &m, float &l, f32x4_t &o) {
+  constexpr int LPR = D / 4;
+  const int gi = threadIdx.x / LPR, c = threadIdx.x % LPR;
+  lds.o[gi][c] = o;
+  if (c == 0) lds.ml[gi] = make_float2(m, l);
+  __syncthreads();
+  if (gi % GR) return;
+#pragma unroll
+  for (int k = 1; k < GR; ++k)
+    add_piece(m, l, o, lds.ml[gi + k].x, lds.ml[gi + k].y, lds.o[gi + k][c]);
 }
 
 // Joins the pieces of cut segments (cross attention): workgroup (w, y) takes
 // rows of the segment that starts, cut, in share w.
-template <int D>
+template <int D, int GR>
 __global__ __launch_bounds__(256) void span_merge_kernel(SpanParams p) {
+  __shared__ JoinLds<D, GR> lds;
   const int w = blockIdx.x;
   const int *hd = p.hdr + kHdr * w;
   const int n = hd[0];
@@ -1284,15 +1342,17 @@ __global__ __launch_bounds__(256) void span_merge_kernel(SpanParams p) {
   constexpr int LPR = D / 4;
   const int c = threadIdx.x % LPR;
   const SpanList &l = p.list[1];
-  const int rloc = blockIdx.y * (256 / LPR) + threadIdx.x / LPR;
+  const int rloc = blockIdx.y * (256 / LPR / GR) + threadIdx.x / LPR / GR;
   const int r = hd[3] * kRows + rloc;
-  if (r >= hd[2] || rloc >= l.part_rows) return;  // whole groups of LPR lanes leave
+  const bool ok = r < hd[2] && rloc < l.part_rows;
   auto prow = [&](int j) {
     return l.part0 + (int64_t)(j == 0 ? 2 * w + 1 : 2 * (w + j)) * l.part_rows + rloc;
   };
   float m = -INFINITY, ls = 0.f;
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-  sum_pieces<LPR>(p, n, prow, c, D, m, ls, o);
+  sum_pieces<D, GR>(p, ok ? n : 0, prow, m, ls, o);
+  if constexpr (GR > 1) sum_groups<D, GR>(lds, m, ls, o);
+  if (!ok || threadIdx.x / LPR % GR) return;
   float inv = ls == 0.f ? 0.f : 1.f / ls;
   const int h = hd[4];
   if (p.v_deq) inv *= p.v_deq[h];
@@ -1307,12 +1367,17 @@ __global__ __launch_bounds__(256) void span_merge_kernel(SpanParams p) {
 // Shared prefix: joins the pieces of a row's prefix and own span, adds the
 // new tokens that not every row of its sequence sees (the last S - 1 keys,
 // row s sees s of them) and the sink.  D / 4 lanes per row.
+constexpr int kJoinGroups = 8;
+
 template <int D, int CT, bool SC>
 __global__ __launch_bounds__(256) void span_join_kernel(SpanParams p, FastDiv hq_div) {
   constexpr int LPR = D / 4;
+  constexpr int GR = kJoinGroups;
+  __shared__ JoinLds<D, GR> lds;
   const int c = threadIdx.x % LPR;
-  const int row = blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
-  if (row >= p.num_tokens * (int)hq_div.d) return;  // whole groups of LPR lanes leave
+  const int n_rows = p.num_tokens * (int)hq_div.d;
+  const int my_row = blockIdx.x * (256 / LPR / GR) + threadIdx.x / LPR / GR;
+  const int row = min(my_row, n_rows - 1);
   const int t = (int)fdiv((uint32_t)row, hq_div);
   const int hq = row - t * (int)hq_div.d;
   const int h = (int)fdiv((uint32_t)hq, p.g_div);
@@ -1342,11 +1407,12 @@ __global__ __launch_bounds__(256) void span_join_kernel(SpanParams p, FastDiv hq
   };
   float m = -INFINITY, ls = 0.f;
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-  if (p.sink) {
+  const int gr = threadIdx.x / LPR % GR;
+  if (p.sink && gr == 0) {
     m = p.sink[hq] * kLog2e;
     ls = 1.f;
   }
-  sum_pieces<LPR>(p, n0 + n1, prow, c, D, m, ls, o);
+  sum_pieces<D, GR>(p, n0 + n1, prow, m, ls, o);
   // the keys between the span that all rows see and row s's own last key
   if (s > 0) {
     const int common = list_len(l1, b);
@@ -1374,7 +1440,7 @@ __global__ __launch_bounds__(256) void span_join_kernel(SpanParams p, FastDiv hq
           }
         }
       };
-      for (int k = common; k < end; ++k) {
+      for (int k = common + gr; k < end; k += GR) {
         const int bj = (int)fdiv((uint32_t)k, p.bs_div);
         const int blk = min(max(l1.bt[(int64_t)b * l1.bt_s + (int64_t)bj * l1.bt_j], 0), p.nb - 1);
         const int off = k - bj * p.bs;
@@ -1392,17 +1458,12 @@ __global__ __launch_bounds__(256) void span_join_kernel(SpanParams p, FastDiv hq
           vs = p.v_sc[(int64_t)blk * p.vs_blk + (int64_t)h * p.vs_h + (int64_t)off * p.vs_t];
         }
         const float sc = dot * c1;
-        const float m2 = fmaxf(m, sc);
-        const float mm2 = m2 == -INFINITY ? 0.f : m2;
-        const float a = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mm2);
-        const float e = __builtin_amdgcn_exp2f(sc - mm2);
-        m = m2;
-        ls = ls * a + e;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = o[i] * a + e * (v[i] * vs);
+        add_piece(m, ls, o, sc, 1.f, f32x4_t{v[0] * vs, v[1] * vs, v[2] * vs, v[3] * vs});
       }
     }
   }
+  sum_groups<D, GR>(lds, m, ls, o);
+  if (gr != 0 || my_row >= n_rows) return;
   float inv = ls == 0.f ? 0.f : 1.f / ls;
   if (p.v_deq) inv *= p.v_deq[h];
   if (c * 4 >= p.d) return;
@@ -1546,7 +1607,7 @@ void launch_span(const SpanParams &p, int grid, hipStream_t s) {
   else span_kernel<D, CT, SC, 2><<<grid, kThreads, 0, s>>>(p);
   if (p.join) {
     const int hq = p.Hkv * p.G;
-    constexpr int RPB = 256 / (D / 4);
+    constexpr int RPB = 256 / (D / 4) / kJoinGroups;
     span_join_kernel<D, CT, SC>
         <<<(p.num_tokens * hq + RPB - 1) / RPB, 256, 0, s>>>(p, make_fastdiv(hq));
   }
@@ -1562,8 +1623,11 @@ void launch_width(const SpanParams &p, int cache_dtype, int grid, hipStream_t s)
   if (!p.join) {
     constexpr int RPB = 256 / (D / 4);
     const SpanList &l = p.list[1];
-    const int units = grid * (l.thin ? kWaves : 1);
-    span_merge_kernel<D><<<dim3(units, (l.part_rows + RPB - 1) / RPB), 256, 0, s>>>(p);
+    if (l.thin)
+      span_merge_kernel<D, kJoinGroups>
+          <<<dim3(grid * kWaves, (l.part_rows * kJoinGroups + RPB - 1) / RPB), 256, 0, s>>>(p);
+    else
+      span_merge_kernel<D, 1><<<dim3(grid, (l.part_rows + RPB - 1) / RPB), 256, 0, s>>>(p);
   }
 }
 
