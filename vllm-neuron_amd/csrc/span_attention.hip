@@ -461,7 +461,7 @@ struct Keys {
   int64_t bt_j;
   const uint8_t *k, *v;
   int64_t k_blk, v_blk;
-  int k_t, v_t;
+  uint32_t k_t, v_t;  // token strides (bytes, below 2^27)
   int seq, len, nb, bs;
   FastDiv bs_div;
 
@@ -472,7 +472,7 @@ struct Keys {
     k = p.k_cache + (int64_t)c.h * p.kc_h;
     v = p.v_cache + (int64_t)c.h * p.vc_h;
     k_blk = p.kc_blk, v_blk = p.vc_blk;
-    k_t = (int)p.kc_t, v_t = (int)p.vc_t;
+    k_t = (uint32_t)p.kc_t, v_t = (uint32_t)p.vc_t;
     seq = c.i, len = c.len, nb = p.nb, bs = p.bs;
     bs_div = p.bs_div;
   }
@@ -484,19 +484,16 @@ struct Keys {
   }
 };
 
-// A 16-key group: block and first key inside it.
+// A 16-key group: its first key, block, and first key inside the block.
 struct Group {
   int k16, blk, off;
+  const uint8_t *k, *v;  // its first rows
   MIA_DEV void set(const Keys &s, int k0, int entry) {
     k16 = s.first(k0);
     blk = s.bt ? min(max(entry, 0), s.nb - 1) : s.seq;
     off = s.bt ? k16 - (int)fdiv((uint32_t)k16, s.bs_div) * s.bs : k16;
-  }
-  MIA_DEV const uint8_t *k(const Keys &s) const {
-    return s.k + (int64_t)blk * s.k_blk + (int64_t)off * s.k_t;
-  }
-  MIA_DEV const uint8_t *v(const Keys &s) const {
-    return s.v + (int64_t)blk * s.v_blk + (int64_t)off * s.v_t;
+    k = s.k + (int64_t)blk * s.k_blk + (int64_t)off * s.k_t;
+    v = s.v + (int64_t)blk * s.v_blk + (int64_t)off * s.v_t;
   }
   MIA_DEV const float *ks(const SpanParams &p, int h) const {
     return p.k_sc + (int64_t)blk * p.ks_blk + (int64_t)h * p.ks_h + (int64_t)off * p.ks_t;
@@ -551,20 +548,63 @@ struct TallLds {
   float sc[2][2][SC ? kTallKeys : 4];            // [stage][K, V]
 };
 
-// One 16-byte-per-lane copy HBM -> LDS: lane data lands at lds_dst + 16 *
-// lane; inactive lanes leave theirs.  Inline assembly, so that the compiler
-// adds no waits before reads of the other stage; the wait for the copies is
-// explicit.  M0 (the LDS base of the copy) is saved and restored around it.
-MIA_DEV void copy16(const uint8_t *src, uint32_t lds_dst) {
+// NP 16-byte-per-lane copies HBM -> LDS: lane data of copy j, from src +
+// off[j], lands at lds_dst + j * 1024 + 16 * lane; inactive lanes leave theirs.
+// Inline assembly, so that the compiler adds no waits before reads of the
+// other stage; the wait for the copies is explicit.  M0 (the LDS base of a
+// copy) is saved and restored around them.
+template <int NP>
+MIA_DEV void copy16(const uint8_t *src, const uint32_t (&off)[NP], uint32_t lds_dst) {
+  static_assert(NP == 2 || NP == 4, "copies per tile");
+  const uint32_t m0 = readfirstlane((int)lds_dst);
+  uint32_t saved;
+  if constexpr (NP == 4) {
+    asm volatile(
+        "s_mov_b32 %0, m0\n\t"
+        "s_mov_b32 m0, %1\n\t"
+        "s_nop 0\n\t"
+        "global_load_lds_dwordx4 %3, %2\n\t"
+        "s_add_u32 m0, m0, 0x400\n\t"
+        "s_nop 0\n\t"
+        "global_load_lds_dwordx4 %4, %2\n\t"
+        "s_add_u32 m0, m0, 0x400\n\t"
+        "s_nop 0\n\t"
+        "global_load_lds_dwordx4 %5, %2\n\t"
+        "s_add_u32 m0, m0, 0x400\n\t"
+        "s_nop 0\n\t"
+        "global_load_lds_dwordx4 %6, %2\n\t"
+        "s_mov_b32 m0, %0"
+        : "=&s"(saved)
+        : "s"(m0), "s"(src), "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3])
+        : "memory", "scc");
+  } else {
+    asm volatile(
+        "s_mov_b32 %0, m0\n\t"
+        "s_mov_b32 m0, %1\n\t"
+        "s_nop 0\n\t"
+        "global_load_lds_dwordx4 %3, %2\n\t"
+        "s_add_u32 m0, m0, 0x400\n\t"
+        "s_nop 0\n\t"
+        "global_load_lds_dwordx4 %4, %2\n\t"
+        "s_mov_b32 m0, %0"
+        : "=&s"(saved)
+        : "s"(m0), "s"(src), "v"(off[0]), "v"(off[1])
+        : "memory", "scc");
+  }
+}
+
+// One such copy.
+MIA_DEV void copy1(const uint8_t *src, uint32_t off, uint32_t lds_dst) {
   const uint32_t m0 = readfirstlane((int)lds_dst);
   uint32_t saved;
   asm volatile(
       "s_mov_b32 %0, m0\n\t"
       "s_mov_b32 m0, %1\n\t"
-      "global_load_lds_dwordx4 %2, off\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %3, %2\n\t"
       "s_mov_b32 m0, %0"
       : "=&s"(saved)
-      : "s"(m0), "v"(src)
+      : "s"(m0), "s"(src), "v"(off)
       : "memory");
 }
 
@@ -575,9 +615,8 @@ MIA_DEV void tall_body(const Share &sh, TallLds<D, CT, SC> &lds) {
   constexpr int CE = 16 / EB;          // elements per 16-byte load
   constexpr int LPR = D / CE;          // lanes per key row
   constexpr int RPW = 64 / LPR;        // key rows per wave and load
-  constexpr int RP = kWaves * RPW;     // key rows per load of the workgroup
-  constexpr int NP = kTallKeys / RP;   // loads per thread and tile (K, V each)
-  static_assert(RPW <= 16, "a wave's rows of a load lie in one 16-key group");
+  constexpr int NP = 16 / RPW;         // loads per thread and tile (K, V each)
+  static_assert(kTallKeys == 16 * kWaves, "a wave loads one 16-key group of a tile");
   constexpr int ROWB = D * 2;
   constexpr int TILEB = kTallKeys * ROWB;
   constexpr int KSTEPS = D / 16;
@@ -591,51 +630,63 @@ MIA_DEV void tall_body(const Share &sh, TallLds<D, CT, SC> &lds) {
   lds_u8_t *const base = (lds_u8_t *)&lds.kv[0][0][0];
   lds_f32_t *const scb = (lds_f32_t *)&lds.sc[0][0][0];
 
-  // ---- loads of a tile: thread -> key row j * RP + lrow, chunk lc
-  const int lrow = wave * RPW + lane / LPR;
+  // ---- loads of a tile: wave w takes the 16 keys 16 w .. (one block: one
+  // table entry), thread -> row j * RPW + lr of them, chunk lc
+  const int lr = lane / LPR;
   const int lc = lane % LPR;
-  const int g16 = (wave * RPW) & ~15;  // 16-key group of load 0
   const int d_used = fresh().d;
   const bool ch_ok = lc * CE < d_used;
   constexpr int NR = DMA ? 1 : NP;
   u32x4_t kr[NR], vr[NR];
   float sr[NR];
-  // table entries of this wave's 16-key groups of a tile, loaded one tile ahead
   Keys ks_;
-  int ent[NP];
-  auto load_entries = [&](int t) {
-#pragma unroll
-    for (int j = 0; j < NP; ++j) ent[j] = ks_.entry(t * kTallKeys + j * RP + g16);
-  };
-  auto load_tile = [&](const Pos &c, int buf) {
-    const int kt = c.t * kTallKeys;
+  int ent = 0;  // the wave's table entry of a tile, loaded one tile ahead
+  auto load_entry = [&](int t) { ent = ks_.entry(t * kTallKeys + wave * 16); };
+  // the chunk a lane loads: for copies the one that the swizzle puts in its slot
+  auto k_chunk = [&](int j) { return DMA ? lc ^ k_swz<D>(j * RPW + lr) : lc; };
+  auto v_chunk = [&](int j) { return DMA ? lc ^ v_swz<D>(j * RPW + lr) : lc; };
+  uint32_t ko[NP], vo[NP];  // a lane's bytes from its group's first row
+  auto set_offsets = [&](int last) {
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
-      // rows past the span read its last key (in bounds) and are masked or
-      // cleared later
-      Group g;
-      g.set(ks_, kt + j * RP + g16, ent[j]);
-      const int row = j * RP + lrow;
-      const int rr = min(kt + row, ks_.len - 1) - g.k16;
-      const uint8_t *kb = g.k(ks_), *vb = g.v(ks_);
-      if constexpr (DMA) {
-        const uint32_t dst = (uint32_t)(uintptr_t)base + (buf * 2) * TILEB +
-                             (j * RP + wave * RPW) * ROWB;
-        // the lane's slot of the copy is chunk lc of its row in LDS: it reads
-        // the chunk that the swizzle puts there
-        const int kc = lc ^ k_swz<D>(row), vc = lc ^ v_swz<D>(row);
-        if (kc * CE < d_used) copy16(kb + rr * ks_.k_t + kc * 16, dst);
-        if (vc * CE < d_used) copy16(vb + rr * ks_.v_t + vc * 16, dst + TILEB);
+      const uint32_t rr = min(j * RPW + lr, last);
+      ko[j] = rr * ks_.k_t + k_chunk(j) * 16;
+      vo[j] = rr * ks_.v_t + v_chunk(j) * 16;
+    }
+  };
+  auto load_tile = [&](const Pos &c, int buf) {
+    const int k0 = c.t * kTallKeys + wave * 16;
+    Group g;
+    g.set(ks_, k0, ent);
+    // rows past the span read its last key (in bounds) and are masked or
+    // cleared later; the tail is a segment's last tile
+    if (k0 + 16 > c.len) set_offsets(c.len - 1 - g.k16);
+    if constexpr (DMA) {
+      const uint32_t dst = (uint32_t)(uintptr_t)base + (buf * 2) * TILEB + wave * 16 * ROWB;
+      if (d_used == D) {
+        copy16<NP>(g.k, ko, dst);
+        copy16<NP>(g.v, vo, dst + TILEB);
       } else {
+        // (one load per row group: its lanes past d differ from the others')
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+          if (k_chunk(j) * CE < d_used) copy1(g.k, ko[j], dst + j * 1024);
+          if (v_chunk(j) * CE < d_used) copy1(g.v, vo[j], dst + TILEB + j * 1024);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < NP; ++j) {
         kr[j] = u32x4_t{0u, 0u, 0u, 0u};
         vr[j] = u32x4_t{0u, 0u, 0u, 0u};
         if (ch_ok) {
-          kr[j] = *reinterpret_cast<const u32x4_t *>(kb + rr * ks_.k_t + lc * 16);
-          vr[j] = *reinterpret_cast<const u32x4_t *>(vb + rr * ks_.v_t + lc * 16);
+          kr[j] = *reinterpret_cast<const u32x4_t *>(g.k + ko[j]);
+          vr[j] = *reinterpret_cast<const u32x4_t *>(g.v + vo[j]);
         }
         if constexpr (SC) {
           const SpanParams &p = fresh();
           const float *ks = g.ks(p, c.h), *vs = g.vs(p, c.h);
+          const int rr = min(k0 + j * RPW + lr, c.len - 1) - g.k16;
           sr[j] = 0.f;
           if (lc < 2) sr[j] = lc ? vs[rr * p.vs_t] : ks[rr * p.ks_t];
         }
@@ -647,10 +698,11 @@ MIA_DEV void tall_body(const Share &sh, TallLds<D, CT, SC> &lds) {
   auto fetch = [&](const Pos &c, int buf, bool anew) {
     if (anew) {
       ks_.set(fresh(), c);
-      load_entries(c.t);
+      load_entry(c.t);
+      set_offsets(15);
     }
     load_tile(c, buf);
-    if (c.t + 1 < c.tiles) load_entries(c.t + 1);
+    if (c.t + 1 < c.tiles) load_entry(c.t + 1);
   };
   // 8-bit caches: the loaded tile widened into stage buf
   auto store_tile = [&](const Pos &c, int buf) {
@@ -659,7 +711,7 @@ MIA_DEV void tall_body(const Share &sh, TallLds<D, CT, SC> &lds) {
     lds_u8_t *const vb = base + (buf * 2 + 1) * TILEB;
 #pragma unroll
     for (int j = 0; j < NR; ++j) {
-      const int row = j * RP + lrow;
+      const int row = wave * 16 + j * RPW + lr;
       // values past the span are cleared: 0 * NaN would reach the sums
       const bool in = kt + row < c.len;
       const u32x4_t v = in ? vr[j] : u32x4_t{0u, 0u, 0u, 0u};
@@ -725,19 +777,30 @@ MIA_DEV void tall_body(const Share &sh, TallLds<D, CT, SC> &lds) {
     // S^T = K . Q^T: lane = row rl, value e of block b: key b*32 + (e/4)*8 +
     // half*4 + e%4
     f32x16_t s[2];
+    auto read_k = [&](int b, int ks) {
+      const int row = b * 32 + rl;
+      return __builtin_bit_cast(
+          bf16x8_t,
+          *(const lds_u32x4_t *)(kb + row * ROWB + (((ks * 2 + half) ^ k_swz<D>(row)) << 4)));
+    };
+    auto read_v = [&](int k2, int db) {
+      u32x2_t t2[2];
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) s[b][e] = 0.f;
-#pragma unroll
-      for (int ks = 0; ks < KSTEPS; ++ks) {
-        const int row = b * 32 + rl;
-        const u32x4_t kf =
-            *(const lds_u32x4_t *)(kb + row * ROWB + (((ks * 2 + half) ^ k_swz<D>(row)) << 4));
-        s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, kf), qf[ks],
-                                                       s[b], 0, 0, 0);
+      for (int rr = 0; rr < 2; ++rr) {
+        const int row = k2 * 16 + rr * 8 + tr_row;
+        const int dd = db * 32 + tr_col;
+        const int off = row * ROWB + (((dd >> 3) ^ v_swz<D>(row)) << 4) + ((dd & 7) << 1);
+        t2[rr] = __builtin_bit_cast(
+            u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t *)(vb + off)));
       }
-    }
+      return __builtin_bit_cast(bf16x8_t, u32x4_t{t2[0][0], t2[0][1], t2[1][0], t2[1][1]});
+    };
+#pragma unroll
+    for (int ks = 0; ks < KSTEPS; ++ks)
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+        s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(read_k(b, ks), qf[ks],
+                                                       ks ? s[b] : f32x16_t{}, 0, 0, 0);
     if constexpr (SC) {
 #pragma unroll
       for (int b = 0; b < 2; ++b)
@@ -785,15 +848,16 @@ MIA_DEV void tall_body(const Share &sh, TallLds<D, CT, SC> &lds) {
         }
       return (ps[0] + ps[1]) + (ps[2] + ps[3]);
     };
-    auto raise = [&]() {  // moves the maximum where it must; true if it did
+    auto tile_max = [&]() {
       float mx = -INFINITY;
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
         for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[b][e]);
-      mx = max32(mx) * c2;
-      const bool bump = mx > m_run + 8.f || (m_run == -INFINITY && mx > -INFINITY);
-      if (!__builtin_amdgcn_ballot_w64(bump)) return false;
+      return max32(mx) * c2;
+    };
+    // moves the maximum of the rows with `bump` to mx
+    auto raise = [&](bool bump, float mx) {
       const float m_new = bump ? mx : m_run;
       const float alpha = m_run == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
       m_run = m_new;
@@ -802,14 +866,11 @@ MIA_DEV void tall_body(const Share &sh, TallLds<D, CT, SC> &lds) {
       for (int i = 0; i < DBLK; ++i)
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[i][e] *= alpha;
-      return true;
     };
-    // A half sum below 2^8 proves that no score passed the maximum by more
-    // than 8, so most tiles need no maximum; a row without one yet does
-    if (__builtin_expect(__builtin_amdgcn_ballot_w64(m_run == -INFINITY) != 0, 0)) raise();
-    float psum = exps();
-    if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(psum < 256.f)) != 0, 0))
-      if (raise()) psum = exps();
+    const float mx = tile_max();
+    const bool bump = mx > m_run + 8.f || (m_run == -INFINITY && mx > -INFINITY);
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(bump) != 0, 0)) raise(bump, mx);
+    const float psum = exps();
     l_run += psum;
     // O^T += V^T . P^T
 #pragma unroll
@@ -818,20 +879,9 @@ MIA_DEV void tall_body(const Share &sh, TallLds<D, CT, SC> &lds) {
       const u32x4_t bw = {pk[b][kh * 4], pk[b][kh * 4 + 1], pk[b][kh * 4 + 2], pk[b][kh * 4 + 3]};
       const bf16x8_t bop = __builtin_bit_cast(bf16x8_t, bw);
 #pragma unroll
-      for (int db = 0; db < DBLK; ++db) {
-        u32x2_t t2[2];
-#pragma unroll
-        for (int rr = 0; rr < 2; ++rr) {
-          const int row = k2 * 16 + rr * 8 + tr_row;
-          const int dd = db * 32 + tr_col;
-          const int off = row * ROWB + (((dd >> 3) ^ v_swz<D>(row)) << 4) + ((dd & 7) << 1);
-          t2[rr] = __builtin_bit_cast(
-              u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t *)(vb + off)));
-        }
-        const u32x4_t vw = {t2[0][0], t2[0][1], t2[1][0], t2[1][1]};
-        acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, vw), bop,
-                                                          acc[db], 0, 0, 0);
-      }
+      for (int db = 0; db < DBLK; ++db)
+        acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+            read_v(k2, db), bop, acc[db], 0, 0, 0);
     }
   };
 
@@ -1006,26 +1056,30 @@ MIA_DEV void thin_body(const Share &sh, ThinLds<D, SC> &lds) {
   // rows past the span read its last key (in bounds) and are masked or
   // cleared later
   auto load_k = [&](const Pos &c) {
+    const bool full = (c.t + 1) * kThinKeys <= ks_.len;
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
-      const int rr = min(c.t * kThinKeys + b * 16 + col, ks_.len - 1) - g[b].k16;
-      const uint8_t *a = g[b].k(ks_) + rr * ks_.k_t;
+      int rr = col;
+      if (!full) rr = min(c.t * kThinKeys + b * 16 + col, ks_.len - 1) - g[b].k16;
+      const uint32_t o = rr * ks_.k_t + k_chan(0, kg) * EB;
 #pragma unroll
       for (int j = 0; j < NK; ++j) {
         kr[b][j] = u32x4_t{0u, 0u, 0u, 0u};
         if (k_chan(j, kg) < d_used)
-          kr[b][j] = *reinterpret_cast<const u32x4_t *>(a + k_chan(j, kg) * EB);
+          kr[b][j] = *reinterpret_cast<const u32x4_t *>(g[b].k + k_chan(j, 0) * EB + o);
       }
     }
   };
   auto load_v = [&](const Pos &c) {
+    const bool full = (c.t + 1) * kThinKeys <= ks_.len;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const Group &x = g[j * TL / 16];
-      const int rr = min(c.t * kThinKeys + j * TL + vtl, ks_.len - 1) - x.k16;
+      int rr = j * TL % 16 + vtl;
+      if (!full) rr = min(c.t * kThinKeys + j * TL + vtl, ks_.len - 1) - x.k16;
       vr[j] = u32x4_t{0u, 0u, 0u, 0u};
       if (vds * VE < d_used)
-        vr[j] = *reinterpret_cast<const u32x4_t *>(x.v(ks_) + rr * ks_.v_t + vds * 16);
+        vr[j] = *reinterpret_cast<const u32x4_t *>(x.v + (uint32_t)(rr * ks_.v_t + vds * 16));
     }
   };
   // lane l: scale of key l (K), of key l - 32 (V)
