@@ -92,7 +92,7 @@ struct SpanParams {
   SpanList list[2];
   int join;        // every piece goes to the workspace (rows have several spans)
   float cost[2];   // time of a tall tile per workgroup, of a thin one per wave
-  int least[2];    // tiles of a share at least
+  int least[2];    // log2 of the tiles of a share at least
   int *hdr;        // see plan()
   float *part_o;   // [partial row][D]
   float2 *part_ml; // [partial row]
@@ -160,20 +160,25 @@ struct Share {
   int x0, x1;  // its tiles
   int u;       // sequence of tile x0
   int xu;      // first tile of that sequence
+  int len, tok0, rows;  // its keys, first query token and rows
 };
 
 struct PlanLds {
   int tot[2][kWaves];
-  int seq[kWaves], first[kWaves];
+  int seq[kWaves], first[kWaves], len[kWaves], tok0[kWaves], rows[kWaves];
   int empty;
 };
 
-MIA_DEV int wave_scan(int x, int lane) {  // inclusive
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int y = __shfl_up(x, o, 64);
-    if (lane >= o) x += y;
-  }
+// Inclusive scan over the wave: shifts inside rows of 16 lanes, then the row
+// totals broadcast (DPP: a few cycles a step, where a shuffle through LDS
+// takes over a hundred).
+MIA_DEV int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31
   return x;
 }
 
@@ -206,39 +211,48 @@ MIA_DEV int plan(const SpanParams &p, PlanLds &lds, Share &sh) {
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = readfirstlane(tid >> 6);
-  const int n_seq = p.list[0].n + p.list[1].n;
+  const int grid = gridDim.x;
+  const int b = blockIdx.x;
+  const int n0 = p.list[0].n;
+  const int n_seq = n0 + p.list[1].n;
   const int per = (n_seq + kThreads - 1) / kThreads;
   const int u0 = min(tid * per, n_seq), u1 = min(u0 + per, n_seq);
-  auto tiles_of = [&](int u, int &thin, bool &empty) {
-    const int li = u < p.list[0].n ? 0 : 1;
-    const SpanList &l = p.list[li];
-    const int i = li ? u - p.list[0].n : u;
-    thin = l.thin;
-    const int len = list_len(l, i);
-    const int rows = list_tokens(l, i, p.num_tokens).y * p.G;
-    empty = len == 0 && rows > 0;
-    return key_tiles(l, len) * row_tiles(l, rows) * p.Hkv;
+  struct Seq {
+    int thin, len, tok0, rows, tiles;
   };
+  auto seq_of = [&](int u) {
+    const int li = u < n0 ? 0 : 1;
+    const SpanList &l = p.list[li];
+    const int i = li ? u - n0 : u;
+    const int2 tk = list_tokens(l, i, p.num_tokens);
+    Seq q;
+    q.thin = l.thin;
+    q.len = list_len(l, i);
+    q.tok0 = tk.x;
+    q.rows = tk.y * p.G;
+    q.tiles = key_tiles(l, q.len) * row_tiles(l, q.rows) * p.Hkv;
+    return q;
+  };
+  // (calls of up to 256 sequences: one per thread, kept)
+  Seq mine = {0, 0, 0, 0, 0};
   int sum[2] = {0, 0};
   bool zero = false;
+#pragma nounroll
   for (int u = u0; u < u1; ++u) {
-    int thin;
-    bool e;
-    const int n = tiles_of(u, thin, e);
-    sum[0] += thin ? 0 : n;
-    sum[1] += thin ? n : 0;
-    zero |= e && u % (int)gridDim.x == (int)blockIdx.x;
+    mine = seq_of(u);
+    sum[0] += mine.thin ? 0 : mine.tiles;
+    sum[1] += mine.thin ? mine.tiles : 0;
+    zero |= mine.len == 0 && mine.rows > 0 && u % grid == b;
   }
-  int inc[2];
+  int inc[2], n[2], base[2];
 #pragma unroll
   for (int f = 0; f < 2; ++f) {
-    inc[f] = wave_scan(sum[f], lane);
+    inc[f] = wave_scan(sum[f]);
     if (lane == 63) lds.tot[f][wave] = inc[f];
   }
   if (tid == 0) lds.empty = 0;
   __syncthreads();
   if (zero && !p.join) lds.empty = 1;
-  int n[2], base[2];
 #pragma unroll
   for (int f = 0; f < 2; ++f) {
     n[f] = 0;
@@ -252,89 +266,81 @@ MIA_DEV int plan(const SpanParams &p, PlanLds &lds, Share &sh) {
   }
   // workgroups of each form: in proportion to the costs, whole multiples of
   // the 8 XCDs where there are enough
-  const int grid = gridDim.x;
-  int wt = (n[0] + p.least[0] - 1) / p.least[0];
-  int ws = (n[1] + kWaves * p.least[1] - 1) / (kWaves * p.least[1]);
+  int wt = (n[0] + (1 << p.least[0]) - 1) >> p.least[0];
+  int ws = (n[1] + kWaves * (1 << p.least[1]) - 1) / (kWaves * (1 << p.least[1]));
   if (wt + ws > grid) {
-    const float a = (float)n[0] * p.cost[0], b = (float)n[1] * p.cost[1];
-    const int share = (int)((float)grid * (a / (a + b)) + 0.5f);
+    const float ca = (float)n[0] * p.cost[0], cb = (float)n[1] * p.cost[1];
+    const int share = readfirstlane((int)((float)grid * (ca / (ca + cb)) + 0.5f));
     wt = n[0] == 0 ? 0 : n[1] == 0 ? grid : min(max(share, 1), grid - 1);
     if (wt > 8 && wt < grid) wt &= ~7;
     ws = n[1] == 0 ? 0 : grid - wt;
   } else if (wt > 8) {
     wt &= ~7;
   }
+  const int form = b < wt ? 0 : b < wt + ws ? 1 : -1;
   const int wv = ws * kWaves;
   Cut cut[2];
   cut[0].base = wt ? n[0] / wt : 0;
   cut[0].rem = n[0] - cut[0].base * wt;
   cut[1].base = wv ? n[1] / wv : 0;
   cut[1].rem = n[1] - cut[1].base * wv;
-  if (p.join) {
-    if (blockIdx.x == 0) {
-      if (tid == 0) {
-        p.hdr[0] = cut[0].base, p.hdr[1] = cut[0].rem;
-        p.hdr[2] = cut[1].base, p.hdr[3] = cut[1].rem;
-      }
-      int x[2] = {base[0], base[1]};
-      for (int u = u0; u < u1; ++u) {
-        int thin;
-        bool e;
-        const int c = tiles_of(u, thin, e);
-        p.hdr[kHdr + u] = thin ? x[1] : x[0];
-        x[0] += thin ? 0 : c;
-        x[1] += thin ? c : 0;
-      }
-    }
+  const bool lists = p.join && b == 0;  // this workgroup writes the header
+  if (lists && tid == 0) {
+    p.hdr[0] = cut[0].base, p.hdr[1] = cut[0].rem;
+    p.hdr[2] = cut[1].base, p.hdr[3] = cut[1].rem;
   }
-  const int b = blockIdx.x;
-  const int form = b < wt ? 0 : b < wt + ws ? 1 : -1;
-  int w;
-  if (form == 0) {
-    // workgroups go round-robin over the 8 XCDs: neighbouring shares (the row
-    // tiles of one head over the same keys) stay on one XCD's L2
-    w = wt >= 8 && wt % 8 == 0 ? (b % 8) * (wt / 8) + b / 8 : b;
-  } else {
-    w = (b - wt) * kWaves;
-  }
+  // workgroups go round-robin over the 8 XCDs: neighbouring tall shares (the
+  // row tiles of one head over the same keys) stay on one XCD's L2
+  const int w = form == 1 ? (b - wt) * kWaves
+                : wt >= 8 && wt % 8 == 0 ? (b % 8) * (wt / 8) + b / 8 : b;
   if (!p.join && lane == 0) {
     // (one form only) no cut segment starts in a share unless it says so: the
     // header is cleared by the thread that may set it
     if (p.list[1].thin) p.hdr[kHdr * (b * kWaves + wave)] = 0;
     else if (wave == 0) p.hdr[kHdr * (form == 0 ? w : b)] = 0;
   }
-  const int f = form == 1 ? 1 : 0;
-  const int shares = form == 1 ? kWaves : 1;
-#pragma unroll
-  for (int k = 0; k < kWaves; ++k) {
-    if (form < 0 || k >= shares) break;
-    const int x = cut_start(cut[f], w + k);
-    if (x < n[f] && base[f] <= x && x < base[f] + sum[f]) {
-      int xu = base[f];
-      for (int u = u0; u < u1; ++u) {
-        int thin;
-        bool e;
-        const int c = tiles_of(u, thin, e);
-        if (thin != f) continue;
-        if (x < xu + c) {
+  // the sequences of this workgroup's first tiles
+  const Cut mycut = form == 1 ? cut[1] : cut[0];
+  const int shares = form < 0 ? 0 : form == 1 ? kWaves : 1;
+  const int x_lo = cut_start(mycut, w), x_hi = cut_start(mycut, w + shares);
+  int x[2] = {base[0], base[1]};
+  const bool find = form == 1 ? x_lo < x[1] + sum[1] && x_hi > x[1]
+                              : form == 0 && x_lo < x[0] + sum[0] && x_hi > x[0];
+  if (lists || find) {
+#pragma nounroll
+    for (int u = u0; u < u1; ++u) {
+      const Seq q = per == 1 ? mine : seq_of(u);
+      const int xu = q.thin ? x[1] : x[0];
+      if (lists) p.hdr[kHdr + u] = xu;
+      if (find && q.thin == form) {
+#pragma nounroll
+        for (int k = 0; k < shares; ++k) {
+          const int xs = cut_start(mycut, w + k);
+          if (xs < xu || xs >= xu + q.tiles) continue;
           lds.seq[k] = u;
           lds.first[k] = xu;
-          break;
+          lds.len[k] = q.len;
+          lds.tok0[k] = q.tok0;
+          lds.rows[k] = q.rows;
         }
-        xu += c;
       }
+      x[0] += q.thin ? 0 : q.tiles;
+      x[1] += q.thin ? q.tiles : 0;
     }
   }
   __syncthreads();
   if (lds.empty) zero_empty(p);
   if (form < 0) return -1;
   const int k = form == 1 ? wave : 0;
-  sh.cut = cut[f];
+  sh.cut = mycut;
   sh.w = w + k;
-  sh.x0 = cut_start(cut[f], sh.w);
-  sh.x1 = cut_start(cut[f], sh.w + 1);
+  sh.x0 = cut_start(mycut, sh.w);
+  sh.x1 = cut_start(mycut, sh.w + 1);
   sh.u = readfirstlane(lds.seq[k]);
   sh.xu = readfirstlane(lds.first[k]);
+  sh.len = readfirstlane(lds.len[k]);
+  sh.tok0 = readfirstlane(lds.tok0[k]);
+  sh.rows = readfirstlane(lds.rows[k]);
   return form;
 }
 
@@ -362,7 +368,11 @@ MIA_DEV Pos first_pos(const SpanParams &p, const Share &sh) {
   Pos c;
   c.li = sh.u < p.list[0].n ? 0 : 1;
   c.i = c.li ? sh.u - p.list[0].n : sh.u;
-  load_seq(p, c);
+  c.len = sh.len;
+  c.tok0 = sh.tok0;
+  c.rows = sh.rows;
+  c.tiles = key_tiles(p.list[c.li], c.len);
+  c.rt_n = row_tiles(p.list[c.li], c.rows);
   const int k = sh.x0 - sh.xu;  // tile of the sequence
   const int seg = k / c.tiles;
   c.t = k - seg * c.tiles;
@@ -541,10 +551,14 @@ MIA_DEV int64_t piece_slot(const SpanParams &p, const Share &sh, const Pos &c, i
 // ---------------------------------------------------------------------------
 // tall form
 // ---------------------------------------------------------------------------
+// Stages of the copy ring (bf16): 64 KB of LDS for either width, so that two
+// workgroups share a CU; the widened tiles of 8-bit caches take two buffers.
+constexpr int tall_stages(int D, int CT) { return CT == kBf16 && D == 64 ? 4 : 2; }
+
 template <int D, int CT, bool SC>
 struct TallLds {
   static constexpr int TILEB = kTallKeys * D * 2;
-  uint8_t kv[2][2][TILEB];                       // [stage][K, V]
+  uint8_t kv[tall_stages(D, CT)][2][TILEB];      // [stage][K, V]
   float sc[2][2][SC ? kTallKeys : 4];            // [stage][K, V]
 };
 
@@ -619,6 +633,7 @@ MIA_DEV void tall_body(const Share &sh, TallLds<D, CT, SC> &lds) {
   static_assert(kTallKeys == 16 * kWaves, "a wave loads one 16-key group of a tile");
   constexpr int ROWB = D * 2;
   constexpr int TILEB = kTallKeys * ROWB;
+  constexpr int STAGES = tall_stages(D, CT);
   constexpr int KSTEPS = D / 16;
   constexpr int DBLK = D / 32;
 
@@ -734,7 +749,9 @@ MIA_DEV void tall_body(const Share &sh, TallLds<D, CT, SC> &lds) {
   float m_run = -INFINITY, l_run = 0.f;
   float c2 = 0.f;
   bool live = false;  // the wave has rows
-  auto begin_piece = [&](const Pos &c) {
+  u32x4_t qw[KSTEPS];
+  // the loads of the rows of a piece, issued ahead of its first tile's
+  auto load_q = [&](const Pos &c) {
     const SpanParams &p = fresh();
     const int r = c.rt * kRows + wave * 32 + rl;
     live = c.rt * kRows + wave * 32 < c.rows;
@@ -742,19 +759,19 @@ MIA_DEV void tall_body(const Share &sh, TallLds<D, CT, SC> &lds) {
     const int pos = (int)fdiv((uint32_t)(ok ? r : 0), p.g_div);
     const int hq = c.h * p.G + (ok ? r - pos * p.G : 0);
     const uint16_t *qp = p.q + tok_off(p, c.tok0 + pos, p.qs_b, p.qs_s) + (int64_t)hq * p.qs_h;
-    uint32_t neg;
-    c2 = score_factor(p, c.h, neg);
 #pragma unroll
     for (int ks = 0; ks < KSTEPS; ++ks) {
-      u32x4_t w = {0u, 0u, 0u, 0u};
+      qw[ks] = u32x4_t{0u, 0u, 0u, 0u};
       const int d0 = ks * 16 + half * 8;
-      if (ok && d0 < p.d) {
-        w = *reinterpret_cast<const u32x4_t *>(qp + d0);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] ^= neg;
-      }
-      qf[ks] = __builtin_bit_cast(bf16x8_t, w);
+      if (ok && d0 < d_used) qw[ks] = *reinterpret_cast<const u32x4_t *>(qp + d0);
     }
+  };
+  auto begin_piece = [&](const Pos &c) {
+    uint32_t neg;
+    c2 = score_factor(fresh(), c.h, neg);
+#pragma unroll
+    for (int ks = 0; ks < KSTEPS; ++ks)
+      qf[ks] = __builtin_bit_cast(bf16x8_t, qw[ks] ^ u32x4_t{neg, neg, neg, neg});
 #pragma unroll
     for (int i = 0; i < DBLK; ++i)
 #pragma unroll
@@ -929,43 +946,63 @@ MIA_DEV void tall_body(const Share &sh, TallLds<D, CT, SC> &lds) {
   Pos nxt = cur;
   int buf = 0, t0 = cur.t;
   if constexpr (DMA) {
-    if (d_used < D) {  // channels past d: zero in both stages, never written again
-      for (int o = tid * 16; o < 4 * TILEB; o += kThreads * 16)
+    if (d_used < D) {  // channels past d: zero in all stages, never written again
+      for (int o = tid * 16; o < 2 * STAGES * TILEB; o += kThreads * 16)
         *(lds_u32x4_t *)(base + o) = u32x4_t{0u, 0u, 0u, 0u};
       __syncthreads();
     }
-    fetch(cur, 0, true);
-    begin_piece(cur);
-    while (true) {
-      // own copies of tile `cur` have landed; the barrier makes every
-      // thread's visible and the other stage free
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __syncthreads();
-      const bool more = cur.left > 1;
+    // nxt: the next tile to copy, STAGES - 1 ahead of cur
+    load_q(cur);
+    bool anew = true, more = true;
+    auto copy_next = [&](int stage) {
+      if (!more) return;
+      fetch(nxt, stage, anew);
+      more = nxt.left > 1;
       if (more) {
         advance(fresh(), nxt);
-        fetch(nxt, buf ^ 1, nxt.t == 0);
+        anew = nxt.t == 0;
       }
+    };
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) copy_next(i);
+    begin_piece(cur);
+    while (true) {
+      // own copies of tile `cur` have landed (those of the STAGES - 2 tiles
+      // behind it may stay in flight; a narrow call's count of copies varies,
+      // so it waits for all); the barrier makes every thread's visible and
+      // the stage of the tile before free
+      if (STAGES > 2 && d_used == D && cur.left > STAGES - 2)
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((STAGES - 2) * 2 * NP) : "memory");
+      else
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      copy_next(buf == 0 ? STAGES - 1 : buf - 1);
       const int left = cur.len - cur.t * kTallKeys;
       if (left < kTallKeys) {
         // values past the span are cleared: 0 * NaN would reach the sums
         lds_u8_t *const vb = base + (buf * 2 + 1) * TILEB;
         for (int o = left * ROWB + tid * 16; o < TILEB; o += kThreads * 16)
           *(lds_u32x4_t *)(vb + o) = u32x4_t{0u, 0u, 0u, 0u};
-        __syncthreads();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
       }
       if (live) compute(cur, buf);
-      const bool ends = !more || nxt.t == 0;
+      const bool last = cur.left == 1;
+      const bool ends = last || cur.t + 1 == cur.tiles;
+      if (ends) end_piece(cur, t0);
+      if (last) return;
+      advance(fresh(), cur);
       if (ends) {
-        end_piece(cur, t0);
-        if (!more) return;
-        begin_piece(nxt);
+        load_q(cur);
+        begin_piece(cur);
         t0 = 0;
       }
-      cur = nxt;
-      buf ^= 1;
+      buf = buf + 1 == STAGES ? 0 : buf + 1;
     }
   } else {
+    load_q(cur);
     fetch(cur, 0, true);
     begin_piece(cur);
     store_tile(cur, 0);
@@ -980,6 +1017,7 @@ MIA_DEV void tall_body(const Share &sh, TallLds<D, CT, SC> &lds) {
       if (!more || nxt.t == 0) {
         end_piece(cur, t0);
         if (!more) return;
+        load_q(nxt);
         begin_piece(nxt);
         t0 = 0;
       }
@@ -1101,10 +1139,10 @@ MIA_DEV void thin_body(const Share &sh, ThinLds<D, SC> &lds) {
   f32x4_t acc[NC][DB16];
   float m_run[NC], l_run[NC];
   float c2 = 0.f;
-  auto begin_piece = [&](const Pos &c) {
+  u32x4_t qw[NC][KSTEPS];
+  // the loads of the rows of a piece, issued ahead of its first tile's
+  auto load_q = [&](const Pos &c) {
     const SpanParams &p = fresh();
-    uint32_t neg;
-    c2 = score_factor(p, c.h, neg);
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
       const int r = n * 16 + col;
@@ -1115,14 +1153,19 @@ MIA_DEV void thin_body(const Share &sh, ThinLds<D, SC> &lds) {
 #pragma unroll
       for (int ks = 0; ks < KSTEPS; ++ks) {
         const int d0 = CT == kBf16 ? k_chan(ks, kg) : k_chan(ks >> 1, kg) + (ks & 1) * 8;
-        u32x4_t w = {0u, 0u, 0u, 0u};
-        if (ok && d0 < p.d) {
-          w = *reinterpret_cast<const u32x4_t *>(qp + d0);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) w[i] ^= neg;
-        }
-        qf[n][ks] = __builtin_bit_cast(bf16x8_t, w);
+        qw[n][ks] = u32x4_t{0u, 0u, 0u, 0u};
+        if (ok && d0 < d_used) qw[n][ks] = *reinterpret_cast<const u32x4_t *>(qp + d0);
       }
+    }
+  };
+  auto begin_piece = [&](const Pos &c) {
+    uint32_t neg;
+    c2 = score_factor(fresh(), c.h, neg);
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+#pragma unroll
+      for (int ks = 0; ks < KSTEPS; ++ks)
+        qf[n][ks] = __builtin_bit_cast(bf16x8_t, qw[n][ks] ^ u32x4_t{neg, neg, neg, neg});
 #pragma unroll
       for (int i = 0; i < DB16; ++i) acc[n][i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
       m_run[n] = -INFINITY;
@@ -1282,6 +1325,7 @@ MIA_DEV void thin_body(const Share &sh, ThinLds<D, SC> &lds) {
   // product (copy to LDS) has freed the registers
   if (sh.x0 >= sh.x1) return;
   Pos cur = first_pos(fresh(), sh);
+  load_q(cur);
   locate(cur, true);
   load_k(cur);
   load_s(cur);
@@ -1308,6 +1352,7 @@ MIA_DEV void thin_body(const Share &sh, ThinLds<D, SC> &lds) {
     if (!more || nxt.t == 0) {
       end_piece(cur, t0);
       if (!more) return;
+      load_q(nxt);
       begin_piece(nxt);
       t0 = 0;
     }
@@ -1423,10 +1468,9 @@ __global__ __launch_bounds__(256) void span_merge_kernel(SpanParams p) {
 // row s sees s of them) and the sink.  D / 4 lanes per row.
 constexpr int kJoinGroups = 8;
 
-template <int D, int CT, bool SC>
+template <int D, int CT, bool SC, int GR>
 __global__ __launch_bounds__(256) void span_join_kernel(SpanParams p, FastDiv hq_div) {
   constexpr int LPR = D / 4;
-  constexpr int GR = kJoinGroups;
   __shared__ JoinLds<D, GR> lds;
   const int c = threadIdx.x % LPR;
   const int n_rows = p.num_tokens * (int)hq_div.d;
@@ -1442,12 +1486,12 @@ __global__ __launch_bounds__(256) void span_join_kernel(SpanParams p, FastDiv hq
   auto pieces = [&](int li, int i, int r, int rows, int64_t &first) {
     const SpanList &l = p.list[li];
     const int tiles = key_tiles(l, list_len(l, i));
-    first = 0;
-    if (tiles == 0) return 0;
     const int rt_n = row_tiles(l, rows), rt = l.thin ? 0 : r / kRows;
     const int in = h * rt_n + rt;  // segment of the sequence
     const Cut cut = {p.hdr[2 * l.thin], p.hdr[2 * l.thin + 1]};
     const int x = p.hdr[kHdr + (li ? p.list[0].n + i : i)] + in * tiles;
+    first = 0;
+    if (tiles == 0) return 0;
     const int w = cut_of(cut, x);
     first = l.part0 + ((int64_t)i * rt_n * p.Hkv + in + w) * l.part_rows + (r - rt * kRows);
     return cut_of(cut, x + tiles - 1) - w + 1;
@@ -1575,8 +1619,8 @@ Layout span_layout(SpanParams &p, int D) {
       hdr += units * kHdr;
     }
   }
-  p.cost[0] = 1.0f, p.cost[1] = 0.6f;
-  p.least[0] = 2, p.least[1] = 2;
+  p.cost[0] = 1.0f, p.cost[1] = D == 64 ? 0.28f : 0.41f;
+  p.least[0] = 1, p.least[1] = 1;
   w.hdr = 0;
   w.ml = (size_t)up(hdr * 4, 256);
   w.o = w.ml + (size_t)up(rows * 8, 256);
@@ -1660,10 +1704,19 @@ void launch_span(const SpanParams &p, int grid, hipStream_t s) {
   if (cols <= 16) span_kernel<D, CT, SC, 1><<<grid, kThreads, 0, s>>>(p);
   else span_kernel<D, CT, SC, 2><<<grid, kThreads, 0, s>>>(p);
   if (p.join) {
+    // lane groups per row by the pieces to expect: those of the prefix (its
+    // share of the workgroups over its segments) and one or two of the row
     const int hq = p.Hkv * p.G;
-    constexpr int RPB = 256 / (D / 4) / kJoinGroups;
-    span_join_kernel<D, CT, SC>
-        <<<(p.num_tokens * hq + RPB - 1) / RPB, 256, 0, s>>>(p, make_fastdiv(hq));
+    const int segs = std::max(1, (p.list[0].tok_max * p.G + kRows - 1) / kRows * p.Hkv);
+    const int units = p.list[0].thin ? grid * kWaves : grid;
+    auto blocks = [&](int groups) {
+      const int rpb = 256 / (D / 4) / groups;
+      return (p.num_tokens * hq + rpb - 1) / rpb;
+    };
+    if (units / segs > 8)
+      span_join_kernel<D, CT, SC, 8><<<blocks(8), 256, 0, s>>>(p, make_fastdiv(hq));
+    else
+      span_join_kernel<D, CT, SC, 2><<<blocks(2), 256, 0, s>>>(p, make_fastdiv(hq));
   }
 }
 
