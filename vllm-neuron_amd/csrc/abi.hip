@@ -75,6 +75,14 @@ static int check_span(const A &a, const int64_t *q_rows, const int64_t *out_rows
                 "span attention: cache head_dim must be contiguous and its rows 16-byte aligned");
     MIA_REQUIRE(s[2] >= 0 && s[2] * eb < (1ll << 27), MIA_ERR_VALUE,
                 "span attention: cache token stride out of range");
+    MIA_REQUIRE(s[0] >= 0 && s[1] >= 0 && s[0] * eb / 16 < (1ll << 32), MIA_ERR_VALUE,
+                "span attention: cache block or head stride out of range");
+    if (a.k_scales) {
+      const int64_t *sc = i ? a.v_scale_stride : a.k_scale_stride;
+      MIA_REQUIRE(sc[0] >= 0 && sc[0] < (1ll << 32) && sc[1] >= 0 && sc[2] >= 0 &&
+                      sc[2] < (1ll << 32),
+                  MIA_ERR_VALUE, "span attention: scale strides out of range");
+    }
   }
   MIA_REQUIRE(aligned(a.q, 16) && q_rows[n_rows] == 1, MIA_ERR_VALUE,
               "span attention: q rows must be contiguous and 16-byte aligned");

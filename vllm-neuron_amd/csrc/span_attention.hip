@@ -81,9 +81,11 @@ struct SpanParams {
   int num_tokens, S;
   int G, Hkv, d;
   const uint8_t *k_cache, *v_cache;
-  int64_t kc_blk, kc_h, kc_t, vc_blk, vc_h, vc_t;  // bytes
+  uint32_t kc_blk16, vc_blk16;       // block strides in 16-byte units
+  int64_t kc_h, kc_t, vc_h, vc_t;    // bytes
   const float *k_sc, *v_sc;  // per-key scales or NULL
-  int64_t ks_blk, ks_h, ks_t, vs_blk, vs_h, vs_t;  // elements
+  uint32_t ks_blk, ks_t, vs_blk, vs_t;  // elements
+  int64_t ks_h, vs_h;
   const float *k_deq, *v_deq;  // per-head scales or NULL
   const float *sink;
   int nb, bs;
@@ -92,7 +94,8 @@ struct SpanParams {
   SpanList list[2];
   int join;        // every piece goes to the workspace (rows have several spans)
   float cost[2];   // time of a tall tile per workgroup, of a thin one per wave
-  int least[2];    // log2 of the tiles of a share at least
+  int over[2];     // cost of a segment's start in tiles (stores, query rows, table)
+  int least[2];    // units of a share at least
   int *hdr;        // see plan()
   float *part_o;   // [partial row][D]
   float2 *part_ml; // [partial row]
@@ -137,18 +140,20 @@ MIA_DEV int key_tiles(const SpanList &l, int len) {
   return l.thin ? (len + kThinKeys - 1) / kThinKeys : (len + kTallKeys - 1) / kTallKeys;
 }
 
-// N tiles cut into W shares: the first `rem` hold base + 1, the others base.
+// A form's segments laid end to end: `over` units for the start of a segment,
+// then one per tile.  N units are cut into W shares: the first `rem` hold
+// base + 1, the others base.
 struct Cut {
   int base, rem;
 };
 MIA_DEV int cut_start(Cut c, int w) { return w * c.base + min(w, c.rem); }
-MIA_DEV int cut_of(Cut c, int x) {  // the share that holds tile x
+MIA_DEV int cut_of(Cut c, int x) {  // the share that holds unit x
   const int head = c.rem * (c.base + 1);
   return x < head ? x / (c.base + 1) : c.rem + (x - head) / c.base;
 }
 
 // Workspace header.  Joined calls: [0..3] the cuts of both forms, [8 + u] the
-// first tile of joined sequence u in its form's stream.  Cross attention: 8
+// first unit of joined sequence u in its form's stream.  Cross attention: 8
 // ints per share: pieces of the cut segment that starts in it (0: none), its
 // first query token, rows, row tile, head.
 constexpr int kHdr = 8;
@@ -157,9 +162,9 @@ constexpr int kHdr = 8;
 struct Share {
   Cut cut;
   int w;       // number of the share
-  int x0, x1;  // its tiles
-  int u;       // sequence of tile x0
-  int xu;      // first tile of that sequence
+  int x0, x1;  // its units
+  int u;       // sequence of unit x0
+  int xu;      // first unit of that sequence
   int len, tok0, rows;  // its keys, first query token and rows
 };
 
@@ -205,8 +210,8 @@ MIA_DEV void zero_empty(const SpanParams &p) {
 // The plan of a launch, in every workgroup: a block scan of the sequences'
 // tiles (each thread a contiguous run of the joined lists), the workgroups of
 // each form, and this workgroup's (tall) or wave's (thin) share.  Returns 0
-// for a tall share, 1 for a thin one, -1 for none; uniform in the workgroup
-// (a thin wave without tiles has x0 == x1).
+// for a tall share, 1 for a thin one, -1 for none; uniform in the workgroup (a
+// share may hold no tile).
 MIA_DEV int plan(const SpanParams &p, PlanLds &lds, Share &sh) {
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -218,7 +223,7 @@ MIA_DEV int plan(const SpanParams &p, PlanLds &lds, Share &sh) {
   const int per = (n_seq + kThreads - 1) / kThreads;
   const int u0 = min(tid * per, n_seq), u1 = min(u0 + per, n_seq);
   struct Seq {
-    int thin, len, tok0, rows, tiles;
+    int thin, len, tok0, rows, units;
   };
   auto seq_of = [&](int u) {
     const int li = u < n0 ? 0 : 1;
@@ -230,7 +235,8 @@ MIA_DEV int plan(const SpanParams &p, PlanLds &lds, Share &sh) {
     q.len = list_len(l, i);
     q.tok0 = tk.x;
     q.rows = tk.y * p.G;
-    q.tiles = key_tiles(l, q.len) * row_tiles(l, q.rows) * p.Hkv;
+    const int kt = key_tiles(l, q.len);
+    q.units = kt ? (kt + p.over[l.thin]) * row_tiles(l, q.rows) * p.Hkv : 0;
     return q;
   };
   // (calls of up to 256 sequences: one per thread, kept)
@@ -240,8 +246,8 @@ MIA_DEV int plan(const SpanParams &p, PlanLds &lds, Share &sh) {
 #pragma nounroll
   for (int u = u0; u < u1; ++u) {
     mine = seq_of(u);
-    sum[0] += mine.thin ? 0 : mine.tiles;
-    sum[1] += mine.thin ? mine.tiles : 0;
+    sum[0] += mine.thin ? 0 : mine.units;
+    sum[1] += mine.thin ? mine.units : 0;
     zero |= mine.len == 0 && mine.rows > 0 && u % grid == b;
   }
   int inc[2], n[2], base[2];
@@ -266,17 +272,16 @@ MIA_DEV int plan(const SpanParams &p, PlanLds &lds, Share &sh) {
   }
   // workgroups of each form: in proportion to the costs, whole multiples of
   // the 8 XCDs where there are enough
-  int wt = (n[0] + (1 << p.least[0]) - 1) >> p.least[0];
-  int ws = (n[1] + kWaves * (1 << p.least[1]) - 1) / (kWaves * (1 << p.least[1]));
+  const int most_t = n[0] ? max(1, n[0] / p.least[0]) : 0;
+  const int most_s = n[1] ? max(1, n[1] / (kWaves * p.least[1])) : 0;
+  int wt = most_t, ws = most_s;
   if (wt + ws > grid) {
     const float ca = (float)n[0] * p.cost[0], cb = (float)n[1] * p.cost[1];
     const int share = readfirstlane((int)((float)grid * (ca / (ca + cb)) + 0.5f));
-    wt = n[0] == 0 ? 0 : n[1] == 0 ? grid : min(max(share, 1), grid - 1);
-    if (wt > 8 && wt < grid) wt &= ~7;
-    ws = n[1] == 0 ? 0 : grid - wt;
-  } else if (wt > 8) {
-    wt &= ~7;
+    wt = n[0] == 0 ? 0 : n[1] == 0 ? grid : min(min(max(share, 1), grid - 1), most_t);
+    ws = n[1] == 0 ? 0 : min(grid - wt, most_s);
   }
+  if (wt > 8) wt &= ~7;
   const int form = b < wt ? 0 : b < wt + ws ? 1 : -1;
   const int wv = ws * kWaves;
   Cut cut[2];
@@ -299,7 +304,7 @@ MIA_DEV int plan(const SpanParams &p, PlanLds &lds, Share &sh) {
     if (p.list[1].thin) p.hdr[kHdr * (b * kWaves + wave)] = 0;
     else if (wave == 0) p.hdr[kHdr * (form == 0 ? w : b)] = 0;
   }
-  // the sequences of this workgroup's first tiles
+  // the sequences of this workgroup's first units
   const Cut mycut = form == 1 ? cut[1] : cut[0];
   const int shares = form < 0 ? 0 : form == 1 ? kWaves : 1;
   const int x_lo = cut_start(mycut, w), x_hi = cut_start(mycut, w + shares);
@@ -316,7 +321,7 @@ MIA_DEV int plan(const SpanParams &p, PlanLds &lds, Share &sh) {
 #pragma nounroll
         for (int k = 0; k < shares; ++k) {
           const int xs = cut_start(mycut, w + k);
-          if (xs < xu || xs >= xu + q.tiles) continue;
+          if (xs < xu || xs >= xu + q.units) continue;
           lds.seq[k] = u;
           lds.first[k] = xu;
           lds.len[k] = q.len;
@@ -324,8 +329,8 @@ MIA_DEV int plan(const SpanParams &p, PlanLds &lds, Share &sh) {
           lds.rows[k] = q.rows;
         }
       }
-      x[0] += q.thin ? 0 : q.tiles;
-      x[1] += q.thin ? q.tiles : 0;
+      x[0] += q.thin ? 0 : q.units;
+      x[1] += q.thin ? q.units : 0;
     }
   }
   __syncthreads();
@@ -351,7 +356,8 @@ struct Pos {
   int len, tiles;     // keys, tiles
   int rt_n, rt, h;    // row tiles, this one, kv head
   int t;              // tile
-  int left;           // tiles of the share from here on
+  int x;              // its unit
+  int over;           // units before a segment's first tile
 };
 
 MIA_DEV void load_seq(const SpanParams &p, Pos &c) {
@@ -364,30 +370,43 @@ MIA_DEV void load_seq(const SpanParams &p, Pos &c) {
   c.rt_n = row_tiles(l, c.rows);
 }
 
-MIA_DEV Pos first_pos(const SpanParams &p, const Share &sh) {
-  Pos c;
+// The share's first tile; false if it has none.
+MIA_DEV bool first_pos(const SpanParams &p, const Share &sh, Pos &c) {
+  if (sh.x0 >= sh.x1) return false;
   c.li = sh.u < p.list[0].n ? 0 : 1;
   c.i = c.li ? sh.u - p.list[0].n : sh.u;
+  const SpanList &l = p.list[c.li];
   c.len = sh.len;
   c.tok0 = sh.tok0;
   c.rows = sh.rows;
-  c.tiles = key_tiles(p.list[c.li], c.len);
-  c.rt_n = row_tiles(p.list[c.li], c.rows);
-  const int k = sh.x0 - sh.xu;  // tile of the sequence
-  const int seg = k / c.tiles;
-  c.t = k - seg * c.tiles;
+  c.tiles = key_tiles(l, c.len);
+  c.rt_n = row_tiles(l, c.rows);
+  c.over = p.over[l.thin];
+  const int k = sh.x0 - sh.xu;  // unit of the sequence
+  const int seg = k / (c.tiles + c.over);
+  c.t = k - seg * (c.tiles + c.over) - c.over;
+  c.x = sh.x0;
+  if (c.t < 0) {  // among the units of a segment's start
+    c.x -= c.t;
+    c.t = 0;
+  }
   c.h = seg / c.rt_n;
   c.rt = seg - c.h * c.rt_n;
-  c.left = sh.x1 - sh.x0;
-  return c;
+  return c.x < sh.x1;
 }
 
-// To the next tile of the share (left > 1), over sequences without tiles and
+// Is there a tile behind c in the share that ends at x1?
+MIA_DEV bool has_next(const Pos &c, int x1) {
+  return c.x + 1 + (c.t + 1 < c.tiles ? 0 : c.over) < x1;
+}
+
+// To the next tile of the share (has_next), over sequences without tiles and
 // lists of the other form.
 MIA_DEV void advance(const SpanParams &p, Pos &c) {
-  --c.left;
+  ++c.x;
   if (++c.t < c.tiles) return;
   c.t = 0;
+  c.x += c.over;
   if (++c.rt < c.rt_n) return;
   c.rt = 0;
   if (++c.h < p.Hkv) return;
@@ -422,14 +441,12 @@ MIA_DEV u32x4_t widen8(uint32_t a, uint32_t b) {
     o[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, false));
     o[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, true));
   } else {
-    // bytes + 128 as unsigned, converted one by one
+    // (one conversion per value: the byte is picked and extended by the operand)
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const uint32_t u = (i ? b : a) ^ 0x80808080u;
-      const float f0 = (float)(u & 0xffu) - 128.f, f1 = (float)((u >> 8) & 0xffu) - 128.f;
-      const float f2 = (float)((u >> 16) & 0xffu) - 128.f, f3 = (float)(u >> 24) - 128.f;
-      o[2 * i] = pack2_bf16(f0, f1);
-      o[2 * i + 1] = pack2_bf16(f2, f3);
+      const uint32_t u = i ? b : a;
+      o[2 * i] = pack2_bf16((float)(int8_t)(u & 0xffu), (float)(int8_t)((u >> 8) & 0xffu));
+      o[2 * i + 1] = pack2_bf16((float)(int8_t)((u >> 16) & 0xffu), (float)(int8_t)(u >> 24));
     }
   }
   return o;
@@ -465,24 +482,34 @@ MIA_DEV int64_t tok_off(const SpanParams &p, int t, int64_t sb, int64_t ss) {
 }
 
 // Where a segment's keys lie (wave-uniform): its table row and the first byte
-// of its head in K and V.
+// of its head in K and V, the first scale of its head.
 struct Keys {
   const int32_t *bt;  // NULL: dense, block = sequence
   int64_t bt_j;
   const uint8_t *k, *v;
-  int64_t k_blk, v_blk;
-  uint32_t k_t, v_t;  // token strides (bytes, below 2^27)
+  const float *ks, *vs;
+  uint32_t k_blk, v_blk;    // block strides in 16-byte units
+  uint32_t k_t, v_t;        // token strides in bytes (below 2^27)
+  uint32_t ks_blk, vs_blk;  // scale strides in elements
+  uint32_t ks_t, vs_t;
   int seq, len, nb, bs;
   FastDiv bs_div;
 
+  template <bool SC>
   MIA_DEV void set(const SpanParams &p, const Pos &c) {
     const SpanList &l = p.list[c.li];
     bt = l.bt ? l.bt + (int64_t)c.i * l.bt_s : nullptr;
     bt_j = l.bt_j;
     k = p.k_cache + (int64_t)c.h * p.kc_h;
     v = p.v_cache + (int64_t)c.h * p.vc_h;
-    k_blk = p.kc_blk, v_blk = p.vc_blk;
+    k_blk = p.kc_blk16, v_blk = p.vc_blk16;
     k_t = (uint32_t)p.kc_t, v_t = (uint32_t)p.vc_t;
+    if constexpr (SC) {
+      ks = p.k_sc + (int64_t)c.h * p.ks_h;
+      vs = p.v_sc + (int64_t)c.h * p.vs_h;
+      ks_blk = p.ks_blk, vs_blk = p.vs_blk;
+      ks_t = p.ks_t, vs_t = p.vs_t;
+    }
     seq = c.i, len = c.len, nb = p.nb, bs = p.bs;
     bs_div = p.bs_div;
   }
@@ -496,20 +523,21 @@ struct Keys {
 
 // A 16-key group: its first key, block, and first key inside the block.
 struct Group {
-  int k16, blk, off;
+  int k16;
+  uint32_t blk, off;
   const uint8_t *k, *v;  // its first rows
   MIA_DEV void set(const Keys &s, int k0, int entry) {
     k16 = s.first(k0);
     blk = s.bt ? min(max(entry, 0), s.nb - 1) : s.seq;
     off = s.bt ? k16 - (int)fdiv((uint32_t)k16, s.bs_div) * s.bs : k16;
-    k = s.k + (int64_t)blk * s.k_blk + (int64_t)off * s.k_t;
-    v = s.v + (int64_t)blk * s.v_blk + (int64_t)off * s.v_t;
+    k = s.k + (((uint64_t)blk * s.k_blk) << 4) + (uint64_t)off * s.k_t;
+    v = s.v + (((uint64_t)blk * s.v_blk) << 4) + (uint64_t)off * s.v_t;
   }
-  MIA_DEV const float *ks(const SpanParams &p, int h) const {
-    return p.k_sc + (int64_t)blk * p.ks_blk + (int64_t)h * p.ks_h + (int64_t)off * p.ks_t;
+  MIA_DEV const float *ks(const Keys &s) const {
+    return s.ks + (uint64_t)blk * s.ks_blk + (uint64_t)off * s.ks_t;
   }
-  MIA_DEV const float *vs(const SpanParams &p, int h) const {
-    return p.v_sc + (int64_t)blk * p.vs_blk + (int64_t)h * p.vs_h + (int64_t)off * p.vs_t;
+  MIA_DEV const float *vs(const Keys &s) const {
+    return s.vs + (uint64_t)blk * s.vs_blk + (uint64_t)off * s.vs_t;
   }
 };
 
@@ -541,8 +569,7 @@ MIA_DEV int64_t piece_slot(const SpanParams &p, const Share &sh, const Pos &c, i
       hd[2] = c.rows;
       hd[3] = c.rt;
       hd[4] = c.h;
-      // the last tile of the segment lies tiles - 1 - t behind the share's last
-      hd[0] = cut_of(sh.cut, sh.x1 - 1 + c.tiles - 1 - c.t) - sh.w + 1;
+      hd[0] = cut_of(sh.cut, c.x + c.tiles - 1 - c.t) - sh.w + 1;
     }
   }
   return ls.part0 + slot * ls.part_rows;
@@ -553,7 +580,7 @@ MIA_DEV int64_t piece_slot(const SpanParams &p, const Share &sh, const Pos &c, i
 // ---------------------------------------------------------------------------
 // Stages of the copy ring (bf16): 64 KB of LDS for either width, so that two
 // workgroups share a CU; the widened tiles of 8-bit caches take two buffers.
-constexpr int tall_stages(int D, int CT) { return CT == kBf16 && D == 64 ? 4 : 2; }
+constexpr int tall_stages(int D, int CT) { return CT == kBf16 && D == 64 ? 3 : 2; }
 
 template <int D, int CT, bool SC>
 struct TallLds {
@@ -622,7 +649,9 @@ MIA_DEV void copy1(const uint8_t *src, uint32_t off, uint32_t lds_dst) {
       : "memory");
 }
 
-template <int D, int CT, bool SC>
+// DU <= D: the products stop there (a head dim of at most DU; channels past
+// the head dim are zero).
+template <int D, int CT, bool SC, int DU>
 MIA_DEV void tall_body(const Share &sh, TallLds<D, CT, SC> &lds) {
   constexpr bool DMA = CT == kBf16;    // else through registers, widened
   constexpr int EB = CT == kBf16 ? 2 : 1;
@@ -634,8 +663,8 @@ MIA_DEV void tall_body(const Share &sh, TallLds<D, CT, SC> &lds) {
   constexpr int ROWB = D * 2;
   constexpr int TILEB = kTallKeys * ROWB;
   constexpr int STAGES = tall_stages(D, CT);
-  constexpr int KSTEPS = D / 16;
-  constexpr int DBLK = D / 32;
+  constexpr int KSTEPS = DU / 16;
+  constexpr int DBLK = DU / 32;
 
   const int tid = threadIdx.x;
   const int wave = readfirstlane(tid >> 6);
@@ -699,11 +728,12 @@ MIA_DEV void tall_body(const Share &sh, TallLds<D, CT, SC> &lds) {
           vr[j] = *reinterpret_cast<const u32x4_t *>(g.v + vo[j]);
         }
         if constexpr (SC) {
-          const SpanParams &p = fresh();
-          const float *ks = g.ks(p, c.h), *vs = g.vs(p, c.h);
-          const int rr = min(k0 + j * RPW + lr, c.len - 1) - g.k16;
-          sr[j] = 0.f;
-          if (lc < 2) sr[j] = lc ? vs[rr * p.vs_t] : ks[rr * p.ks_t];
+          // lanes 0 and 1 of a row: its K and V scale (one load: a second
+          // into the same register would wait for the first)
+          const uint32_t rr = min(k0 + j * RPW + lr, c.len - 1) - g.k16;
+          const float *sp = lc ? g.vs(ks_) : g.ks(ks_);
+          const uint32_t st = lc ? ks_.vs_t : ks_.ks_t;
+          if (lc < 2) sr[j] = sp[(uint64_t)rr * st];
         }
       }
     }
@@ -712,7 +742,7 @@ MIA_DEV void tall_body(const Share &sh, TallLds<D, CT, SC> &lds) {
   // entries of the one behind it
   auto fetch = [&](const Pos &c, int buf, bool anew) {
     if (anew) {
-      ks_.set(fresh(), c);
+      ks_.set<SC>(fresh(), c);
       load_entry(c.t);
       set_offsets(15);
     }
@@ -736,6 +766,8 @@ MIA_DEV void tall_body(const Share &sh, TallLds<D, CT, SC> &lds) {
             widen8<CT>(kr[j][2 * x], kr[j][2 * x + 1]);
         *(lds_u32x4_t *)(vb + row * ROWB + (((2 * lc + x) ^ v_swz<D>(row)) << 4)) =
             widen8<CT>(v[2 * x], v[2 * x + 1]);
+        // converted a chunk at a time: all of them at once spill
+        if constexpr (CT == kI8) __builtin_amdgcn_sched_barrier(0);
       }
       if constexpr (SC) {
         if (lc < 2) scb[(buf * 2 + lc) * kTallKeys + row] = in ? sr[j] : 0.f;
@@ -941,8 +973,8 @@ MIA_DEV void tall_body(const Share &sh, TallLds<D, CT, SC> &lds) {
   };
 
   // ---- the stream
-  if (sh.x0 >= sh.x1) return;
-  Pos cur = first_pos(fresh(), sh);
+  Pos cur;
+  if (!first_pos(fresh(), sh, cur)) return;
   Pos nxt = cur;
   int buf = 0, t0 = cur.t;
   if constexpr (DMA) {
@@ -957,7 +989,7 @@ MIA_DEV void tall_body(const Share &sh, TallLds<D, CT, SC> &lds) {
     auto copy_next = [&](int stage) {
       if (!more) return;
       fetch(nxt, stage, anew);
-      more = nxt.left > 1;
+      more = has_next(nxt, sh.x1);
       if (more) {
         advance(fresh(), nxt);
         anew = nxt.t == 0;
@@ -971,7 +1003,7 @@ MIA_DEV void tall_body(const Share &sh, TallLds<D, CT, SC> &lds) {
       // behind it may stay in flight; a narrow call's count of copies varies,
       // so it waits for all); the barrier makes every thread's visible and
       // the stage of the tile before free
-      if (STAGES > 2 && d_used == D && cur.left > STAGES - 2)
+      if (STAGES > 2 && d_used == D && more)
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((STAGES - 2) * 2 * NP) : "memory");
       else
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
@@ -988,14 +1020,16 @@ MIA_DEV void tall_body(const Share &sh, TallLds<D, CT, SC> &lds) {
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
       }
-      if (live) compute(cur, buf);
-      const bool last = cur.left == 1;
+      const bool last = !has_next(cur, sh.x1);
       const bool ends = last || cur.t + 1 == cur.tiles;
-      if (ends) end_piece(cur, t0);
+      const Pos at = cur;
+      const bool at_live = live;
+      if (!last) advance(fresh(), cur);
+      if (ends && !last) load_q(cur);  // (sets live for the next piece)
+      if (at_live) compute(at, buf);
+      if (ends) end_piece(at, t0);
       if (last) return;
-      advance(fresh(), cur);
       if (ends) {
-        load_q(cur);
         begin_piece(cur);
         t0 = 0;
       }
@@ -1006,24 +1040,25 @@ MIA_DEV void tall_body(const Share &sh, TallLds<D, CT, SC> &lds) {
     fetch(cur, 0, true);
     begin_piece(cur);
     store_tile(cur, 0);
-    bool more = cur.left > 1;
+    bool more = has_next(cur, sh.x1);
     if (more) {
       advance(fresh(), nxt);
       fetch(nxt, 0, nxt.t == 0);
     }
     __syncthreads();
     while (true) {
+      const bool ends = !more || nxt.t == 0;
       if (live) compute(cur, buf);
-      if (!more || nxt.t == 0) {
+      if (ends) {
         end_piece(cur, t0);
         if (!more) return;
-        load_q(nxt);
+        load_q(nxt);  // (ahead of the products its registers would spill others)
         begin_piece(nxt);
         t0 = 0;
       }
       store_tile(nxt, buf ^ 1);
       cur = nxt;
-      more = cur.left > 1;
+      more = has_next(cur, sh.x1);
       if (more) {
         advance(fresh(), nxt);
         fetch(nxt, 0, nxt.t == 0);
@@ -1044,10 +1079,11 @@ struct ThinLds {
 };
 
 // NC groups of 16 columns (rows of the segment).
-template <int D, int CT, bool SC, int NC>
+template <int D, int CT, bool SC, int DU, int NC>
 MIA_DEV void thin_body(const Share &sh, ThinLds<D, SC> &lds) {
   constexpr int EB = CT == kBf16 ? 2 : 1;
-  constexpr int KSTEPS = D / 32;
+  // (8-bit k-steps come in pairs: all of D)
+  constexpr int KSTEPS = (CT == kBf16 ? DU : D) / 32;
   constexpr int VE = 16 / EB;          // V elements per 16-byte load
   constexpr int DS = D / VE;           // lanes per V row
   constexpr int TL = 64 / DS;          // V rows per load
@@ -1058,7 +1094,7 @@ MIA_DEV void thin_body(const Share &sh, ThinLds<D, SC> &lds) {
   constexpr int NK = CT == kBf16 ? KSTEPS : KSTEPS / 2;  // K loads per 16 keys
   constexpr int ROWB = D * 2;
   constexpr int VNCH = D / 8;
-  constexpr int DB16 = D / 16;
+  constexpr int DB16 = DU / 16;
 
   const int wave = readfirstlane((int)threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
@@ -1084,7 +1120,7 @@ MIA_DEV void thin_body(const Share &sh, ThinLds<D, SC> &lds) {
   // segment), and the entries of the one behind it
   auto locate = [&](const Pos &c, bool anew) {
     if (anew) {
-      ks_.set(fresh(), c);
+      ks_.set<SC>(fresh(), c);
       load_entries(c.t);
     }
     g[0].set(ks_, c.t * kThinKeys, ent[0]);
@@ -1123,14 +1159,13 @@ MIA_DEV void thin_body(const Share &sh, ThinLds<D, SC> &lds) {
   // lane l: scale of key l (K), of key l - 32 (V)
   auto load_s = [&](const Pos &c) {
     if constexpr (SC) {
-      const SpanParams &p = fresh();
       const int k = lane & 31;
       const bool hi = k >= 16;
-      const int rr = min(c.t * kThinKeys + k, ks_.len - 1) - (hi ? g[1].k16 : g[0].k16);
-      const float *ks = hi ? g[1].ks(p, c.h) : g[0].ks(p, c.h);
-      const float *vs = hi ? g[1].vs(p, c.h) : g[0].vs(p, c.h);
-      sr = lane < 32 ? ks[rr * p.ks_t] : vs[rr * p.vs_t];
-      if (c.t * kThinKeys + k >= ks_.len) sr = 0.f;
+      const uint32_t rr = min(c.t * kThinKeys + k, ks_.len - 1) - (hi ? g[1].k16 : g[0].k16);
+      const float *ks = hi ? g[1].ks(ks_) : g[0].ks(ks_);
+      const float *vs = hi ? g[1].vs(ks_) : g[0].vs(ks_);
+      const float *sp = lane < 32 ? ks : vs;
+      sr = sp[(uint64_t)rr * (lane < 32 ? ks_.ks_t : ks_.vs_t)];
     }
   };
 
@@ -1196,6 +1231,7 @@ MIA_DEV void thin_body(const Share &sh, ThinLds<D, SC> &lds) {
         for (int n = 0; n < NC; ++n)
           s[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, w),
                                                             qf[n][ks], s[n][b], 0, 0, 0);
+        if constexpr (CT == kI8) __builtin_amdgcn_sched_barrier(0);
       }
     }
   };
@@ -1213,6 +1249,7 @@ MIA_DEV void thin_body(const Share &sh, ThinLds<D, SC> &lds) {
         for (int x = 0; x < 2; ++x)
           *(lds_u32x4_t *)(vw + t * ROWB + (((2 * vds + x) ^ (t & (VNCH - 1))) << 4)) =
               widen8<CT>(v[2 * x], v[2 * x + 1]);
+        if constexpr (CT == kI8) __builtin_amdgcn_sched_barrier(0);
       }
     }
   };
@@ -1323,8 +1360,8 @@ MIA_DEV void thin_body(const Share &sh, ThinLds<D, SC> &lds) {
 
   // ---- the stream: K (V) of the next tile is issued once this tile's
   // product (copy to LDS) has freed the registers
-  if (sh.x0 >= sh.x1) return;
-  Pos cur = first_pos(fresh(), sh);
+  Pos cur;
+  if (!first_pos(fresh(), sh, cur)) return;
   load_q(cur);
   locate(cur, true);
   load_k(cur);
@@ -1333,14 +1370,15 @@ MIA_DEV void thin_body(const Share &sh, ThinLds<D, SC> &lds) {
   begin_piece(cur);
   int t0 = cur.t;
   while (true) {
-    const bool more = cur.left > 1;
+    const bool more = has_next(cur, sh.x1);
     Pos nxt = cur;
     if (more) {
       advance(fresh(), nxt);
+      if (NC == 1 && nxt.t == 0) load_q(nxt);
       locate(nxt, nxt.t == 0);
     }
     scores();
-    if constexpr (SC) sw[lane] = sr;
+    if constexpr (SC) sw[lane] = cur.t * kThinKeys + (lane & 31) < cur.len ? sr : 0.f;
     if (more) {
       load_k(nxt);
       load_s(nxt);
@@ -1352,7 +1390,7 @@ MIA_DEV void thin_body(const Share &sh, ThinLds<D, SC> &lds) {
     if (!more || nxt.t == 0) {
       end_piece(cur, t0);
       if (!more) return;
-      load_q(nxt);
+      if (NC > 1) load_q(nxt);  // (ahead of the products it would spill)
       begin_piece(nxt);
       t0 = 0;
     }
@@ -1360,9 +1398,9 @@ MIA_DEV void thin_body(const Share &sh, ThinLds<D, SC> &lds) {
   }
 }
 
-template <int D, int CT, bool SC, int NC>
-__global__ __launch_bounds__(kThreads, 2) void span_kernel(SpanParams p) {
-  static_assert(D == 64 || D == 128, "tile widths");
+template <int D, int CT, bool SC, int DU, int NC>
+__global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void span_kernel(SpanParams p) {
+  static_assert((D == 64 && DU == 64) || (D == 128 && (DU == 96 || DU == 128)), "tile widths");
   static_assert(CT != kBf16 || !SC, "bf16 caches have no per-key scales");
   __shared__ union __attribute__((aligned(1024))) {
     TallLds<D, CT, SC> tall;
@@ -1371,8 +1409,8 @@ __global__ __launch_bounds__(kThreads, 2) void span_kernel(SpanParams p) {
   __shared__ PlanLds plan_lds;
   Share sh;
   const int form = plan(fresh(), plan_lds, sh);
-  if (form == 0) tall_body<D, CT, SC>(sh, lds.tall);
-  else if (form == 1) thin_body<D, CT, SC, NC>(sh, lds.thin);
+  if (form == 0) tall_body<D, CT, SC, DU>(sh, lds.tall);
+  else if (form == 1) thin_body<D, CT, SC, DU, NC>(sh, lds.thin);
 }
 
 // A row is joined by GR groups of D / 4 lanes, four channels a lane.
@@ -1489,7 +1527,8 @@ __global__ __launch_bounds__(256) void span_join_kernel(SpanParams p, FastDiv hq
     const int rt_n = row_tiles(l, rows), rt = l.thin ? 0 : r / kRows;
     const int in = h * rt_n + rt;  // segment of the sequence
     const Cut cut = {p.hdr[2 * l.thin], p.hdr[2 * l.thin + 1]};
-    const int x = p.hdr[kHdr + (li ? p.list[0].n + i : i)] + in * tiles;
+    const int over = p.over[l.thin];
+    const int x = p.hdr[kHdr + (li ? p.list[0].n + i : i)] + in * (tiles + over) + over;
     first = 0;
     if (tiles == 0) return 0;
     const int w = cut_of(cut, x);
@@ -1503,61 +1542,84 @@ __global__ __launch_bounds__(256) void span_join_kernel(SpanParams p, FastDiv hq
   auto prow = [&](int j) {
     return j < n0 ? f0 + (int64_t)j * l0.part_rows : f1 + (int64_t)(j - n0) * l1.part_rows;
   };
+  const int gr = threadIdx.x / LPR % GR;
+  // the keys between the span that all rows see and row s's own last key:
+  // group g takes common + g, ..., the first of them loaded ahead of the pieces
+  struct Late {
+    u32x2_t k, v;
+    float ks, vs;
+  };
+  const bool c_ok = c * 4 < p.d;
+  auto load_late = [&](int k) {
+    const int bj = (int)fdiv((uint32_t)k, p.bs_div);
+    const uint32_t blk =
+        min(max(scalar_load(l1.bt, (int64_t)b * l1.bt_s + (int64_t)bj * l1.bt_j), 0), p.nb - 1);
+    const uint32_t off = k - bj * p.bs;
+    const uint8_t *ka =
+        p.k_cache + (((uint64_t)blk * p.kc_blk16) << 4) + (int64_t)h * p.kc_h + off * p.kc_t;
+    const uint8_t *va =
+        p.v_cache + (((uint64_t)blk * p.vc_blk16) << 4) + (int64_t)h * p.vc_h + off * p.vc_t;
+    Late x = {u32x2_t{0u, 0u}, u32x2_t{0u, 0u}, 1.f, 1.f};
+    if (c_ok) {
+      if constexpr (CT == kBf16) {
+        x.k = *reinterpret_cast<const u32x2_t *>(ka + c * 8);
+        x.v = *reinterpret_cast<const u32x2_t *>(va + c * 8);
+      } else {
+        x.k[0] = *reinterpret_cast<const uint32_t *>(ka + c * 4);
+        x.v[0] = *reinterpret_cast<const uint32_t *>(va + c * 4);
+      }
+    }
+    if constexpr (SC) {
+      x.ks = p.k_sc[(uint64_t)blk * p.ks_blk + h * p.ks_h + (uint64_t)off * p.ks_t];
+      x.vs = p.v_sc[(uint64_t)blk * p.vs_blk + h * p.vs_h + (uint64_t)off * p.vs_t];
+    }
+    return x;
+  };
+  auto four = [&](u32x2_t w, float (&x)[4]) {
+    if constexpr (CT == kBf16) {
+      x[0] = bf16lo(w[0]), x[1] = bf16hi(w[0]), x[2] = bf16lo(w[1]), x[3] = bf16hi(w[1]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t byte = (w[0] >> (8 * i)) & 0xffu;
+        x[i] = CT == kI8 ? (float)(int8_t)byte : e4m3fn_bits_to_f32(byte);
+      }
+    }
+  };
+  int late0 = 0, late1 = 0;
+  u32x2_t qw = {0u, 0u};
+  Late late;
+  if (s > 0) {
+    late0 = list_len(l1, b) + gr;
+    late1 = min(scalar_load(l1.len, b) - l1.len_sub + s, l1.len_cap);
+    if (late0 < late1) {
+      late = load_late(late0);
+      if (c_ok)
+        qw = *reinterpret_cast<const u32x2_t *>(p.q + (int64_t)b * p.qs_b + (int64_t)s * p.qs_s +
+                                                (int64_t)hq * p.qs_h + c * 4);
+    }
+  }
   float m = -INFINITY, ls = 0.f;
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-  const int gr = threadIdx.x / LPR % GR;
   if (p.sink && gr == 0) {
     m = p.sink[hq] * kLog2e;
     ls = 1.f;
   }
   sum_pieces<D, GR>(p, n0 + n1, prow, m, ls, o);
-  // the keys between the span that all rows see and row s's own last key
-  if (s > 0) {
-    const int common = list_len(l1, b);
-    const int end = min(l1.len[b] - l1.len_sub + s, l1.len_cap);
-    if (common < end) {
-      float qv[4] = {0.f, 0.f, 0.f, 0.f};
-      const bool c_ok = c * 4 < p.d;
-      if (c_ok) {
-        const uint16_t *qp = p.q + (int64_t)b * p.qs_b + (int64_t)s * p.qs_s + (int64_t)hq * p.qs_h;
-        const u32x2_t w = *reinterpret_cast<const u32x2_t *>(qp + c * 4);
-        qv[0] = bf16lo(w[0]), qv[1] = bf16hi(w[0]), qv[2] = bf16lo(w[1]), qv[3] = bf16hi(w[1]);
-      }
-      float c1 = p.scale_log2;
-      if (p.k_deq) c1 *= p.k_deq[h];
-      auto load4 = [&](const uint8_t *a, float (&x)[4]) {
-        if constexpr (CT == kBf16) {
-          const u32x2_t w = *reinterpret_cast<const u32x2_t *>(a + c * 8);
-          x[0] = bf16lo(w[0]), x[1] = bf16hi(w[0]), x[2] = bf16lo(w[1]), x[3] = bf16hi(w[1]);
-        } else {
-          const uint32_t w = *reinterpret_cast<const uint32_t *>(a + c * 4);
+  if (late0 < late1) {
+    float c1 = p.scale_log2;
+    if (p.k_deq) c1 *= p.k_deq[h];
+    const float qv[4] = {bf16lo(qw[0]), bf16hi(qw[0]), bf16lo(qw[1]), bf16hi(qw[1])};
+    for (int k = late0; k < late1; k += GR) {
+      if (k > late0) late = load_late(k);
+      float x[4], v[4];
+      four(late.k, x);
+      four(late.v, v);
+      float dot = qv[0] * x[0] + qv[1] * x[1] + qv[2] * x[2] + qv[3] * x[3];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t byte = (w >> (8 * i)) & 0xffu;
-            x[i] = CT == kI8 ? (float)(int8_t)byte : e4m3fn_bits_to_f32(byte);
-          }
-        }
-      };
-      for (int k = common + gr; k < end; k += GR) {
-        const int bj = (int)fdiv((uint32_t)k, p.bs_div);
-        const int blk = min(max(l1.bt[(int64_t)b * l1.bt_s + (int64_t)bj * l1.bt_j], 0), p.nb - 1);
-        const int off = k - bj * p.bs;
-        float x[4] = {0.f, 0.f, 0.f, 0.f}, v[4] = {0.f, 0.f, 0.f, 0.f};
-        if (c_ok) {
-          load4(p.k_cache + (int64_t)blk * p.kc_blk + (int64_t)h * p.kc_h + (int64_t)off * p.kc_t, x);
-          load4(p.v_cache + (int64_t)blk * p.vc_blk + (int64_t)h * p.vc_h + (int64_t)off * p.vc_t, v);
-        }
-        float dot = qv[0] * x[0] + qv[1] * x[1] + qv[2] * x[2] + qv[3] * x[3];
-#pragma unroll
-        for (int q = 1; q < LPR; q <<= 1) dot += __shfl_xor(dot, q, 64);
-        float vs = 1.f;
-        if constexpr (SC) {
-          dot *= p.k_sc[(int64_t)blk * p.ks_blk + (int64_t)h * p.ks_h + (int64_t)off * p.ks_t];
-          vs = p.v_sc[(int64_t)blk * p.vs_blk + (int64_t)h * p.vs_h + (int64_t)off * p.vs_t];
-        }
-        const float sc = dot * c1;
-        add_piece(m, ls, o, sc, 1.f, f32x4_t{v[0] * vs, v[1] * vs, v[2] * vs, v[3] * vs});
-      }
+      for (int q = 1; q < LPR; q <<= 1) dot += __shfl_xor(dot, q, 64);
+      add_piece(m, ls, o, dot * late.ks * c1, 1.f,
+                f32x4_t{v[0] * late.vs, v[1] * late.vs, v[2] * late.vs, v[3] * late.vs});
     }
   }
   sum_groups<D, GR>(lds, m, ls, o);
@@ -1597,7 +1659,7 @@ struct Layout {
 // Launch size and workspace of a call; fills the lists' forms and partials.
 Layout span_layout(SpanParams &p, int D) {
   Layout w;
-  w.grid = 2 * cu_count();
+  w.grid = (D == 64 ? 3 : 2) * cu_count();
   int64_t rows = 0, hdr = kHdr;
   for (int li = 0; li < 2; ++li) {
     SpanList &l = p.list[li];
@@ -1620,7 +1682,8 @@ Layout span_layout(SpanParams &p, int D) {
     }
   }
   p.cost[0] = 1.0f, p.cost[1] = D == 64 ? 0.28f : 0.41f;
-  p.least[0] = 1, p.least[1] = 1;
+  p.over[0] = 2, p.over[1] = 2;
+  p.least[0] = 4, p.least[1] = 4;
   w.hdr = 0;
   w.ml = (size_t)up(hdr * 4, 256);
   w.o = w.ml + (size_t)up(rows * 8, 256);
@@ -1639,13 +1702,14 @@ void set_cache(SpanParams &p, const A &a) {
   const int eb = a.cache_dtype == MIA_DTYPE_BF16 ? 2 : 1;
   p.k_cache = (const uint8_t *)a.k_cache;
   p.v_cache = (const uint8_t *)a.v_cache;
-  p.kc_blk = a.k_cache_stride[0] * eb, p.kc_h = a.k_cache_stride[1] * eb,
-  p.kc_t = a.k_cache_stride[2] * eb;
-  p.vc_blk = a.v_cache_stride[0] * eb, p.vc_h = a.v_cache_stride[1] * eb,
-  p.vc_t = a.v_cache_stride[2] * eb;
+  p.kc_blk16 = (uint32_t)(a.k_cache_stride[0] * eb / 16);
+  p.vc_blk16 = (uint32_t)(a.v_cache_stride[0] * eb / 16);
+  p.kc_h = a.k_cache_stride[1] * eb, p.kc_t = a.k_cache_stride[2] * eb;
+  p.vc_h = a.v_cache_stride[1] * eb, p.vc_t = a.v_cache_stride[2] * eb;
   p.k_sc = a.k_scales, p.v_sc = a.v_scales;
-  p.ks_blk = a.k_scale_stride[0], p.ks_h = a.k_scale_stride[1], p.ks_t = a.k_scale_stride[2];
-  p.vs_blk = a.v_scale_stride[0], p.vs_h = a.v_scale_stride[1], p.vs_t = a.v_scale_stride[2];
+  p.ks_blk = (uint32_t)a.k_scale_stride[0], p.ks_t = (uint32_t)a.k_scale_stride[2];
+  p.vs_blk = (uint32_t)a.v_scale_stride[0], p.vs_t = (uint32_t)a.v_scale_stride[2];
+  p.ks_h = a.k_scale_stride[1], p.vs_h = a.v_scale_stride[1];
   p.k_deq = a.k_dequant, p.v_deq = a.v_dequant;
   p.nb = a.num_blocks, p.bs = a.block_size;
   p.bs_div = make_fastdiv(a.block_size);
@@ -1701,8 +1765,15 @@ template <int D, int CT, bool SC>
 void launch_span(const SpanParams &p, int grid, hipStream_t s) {
   const int cols = std::max(p.list[0].thin && p.list[0].n ? p.list[0].part_rows : 0,
                             p.list[1].thin ? p.list[1].part_rows : 0);
-  if (cols <= 16) span_kernel<D, CT, SC, 1><<<grid, kThreads, 0, s>>>(p);
-  else span_kernel<D, CT, SC, 2><<<grid, kThreads, 0, s>>>(p);
+  // head dims of 65 to 96 leave a quarter of the 128-wide products out
+  constexpr int DN = D == 128 ? 96 : D;
+  if (D == 128 && p.d <= DN) {
+    if (cols <= 16) span_kernel<D, CT, SC, DN, 1><<<grid, kThreads, 0, s>>>(p);
+    else span_kernel<D, CT, SC, DN, 2><<<grid, kThreads, 0, s>>>(p);
+  } else {
+    if (cols <= 16) span_kernel<D, CT, SC, D, 1><<<grid, kThreads, 0, s>>>(p);
+    else span_kernel<D, CT, SC, D, 2><<<grid, kThreads, 0, s>>>(p);
+  }
   if (p.join) {
     // lane groups per row by the pieces to expect: those of the prefix (its
     // share of the workgroups over its segments) and one or two of the row

@@ -1009,46 +1009,42 @@ def skinny_linear(x: torch.Tensor, w: torch.Tensor, norm: bool = False,
 # ---------------------------------------------------------------------------
 # quantised cache: write and read back
 # ---------------------------------------------------------------------------
-def _quant_pool(k_cache, v_cache, k_scales, v_scales):
-    """(num_blocks, Hkv, block_size, d) of a quantised cache, checked."""
-    if k_cache.dim() != 4:
-        raise ValueError(f"quantised cache must be [nb, Hkv, bs, d], got {tuple(k_cache.shape)}")
-    if v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype:
-        raise ValueError("K and V caches have different geometry or dtypes")
-    if k_scales.shape != k_cache.shape[:3] or v_scales.shape != k_cache.shape[:3]:
-        raise ValueError(
-            f"scales must be [nb, Hkv, bs] = {tuple(k_cache.shape[:3])}, got "
-            f"{tuple(k_scales.shape)} / {tuple(v_scales.shape)}")
+def _check_scales(shape, k_scales, v_scales) -> None:
+    """Scales of a quantised cache [nb, Hkv, bs, d]."""
+    if k_scales.shape != shape[:3] or v_scales.shape != shape[:3]:
+        raise ValueError(f"scales must be [nb, Hkv, bs] = {tuple(shape[:3])}, got "
+                         f"{tuple(k_scales.shape)} / {tuple(v_scales.shape)}")
     if k_scales.dtype != torch.float32 or v_scales.dtype != torch.float32:
         raise ValueError("scales must be float32")
-    return k_cache.shape
 
 
 def _quant_kv(fn, what, k, v, slots, k_cache, v_cache, k_scales, v_scales) -> None:
-    dev = N.require_gpu(k, v, slots, k_cache, v_cache, k_scales, v_scales)
-    nb, hkv, bs, d = _quant_pool(k_cache, v_cache, k_scales, v_scales)
-    if k.dim() != 3 or k.shape[1:] != (hkv, d) or v.shape != k.shape:
-        raise ValueError(f"K/V rows must be [T, {hkv}, {d}], got {tuple(k.shape)} / "
+    dev = N.same_gpu(k, v, slots, k_cache, v_cache, k_scales, v_scales)
+    shape = k_cache.shape
+    if len(shape) != 4:
+        raise ValueError(f"quantised cache must be [nb, Hkv, bs, d], got {tuple(shape)}")
+    if v_cache.shape != shape or v_cache.dtype != k_cache.dtype:
+        raise ValueError("K and V caches have different geometry or dtypes")
+    _check_scales(shape, k_scales, v_scales)
+    nb, hkv, bs, d = shape
+    rows = k.shape
+    if len(rows) != 3 or rows[1] != hkv or rows[2] != d or v.shape != rows:
+        raise ValueError(f"K/V rows must be [T, {hkv}, {d}], got {tuple(rows)} / "
                          f"{tuple(v.shape)}")
     if v.dtype != k.dtype:
         raise ValueError("K and V rows have different dtypes")
-    if slots.dim() != 1 or slots.shape[0] != k.shape[0]:
-        raise ValueError(f"slots must be [T] = [{k.shape[0]}], got {tuple(slots.shape)}")
+    T = rows[0]
+    if slots.dim() != 1 or slots.shape[0] != T:
+        raise ValueError(f"slots must be [T] = [{T}], got {tuple(slots.shape)}")
     if not slots.is_contiguous():
         slots = slots.contiguous()
     a = N.QuantKvArgs()
-    a.k, a.v = k.data_ptr(), v.data_ptr()
-    a.row_dtype = N.mia_dtype(k.dtype)
-    a.code_dtype = N.mia_dtype(k_cache.dtype)
-    a.k_stride, a.v_stride = k.stride(), v.stride()
-    a.slots = slots.data_ptr()
-    a.slot_dtype = N.mia_dtype(slots.dtype)
-    a.num_tokens = k.shape[0]
-    a.k_cache, a.v_cache = k_cache.data_ptr(), v_cache.data_ptr()
-    a.k_cache_stride, a.v_cache_stride = k_cache.stride(), v_cache.stride()
-    a.k_scales, a.v_scales = k_scales.data_ptr(), v_scales.data_ptr()
-    a.k_scale_stride, a.v_scale_stride = k_scales.stride(), v_scales.stride()
-    a.num_blocks, a.block_size, a.num_kv_heads, a.head_dim = nb, bs, hkv, d
+    N.PACK_QUANT.pack_into(
+        a, 0, k.data_ptr(), v.data_ptr(), N.mia_dtype(k.dtype), N.mia_dtype(k_cache.dtype),
+        *k.stride(), *v.stride(), slots.data_ptr(), N.mia_dtype(slots.dtype), 0, T,
+        k_cache.data_ptr(), v_cache.data_ptr(), *k_cache.stride(), *v_cache.stride(),
+        k_scales.data_ptr(), v_scales.data_ptr(), *k_scales.stride(), *v_scales.stride(),
+        nb, bs, hkv, d)
     with N.on_device(dev):
         N.check(fn(ctypes.byref(a), N.stream_ptr(dev)), what)
 
@@ -1062,11 +1058,12 @@ def quant_kv_write(k, v, slots, k_cache, v_cache, k_scales, v_scales) -> None:
 
 def quant_kv_read(k_cache, v_cache, k_scales, v_scales, slots, dtype=torch.bfloat16):
     """Rows ``slots [T]`` of a quantised cache as ``(k, v) [T, Hkv, d]``."""
-    if k_cache.dim() != 4 or slots.dim() != 1:
+    shape = k_cache.shape
+    if len(shape) != 4 or slots.dim() != 1:
         raise ValueError("quant_kv_read: the cache must be [nb, Hkv, bs, d] and slots [T]")
-    shape = (slots.shape[0], k_cache.shape[1], k_cache.shape[3])
-    k = torch.empty(shape, dtype=dtype, device=k_cache.device)
-    v = torch.empty(shape, dtype=dtype, device=k_cache.device)
+    rows = (slots.shape[0], shape[1], shape[3])
+    k = torch.empty(rows, dtype=dtype, device=k_cache.device)
+    v = torch.empty(rows, dtype=dtype, device=k_cache.device)
     _quant_kv(N.lib().mia_quant_kv_read, "quant_kv_read", k, v, slots, k_cache, v_cache,
               k_scales, v_scales)
     return k, v
@@ -1075,47 +1072,53 @@ def quant_kv_read(k_cache, v_cache, k_scales, v_scales, slots, dtype=torch.bfloa
 # ---------------------------------------------------------------------------
 # attention over key spans of another length
 # ---------------------------------------------------------------------------
-def _span_cache(a, q, k_cache, v_cache, k_scales, v_scales, k_dequant, v_dequant, dev):
-    """Cache fields shared by the cross and shared-prefix arguments; returns
-    what must stay alive until the launch."""
-    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype:
+_NO_STRIDES = (0, 0, 0)
+
+
+def _span_cache(q, k_cache, v_cache, k_scales, v_scales, k_dequant, v_dequant, dev):
+    """Checks what the cross and shared-prefix calls share; returns the cache's
+    shape, q heads, dtype code, scale pointers and strides, and the dequant
+    factors (to be kept alive until the launch)."""
+    shape = k_cache.shape
+    if len(shape) != 4 or v_cache.shape != shape or v_cache.dtype != k_cache.dtype:
         raise ValueError(f"K and V caches must be [nb, Hkv, bs, d] of one dtype, got "
-                         f"{tuple(k_cache.shape)} / {tuple(v_cache.shape)}")
-    nb, hkv, bs, d = k_cache.shape
-    hq = q.shape[-2]
+                         f"{tuple(shape)} / {tuple(v_cache.shape)}")
+    hq, d = q.shape[-2:]
     if q.dtype != torch.bfloat16:
         raise NotImplementedError("q must be bf16")
-    if q.shape[-1] != d:
-        raise ValueError(f"head_dim mismatch: q {q.shape[-1]}, cache {d}")
+    if d != shape[3]:
+        raise ValueError(f"head_dim mismatch: q {d}, cache {shape[3]}")
+    hkv = shape[1]
     if hkv == 0 or hq % hkv:
         raise ValueError("GQA requires q_heads divisible by kv_heads")
     if (k_scales is None) != (v_scales is None) or (k_dequant is None) != (v_dequant is None):
         raise ValueError("the scales of K and V go together")
+    scales = (0, 0, *_NO_STRIDES, *_NO_STRIDES)
     if k_scales is not None:
         if k_dequant is not None:
             raise ValueError("per-token scales and per-head dequant scales exclude each other")
-        _quant_pool(k_cache, v_cache, k_scales, v_scales)
-        a.k_scales, a.v_scales = k_scales.data_ptr(), v_scales.data_ptr()
-        a.k_scale_stride, a.v_scale_stride = k_scales.stride(), v_scales.stride()
-    if k_dequant is not None and k_cache.dtype != torch.float8_e4m3fn:
-        raise ValueError("per-head dequant scales belong to an fp8 cache")
-    kd = _scale_f32(k_dequant, dev, hkv, "k_dequant_scale")
-    vd = _scale_f32(v_dequant, dev, hkv, "v_dequant_scale")
-    a.k_dequant, a.v_dequant = N.ptr(kd), N.ptr(vd)
-    a.k_cache, a.v_cache = k_cache.data_ptr(), v_cache.data_ptr()
-    a.cache_dtype = N.mia_dtype(k_cache.dtype)
-    a.k_cache_stride, a.v_cache_stride = k_cache.stride(), v_cache.stride()
-    a.num_blocks, a.block_size = nb, bs
-    a.num_q_heads, a.num_kv_heads, a.head_dim = hq, hkv, d
-    a.q, a.q_stride = q.data_ptr(), q.stride()
-    return kd, vd
+        _check_scales(shape, k_scales, v_scales)
+        scales = (k_scales.data_ptr(), v_scales.data_ptr(), *k_scales.stride(),
+                  *v_scales.stride())
+    kd = vd = None
+    if k_dequant is not None:
+        if k_cache.dtype != torch.float8_e4m3fn:
+            raise ValueError("per-head dequant scales belong to an fp8 cache")
+        kd = _scale_f32(k_dequant, dev, hkv, "k_dequant_scale")
+        vd = _scale_f32(v_dequant, dev, hkv, "v_dequant_scale")
+    return shape, hq, N.mia_dtype(k_cache.dtype), scales, kd, vd
 
 
-def _int32(t, shape, what):
-    if t.dtype != torch.int32 or tuple(t.shape) != shape:
-        raise ValueError(f"{what} must be an int32 tensor of shape {shape}, got {t.dtype} "
+def _int32(t, n, what):
+    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n:
+        raise ValueError(f"{what} must be an int32 tensor of {n} entries, got {t.dtype} "
                          f"{tuple(t.shape)}")
     return t if t.is_contiguous() else t.contiguous()
+
+
+def _check_out(out, q) -> None:
+    if out.shape != q.shape or out.dtype != torch.bfloat16:
+        raise ValueError(f"out must be a bf16 tensor of shape {tuple(q.shape)}")
 
 
 def _span_launch(a, query, launch, what, workspace, dev) -> None:
@@ -1126,7 +1129,7 @@ def _span_launch(a, query, launch, what, workspace, dev) -> None:
             if workspace is None or workspace.numel() * workspace.element_size() < need:
                 workspace = torch.empty(need, dtype=torch.uint8, device=dev)
             a.workspace = workspace.data_ptr()
-            a.workspace_bytes = workspace.numel() * workspace.element_size()
+            a.workspace_bytes = need
         # without a workspace the arguments were refused (the launch says
         # why) or there is nothing to compute
         N.check(launch(ctypes.byref(a), N.stream_ptr(dev)), what)
@@ -1136,42 +1139,40 @@ def cross_attention(q, k_cache, v_cache, key_lens, out, *, softmax_scale, block_
                     cu_seqlens_q=None, max_seqlen_q=0, k_scales=None, v_scales=None,
                     k_dequant=None, v_dequant=None, workspace=None) -> None:
     """Attention of ``q [T, Hq, d]`` over ragged keys into ``out``."""
-    dev = N.require_gpu(q, k_cache, v_cache, key_lens, out, block_table, cu_seqlens_q, k_scales,
-                        v_scales, k_dequant, v_dequant, workspace)
+    dev = N.same_gpu(q, k_cache, v_cache, key_lens, out, block_table, cu_seqlens_q, k_scales,
+                     v_scales, k_dequant, v_dequant, workspace)
     if q.dim() != 3:
         raise ValueError(f"q must be [T, Hq, d], got {tuple(q.shape)}")
-    if out.shape != q.shape or out.dtype != torch.bfloat16:
-        raise ValueError(f"out must be a bf16 tensor of shape {tuple(q.shape)}")
+    _check_out(out, q)
     if key_lens.dim() != 1:
         raise ValueError("the key lengths must be one int32 per sequence")
-    n = key_lens.shape[0]
-    key_lens = _int32(key_lens, (n,), "the key lengths")
-    a = N.CrossArgs()
-    alive = _span_cache(a, q, k_cache, v_cache, k_scales, v_scales, k_dequant, v_dequant, dev)
-    a.num_tokens, a.num_seqs = q.shape[0], n
+    T, n = q.shape[0], key_lens.shape[0]
+    key_lens = _int32(key_lens, n, "the key lengths")
+    (nb, hkv, bs, d), hq, code, scales, kd, vd = _span_cache(
+        q, k_cache, v_cache, k_scales, v_scales, k_dequant, v_dequant, dev)
+    cu = 0
     if cu_seqlens_q is not None:
-        cu_seqlens_q = _int32(cu_seqlens_q, (n + 1,), "cu_seqlens_q")
-        a.cu_seqlens_q = cu_seqlens_q.data_ptr()
-        a.max_seqlen_q = max_seqlen_q
-    elif q.shape[0] < n:
-        raise ValueError(f"q holds {q.shape[0]} tokens for {n} sequences of one token")
+        cu_seqlens_q = _int32(cu_seqlens_q, n + 1, "cu_seqlens_q")
+        cu = cu_seqlens_q.data_ptr()
+    elif T < n:
+        raise ValueError(f"q holds {T} tokens for {n} sequences of one token")
+    table, bts, nblk = 0, (0, 0), 1
     if block_table is not None:
         if block_table.dim() != 2 or block_table.shape[0] != n or block_table.dtype != torch.int32:
             raise ValueError(f"block table must be int32 [{n}, blocks], got {block_table.dtype} "
                              f"{tuple(block_table.shape)}")
-        a.block_table, a.bt_stride = block_table.data_ptr(), block_table.stride()
-        a.blocks_per_seq = block_table.shape[1]
-    else:
-        if k_cache.shape[0] < n:
-            raise ValueError(f"dense keys of {k_cache.shape[0]} sequences for {n}")
-        a.blocks_per_seq = 1
-    a.key_lens = key_lens.data_ptr()
-    a.softmax_scale = softmax_scale
-    a.out, a.out_stride = out.data_ptr(), out.stride()
+        table, bts, nblk = block_table.data_ptr(), block_table.stride(), block_table.shape[1]
+    elif nb < n:
+        raise ValueError(f"dense keys of {nb} sequences for {n}")
+    a = N.CrossArgs()
+    N.PACK_CROSS.pack_into(
+        a, 0, q.data_ptr(), *q.stride(), out.data_ptr(), *out.stride(), T, n, cu, max_seqlen_q,
+        hq, hkv, d, k_cache.data_ptr(), v_cache.data_ptr(), code, nb, *k_cache.stride(),
+        *v_cache.stride(), bs, nblk, table, *bts, key_lens.data_ptr(), *scales, N.ptr(kd) or 0,
+        N.ptr(vd) or 0, softmax_scale, 0, 0, 0)
     L = N.lib()
     _span_launch(a, L.mia_cross_workspace_bytes, L.mia_cross_attention, "cross_attention",
                  workspace, dev)
-    del alive
 
 
 def shared_prefix_attention(q, k_cache, v_cache, prefix_table, prefix_len, block_table, seq_lens,
@@ -1179,13 +1180,12 @@ def shared_prefix_attention(q, k_cache, v_cache, prefix_table, prefix_len, block
                             k_dequant=None, v_dequant=None, workspace=None) -> None:
     """Attention of ``q [B, S, Hq, d]`` over a shared prefix and each row's
     own keys into ``out``."""
-    dev = N.require_gpu(q, k_cache, v_cache, prefix_table, prefix_len, block_table, seq_lens, out,
-                        sink, k_scales, v_scales, k_dequant, v_dequant, workspace)
+    dev = N.same_gpu(q, k_cache, v_cache, prefix_table, prefix_len, block_table, seq_lens, out,
+                     sink, k_scales, v_scales, k_dequant, v_dequant, workspace)
     if q.dim() != 4:
         raise ValueError(f"q must be [B, S, Hq, d], got {tuple(q.shape)}")
-    if out.shape != q.shape or out.dtype != torch.bfloat16:
-        raise ValueError(f"out must be a bf16 tensor of shape {tuple(q.shape)}")
-    B, S, hq, _ = q.shape
+    _check_out(out, q)
+    B, S = q.shape[:2]
     if prefix_table.dim() != 1 or prefix_table.dtype != torch.int32:
         raise ValueError("the prefix table must be int32 [blocks]")
     if prefix_len.dtype != torch.int32 or prefix_len.numel() != 1:
@@ -1193,23 +1193,20 @@ def shared_prefix_attention(q, k_cache, v_cache, prefix_table, prefix_len, block
     if block_table.dim() != 2 or block_table.shape[0] != B or block_table.dtype != torch.int32:
         raise ValueError(f"block table must be int32 [{B}, blocks], got {block_table.dtype} "
                          f"{tuple(block_table.shape)}")
-    seq_lens = _int32(seq_lens, (B,), "seq_lens")
-    a = N.SharedPrefixArgs()
-    alive = _span_cache(a, q, k_cache, v_cache, k_scales, v_scales, k_dequant, v_dequant, dev)
+    seq_lens = _int32(seq_lens, B, "seq_lens")
+    (nb, hkv, bs, d), hq, code, scales, kd, vd = _span_cache(
+        q, k_cache, v_cache, k_scales, v_scales, k_dequant, v_dequant, dev)
     sk = _scale_f32(sink, dev, hq, "sink")
     if sk is not None and sk.numel() != hq:
         raise ValueError(f"sink must have {hq} entries, got {sk.numel()}")
-    a.batch, a.s_active = B, S
-    a.prefix_table, a.prefix_stride = prefix_table.data_ptr(), prefix_table.stride(0)
-    a.prefix_blocks = prefix_table.shape[0]
-    a.prefix_len = prefix_len.data_ptr()
-    a.block_table, a.bt_stride = block_table.data_ptr(), block_table.stride()
-    a.blocks_per_seq = block_table.shape[1]
-    a.seq_lens = seq_lens.data_ptr()
-    a.sink = N.ptr(sk)
-    a.softmax_scale = softmax_scale
-    a.out, a.out_stride = out.data_ptr(), out.stride()
+    a = N.SharedPrefixArgs()
+    N.PACK_PREFIX.pack_into(
+        a, 0, q.data_ptr(), *q.stride(), out.data_ptr(), *out.stride(), B, S, hq, hkv, d, code,
+        k_cache.data_ptr(), v_cache.data_ptr(), *k_cache.stride(), *v_cache.stride(), nb, bs,
+        prefix_table.data_ptr(), prefix_table.stride(0), prefix_len.data_ptr(),
+        block_table.data_ptr(), *block_table.stride(), seq_lens.data_ptr(),
+        prefix_table.shape[0], block_table.shape[1], *scales, N.ptr(kd) or 0, N.ptr(vd) or 0,
+        N.ptr(sk) or 0, softmax_scale, 0, 0, 0)
     L = N.lib()
     _span_launch(a, L.mia_shared_prefix_workspace_bytes, L.mia_shared_prefix_attention,
                  "shared_prefix_attention", workspace, dev)
-    del alive

@@ -8,6 +8,7 @@ calls raise.
 from __future__ import annotations
 
 import ctypes
+import struct
 import threading
 from pathlib import Path
 
@@ -254,6 +255,24 @@ class SharedPrefixArgs(ctypes.Structure):
     ]
 
 
+_CODES = {c_vp: "P", c_i32: "i", c_i64: "q", c_f32: "f", ctypes.c_size_t: "N"}
+
+
+def _packer(st) -> struct.Struct:
+    """Packs an argument struct's fields (arrays flattened) in one call; a
+    field set one by one costs ~0.2 us of a launch's host time."""
+    code = ""
+    for _, t in st._fields_:
+        n = getattr(t, "_length_", None)
+        code += _CODES[t] if n is None else f"{n}{_CODES[t._type_]}"
+    return struct.Struct("@" + code)
+
+
+PACK_QUANT = _packer(QuantKvArgs)
+PACK_CROSS = _packer(CrossArgs)
+PACK_PREFIX = _packer(SharedPrefixArgs)
+
+
 ARGS_STRUCTS = {
     0: KvWriteArgs, 1: GatherArgs, 2: MaskArgs, 3: DecodeArgs, 4: PrefillArgs,
     5: SlotMappingArgs, 6: PackedKArgs, 7: SwaTrimArgs, 8: ScatterRowsArgs, 9: StageArgs,
@@ -375,6 +394,16 @@ def require_gpu(*tensors: torch.Tensor | None) -> torch.device:
     if dev is None:
         raise ValueError("no tensor given")
     return dev
+
+
+def same_gpu(*tensors: torch.Tensor | None) -> torch.device:
+    """``require_gpu`` for many tensors: one index each where all is well."""
+    first = tensors[0]
+    index = first.get_device()
+    for t in tensors:
+        if t is not None and t.get_device() != index:
+            return require_gpu(*tensors)
+    return first.device if index >= 0 else require_gpu(*tensors)
 
 
 def stream_ptr(device: torch.device) -> int:
