@@ -19,8 +19,8 @@
 //
 // Layout.  A row is read by LPR lanes with 16 bytes each (8 elements), the
 // maximum goes over those lanes with xor shuffles, and each lane stores its 8
-// codes; K and V are grid rows y = 0 and 1 of one launch.  Bound by HBM for
-// long writes, by the launch for a step's few rows.
+// codes; a thread takes K and V of its (token, head).  Bound by HBM for long
+// writes, by the launch for a step's few rows.
 #include <algorithm>
 
 #include "mia_device.h"
@@ -118,130 +118,144 @@ MIA_DEV void load8(const uint8_t *row, int64_t sd, int c0, int d, float (&x)[8])
   }
 }
 
-// LPR lanes per row, 8 channels each (d <= 8 LPR).  VEC: d is a multiple of
-// 8, rows are contiguous and 16-byte (cache: 8-byte) aligned.
+// LPR lanes per row, 8 channels each (d <= 8 LPR); a thread takes its chunk of
+// the K and of the V row, so that two loads are in flight and the slot is
+// resolved once.  VEC: d is a multiple of 8, rows are contiguous and 16-byte
+// (cache: 8-byte) aligned.
 template <int SRC, bool I8, int LPR, bool VEC>
 __global__ __launch_bounds__(256) void quant_write_kernel(QuantKParams p) {
-  const int y = blockIdx.y;
   const uint32_t row = blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
   const int c0 = (threadIdx.x % LPR) * 8;
   const bool in = row < p.n_rows;
   const RowPos r = row_pos(p, in ? row : 0);
   const bool act = c0 < p.d;
-  float x[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = 0.f;
   constexpr int SB = SRC == MIA_DTYPE_F32 ? 4 : 2;
-  if (act)
-    load8<SRC, VEC>(p.rows[y] + ((int64_t)r.t * p.r_t[y] + (int64_t)r.h * p.r_h[y]) * SB,
-                    p.r_d[y], c0, p.d, x);
-  // maximum of the magnitudes as integers: an infinity or NaN is the largest
-  uint32_t mag = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) mag = max(mag, __float_as_uint(x[i]) & 0x7fffffffu);
-#pragma unroll
-  for (int o = 1; o < LPR; o <<= 1) mag = max(mag, (uint32_t)__shfl_xor((int)mag, o, 64));
-  if (!in || r.slot < 0) return;
   constexpr float Q = I8 ? 127.0f : 448.0f;
-  const float amax = __uint_as_float(mag);
-  const bool bad = mag >= 0x7f800000u;
-  const bool zero = bad || mag == 0;
-  const int e = __builtin_amdgcn_frexp_expf(amax);
-  const float b = zero ? 1.0f : ldexpf(amax, -e);  // [0.5, 1)
-  float rc = __builtin_amdgcn_rcpf(b);
-  rc = fmaf(fmaf(-b, rc, 1.0f), rc, rc);
-  float y8[8];
+  float x[2][8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float a = (zero ? 0.f : ldexpf(x[i], -e)) * Q;
-    const float q = a * rc;
-    y8[i] = fmaf(fmaf(-b, q, a), rc, q);
+  for (int y = 0; y < 2; ++y) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[y][i] = 0.f;
+    if (act)
+      load8<SRC, VEC>(p.rows[y] + ((int64_t)r.t * p.r_t[y] + (int64_t)r.h * p.r_h[y]) * SB,
+                      p.r_d[y], c0, p.d, x[y]);
   }
-  u32x2_t w;
-  if constexpr (I8) {
 #pragma unroll
-    for (int g = 0; g < 2; ++g) {
-      uint32_t v = 0;
+  for (int y = 0; y < 2; ++y) {
+    // maximum of the magnitudes as integers: an infinity or NaN is the largest
+    uint32_t mag = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        v |= ((uint32_t)(int)rintf(y8[4 * g + i]) & 0xffu) << (8 * i);
-      w[g] = v;
+    for (int i = 0; i < 8; ++i) mag = max(mag, __float_as_uint(x[y][i]) & 0x7fffffffu);
+#pragma unroll
+    for (int o = 1; o < LPR; o <<= 1) mag = max(mag, (uint32_t)__shfl_xor((int)mag, o, 64));
+    if (!in || r.slot < 0) continue;
+    const float amax = __uint_as_float(mag);
+    const bool bad = mag >= 0x7f800000u;
+    const bool zero = bad || mag == 0;
+    const int e = __builtin_amdgcn_frexp_expf(amax);
+    const float b = zero ? 1.0f : ldexpf(amax, -e);  // [0.5, 1)
+    float rc = __builtin_amdgcn_rcpf(b);
+    rc = fmaf(fmaf(-b, rc, 1.0f), rc, rc);
+    float y8[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float a = (zero ? 0.f : ldexpf(x[y][i], -e)) * Q;
+      const float q = a * rc;
+      y8[i] = fmaf(fmaf(-b, q, a), rc, q);
     }
-  } else {
-    w[0] = e4m3fn_x4(y8[0], y8[1], y8[2], y8[3]);
-    w[1] = e4m3fn_x4(y8[4], y8[5], y8[6], y8[7]);
-  }
-  uint8_t *dst = p.cache[y] + r.blk * p.c_blk[y] + (int64_t)r.h * p.c_h[y] + r.off * p.c_t[y];
-  if constexpr (VEC) {
-    if (act) *reinterpret_cast<u32x2_t *>(dst + c0) = w;
-  } else {
+    u32x2_t w;
+    if constexpr (I8) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (c0 + i < p.d) dst[(int64_t)(c0 + i) * p.c_d[y]] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
-  }
-  if (threadIdx.x % LPR == 0) {
-    float sc = amax / Q;
-    // the largest fp32 values: code Q must not read back as an infinity
-    if (SRC == MIA_DTYPE_F32 && sc * Q > 3.402823466e38f)
-      sc = __uint_as_float(__float_as_uint(sc) - 1u);
-    p.scales[y][r.blk * p.s_blk[y] + (int64_t)r.h * p.s_h[y] + r.off * p.s_t[y]] =
-        bad ? __uint_as_float(0x7fc00000u) : sc;
+      for (int g = 0; g < 2; ++g) {
+        uint32_t v = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          v |= ((uint32_t)(int)rintf(y8[4 * g + i]) & 0xffu) << (8 * i);
+        w[g] = v;
+      }
+    } else {
+      w[0] = e4m3fn_x4(y8[0], y8[1], y8[2], y8[3]);
+      w[1] = e4m3fn_x4(y8[4], y8[5], y8[6], y8[7]);
+    }
+    uint8_t *dst = p.cache[y] + r.blk * p.c_blk[y] + (int64_t)r.h * p.c_h[y] + r.off * p.c_t[y];
+    if constexpr (VEC) {
+      if (act) *reinterpret_cast<u32x2_t *>(dst + c0) = w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (c0 + i < p.d)
+          dst[(int64_t)(c0 + i) * p.c_d[y]] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
+    }
+    if (threadIdx.x % LPR == 0) {
+      float sc = amax / Q;
+      // the largest fp32 values: code Q must not read back as an infinity
+      if (SRC == MIA_DTYPE_F32 && sc * Q > 3.402823466e38f)
+        sc = __uint_as_float(__float_as_uint(sc) - 1u);
+      p.scales[y][r.blk * p.s_blk[y] + (int64_t)r.h * p.s_h[y] + r.off * p.s_t[y]] =
+          bad ? __uint_as_float(0x7fc00000u) : sc;
+    }
   }
 }
 
 template <int DST, bool I8, int LPR, bool VEC>
 __global__ __launch_bounds__(256) void quant_read_kernel(QuantKParams p) {
-  const int y = blockIdx.y;
   const uint32_t row = blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
   const int c0 = (threadIdx.x % LPR) * 8;
   if (row >= p.n_rows || c0 >= p.d) return;
   const RowPos r = row_pos(p, row);
-  float x[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = 0.f;
+  uint32_t w[2][2] = {{0u, 0u}, {0u, 0u}};
+  float s[2] = {0.f, 0.f};
   if (r.slot >= 0) {
-    const uint8_t *src =
-        p.cache[y] + r.blk * p.c_blk[y] + (int64_t)r.h * p.c_h[y] + r.off * p.c_t[y];
-    const float s = p.scales[y][r.blk * p.s_blk[y] + (int64_t)r.h * p.s_h[y] + r.off * p.s_t[y]];
-    uint32_t w[2] = {0u, 0u};
-    if constexpr (VEC) {
-      const u32x2_t v = *reinterpret_cast<const u32x2_t *>(src + c0);
-      w[0] = v[0];
-      w[1] = v[1];
-    } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (c0 + i < p.d)
-          w[i >> 2] |= (uint32_t)src[(int64_t)(c0 + i) * p.c_d[y]] << (8 * (i & 3));
-    }
+    for (int y = 0; y < 2; ++y) {
+      const uint8_t *src =
+          p.cache[y] + r.blk * p.c_blk[y] + (int64_t)r.h * p.c_h[y] + r.off * p.c_t[y];
+      s[y] = p.scales[y][r.blk * p.s_blk[y] + (int64_t)r.h * p.s_h[y] + r.off * p.s_t[y]];
+      if constexpr (VEC) {
+        const u32x2_t v = *reinterpret_cast<const u32x2_t *>(src + c0);
+        w[y][0] = v[0];
+        w[y][1] = v[1];
+      } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t byte = (w[i >> 2] >> (8 * (i & 3))) & 0xffu;
-      const float c = I8 ? (float)(int8_t)byte : e4m3fn_bits_to_f32(byte);
-      x[i] = c * s;
+        for (int i = 0; i < 8; ++i)
+          if (c0 + i < p.d)
+            w[y][i >> 2] |= (uint32_t)src[(int64_t)(c0 + i) * p.c_d[y]] << (8 * (i & 3));
+      }
     }
   }
   constexpr int DB = DST == MIA_DTYPE_F32 ? 4 : 2;
-  uint8_t *dst = const_cast<uint8_t *>(p.rows[y]) +
-                 ((int64_t)r.t * p.r_t[y] + (int64_t)r.h * p.r_h[y]) * DB;
-  if constexpr (VEC) {
-    if constexpr (DST == MIA_DTYPE_F32) {
-      *reinterpret_cast<f32x4_t *>(dst + c0 * 4) = f32x4_t{x[0], x[1], x[2], x[3]};
-      *reinterpret_cast<f32x4_t *>(dst + c0 * 4 + 16) = f32x4_t{x[4], x[5], x[6], x[7]};
-    } else {
-      u32x4_t w;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        w[i] = to_bits16<DST>(x[2 * i]) | (to_bits16<DST>(x[2 * i + 1]) << 16);
-      *reinterpret_cast<u32x4_t *>(dst + c0 * 2) = w;
-    }
-  } else {
+  for (int y = 0; y < 2; ++y) {
+    float x[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      if (c0 + i >= p.d) break;
-      const int64_t o = (int64_t)(c0 + i) * p.r_d[y];
-      if constexpr (DST == MIA_DTYPE_F32) reinterpret_cast<float *>(dst)[o] = x[i];
-      else reinterpret_cast<uint16_t *>(dst)[o] = (uint16_t)to_bits16<DST>(x[i]);
+      const uint32_t byte = (w[y][i >> 2] >> (8 * (i & 3))) & 0xffu;
+      x[i] = (I8 ? (float)(int8_t)byte : e4m3fn_bits_to_f32(byte)) * s[y];
+      // the product is rounded to fp32 in every case (an f16 result would
+      // otherwise be formed by one mixed multiply, rounded once)
+      if constexpr (DST == MIA_DTYPE_F16) asm("" : "+v"(x[i]));
+    }
+    uint8_t *dst = const_cast<uint8_t *>(p.rows[y]) +
+                   ((int64_t)r.t * p.r_t[y] + (int64_t)r.h * p.r_h[y]) * DB;
+    if constexpr (VEC) {
+      if constexpr (DST == MIA_DTYPE_F32) {
+        *reinterpret_cast<f32x4_t *>(dst + c0 * 4) = f32x4_t{x[0], x[1], x[2], x[3]};
+        *reinterpret_cast<f32x4_t *>(dst + c0 * 4 + 16) = f32x4_t{x[4], x[5], x[6], x[7]};
+      } else {
+        u32x4_t o;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          o[i] = to_bits16<DST>(x[2 * i]) | (to_bits16<DST>(x[2 * i + 1]) << 16);
+        *reinterpret_cast<u32x4_t *>(dst + c0 * 2) = o;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (c0 + i >= p.d) break;
+        const int64_t o = (int64_t)(c0 + i) * p.r_d[y];
+        if constexpr (DST == MIA_DTYPE_F32) reinterpret_cast<float *>(dst)[o] = x[i];
+        else reinterpret_cast<uint16_t *>(dst)[o] = (uint16_t)to_bits16<DST>(x[i]);
+      }
     }
   }
 }
@@ -287,7 +301,7 @@ QuantKParams kparams(const mia_quant_kv_args &a) {
 
 template <int DT, bool I8, int LPR, bool VEC>
 void launch_one(const QuantKParams &p, bool write, hipStream_t s) {
-  const dim3 grid((p.n_rows + 256 / LPR - 1) / (256 / LPR), 2);
+  const dim3 grid((p.n_rows + 256 / LPR - 1) / (256 / LPR));
   if (write) quant_write_kernel<DT, I8, LPR, VEC><<<grid, 256, 0, s>>>(p);
   else quant_read_kernel<DT, I8, LPR, VEC><<<grid, 256, 0, s>>>(p);
 }

@@ -686,9 +686,10 @@ MIA_DEV void tall_body(const Share &sh, TallLds<D, CT, SC> &lds) {
   Keys ks_;
   int ent = 0;  // the wave's table entry of a tile, loaded one tile ahead
   auto load_entry = [&](int t) { ent = ks_.entry(t * kTallKeys + wave * 16); };
-  // the chunk a lane loads: for copies the one that the swizzle puts in its slot
-  auto k_chunk = [&](int j) { return DMA ? lc ^ k_swz<D>(j * RPW + lr) : lc; };
-  auto v_chunk = [&](int j) { return DMA ? lc ^ v_swz<D>(j * RPW + lr) : lc; };
+  // the chunk a lane loads: for copies the one that the swizzle puts in its
+  // slot, else its own (past the head dim: the first, stored nowhere)
+  auto k_chunk = [&](int j) { return DMA ? lc ^ k_swz<D>(j * RPW + lr) : ch_ok ? lc : 0; };
+  auto v_chunk = [&](int j) { return DMA ? lc ^ v_swz<D>(j * RPW + lr) : ch_ok ? lc : 0; };
   uint32_t ko[NP], vo[NP];  // a lane's bytes from its group's first row
   auto set_offsets = [&](int last) {
 #pragma unroll
@@ -721,19 +722,14 @@ MIA_DEV void tall_body(const Share &sh, TallLds<D, CT, SC> &lds) {
     } else {
 #pragma unroll
       for (int j = 0; j < NP; ++j) {
-        kr[j] = u32x4_t{0u, 0u, 0u, 0u};
-        vr[j] = u32x4_t{0u, 0u, 0u, 0u};
-        if (ch_ok) {
-          kr[j] = *reinterpret_cast<const u32x4_t *>(g.k + ko[j]);
-          vr[j] = *reinterpret_cast<const u32x4_t *>(g.v + vo[j]);
-        }
+        // (no condition on a load: the merge of its two results would wait)
+        kr[j] = *reinterpret_cast<const u32x4_t *>(g.k + ko[j]);
+        vr[j] = *reinterpret_cast<const u32x4_t *>(g.v + vo[j]);
         if constexpr (SC) {
-          // lanes 0 and 1 of a row: its K and V scale (one load: a second
-          // into the same register would wait for the first)
+          // even lanes of a row its K scale, odd ones its V scale
           const uint32_t rr = min(k0 + j * RPW + lr, c.len - 1) - g.k16;
-          const float *sp = lc ? g.vs(ks_) : g.ks(ks_);
-          const uint32_t st = lc ? ks_.vs_t : ks_.ks_t;
-          if (lc < 2) sr[j] = sp[(uint64_t)rr * st];
+          const float *sp = lc & 1 ? g.vs(ks_) : g.ks(ks_);
+          sr[j] = sp[(uint64_t)rr * (lc & 1 ? ks_.vs_t : ks_.ks_t)];
         }
       }
     }
@@ -760,6 +756,7 @@ MIA_DEV void tall_body(const Share &sh, TallLds<D, CT, SC> &lds) {
       // values past the span are cleared: 0 * NaN would reach the sums
       const bool in = kt + row < c.len;
       const u32x4_t v = in ? vr[j] : u32x4_t{0u, 0u, 0u, 0u};
+      if (ch_ok)
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         *(lds_u32x4_t *)(kb + row * ROWB + (((2 * lc + x) ^ k_swz<D>(row)) << 4)) =
@@ -977,12 +974,12 @@ MIA_DEV void tall_body(const Share &sh, TallLds<D, CT, SC> &lds) {
   if (!first_pos(fresh(), sh, cur)) return;
   Pos nxt = cur;
   int buf = 0, t0 = cur.t;
+  if (d_used < D) {  // channels past d: zero in all stages, never written again
+    for (int o = tid * 16; o < 2 * STAGES * TILEB; o += kThreads * 16)
+      *(lds_u32x4_t *)(base + o) = u32x4_t{0u, 0u, 0u, 0u};
+    __syncthreads();
+  }
   if constexpr (DMA) {
-    if (d_used < D) {  // channels past d: zero in all stages, never written again
-      for (int o = tid * 16; o < 2 * STAGES * TILEB; o += kThreads * 16)
-        *(lds_u32x4_t *)(base + o) = u32x4_t{0u, 0u, 0u, 0u};
-      __syncthreads();
-    }
     // nxt: the next tile to copy, STAGES - 1 ahead of cur
     load_q(cur);
     bool anew = true, more = true;
@@ -1109,6 +1106,13 @@ MIA_DEV void thin_body(const Share &sh, ThinLds<D, SC> &lds) {
 
   u32x4_t kr[2][NK], vr[NV];
   float sr = 0.f;
+  // bytes of a lane's chunks in a row; past the head dim the first chunk: K is
+  // cleared at its use, what V gives there is stored nowhere
+  uint32_t kch[NK];
+#pragma unroll
+  for (int j = 0; j < NK; ++j) kch[j] = k_chan(j, kg) < d_used ? k_chan(j, kg) * EB : 0;
+  const uint32_t vch = vds * VE < d_used ? vds * 16 : 0;
+  const bool narrow = d_used < D;
   Keys ks_;
   Group g[2];
   int ent[2];  // table entries of a tile, loaded one tile ahead
@@ -1135,13 +1139,10 @@ MIA_DEV void thin_body(const Share &sh, ThinLds<D, SC> &lds) {
     for (int b = 0; b < 2; ++b) {
       int rr = col;
       if (!full) rr = min(c.t * kThinKeys + b * 16 + col, ks_.len - 1) - g[b].k16;
-      const uint32_t o = rr * ks_.k_t + k_chan(0, kg) * EB;
+      // (no condition on a load: the merge of its two results would wait)
 #pragma unroll
-      for (int j = 0; j < NK; ++j) {
-        kr[b][j] = u32x4_t{0u, 0u, 0u, 0u};
-        if (k_chan(j, kg) < d_used)
-          kr[b][j] = *reinterpret_cast<const u32x4_t *>(g[b].k + k_chan(j, 0) * EB + o);
-      }
+      for (int j = 0; j < NK; ++j)
+        kr[b][j] = *reinterpret_cast<const u32x4_t *>(g[b].k + (rr * ks_.k_t + kch[j]));
     }
   };
   auto load_v = [&](const Pos &c) {
@@ -1151,9 +1152,7 @@ MIA_DEV void thin_body(const Share &sh, ThinLds<D, SC> &lds) {
       const Group &x = g[j * TL / 16];
       int rr = j * TL % 16 + vtl;
       if (!full) rr = min(c.t * kThinKeys + j * TL + vtl, ks_.len - 1) - x.k16;
-      vr[j] = u32x4_t{0u, 0u, 0u, 0u};
-      if (vds * VE < d_used)
-        vr[j] = *reinterpret_cast<const u32x4_t *>(x.v + (uint32_t)(rr * ks_.v_t + vds * 16));
+      vr[j] = *reinterpret_cast<const u32x4_t *>(x.v + (rr * ks_.v_t + vch));
     }
   };
   // lane l: scale of key l (K), of key l - 32 (V)
@@ -1218,6 +1217,13 @@ MIA_DEV void thin_body(const Share &sh, ThinLds<D, SC> &lds) {
   // S^T of the tile; frees the K registers
   f32x4_t s[NC][2];
   auto scores = [&]() {
+    if (narrow) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int j = 0; j < NK; ++j)
+          if (k_chan(j, kg) >= d_used) kr[b][j] = u32x4_t{0u, 0u, 0u, 0u};
+    }
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
 #pragma unroll
@@ -1775,19 +1781,20 @@ void launch_span(const SpanParams &p, int grid, hipStream_t s) {
     else span_kernel<D, CT, SC, D, 2><<<grid, kThreads, 0, s>>>(p);
   }
   if (p.join) {
-    // lane groups per row by the pieces to expect: those of the prefix (its
-    // share of the workgroups over its segments) and one or two of the row
+    // Lane groups per row: as many as one round of resident waves (8 per SIMD)
+    // holds, since a row's pieces are loaded one after the other within a
+    // group.  128 rows of 64 heads, d = 64: 14.4 us by 8 groups, 7 by 2; 64
+    // rows of 32 heads, d = 128: 9 us by 8.
     const int hq = p.Hkv * p.G;
-    const int segs = std::max(1, (p.list[0].tok_max * p.G + kRows - 1) / kRows * p.Hkv);
-    const int units = p.list[0].thin ? grid * kWaves : grid;
-    auto blocks = [&](int groups) {
+    const int rows = p.num_tokens * hq;
+    const int64_t waves = (int64_t)rows * (D / 4) / 64, resident = 32 * cu_count();
+    auto join = [&](auto kernel, int groups) {
       const int rpb = 256 / (D / 4) / groups;
-      return (p.num_tokens * hq + rpb - 1) / rpb;
+      kernel<<<(rows + rpb - 1) / rpb, 256, 0, s>>>(p, make_fastdiv(hq));
     };
-    if (units / segs > 8)
-      span_join_kernel<D, CT, SC, 8><<<blocks(8), 256, 0, s>>>(p, make_fastdiv(hq));
-    else
-      span_join_kernel<D, CT, SC, 2><<<blocks(2), 256, 0, s>>>(p, make_fastdiv(hq));
+    if (waves * 8 <= resident) join(span_join_kernel<D, CT, SC, 8>, 8);
+    else if (waves * 4 <= resident) join(span_join_kernel<D, CT, SC, 4>, 4);
+    else join(span_join_kernel<D, CT, SC, 2>, 2);
   }
 }
 
