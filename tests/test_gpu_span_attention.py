@@ -429,6 +429,115 @@ def test_cross_random_shapes(gpu):
                [r.randint(0, r.choice([3, 70, 900])) for _ in range(B)], new, seed=i * 10)
 
 
+def test_prefix_many_new_tokens(gpu):
+    """Up to 64 new tokens a row: the last 63 keys are seen by some rows only."""
+    _prefix(gpu, "bf16", 2, 1, 64, 16, 50, [64, 100, 10, 200], S=64)
+    _prefix(gpu, "int8", 4, 2, 128, 16, 0, [40, 33], S=33)
+
+
+def test_lengths_of_any_int32(gpu):
+    """The ends of int32 as lengths: nothing, or all that the tables hold."""
+    hq, hkv, d, bs = 4, 2, 64, 16
+    pool = Pool("bf16", 12, hkv, bs, d, 2, gpu).up()
+    lo, hi = -2 ** 31, 2 ** 31 - 1
+    q = _randn(_gen(4), 2, 3, hq, d)
+    t = torch.tensor([[1, 2], [3, 4]], dtype=torch.int32)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=gpu)
+    out = shared_prefix_attention(q.to(gpu), pool.gk, pool.gv, i32(5, 6, 7), i32(hi), t.to(gpu), i32(lo, hi))
+    kp, vp = pool.rows([5, 6, 7], 48)
+    k, v = pool.rows([3, 4], 32)
+    for s in range(3):
+        o, bound = attend(q[0, s:s + 1], kp, vp, d ** -0.5)
+        check(out[0, s:s + 1], o, bound)
+        o, bound = attend(q[1, s:s + 1], torch.cat([kp, k]), torch.cat([vp, v]), d ** -0.5)
+        check(out[1, s:s + 1], o, bound)
+    out = shared_prefix_attention(q.to(gpu), pool.gk, pool.gv, i32(5, 6, 7), i32(lo), t.to(gpu), i32(lo, 2))
+    assert (out[0] == 0).all() and (out[1, 0] == 0).all()
+    out = cross_attention(q[:, 0].to(gpu), pool.gk, pool.gv, i32(lo, hi), block_table=t.to(gpu))
+    o, bound = attend(q[1:2, 0], k, v, d ** -0.5)
+    assert (out[0] == 0).all()
+    check(out[1:], o, bound)
+
+
+def test_axes_of_one_entry_have_any_stride(gpu):
+    """Strides that no address uses are not asked to be aligned."""
+    hkv, bs, d, n = 1, 16, 64, 40
+    big = _randn(_gen(3), 8, 3 * d + 1).to(gpu)
+    q = big[2:3, :2 * d].as_strided((1, 2, d), (3 * d + 1, d, 1), 0)  # one token, odd row stride
+    pool = Pool("bf16", 4, hkv, bs, d, 2, gpu).up()
+    k, v = (x.as_strided(x.shape, (x.stride(0), 3, d, 1)) for x in (pool.gk, pool.gv))
+    t = torch.tensor([[2, 0, 3]], dtype=torch.int32)
+    lens = torch.tensor([n], dtype=torch.int32, device=gpu)
+    out = cross_attention(q, k, v, lens, block_table=t.to(gpu))
+    o, bound = attend(q.cpu(), *pool.rows(t[0], n), d ** -0.5)
+    check(out, o, bound)
+
+
+def test_query_tokens_past_the_maximum(gpu):
+    """max_seqlen_q bounds what is computed; the rest of out stays."""
+    hq, hkv, d, L = 4, 2, 64, 33
+    g = _gen(5)
+    q, k, v = _randn(g, 10, hq, d), _randn(g, 2, hkv, L, d), _randn(g, 2, hkv, L, d)
+    out = torch.full((10, hq, d), 5.0, dtype=BF, device=gpu)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=gpu)
+    cross_attention(q.to(gpu), k.to(gpu), v.to(gpu), i32(L, L), cu_seqlens_q=i32(0, 6, 8), max_seqlen_q=4, out=out)
+    for i, (a, b) in enumerate([(0, 4), (6, 8)]):
+        o, bound = attend(q[a:b], k[i].transpose(0, 1).double(), v[i].transpose(0, 1).double(), d ** -0.5)
+        check(out[a:b], o, bound)
+    assert (out[4:6] == 5.0).all() and (out[8:] == 5.0).all()
+
+
+def test_two_streams_and_a_given_workspace(gpu):
+    """Calls at once on two streams; a given workspace is used and gives the
+    same bits, one too small is not."""
+    hq, hkv, d, bs, B = 8, 2, 64, 16, 6
+    tp, nb = _tables([300], bs, 1, 0)
+    t, nb = _tables([96] * B, bs, nb, 1)
+    pool = Pool("bf16", nb, hkv, bs, d, 2, gpu).up()
+    q = _randn(_gen(3), B, 1, hq, d).to(gpu)
+    args = (pool.gk, pool.gv, tp[0].to(gpu), torch.tensor([300], dtype=torch.int32, device=gpu), t.to(gpu),
+            torch.tensor([96, 1, 5, 64, 65, 33], dtype=torch.int32, device=gpu))
+    want = shared_prefix_attention(q, *args)
+    ws = torch.full((64 << 20,), 255, dtype=torch.uint8, device=gpu)
+    assert torch.equal(want, shared_prefix_attention(q, *args, workspace=ws))
+    assert (ws != 255).any()
+    assert torch.equal(want, shared_prefix_attention(q, *args, workspace=ws[:100]))
+    with pytest.raises(ValueError):
+        shared_prefix_attention(q, *args, workspace=ws[::2])
+    with pytest.raises(ValueError):
+        shared_prefix_attention(q, *args, workspace=ws[1:])
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = []
+    for i in range(6):
+        with torch.cuda.stream(streams[i % 2]):
+            outs.append(shared_prefix_attention(q, *args))
+    torch.cuda.synchronize()
+    assert all(torch.equal(want, o) for o in outs)
+
+
+def test_prefix_compiles(gpu):
+    hq, hkv, d, bs, B = 8, 2, 64, 16, 3
+    tp, nb = _tables([50], bs, 1, 0)
+    t, nb = _tables([20] * B, bs, nb, 1)
+    pool = Pool("int8", nb, hkv, bs, d, 2, gpu).up()
+    q = _randn(_gen(3), B, 1, hq, d).to(gpu)
+    P = torch.tensor([50], dtype=torch.int32, device=gpu)
+    lens = torch.tensor([20, 3, 7], dtype=torch.int32, device=gpu)
+    tp, t = tp[0].to(gpu), t.to(gpu)
+    slots = torch.tensor([7, 8, 9], device=gpu)
+    rows = _randn(_gen(4), B, hkv, d).to(gpu)
+    kv = (pool.gk, pool.gv, pool.kw["k_scales"], pool.kw["v_scales"])
+
+    def step(q, rows):
+        quant_kv_write(rows, rows, slots, *kv)
+        return shared_prefix_attention(q, pool.gk, pool.gv, tp, P, t, lens, **pool.kw) + 1
+
+    want = step(q, rows)
+    got = torch.compile(step, fullgraph=True, backend="aot_eager")(q, rows)
+    assert torch.equal(want, got)
+
+
 # ---------------------------------------------------------------------------
 # the operators together, and against the framework's decode
 # ---------------------------------------------------------------------------

@@ -108,6 +108,7 @@ SHARED = [
     (dict(block_table=None), ValueError, "dense"),
     (dict(num_seqs=-1), ValueError, "shape"),
     (dict(num_tokens=1 << 28), ValueError, "2\\^30"),
+    (dict(num_tokens=1 << 24, blocks_per_seq=1 << 16), ValueError, "key tiles"),
 ])
 def test_cross_refusals(over, err, text):
     L = N.lib()
@@ -120,6 +121,7 @@ def test_cross_refusals(over, err, text):
     (dict(s_active=0), ValueError, "shape"),
     (dict(s_active=65), NotImplementedError, "64"),
     (dict(prefix_blocks=0), ValueError, "prefix"),
+    (dict(batch=1 << 20, blocks_per_seq=1 << 16), ValueError, "key tiles"),
 ])
 def test_prefix_refusals(over, err, text):
     L = N.lib()

@@ -40,8 +40,8 @@ static bool aligned(const void *p, size_t a) {
 
 // What cross and shared-prefix attention ask of their heads, rows and cache.
 template <typename A>
-static int check_span(const A &a, const int64_t *q_rows, const int64_t *out_rows, int n_rows,
-                      int64_t rows, bool paged) {
+static int check_span(const A &a, const int64_t *q_rows, const int64_t *out_rows,
+                      const int *extents, int n_rows, int64_t rows, bool paged) {
   MIA_REQUIRE(a.num_q_heads > 0 && a.num_kv_heads > 0 && a.num_q_heads % a.num_kv_heads == 0,
               MIA_ERR_VALUE, "GQA requires q_heads divisible by kv_heads");
   MIA_REQUIRE(a.cache_dtype == MIA_DTYPE_BF16 || a.cache_dtype == MIA_DTYPE_FP8_E4M3FN ||
@@ -69,8 +69,11 @@ static int check_span(const A &a, const int64_t *q_rows, const int64_t *out_rows
   for (int i = 0; i < 2; ++i) {
     const void *c = i ? a.v_cache : a.k_cache;
     const int64_t *s = i ? a.v_cache_stride : a.k_cache_stride;
-    MIA_REQUIRE(s[3] == 1 && aligned(c, 16) && s[0] * eb % 16 == 0 && s[1] * eb % 16 == 0 &&
-                    s[2] * eb % 16 == 0,
+    // (the stride of an axis of one entry is never used)
+    MIA_REQUIRE((s[3] == 1 || a.head_dim == 1) && aligned(c, 16) &&
+                    (s[0] * eb % 16 == 0 || a.num_blocks == 1) &&
+                    (s[1] * eb % 16 == 0 || a.num_kv_heads == 1) &&
+                    (s[2] * eb % 16 == 0 || a.block_size == 1),
                 MIA_ERR_VALUE,
                 "span attention: cache head_dim must be contiguous and its rows 16-byte aligned");
     MIA_REQUIRE(s[2] >= 0 && s[2] * eb < (1ll << 27), MIA_ERR_VALUE,
@@ -89,6 +92,7 @@ static int check_span(const A &a, const int64_t *q_rows, const int64_t *out_rows
   MIA_REQUIRE(aligned(a.out, 8) && out_rows[n_rows] == 1, MIA_ERR_VALUE,
               "span attention: out rows must be contiguous and 8-byte aligned");
   for (int i = 0; i < n_rows; ++i) {
+    if (extents[i] == 1) continue;
     MIA_REQUIRE(q_rows[i] % 8 == 0, MIA_ERR_VALUE,
                 "span attention: q rows must be contiguous and 16-byte aligned");
     MIA_REQUIRE(out_rows[i] % 4 == 0, MIA_ERR_VALUE,
@@ -729,7 +733,18 @@ static int validate_cross(const mia_cross_args *a) {
               "cross_attention: max_seqlen_q must be positive");
   MIA_REQUIRE(a->block_table || (a->num_blocks >= a->num_seqs && a->blocks_per_seq == 1),
               MIA_ERR_VALUE, "cross_attention: dense keys need one block per sequence");
-  return check_span(*a, a->q_stride, a->out_stride, 2, a->num_tokens, a->block_table != nullptr);
+  const int extents[2] = {a->num_tokens, a->num_q_heads};
+  const int rc = check_span(*a, a->q_stride, a->out_stride, extents, 2, a->num_tokens,
+                            a->block_table != nullptr);
+  if (rc) return rc;
+  // the tiles of all segments are counted in 32-bit integers: at most those
+  // of full tables
+  const int64_t G = a->num_q_heads / a->num_kv_heads;
+  const int64_t row_tiles = a->num_tokens * G / 32 + a->num_seqs;
+  const int64_t key_tiles = (int64_t)a->blocks_per_seq * a->block_size / 32 + 4;
+  MIA_REQUIRE(row_tiles * a->num_kv_heads < (1ll << 31) / key_tiles, MIA_ERR_VALUE,
+              "cross_attention: query rows * kv heads * key tiles beyond 2^31");
+  return MIA_OK;
 }
 
 size_t mia_cross_workspace_bytes(const mia_cross_args *a) {
@@ -761,7 +776,19 @@ static int validate_shared_prefix(const mia_shared_prefix_args *a) {
   MIA_REQUIRE(a->prefix_blocks > 0 &&
                   (int64_t)a->prefix_blocks * a->block_size < (1ll << 30),
               MIA_ERR_VALUE, "shared_prefix: empty prefix table or prefix beyond 2^30 tokens");
-  return check_span(*a, a->q_stride, a->out_stride, 3, (int64_t)a->batch * a->s_active, true);
+  const int extents[3] = {a->batch, a->s_active, a->num_q_heads};
+  const int64_t tokens = (int64_t)a->batch * a->s_active;
+  const int rc = check_span(*a, a->q_stride, a->out_stride, extents, 3, tokens, true);
+  if (rc) return rc;
+  // as for cross attention
+  const int64_t G = a->num_q_heads / a->num_kv_heads;
+  const int64_t row_tiles = tokens * G / 32 + a->batch + 1;
+  const int64_t blocks = a->prefix_blocks > a->blocks_per_seq ? a->prefix_blocks
+                                                              : a->blocks_per_seq;
+  const int64_t key_tiles = blocks * a->block_size / 32 + 4;
+  MIA_REQUIRE(row_tiles * a->num_kv_heads < (1ll << 31) / key_tiles, MIA_ERR_VALUE,
+              "shared_prefix: query rows * kv heads * key tiles beyond 2^31");
+  return MIA_OK;
 }
 
 size_t mia_shared_prefix_workspace_bytes(const mia_shared_prefix_args *a) {

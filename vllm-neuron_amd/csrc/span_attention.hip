@@ -119,7 +119,8 @@ MIA_DEV int scalar_load(const int32_t *p, int64_t i) {
 }
 
 MIA_DEV int list_len(const SpanList &l, int i) {
-  return max(0, min(scalar_load(l.len, i) - l.len_sub, l.len_cap));
+  const int n = scalar_load(l.len, i);  // (any int32: no difference below zero)
+  return n > l.len_sub ? min(n - l.len_sub, l.len_cap) : 0;
 }
 // first query token and token count of sequence i
 MIA_DEV int2 list_tokens(const SpanList &l, int i, int num_tokens) {
@@ -1450,7 +1451,7 @@ MIA_DEV void sum_pieces(const SpanParams &p, int n, F prow, float &m, float &l, 
     for (int u = 0; u < 4; ++u) {
       const int64_t r = prow(min(j + u * GR, n - 1));
       ml[u] = p.part_ml[r];
-      v[u] = *reinterpret_cast<const f32x4_t *>(p.part_o + r * D + c * 4);
+      v[u] = *reinterpret_cast<const f32x4_t *>(p.part_o + r * D + (c * 4 < p.d ? c * 4 : 0));
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u)
@@ -1597,7 +1598,7 @@ __global__ __launch_bounds__(256) void span_join_kernel(SpanParams p, FastDiv hq
   Late late;
   if (s > 0) {
     late0 = list_len(l1, b) + gr;
-    late1 = min(scalar_load(l1.len, b) - l1.len_sub + s, l1.len_cap);
+    late1 = min(max(scalar_load(l1.len, b), 0) - l1.len_sub + s, l1.len_cap);
     if (late0 < late1) {
       late = load_late(late0);
       if (c_ok)

@@ -1045,8 +1045,7 @@ def _quant_kv(fn, what, k, v, slots, k_cache, v_cache, k_scales, v_scales) -> No
         k_cache.data_ptr(), v_cache.data_ptr(), *k_cache.stride(), *v_cache.stride(),
         k_scales.data_ptr(), v_scales.data_ptr(), *k_scales.stride(), *v_scales.stride(),
         nb, bs, hkv, d)
-    with N.on_device(dev):
-        N.check(fn(ctypes.byref(a), N.stream_ptr(dev)), what)
+    N.launch(fn, a, dev, what)
 
 
 def quant_kv_write(k, v, slots, k_cache, v_cache, k_scales, v_scales) -> None:
@@ -1122,17 +1121,22 @@ def _check_out(out, q) -> None:
 
 
 def _span_launch(a, query, launch, what, workspace, dev) -> None:
-    """Workspace and launch of a span attention call."""
-    with N.on_device(dev):
-        need = query(ctypes.byref(a))
-        if need:
-            if workspace is None or workspace.numel() * workspace.element_size() < need:
-                workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-            a.workspace = workspace.data_ptr()
-            a.workspace_bytes = need
-        # without a workspace the arguments were refused (the launch says
-        # why) or there is nothing to compute
-        N.check(launch(ctypes.byref(a), N.stream_ptr(dev)), what)
+    """Workspace (sized for the device's compute units) and launch of a span
+    attention call."""
+    if dev.index is not None and dev.index != torch._C._cuda_getDevice():
+        with torch.cuda.device(dev):
+            return _span_launch(a, query, launch, what, workspace, dev)
+    need = query(ctypes.byref(a))
+    if need:
+        if workspace is None or workspace.numel() * workspace.element_size() < need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        elif not workspace.is_contiguous():
+            raise ValueError("workspace must be contiguous")
+        a.workspace = workspace.data_ptr()
+        a.workspace_bytes = need
+    # without a workspace the arguments were refused (the launch says why) or
+    # there is nothing to compute
+    N.launch(launch, a, dev, what)
 
 
 def cross_attention(q, k_cache, v_cache, key_lens, out, *, softmax_scale, block_table=None,

@@ -413,25 +413,18 @@ def stream_ptr(device: torch.device) -> int:
         torch.cuda.current_device() if device.index is None else device.index)
 
 
-class _Here:
-    """A guard that does nothing (a context of contextlib costs ~1 us)."""
-
-    def __enter__(self):
-        return None
-
-    def __exit__(self, *exc):
-        return None
-
-
-_HERE = _Here()
-
-
-def on_device(device: torch.device):
-    """Guard for a launch on ``device``, a no-op where it is the current one:
-    a kernel goes to the current device, whatever its stream's is."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return _HERE
-    return torch.cuda.device(device)
+def launch(fn, args, device: torch.device, what: str) -> None:
+    """``fn(args, stream)`` on torch's current stream of ``device``, with that
+    device current (a kernel goes to the current device, whatever its stream's
+    is), and its return code checked."""
+    here = torch._C._cuda_getDevice()
+    if device.index is None or device.index == here:
+        rc = fn(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(here))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(device.index))
+    if rc:
+        check(rc, what)
 
 
 def ptr(t: torch.Tensor | None) -> int | None:
