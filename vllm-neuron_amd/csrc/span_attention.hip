@@ -1688,9 +1688,17 @@ Layout span_layout(SpanParams &p, int D) {
       hdr += units * kHdr;
     }
   }
-  p.cost[0] = 1.0f, p.cost[1] = D == 64 ? 0.28f : 0.41f;
-  p.over[0] = 2, p.over[1] = 2;
-  p.least[0] = 4, p.least[1] = 4;
+  // Measured: a thin tile takes a wave 1.7 us and a tall one a workgroup 1.8
+  // us at d = 64 (4 and 2.6 us at d = 128), side by side.  64 rows behind 8192
+  // keys (d = 128): 54.2 us at 0.33, 55.8 at 0.41, 58.7 at 0.5; 128 rows
+  // behind 4133 (d = 64): 47.0 at 0.22 and 0.28, 45.5 at 0.35.  A segment's
+  // start costs about two tiles at d = 128 (one: 57.1 and 124.3 us for the 16
+  // drafted int8 rows, two: 55.8 and 120) and for tall ones at d = 64 (ragged
+  // prompts 33.1 against 34.4), one for thin ones there (45.0 against 47.0).
+  // Shares of six units and more leave CUs idle on short calls (15.6 -> 18.3).
+  p.cost[0] = 1.0f, p.cost[1] = 0.35f;
+  p.over[0] = 2, p.over[1] = D == 64 ? 1 : 2;
+  p.least[0] = 4, p.least[1] = D == 64 ? 3 : 4;
   w.hdr = 0;
   w.ml = (size_t)up(hdr * 4, 256);
   w.o = w.ml + (size_t)up(rows * 8, 256);
