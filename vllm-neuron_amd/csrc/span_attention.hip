@@ -350,18 +350,19 @@ MIA_DEV int plan(const SpanParams &p, PlanLds &lds, Share &sh) {
   return form;
 }
 
-// A position in a stream of tiles (wave-uniform).
-struct Pos {
+// A piece: consecutive tiles of one segment in a share (wave-uniform).
+struct Piece {
   int li, i;          // list, sequence
   int tok0, rows;     // first query token, rows (tokens x G)
-  int len, tiles;     // keys, tiles
+  int len, tiles;     // keys, tiles of the segment
   int rt_n, rt, h;    // row tiles, this one, kv head
-  int t;              // tile
-  int x;              // its unit
+  int t, n;           // its tiles [t, t + n)
+  int x;              // unit of tile t
   int over;           // units before a segment's first tile
+  MIA_DEV bool whole() const { return t == 0 && n == tiles; }
 };
 
-MIA_DEV void load_seq(const SpanParams &p, Pos &c) {
+MIA_DEV void load_seq(const SpanParams &p, Piece &c) {
   const SpanList &l = p.list[c.li];
   const int2 tk = list_tokens(l, c.i, p.num_tokens);
   c.tok0 = readfirstlane(tk.x);
@@ -371,8 +372,8 @@ MIA_DEV void load_seq(const SpanParams &p, Pos &c) {
   c.rt_n = row_tiles(l, c.rows);
 }
 
-// The share's first tile; false if it has none.
-MIA_DEV bool first_pos(const SpanParams &p, const Share &sh, Pos &c) {
+// The share's first piece; false if it has no tile.
+MIA_DEV bool first_piece(const SpanParams &p, const Share &sh, Piece &c) {
   if (sh.x0 >= sh.x1) return false;
   c.li = sh.u < p.list[0].n ? 0 : 1;
   c.i = c.li ? sh.u - p.list[0].n : sh.u;
@@ -393,38 +394,38 @@ MIA_DEV bool first_pos(const SpanParams &p, const Share &sh, Pos &c) {
   }
   c.h = seg / c.rt_n;
   c.rt = seg - c.h * c.rt_n;
-  return c.x < sh.x1;
+  c.n = min(c.tiles - c.t, sh.x1 - c.x);
+  return c.n > 0;
 }
 
-// Is there a tile behind c in the share that ends at x1?
-MIA_DEV bool has_next(const Pos &c, int x1) {
-  return c.x + 1 + (c.t + 1 < c.tiles ? 0 : c.over) < x1;
-}
-
-// To the next tile of the share (has_next), over sequences without tiles and
-// lists of the other form.
-MIA_DEV void advance(const SpanParams &p, Pos &c) {
-  ++c.x;
-  if (++c.t < c.tiles) return;
+// To the piece behind c, over sequences without tiles and lists of the other
+// form; false at the end of the share.
+MIA_DEV bool next_piece(const SpanParams &p, const Share &sh, Piece &c) {
+  if (c.t + c.n < c.tiles) return false;
+  c.x += c.n + c.over;
+  if (c.x >= sh.x1) return false;
   c.t = 0;
-  c.x += c.over;
-  if (++c.rt < c.rt_n) return;
-  c.rt = 0;
-  if (++c.h < p.Hkv) return;
-  c.h = 0;
-  const int form = p.list[c.li].thin;
-  ++c.i;
-  while (true) {
-    if (c.i >= p.list[c.li].n || p.list[c.li].thin != form) {
-      if (c.li == 1) return;  // not reached while tiles are left
-      c.li = 1;
-      c.i = 0;
-      continue;
+  if (++c.rt >= c.rt_n) {
+    c.rt = 0;
+    if (++c.h >= p.Hkv) {
+      c.h = 0;
+      const int form = p.list[c.li].thin;
+      ++c.i;
+      while (true) {
+        if (c.i >= p.list[c.li].n || p.list[c.li].thin != form) {
+          if (c.li == 1) return false;  // not reached while units are left
+          c.li = 1;
+          c.i = 0;
+          continue;
+        }
+        load_seq(p, c);
+        if (c.tiles > 0 && c.rt_n > 0) break;
+        ++c.i;
+      }
     }
-    load_seq(p, c);
-    if (c.tiles > 0 && c.rt_n > 0) return;
-    ++c.i;
   }
+  c.n = min(c.tiles, sh.x1 - c.x);
+  return true;
 }
 
 template <int D>
@@ -497,7 +498,7 @@ struct Keys {
   FastDiv bs_div;
 
   template <bool SC>
-  MIA_DEV void set(const SpanParams &p, const Pos &c) {
+  MIA_DEV void set(const SpanParams &p, const Piece &c) {
     const SpanList &l = p.list[c.li];
     bt = l.bt ? l.bt + (int64_t)c.i * l.bt_s : nullptr;
     bt_j = l.bt_j;
@@ -553,24 +554,22 @@ MIA_DEV float score_factor(const SpanParams &p, int h, uint32_t &neg) {
   return c2 == 0.f ? 1e-37f : c2;  // masked scores (-inf) stay masked
 }
 
-// Partial row (or none: < 0) of row `rloc` of the piece [t0, c.t] of c's
-// segment in share sh.w, and the header of a cut segment.
-MIA_DEV int64_t piece_slot(const SpanParams &p, const Share &sh, const Pos &c, int t0,
-                           bool writer) {
+// First partial row of piece c in share sh.w, and the header of a cut segment.
+MIA_DEV int64_t piece_slot(const SpanParams &p, const Share &sh, const Piece &c, bool writer) {
   const SpanList &ls = p.list[c.li];
   int64_t slot;
   if (p.join) {
     const int segs = c.rt_n * p.Hkv;
     slot = (int64_t)(c.li ? c.i * segs : 0) + c.h * c.rt_n + c.rt + sh.w;
   } else {
-    slot = 2 * sh.w + (t0 == 0 ? 1 : 0);
-    if (t0 == 0 && writer) {
+    slot = 2 * sh.w + (c.t == 0 ? 1 : 0);
+    if (c.t == 0 && writer) {
       int *hd = p.hdr + kHdr * sh.w;
       hd[1] = c.tok0;
       hd[2] = c.rows;
       hd[3] = c.rt;
       hd[4] = c.h;
-      hd[0] = cut_of(sh.cut, c.x + c.tiles - 1 - c.t) - sh.w + 1;
+      hd[0] = cut_of(sh.cut, c.x + c.tiles - 1) - sh.w + 1;
     }
   }
   return ls.part0 + slot * ls.part_rows;
@@ -579,14 +578,10 @@ MIA_DEV int64_t piece_slot(const SpanParams &p, const Share &sh, const Pos &c, i
 // ---------------------------------------------------------------------------
 // tall form
 // ---------------------------------------------------------------------------
-// Stages of the copy ring (bf16): 64 KB of LDS for either width, so that two
-// workgroups share a CU; the widened tiles of 8-bit caches take two buffers.
-constexpr int tall_stages(int D, int CT) { return CT == kBf16 && D == 64 ? 3 : 2; }
-
 template <int D, int CT, bool SC>
 struct TallLds {
   static constexpr int TILEB = kTallKeys * D * 2;
-  uint8_t kv[tall_stages(D, CT)][2][TILEB];      // [stage][K, V]
+  uint8_t kv[2][2][TILEB];                       // [stage][K, V]
   float sc[2][2][SC ? kTallKeys : 4];            // [stage][K, V]
 };
 
@@ -663,7 +658,6 @@ MIA_DEV void tall_body(const Share &sh, TallLds<D, CT, SC> &lds) {
   static_assert(kTallKeys == 16 * kWaves, "a wave loads one 16-key group of a tile");
   constexpr int ROWB = D * 2;
   constexpr int TILEB = kTallKeys * ROWB;
-  constexpr int STAGES = tall_stages(D, CT);
   constexpr int KSTEPS = DU / 16;
   constexpr int DBLK = DU / 32;
 
@@ -700,15 +694,22 @@ MIA_DEV void tall_body(const Share &sh, TallLds<D, CT, SC> &lds) {
       vo[j] = rr * ks_.v_t + v_chunk(j) * 16;
     }
   };
-  auto load_tile = [&](const Pos &c, int buf) {
-    const int k0 = c.t * kTallKeys + wave * 16;
+  auto set_keys = [&](const Piece &c) {
+    ks_.set<SC>(fresh(), c);
+    load_entry(c.t);
+    set_offsets(15);
+  };
+  // Tile t of the segment of ks_ (its entry is loaded): copied into stage st,
+  // or loaded into registers; the entry of the tile behind it.
+  auto load_tile = [&](int t, int st) {
+    const int k0 = t * kTallKeys + wave * 16;
     Group g;
     g.set(ks_, k0, ent);
     // rows past the span read its last key (in bounds) and are masked or
     // cleared later; the tail is a segment's last tile
-    if (k0 + 16 > c.len) set_offsets(c.len - 1 - g.k16);
+    if (k0 + 16 > ks_.len) set_offsets(ks_.len - 1 - g.k16);
     if constexpr (DMA) {
-      const uint32_t dst = (uint32_t)(uintptr_t)base + (buf * 2) * TILEB + wave * 16 * ROWB;
+      const uint32_t dst = (uint32_t)(uintptr_t)base + (st * 2) * TILEB + wave * 16 * ROWB;
       if (d_used == D) {
         copy16<NP>(g.k, ko, dst);
         copy16<NP>(g.v, vo, dst + TILEB);
@@ -728,34 +729,24 @@ MIA_DEV void tall_body(const Share &sh, TallLds<D, CT, SC> &lds) {
         vr[j] = *reinterpret_cast<const u32x4_t *>(g.v + vo[j]);
         if constexpr (SC) {
           // even lanes of a row its K scale, odd ones its V scale
-          const uint32_t rr = min(k0 + j * RPW + lr, c.len - 1) - g.k16;
+          const uint32_t rr = min(k0 + j * RPW + lr, ks_.len - 1) - g.k16;
           const float *sp = lc & 1 ? g.vs(ks_) : g.ks(ks_);
           sr[j] = sp[(uint64_t)rr * (lc & 1 ? ks_.vs_t : ks_.ks_t)];
         }
       }
     }
-  };
-  // the tile at c (its entries are loaded, or c starts a segment) and the
-  // entries of the one behind it
-  auto fetch = [&](const Pos &c, int buf, bool anew) {
-    if (anew) {
-      ks_.set<SC>(fresh(), c);
-      load_entry(c.t);
-      set_offsets(15);
-    }
-    load_tile(c, buf);
-    if (c.t + 1 < c.tiles) load_entry(c.t + 1);
+    if ((t + 1) * kTallKeys < ks_.len) load_entry(t + 1);
   };
   // 8-bit caches: the loaded tile widened into stage buf
-  auto store_tile = [&](const Pos &c, int buf) {
-    const int kt = c.t * kTallKeys;
+  auto store_tile = [&](int t, int len, int buf) {
+    const int kt = t * kTallKeys;
     lds_u8_t *const kb = base + (buf * 2) * TILEB;
     lds_u8_t *const vb = base + (buf * 2 + 1) * TILEB;
 #pragma unroll
     for (int j = 0; j < NR; ++j) {
       const int row = wave * 16 + j * RPW + lr;
       // values past the span are cleared: 0 * NaN would reach the sums
-      const bool in = kt + row < c.len;
+      const bool in = kt + row < len;
       const u32x4_t v = in ? vr[j] : u32x4_t{0u, 0u, 0u, 0u};
       if (ch_ok)
 #pragma unroll
@@ -781,7 +772,7 @@ MIA_DEV void tall_body(const Share &sh, TallLds<D, CT, SC> &lds) {
   bool live = false;  // the wave has rows
   u32x4_t qw[KSTEPS];
   // the loads of the rows of a piece, issued ahead of its first tile's
-  auto load_q = [&](const Pos &c) {
+  auto load_q = [&](const Piece &c) {
     const SpanParams &p = fresh();
     const int r = c.rt * kRows + wave * 32 + rl;
     live = c.rt * kRows + wave * 32 < c.rows;
@@ -796,7 +787,7 @@ MIA_DEV void tall_body(const Share &sh, TallLds<D, CT, SC> &lds) {
       if (ok && d0 < d_used) qw[ks] = *reinterpret_cast<const u32x4_t *>(qp + d0);
     }
   };
-  auto begin_piece = [&](const Pos &c) {
+  auto begin_piece = [&](const Piece &c) {
     uint32_t neg;
     c2 = score_factor(fresh(), c.h, neg);
 #pragma unroll
@@ -816,7 +807,7 @@ MIA_DEV void tall_body(const Share &sh, TallLds<D, CT, SC> &lds) {
   const int tr_col = ((lane >> 4) & 1) * 16 + 4 * (tr_k & 3);
   const int tr_row = half * 4 + (tr_k >> 2);
 
-  auto compute = [&](const Pos &c, int buf) {
+  auto compute = [&](int t, int len, int buf) {
     const lds_u8_t *kb = base + (buf * 2) * TILEB;
     const lds_u8_t *vb = base + (buf * 2 + 1) * TILEB;
     const lds_f32_t *ksb = scb + (buf * 2) * kTallKeys;
@@ -858,8 +849,8 @@ MIA_DEV void tall_body(const Share &sh, TallLds<D, CT, SC> &lds) {
           for (int i = 0; i < 4; ++i) s[b][g * 4 + i] *= ks4[i];
         }
     }
-    const int left = c.len - c.t * kTallKeys - half * 4;
-    if (c.t == c.tiles - 1) {
+    const int left = len - t * kTallKeys - half * 4;
+    if ((t + 1) * kTallKeys > len) {
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -932,14 +923,13 @@ MIA_DEV void tall_body(const Share &sh, TallLds<D, CT, SC> &lds) {
     }
   };
 
-  // ---- end of a piece: final rows, or a partial.  t0: its first tile, c:
-  // its last
-  auto end_piece = [&](const Pos &c, int t0) {
+  // ---- end of a piece: final rows, or a partial
+  auto end_piece = [&](const Piece &c) {
     const SpanParams &p = fresh();
     const float l = sum32(l_run);
     const int rloc = wave * 32 + rl;
     const int r = c.rt * kRows + rloc;
-    if (!p.join && t0 == 0 && c.t == c.tiles - 1) {
+    if (!p.join && c.whole()) {
       if (r >= c.rows) return;
       const int pos = (int)fdiv((uint32_t)r, p.g_div);
       uint16_t *op = p.out + tok_off(p, c.tok0 + pos, p.os_b, p.os_s) +
@@ -958,7 +948,7 @@ MIA_DEV void tall_body(const Share &sh, TallLds<D, CT, SC> &lds) {
         }
       return;
     }
-    const int64_t pr = piece_slot(p, sh, c, t0, tid == 0) + rloc;
+    const int64_t pr = piece_slot(p, sh, c, tid == 0) + rloc;
     if (r >= c.rows || rloc >= p.list[c.li].part_rows) return;
     float *po = p.part_o + pr * D;
 #pragma unroll
@@ -971,44 +961,44 @@ MIA_DEV void tall_body(const Share &sh, TallLds<D, CT, SC> &lds) {
   };
 
   // ---- the stream
-  Pos cur;
-  if (!first_pos(fresh(), sh, cur)) return;
-  Pos nxt = cur;
-  int buf = 0, t0 = cur.t;
-  if (d_used < D) {  // channels past d: zero in all stages, never written again
-    for (int o = tid * 16; o < 2 * STAGES * TILEB; o += kThreads * 16)
+  Piece cur, nxt;
+  if (!first_piece(fresh(), sh, cur)) return;
+  if (d_used < D) {  // channels past d: zero in both stages, never written again
+    for (int o = tid * 16; o < 4 * TILEB; o += kThreads * 16)
       *(lds_u32x4_t *)(base + o) = u32x4_t{0u, 0u, 0u, 0u};
     __syncthreads();
   }
+  load_q(cur);
+  set_keys(cur);
+  int t = cur.t, end = cur.t + cur.n, buf = 0;
+  // The tile behind t, of the next piece behind the last of this one: go: there
+  // is one, anew: it starts piece nxt.
+  int tn = 0;
+  bool go = false, anew = false;
+  auto step = [&]() {
+    tn = t + 1;
+    go = true;
+    anew = false;
+    if (tn < end) return;
+    nxt = cur;
+    go = anew = next_piece(fresh(), sh, nxt);
+    tn = 0;
+    if (go) set_keys(nxt);
+  };
   if constexpr (DMA) {
-    // nxt: the next tile to copy, STAGES - 1 ahead of cur
-    load_q(cur);
-    bool anew = true, more = true;
-    auto copy_next = [&](int stage) {
-      if (!more) return;
-      fetch(nxt, stage, anew);
-      more = has_next(nxt, sh.x1);
-      if (more) {
-        advance(fresh(), nxt);
-        anew = nxt.t == 0;
-      }
-    };
-#pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) copy_next(i);
+    load_tile(t, 0);
     begin_piece(cur);
+    bool at_live = live;
     while (true) {
-      // own copies of tile `cur` have landed (those of the STAGES - 2 tiles
-      // behind it may stay in flight; a narrow call's count of copies varies,
-      // so it waits for all); the barrier makes every thread's visible and
-      // the stage of the tile before free
-      if (STAGES > 2 && d_used == D && more)
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((STAGES - 2) * 2 * NP) : "memory");
-      else
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      // own copies of this tile have landed; the barrier makes every thread's
+      // visible and the other stage free
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
-      copy_next(buf == 0 ? STAGES - 1 : buf - 1);
-      const int left = cur.len - cur.t * kTallKeys;
+      step();
+      if (anew) load_q(nxt);  // (sets live for the next piece)
+      if (go) load_tile(tn, buf ^ 1);
+      const int left = cur.len - t * kTallKeys;
       if (left < kTallKeys) {
         // values past the span are cleared: 0 * NaN would reach the sums
         lds_u8_t *const vb = base + (buf * 2 + 1) * TILEB;
@@ -1018,49 +1008,39 @@ MIA_DEV void tall_body(const Share &sh, TallLds<D, CT, SC> &lds) {
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
       }
-      const bool last = !has_next(cur, sh.x1);
-      const bool ends = last || cur.t + 1 == cur.tiles;
-      const Pos at = cur;
-      const bool at_live = live;
-      if (!last) advance(fresh(), cur);
-      if (ends && !last) load_q(cur);  // (sets live for the next piece)
-      if (at_live) compute(at, buf);
-      if (ends) end_piece(at, t0);
-      if (last) return;
-      if (ends) {
+      if (at_live) compute(t, cur.len, buf);
+      if (!go || anew) {
+        end_piece(cur);
+        if (!go) return;
+        cur = nxt;
+        end = cur.n;
         begin_piece(cur);
-        t0 = 0;
+        at_live = live;
       }
-      buf = buf + 1 == STAGES ? 0 : buf + 1;
+      t = tn;
+      buf ^= 1;
     }
   } else {
-    load_q(cur);
-    fetch(cur, 0, true);
+    load_tile(t, 0);
     begin_piece(cur);
-    store_tile(cur, 0);
-    bool more = has_next(cur, sh.x1);
-    if (more) {
-      advance(fresh(), nxt);
-      fetch(nxt, 0, nxt.t == 0);
-    }
+    store_tile(t, cur.len, 0);
+    step();
+    if (go) load_tile(tn, 0);
     __syncthreads();
     while (true) {
-      const bool ends = !more || nxt.t == 0;
-      if (live) compute(cur, buf);
-      if (ends) {
-        end_piece(cur, t0);
-        if (!more) return;
-        load_q(nxt);  // (ahead of the products its registers would spill others)
-        begin_piece(nxt);
-        t0 = 0;
+      if (live) compute(t, cur.len, buf);
+      if (!go || anew) {
+        end_piece(cur);
+        if (!go) return;
+        cur = nxt;
+        end = cur.n;
+        load_q(cur);  // (ahead of the products its registers would spill others)
+        begin_piece(cur);
       }
-      store_tile(nxt, buf ^ 1);
-      cur = nxt;
-      more = has_next(cur, sh.x1);
-      if (more) {
-        advance(fresh(), nxt);
-        fetch(nxt, 0, nxt.t == 0);
-      }
+      store_tile(tn, cur.len, buf ^ 1);
+      t = tn;
+      step();
+      if (go) load_tile(tn, 0);
       __syncthreads();
       buf ^= 1;
     }
@@ -1121,47 +1101,47 @@ MIA_DEV void thin_body(const Share &sh, ThinLds<D, SC> &lds) {
     ent[0] = ks_.entry(t * kThinKeys);
     ent[1] = ks_.entry(t * kThinKeys + 16);
   };
-  // the groups of the tile at c (its entries are loaded, or c starts a
-  // segment), and the entries of the one behind it
-  auto locate = [&](const Pos &c, bool anew) {
-    if (anew) {
-      ks_.set<SC>(fresh(), c);
-      load_entries(c.t);
-    }
-    g[0].set(ks_, c.t * kThinKeys, ent[0]);
-    g[1].set(ks_, c.t * kThinKeys + 16, ent[1]);
-    if (c.t + 1 < c.tiles) load_entries(c.t + 1);
+  auto set_keys = [&](const Piece &c) {
+    ks_.set<SC>(fresh(), c);
+    load_entries(c.t);
+  };
+  // the groups of tile t of the segment of ks_ (its entries are loaded), and
+  // the entries of the tile behind it
+  auto locate = [&](int t) {
+    g[0].set(ks_, t * kThinKeys, ent[0]);
+    g[1].set(ks_, t * kThinKeys + 16, ent[1]);
+    if ((t + 1) * kThinKeys < ks_.len) load_entries(t + 1);
   };
   // rows past the span read its last key (in bounds) and are masked or
   // cleared later
-  auto load_k = [&](const Pos &c) {
-    const bool full = (c.t + 1) * kThinKeys <= ks_.len;
+  auto load_k = [&](int t) {
+    const bool full = (t + 1) * kThinKeys <= ks_.len;
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       int rr = col;
-      if (!full) rr = min(c.t * kThinKeys + b * 16 + col, ks_.len - 1) - g[b].k16;
+      if (!full) rr = min(t * kThinKeys + b * 16 + col, ks_.len - 1) - g[b].k16;
       // (no condition on a load: the merge of its two results would wait)
 #pragma unroll
       for (int j = 0; j < NK; ++j)
         kr[b][j] = *reinterpret_cast<const u32x4_t *>(g[b].k + (rr * ks_.k_t + kch[j]));
     }
   };
-  auto load_v = [&](const Pos &c) {
-    const bool full = (c.t + 1) * kThinKeys <= ks_.len;
+  auto load_v = [&](int t) {
+    const bool full = (t + 1) * kThinKeys <= ks_.len;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const Group &x = g[j * TL / 16];
       int rr = j * TL % 16 + vtl;
-      if (!full) rr = min(c.t * kThinKeys + j * TL + vtl, ks_.len - 1) - x.k16;
+      if (!full) rr = min(t * kThinKeys + j * TL + vtl, ks_.len - 1) - x.k16;
       vr[j] = *reinterpret_cast<const u32x4_t *>(x.v + (rr * ks_.v_t + vch));
     }
   };
   // lane l: scale of key l (K), of key l - 32 (V)
-  auto load_s = [&](const Pos &c) {
+  auto load_s = [&](int t) {
     if constexpr (SC) {
       const int k = lane & 31;
       const bool hi = k >= 16;
-      const uint32_t rr = min(c.t * kThinKeys + k, ks_.len - 1) - (hi ? g[1].k16 : g[0].k16);
+      const uint32_t rr = min(t * kThinKeys + k, ks_.len - 1) - (hi ? g[1].k16 : g[0].k16);
       const float *ks = hi ? g[1].ks(ks_) : g[0].ks(ks_);
       const float *vs = hi ? g[1].vs(ks_) : g[0].vs(ks_);
       const float *sp = lane < 32 ? ks : vs;
@@ -1176,7 +1156,7 @@ MIA_DEV void thin_body(const Share &sh, ThinLds<D, SC> &lds) {
   float c2 = 0.f;
   u32x4_t qw[NC][KSTEPS];
   // the loads of the rows of a piece, issued ahead of its first tile's
-  auto load_q = [&](const Pos &c) {
+  auto load_q = [&](const Piece &c) {
     const SpanParams &p = fresh();
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
@@ -1193,7 +1173,7 @@ MIA_DEV void thin_body(const Share &sh, ThinLds<D, SC> &lds) {
       }
     }
   };
-  auto begin_piece = [&](const Pos &c) {
+  auto begin_piece = [&](const Piece &c) {
     uint32_t neg;
     c2 = score_factor(fresh(), c.h, neg);
 #pragma unroll
@@ -1242,8 +1222,7 @@ MIA_DEV void thin_body(const Share &sh, ThinLds<D, SC> &lds) {
       }
     }
   };
-  auto store_v = [&](const Pos &c) {
-    const int left = c.len - c.t * kThinKeys;
+  auto store_v = [&](int left) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int t = j * TL + vtl;
@@ -1261,7 +1240,7 @@ MIA_DEV void thin_body(const Share &sh, ThinLds<D, SC> &lds) {
     }
   };
   u32x4_t pk[NC];
-  auto softmax = [&](const Pos &c) {
+  auto softmax = [&](int left0) {
     f32x4_t ks4[2], vs4[2];
     if constexpr (SC) {
 #pragma unroll
@@ -1270,7 +1249,7 @@ MIA_DEV void thin_body(const Share &sh, ThinLds<D, SC> &lds) {
         vs4[b] = *(const lds_f32x4_t *)(sw + 32 + b * 16 + kg * 4);
       }
     }
-    const int left = c.len - c.t * kThinKeys - kg * 4;
+    const int left = left0 - kg * 4;
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
       float mx = -INFINITY;
@@ -1332,10 +1311,10 @@ MIA_DEV void thin_body(const Share &sh, ThinLds<D, SC> &lds) {
             0, 0);
     }
   };
-  auto end_piece = [&](const Pos &c, int t0) {
+  auto end_piece = [&](const Piece &c) {
     const SpanParams &p = fresh();
-    const bool whole = !p.join && t0 == 0 && c.t == c.tiles - 1;
-    const int64_t pr0 = whole ? 0 : piece_slot(p, sh, c, t0, lane == 0);
+    const bool whole = !p.join && c.whole();
+    const int64_t pr0 = whole ? 0 : piece_slot(p, sh, c, lane == 0);
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
       const float l = sum32(sum16(l_run[n]));
@@ -1367,41 +1346,50 @@ MIA_DEV void thin_body(const Share &sh, ThinLds<D, SC> &lds) {
 
   // ---- the stream: K (V) of the next tile is issued once this tile's
   // product (copy to LDS) has freed the registers
-  Pos cur;
-  if (!first_pos(fresh(), sh, cur)) return;
+  Piece cur, nxt;
+  if (!first_piece(fresh(), sh, cur)) return;
   load_q(cur);
-  locate(cur, true);
-  load_k(cur);
-  load_s(cur);
-  load_v(cur);
+  set_keys(cur);
+  int t = cur.t, end = cur.t + cur.n;
+  locate(t);
+  load_k(t);
+  load_s(t);
+  load_v(t);
   begin_piece(cur);
-  int t0 = cur.t;
   while (true) {
-    const bool more = has_next(cur, sh.x1);
-    Pos nxt = cur;
-    if (more) {
-      advance(fresh(), nxt);
-      if (NC == 1 && nxt.t == 0) load_q(nxt);
-      locate(nxt, nxt.t == 0);
+    // the tile behind t, of the next piece behind the last of this one
+    int tn = t + 1;
+    bool go = true, anew = false;
+    if (tn >= end) {
+      nxt = cur;
+      go = anew = next_piece(fresh(), sh, nxt);
+      tn = 0;
+      if (go) {
+        if (NC == 1) load_q(nxt);
+        set_keys(nxt);
+      }
     }
+    if (go) locate(tn);
+    const int left = cur.len - t * kThinKeys;
     scores();
-    if constexpr (SC) sw[lane] = cur.t * kThinKeys + (lane & 31) < cur.len ? sr : 0.f;
-    if (more) {
-      load_k(nxt);
-      load_s(nxt);
+    if constexpr (SC) sw[lane] = (lane & 31) < left ? sr : 0.f;
+    if (go) {
+      load_k(tn);
+      load_s(tn);
     }
-    softmax(cur);
-    store_v(cur);
-    if (more) load_v(nxt);
+    softmax(left);
+    store_v(left);
+    if (go) load_v(tn);
     values();
-    if (!more || nxt.t == 0) {
-      end_piece(cur, t0);
-      if (!more) return;
-      if (NC > 1) load_q(nxt);  // (ahead of the products it would spill)
-      begin_piece(nxt);
-      t0 = 0;
+    if (!go || anew) {
+      end_piece(cur);
+      if (!go) return;
+      cur = nxt;
+      end = cur.n;
+      if (NC > 1) load_q(cur);  // (ahead of the products it would spill)
+      begin_piece(cur);
     }
-    cur = nxt;
+    t = tn;
   }
 }
 
