@@ -701,6 +701,8 @@ int mia_quant_kv_read(const mia_quant_kv_args *args, mia_stream_t stream);
 /* computed) and keys [0, key_lens[i]) in the cache through block_table row  */
 /* i, or, with block_table NULL, in "block" i of a dense [num_seqs, head,    */
 /* block_size, d] tensor.  key_lens are clamped to what the table holds.     */
+/* Table entries outside the pool read its first or last block.  A list      */
+/* cu_seqlens_q that decreases somewhere computes nothing.                   */
 /* Rows of a sequence without keys give 0; rows of no sequence are left as   */
 /* they were.                                                                */
 /* Caches: bf16; e4m3fn with per-head factors k_dequant / v_dequant (NULL =  */
@@ -754,7 +756,7 @@ int mia_cross_attention(const mia_cross_args *args, mia_stream_t stream);
 /* which hold the S active tokens last (already written).  One softmax over  */
 /* both, and the sink logit in the denominator.  Rows without keys give 0.   */
 /* prefix_len is one int32 on the device; lengths are clamped to what the    */
-/* tables hold.  Caches as for mia_cross_attention.                          */
+/* tables hold.  Caches and table entries as for mia_cross_attention.        */
 /* ------------------------------------------------------------------------ */
 typedef struct {
   const void *q; /* bf16 */

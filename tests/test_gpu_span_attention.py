@@ -487,6 +487,28 @@ def test_query_tokens_past_the_maximum(gpu):
     assert (out[4:6] == 5.0).all() and (out[8:] == 5.0).all()
 
 
+@pytest.mark.parametrize("new_max", [2, 64])
+def test_decreasing_first_tokens_compute_nothing(gpu, new_max):
+    """Sequences would share tokens: the rows stay as they were, captured pieces
+    of an earlier call in the workspace included; a rising list is computed."""
+    B, hq, hkv, d, L = 6, 8, 2, 64, 900
+    g = _gen(5)
+    q = _randn(g, B * new_max, hq, d).to(gpu)
+    k, v = (_randn(g, B, hkv, L, d).to(gpu) for _ in range(2))
+    lens = torch.tensor([L, 0, 17, L, 300, L], dtype=torch.int32, device=gpu)
+    rising = torch.arange(B + 1, dtype=torch.int32, device=gpu) * new_max
+    want = cross_attention(q, k, v, lens, cu_seqlens_q=rising, max_seqlen_q=new_max)
+    ws = torch.empty(1 << 28, dtype=torch.uint8, device=gpu)
+    got = cross_attention(q, k, v, lens, cu_seqlens_q=rising, max_seqlen_q=new_max, workspace=ws)
+    assert torch.equal(got, want)
+    falling = rising.clone()
+    falling[3] = 0
+    out = torch.full_like(q, 7.0)
+    cross_attention(q, k, v, lens, cu_seqlens_q=falling, max_seqlen_q=new_max, out=out,
+                    workspace=ws)
+    assert (out == 7.0).all()
+
+
 def test_two_streams_and_a_given_workspace(gpu):
     """Calls at once on two streams; a given workspace is used and gives the
     same bits, one too small is not."""

@@ -248,19 +248,26 @@ MIA_DEV int plan(const SpanParams &p, PlanLds &lds, Share &sh) {
   // (calls of up to 256 sequences: one per thread, kept)
   Seq mine = {0, 0, 0, 0, 0};
   int sum[2] = {0, 0};
-  bool zero = false;
+  bool zero = false, bad = false;
 #pragma nounroll
   for (int u = u0; u < u1; ++u) {
     mine = seq_of(u);
+    if (u >= n0 && p.list[1].cu) {
+      const int32_t *cu = p.list[1].cu + (u - n0);
+      bad |= scalar_load(cu, 1) < scalar_load(cu, 0);
+    }
     sum[0] += mine.thin ? 0 : mine.units;
     sum[1] += mine.thin ? mine.units : 0;
     zero |= mine.len == 0 && mine.rows > 0 && u % grid == b;
   }
+  // (first tokens that decrease would let sequences share tokens: more units
+  // than the host counted, rows written twice; the call then has no tiles)
+  bad = __builtin_amdgcn_ballot_w64(bad) != 0;
   int inc[2], n[2], base[2];
 #pragma unroll
   for (int f = 0; f < 2; ++f) {
     inc[f] = wave_scan(sum[f]);
-    if (lane == 63) lds.tot[f][wave] = inc[f];
+    if (lane == 63) lds.tot[f][wave] = bad ? -1 : inc[f];
   }
   if (tid == 0) lds.empty = 0;
   __syncthreads();
@@ -269,12 +276,14 @@ MIA_DEV int plan(const SpanParams &p, PlanLds &lds, Share &sh) {
   for (int f = 0; f < 2; ++f) {
     n[f] = 0;
     base[f] = inc[f] - sum[f];
+    bad = false;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
       base[f] += w < wave ? lds.tot[f][w] : 0;
       n[f] += lds.tot[f][w];
+      bad |= lds.tot[f][w] < 0;
     }
-    n[f] = readfirstlane(n[f]);
+    n[f] = bad ? 0 : readfirstlane(n[f]);
   }
   // workgroups of each form: in proportion to the costs, whole multiples of
   // the 8 XCDs where there are enough
@@ -340,7 +349,7 @@ MIA_DEV int plan(const SpanParams &p, PlanLds &lds, Share &sh) {
     }
   }
   __syncthreads();
-  if (lds.empty) zero_empty(p);
+  if (lds.empty && !bad) zero_empty(p);
   if (form < 0) return -1;
   const int k = form == 1 ? wave : 0;
   sh.cut = mycut;

@@ -40,7 +40,8 @@ def cross_attention(
     follows them) and clamped to what the table or ``L`` holds;
     ``max_seqlen_q`` bounds the query tokens of a sequence (default: T), those
     past it are not computed.  A sequence without keys gives zeros; rows of
-    ``out`` that belong to no sequence are left as they were.
+    ``out`` that belong to no sequence are left as they were.  A
+    ``cu_seqlens_q`` that decreases somewhere computes nothing.
 
     Caches: bf16; e4m3fn with static per-head scales; e4m3fn or int8 with the
     per-token scales of ``quant_kv_write``.  ``d`` is a multiple of 8 (8-bit
