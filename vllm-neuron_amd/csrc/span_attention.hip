@@ -58,6 +58,11 @@ constexpr int kThinKeys = 32;  // keys per thin tile
 // the compiler reads each right before it: 2048 tokens of 32 heads over 6404
 // keys (d = 128) 246 us, 230 with 2 or 3 ahead.
 constexpr int kAhead = 2;
+// Tall waves issue their products at a lower priority than the rest, so that
+// of a SIMD's two waves the one in its softmax is not held up by the other's
+// products: the same call 234 us at one priority, 226 with the products above
+// and 223 with them below.  (Products of one half of a tile between the
+// softmax of the other, at one priority: 245.)
 
 enum CacheKind { kBf16 = 0, kFp8 = 1, kI8 = 2 };
 
@@ -849,6 +854,7 @@ MIA_DEV void tall_body(const Share &sh, TallLds<D, CT, SC> &lds) {
     };
     // (fragments are read kAhead products ahead, an order held by the
     // scheduling barriers)
+    __builtin_amdgcn_s_setprio(0);
     {
       constexpr int AHEAD = kAhead, N = 2 * KSTEPS;
       bf16x8_t kf[AHEAD + 1];
@@ -864,6 +870,7 @@ MIA_DEV void tall_body(const Share &sh, TallLds<D, CT, SC> &lds) {
         __builtin_amdgcn_sched_barrier(0);
       }
     }
+    __builtin_amdgcn_s_setprio(1);
     if constexpr (SC) {
 #pragma unroll
       for (int b = 0; b < 2; ++b)
@@ -936,6 +943,7 @@ MIA_DEV void tall_body(const Share &sh, TallLds<D, CT, SC> &lds) {
     const float psum = exps();
     l_run += psum;
     // O^T += V^T . P^T
+    __builtin_amdgcn_s_setprio(0);
     {
       constexpr int AHEAD = kAhead, N = 4 * DBLK;
       bf16x8_t vf[AHEAD + 1];
@@ -953,6 +961,7 @@ MIA_DEV void tall_body(const Share &sh, TallLds<D, CT, SC> &lds) {
         __builtin_amdgcn_sched_barrier(0);
       }
     }
+    __builtin_amdgcn_s_setprio(1);
   };
 
   // ---- end of a piece: final rows, or a partial
