@@ -1724,15 +1724,16 @@ Layout span_layout(SpanParams &p, int D) {
       hdr += units * kHdr;
     }
   }
-  // Measured: a thin tile takes a wave 1.7 us and a tall one a workgroup 1.8
-  // us at d = 64 (4 and 2.6 us at d = 128), side by side.  64 rows behind 8192
-  // keys (d = 128): 54.2 us at 0.33, 55.8 at 0.41, 58.7 at 0.5; 128 rows
-  // behind 4133 (d = 64): 47.0 at 0.22 and 0.28, 45.5 at 0.35.  A segment's
-  // start costs about two tiles at d = 128 (one: 57.1 and 124.3 us for the 16
-  // drafted int8 rows, two: 55.8 and 120) and for tall ones at d = 64 (ragged
-  // prompts 33.1 against 34.4), one for thin ones there (45.0 against 47.0).
-  // Shares of six units and more leave CUs idle on short calls (15.6 -> 18.3).
-  p.cost[0] = 1.0f, p.cost[1] = 0.35f;
+  // Measured, side by side: a thin tile takes a wave 2.3 us and a tall one a
+  // workgroup 1.7 us at d = 64 (3.8 and 2.6 us at d = 128).  Thin costs of
+  // 0.30 / 0.35 / 0.40 / 0.45: 64 rows behind 8192 keys (d = 128) 53.8 / 53.5 /
+  // 53.1 / 53.2 us; 128 rows behind 4133 (d = 64) 44.9 / 44.2 / 44.1 / 44.7; 64
+  // drafted int8 rows behind 32768 127.3 / 119.9 / 119.7 / 122.7.  A segment's
+  // start costs about two tiles (tall, three: ragged prompts of d = 80 61.4 us
+  // against 59.8; thin at d = 128, one: 57.1 against 55.8), one for thin ones at
+  // d = 64 (45.0 against 47.0).  Shares of six units and more leave CUs idle
+  // on short calls (15.6 -> 18.3).
+  p.cost[0] = 1.0f, p.cost[1] = 0.40f;
   p.over[0] = 2, p.over[1] = D == 64 ? 1 : 2;
   p.least[0] = 4, p.least[1] = D == 64 ? 3 : 4;
   w.hdr = 0;
