@@ -131,7 +131,7 @@ int mia_kv_write(const mia_kv_write_args *args, mia_stream_t stream);
 /* ------------------------------------------------------------------------ */
 typedef struct {
   const void *cache;
-  int32_t cache_dtype;
+  int32_t cache_dtype; /* BF16, F16, F32 or FP8_E4M3FN */
   int32_t k_packed;
   int64_t cache_stride[5];
   const int32_t *block_table;
