@@ -59,6 +59,15 @@ struct RowPos {
   int64_t slot, blk, off;
 };
 
+// Workgroups of a launch lie in rows of at most kGridX: a grid of 2^32 threads
+// or more along x is cut to its low 32 bits without an error, and 2^26 rows of
+// 64 lanes are that many.
+constexpr uint32_t kGridX = 1u << 23;
+template <int LPR>
+MIA_DEV uint32_t row_of() {
+  return (blockIdx.y * gridDim.x + blockIdx.x) * (256 / LPR) + threadIdx.x / LPR;
+}
+
 // Row `row` of the call and its place in the cache (slot < 0: a sentinel).
 MIA_DEV RowPos row_pos(const QuantKParams &p, uint32_t row) {
   RowPos r;
@@ -128,7 +137,7 @@ MIA_DEV void load8(const uint8_t *row, int64_t sd, int c0, int d, float (&x)[8])
 // (cache: 8-byte) aligned.
 template <int SRC, bool I8, int LPR, bool VEC>
 __global__ __launch_bounds__(256) void quant_write_kernel(QuantKParams p) {
-  const uint32_t row = blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
+  const uint32_t row = row_of<LPR>();
   const int c0 = (threadIdx.x % LPR) * 8;
   const bool in = row < p.n_rows;
   const RowPos r = row_pos(p, in ? row : 0);
@@ -203,7 +212,7 @@ __global__ __launch_bounds__(256) void quant_write_kernel(QuantKParams p) {
 
 template <int DST, bool I8, int LPR, bool VEC>
 __global__ __launch_bounds__(256) void quant_read_kernel(QuantKParams p) {
-  const uint32_t row = blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
+  const uint32_t row = row_of<LPR>();
   const int c0 = (threadIdx.x % LPR) * 8;
   if (row >= p.n_rows || c0 >= p.d) return;
   const RowPos r = row_pos(p, row);
@@ -305,7 +314,8 @@ QuantKParams kparams(const mia_quant_kv_args &a) {
 
 template <int DT, bool I8, int LPR, bool VEC>
 void launch_one(const QuantKParams &p, bool write, hipStream_t s) {
-  const dim3 grid((p.n_rows + 256 / LPR - 1) / (256 / LPR));
+  const uint32_t n = (p.n_rows + 256 / LPR - 1) / (256 / LPR), x = std::min(n, kGridX);
+  const dim3 grid(x, (n + x - 1) / x);
   if (write) quant_write_kernel<DT, I8, LPR, VEC><<<grid, 256, 0, s>>>(p);
   else quant_read_kernel<DT, I8, LPR, VEC><<<grid, 256, 0, s>>>(p);
 }
