@@ -757,6 +757,7 @@ int mia_cross_attention(const mia_cross_args *args, mia_stream_t stream);
 /* both, and the sink logit in the denominator.  Rows without keys give 0.   */
 /* prefix_len is one int32 on the device; lengths are clamped to what the    */
 /* tables hold.  Caches and table entries as for mia_cross_attention.        */
+/* batch * s_active * num_q_heads < 2^26.                                    */
 /* ------------------------------------------------------------------------ */
 typedef struct {
   const void *q; /* bf16 */

@@ -784,6 +784,9 @@ static int validate_shared_prefix(const mia_shared_prefix_args *a) {
   const int64_t tokens = (int64_t)a->batch * a->s_active;
   const int rc = check_span(*a, a->q_stride, a->out_stride, extents, 3, tokens, true);
   if (rc) return rc;
+  // the join's 64 threads per row and head lie along one grid axis (2^32)
+  MIA_REQUIRE(tokens * a->num_q_heads < (1ll << 26), MIA_ERR_VALUE,
+              "shared_prefix: query tokens * heads beyond 2^26");
   // as for cross attention
   const int64_t G = a->num_q_heads / a->num_kv_heads;
   const int64_t row_tiles = tokens * G / 32 + a->batch + 1;

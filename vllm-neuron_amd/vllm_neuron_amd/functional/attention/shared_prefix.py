@@ -43,7 +43,8 @@ def shared_prefix_attention(
     any key gives zeros.  Lengths are read on the device (a captured call
     follows them) and clamped to what the tables hold.
 
-    Caches as for ``cross_attention``; at most 64 new tokens per row.
+    Caches as for ``cross_attention``; at most 64 new tokens per row, and fewer
+    than 2^26 (token, head) rows in a call.
     """
     return K.shared_prefix_attention(
         q, k_cache, v_cache, prefix_table, prefix_len, block_table, seq_lens,
