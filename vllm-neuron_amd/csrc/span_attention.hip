@@ -188,7 +188,6 @@ struct Share {
 struct PlanLds {
   int tot[2][kWaves];
   int seq[kWaves], first[kWaves], len[kWaves], tok0[kWaves], rows[kWaves];
-  int empty;
 };
 
 // Inclusive scan over the wave: shifts inside rows of 16 lanes, then the row
@@ -204,22 +203,19 @@ MIA_DEV int wave_scan(int x) {
   return x;
 }
 
-// Rows of sequences without any key (cross attention): zeros.
-MIA_DEV void zero_empty(const SpanParams &p) {
-  const SpanList &l = p.list[1];
-  for (int i = blockIdx.x; i < l.n; i += gridDim.x) {
-    if (list_len(l, i) > 0) continue;
-    const int2 tk = list_tokens(l, i, p.num_tokens);
-    const int c8 = p.d / 8, hq = p.Hkv * p.G;
-    const int per_tok = hq * c8;
-    for (int t = tk.x; t < tk.x + tk.y; ++t)
-      for (int k = threadIdx.x; k < per_tok; k += kThreads) {
-        const int h = k / c8, c = k - h * c8;
-        const int b = (int)fdiv((uint32_t)t, p.s_div);
-        uint16_t *op = p.out + (int64_t)b * p.os_b + (int64_t)(t - b * p.S) * p.os_s +
-                       (int64_t)h * p.os_h + c * 8;
-        *reinterpret_cast<u32x2_t *>(op) = u32x2_t{0u, 0u};
-        *reinterpret_cast<u32x2_t *>(op + 4) = u32x2_t{0u, 0u};
+// Zeros in the output rows of tokens [t0, t1); a wave calls it.
+MIA_DEV void zero_rows(const SpanParams &p, int t0, int t1) {
+  const int lane = threadIdx.x & 63;
+  const int c8 = p.d / 8, heads = 64 / c8;  // 16-byte chunks of a head, heads at once
+  const int h0 = lane / c8, c = lane - h0 * c8;
+  for (int t = t0; t < t1; ++t) {
+    const int b = (int)fdiv((uint32_t)t, p.s_div);
+    uint16_t *op = p.out + (int64_t)b * p.os_b + (int64_t)(t - b * p.S) * p.os_s + c * 8;
+    if (h0 < heads)
+      for (int h = h0; h < p.Hkv * p.G; h += heads) {
+        u32x2_t *x = reinterpret_cast<u32x2_t *>(op + (int64_t)h * p.os_h);
+        x[0] = u32x2_t{0u, 0u};
+        x[1] = u32x2_t{0u, 0u};
       }
   }
 }
@@ -256,10 +252,26 @@ MIA_DEV int plan(const SpanParams &p, PlanLds &lds, Share &sh) {
     q.units = kt ? (kt + p.over[l.thin]) * row_tiles(l, q.rows) * p.Hkv : 0;
     return q;
   };
+  // The tokens [x, y) of sequence u that this workgroup clears: those of a
+  // sequence without any key (cross attention) in equal runs over the launch,
+  // from workgroup `at` = u % grid on.
+  auto cleared = [&](int at, const Seq &q) {
+    int2 t = {0, 0};
+    if (q.len == 0 && q.rows > 0 && !p.join) {
+      const int n = (int)fdiv((uint32_t)q.rows, p.g_div);
+      const int each = n <= grid ? 1 : (n + grid - 1) / grid;
+      const int k = b < at ? b - at + grid : b - at;
+      t.x = q.tok0 + min(k * each, n);
+      t.y = q.tok0 + min((k + 1) * each, n);
+    }
+    return t;
+  };
   // (calls of up to 256 sequences: one per thread, kept)
   Seq mine = {0, 0, 0, 0, 0};
   int sum[2] = {0, 0};
-  bool zero = false, bad = false;
+  int2 zero = {0, 0};  // tokens to be cleared, of the last such sequence
+  bool more = false, bad = false;
+  int at = u0 < grid ? u0 : u0 % grid;
 #pragma nounroll
   for (int u = u0; u < u1; ++u) {
     mine = seq_of(u);
@@ -269,7 +281,12 @@ MIA_DEV int plan(const SpanParams &p, PlanLds &lds, Share &sh) {
     }
     sum[0] += mine.thin ? 0 : mine.units;
     sum[1] += mine.thin ? mine.units : 0;
-    zero |= mine.len == 0 && mine.rows > 0 && u % grid == b;
+    const int2 t = cleared(at, mine);
+    if (t.x < t.y) {
+      more |= zero.x < zero.y;
+      zero = t;
+    }
+    at = at + 1 == grid ? 0 : at + 1;
   }
   // (first tokens that decrease would let sequences share tokens: more units
   // than the host counted, rows written twice; the call then has no tiles)
@@ -280,9 +297,7 @@ MIA_DEV int plan(const SpanParams &p, PlanLds &lds, Share &sh) {
     inc[f] = wave_scan(sum[f]);
     if (lane == 63) lds.tot[f][wave] = bad ? -1 : inc[f];
   }
-  if (tid == 0) lds.empty = 0;
   __syncthreads();
-  if (zero && !p.join) lds.empty = 1;
 #pragma unroll
   for (int f = 0; f < 2; ++f) {
     n[f] = 0;
@@ -360,7 +375,27 @@ MIA_DEV int plan(const SpanParams &p, PlanLds &lds, Share &sh) {
     }
   }
   __syncthreads();
-  if (lds.empty && !bad) zero_empty(p);
+  // (2048 tokens of 32 heads, d = 128, beside 16 with keys: 32 us, by one
+  // workgroup 705)
+  auto clear = [&](int2 t) {
+    uint64_t left = __builtin_amdgcn_ballot_w64(t.x < t.y);
+    while (left) {
+      const int src = __builtin_ctzll(left);
+      left &= left - 1;
+      zero_rows(p, __builtin_amdgcn_readlane(t.x, src), __builtin_amdgcn_readlane(t.y, src));
+    }
+  };
+  if (!bad) {
+    clear(zero);
+    if (__builtin_amdgcn_ballot_w64(more)) {  // (a thread of several sequences)
+      at = u0 < grid ? u0 : u0 % grid;
+#pragma nounroll
+      for (int u = u0; u < u0 + per; ++u) {
+        clear(u < u1 ? cleared(at, seq_of(u)) : int2{0, 0});
+        at = at + 1 == grid ? 0 : at + 1;
+      }
+    }
+  }
   if (form < 0) return -1;
   const int k = form == 1 ? wave : 0;
   sh.cut = mycut;
