@@ -703,8 +703,9 @@ int mia_quant_kv_read(const mia_quant_kv_args *args, mia_stream_t stream);
 /* block_size, d] tensor.  key_lens are clamped to what the table holds.     */
 /* Table entries outside the pool read its first or last block.  A list      */
 /* cu_seqlens_q that decreases somewhere computes nothing.                   */
-/* Rows of a sequence without keys give 0; rows of no sequence are left as   */
-/* they were.                                                                */
+/* Rows of a sequence without keys give 0; rows that nothing computes (past  */
+/* max_seqlen_q, of no sequence) stay as they were, or give 0 with zero_rest.*/
+/* A call with num_seqs = 0 writes nothing.                                  */
 /* Caches: bf16; e4m3fn with per-head factors k_dequant / v_dequant (NULL =  */
 /* 1) or with the per-token scales of mia_quant_kv_write; int8 with those.   */
 /* head_dim: a multiple of 8 (8-bit caches: 16) up to 128.  With a table,    */
@@ -740,7 +741,7 @@ typedef struct {
   const float *k_dequant; /* [Hkv] or NULL */
   const float *v_dequant;
   float softmax_scale;
-  int32_t _pad0;
+  int32_t zero_rest; /* nonzero: rows that nothing computes give 0 */
   void *workspace; /* mia_cross_workspace_bytes(), 256-byte aligned */
   size_t workspace_bytes;
 } mia_cross_args;

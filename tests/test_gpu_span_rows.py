@@ -1,4 +1,5 @@
-"""Rows that no key reaches: sequences without keys beside ordinary ones."""
+"""Rows that no key reaches (sequences without keys beside ordinary ones) and
+rows that nothing computes."""
 import random
 
 import pytest
@@ -80,3 +81,114 @@ def test_a_prompt_without_keys_costs_no_more_than_one_with_keys(gpu):
     call = lambda lens: lambda: cross_attention(q, k, k, lens, cu_seqlens_q=cu, max_seqlen_q=2048, out=out)
     none, one = _median(call(_i32(gpu, 0, 400))), _median(call(_i32(gpu, 1, 400)))
     assert none <= 4 * one, (none, one)
+
+
+def _into_used_memory(q, *args, **kw):
+    """A call without ``out`` whose output takes memory that held sevens."""
+    used = torch.full(q.shape, 7.0, dtype=BF, device=q.device)
+    del used
+    return cross_attention(q, *args, **kw)
+
+
+def _computed(cu, most, T):
+    """Tokens that the call computes, by sequence."""
+    if any(b < a for a, b in zip(cu, cu[1:])):
+        return []
+    clip = lambda x: min(max(x, 0), T)
+    return [(clip(a), min(clip(b), clip(a) + most)) for a, b in zip(cu, cu[1:])]
+
+
+@pytest.mark.parametrize("cu,most", [
+    ([0, 4, 9, 9, 12], 12),          # rows behind the last sequence
+    ([3, 4, 9, 9, 20], 20),          # and before the first
+    ([0, 6, 9, 15, 20], 4),          # past the maximum
+    ([-5, 6, 9, 15, 99], 4),
+    ([20, 20, 20, 20, 20], 3),       # sequences without tokens
+    ([0, 9, 5, 15, 20], 20),         # a list that decreases
+])
+def test_rows_of_an_allocated_output(gpu, cu, most):
+    """Rows that nothing computes are zeros there, and stay in a given one."""
+    T, B, hq, hkv, d, L = 20, 4, 6, 2, 80, 33
+    q, k, v = _randn(1, T, hq, d), _randn(2, B, hkv, L, d), _randn(3, B, hkv, L, d)
+    lens = [33, 7, 5, 0]
+    args = (q.to(gpu), k.to(gpu), v.to(gpu), _i32(gpu, *lens))
+    kw = dict(cu_seqlens_q=_i32(gpu, *cu), max_seqlen_q=most)
+    got = _into_used_memory(*args, **kw)
+    kept = cross_attention(*args, out=torch.full((T, hq, d), 7.0, dtype=BF, device=gpu), **kw)
+    rest = torch.ones(T, dtype=torch.bool)
+    for i, (a, b) in enumerate(_computed(cu, most, T)):
+        rest[a:b] = False
+        n = lens[i]
+        o, bound = attend(q[a:b], k[i, :, :n].transpose(0, 1).double(), v[i, :, :n].transpose(0, 1).double(),
+                          d ** -0.5)
+        check(got[a:b], o, bound, f"sequence {i}")
+        assert torch.equal(got[a:b], kept[a:b])
+    assert (got.cpu()[rest] == 0).all() and (kept.cpu()[rest] == 7.0).all()
+
+
+def test_more_tokens_than_sequences(gpu):
+    """One token each without a list of first tokens; no sequence at all; one
+    row tile form and the other, and more rows than workgroups."""
+    hq, hkv, d, L = 4, 2, 64, 20
+    q = _randn(1, 3000, hq, d).to(gpu)
+    k = _randn(2, 5, hkv, L, d).to(gpu)
+    got = _into_used_memory(q, k, k, _i32(gpu, 20, 3, 0, 9, 20))
+    assert (got[5:] == 0).all() and (got[2] == 0).all() and (got[[0, 1, 3, 4]] != 0).any(-1).all()
+    none = _into_used_memory(q, k, k, _i32(gpu))
+    assert (none == 0).all()
+    tall = _into_used_memory(q, k, k, _i32(gpu, 20, 3, 0, 9, 20), cu_seqlens_q=_i32(gpu, 0, 40, 41, 90, 91, 130))
+    assert (tall[130:] == 0).all() and (tall[41:90] == 0).all() and (tall[:41] != 0).any(-1).all()
+
+
+def test_many_sequences_past_the_maximum(gpu):
+    """Several sequences to a thread of the plan, each with rows left over."""
+    r = random.Random(7)
+    cu = [2]
+    for _ in range(600):
+        cu.append(cu[-1] + r.choice([0, 1, 2, 5]))
+    T, most = cu[-1] + 3, 2
+    q, k = _randn(1, T, 2, 16), _randn(2, 600, 1, 9, 16)
+    lens = [r.choice([0, 4, 9]) for _ in range(600)]
+    got = _into_used_memory(q.to(gpu), k.to(gpu), k.to(gpu), _i32(gpu, *lens), cu_seqlens_q=_i32(gpu, *cu),
+                            max_seqlen_q=most).cpu()
+    rest = torch.ones(T, dtype=torch.bool)
+    for i, (a, b) in enumerate(_computed(cu, most, T)):
+        if lens[i]:
+            rest[a:b] = False
+            kk = k[i, :, :lens[i]].transpose(0, 1).double()
+            check(got[a:b], *attend(q[a:b], kk, kk, 0.25), f"sequence {i}")
+    assert (got[rest] == 0).all()
+
+
+def test_padded_batch_in_a_graph(gpu):
+    """A captured call without ``out``: replays clear what earlier ones wrote."""
+    T, B, hq, hkv, d, L = 64, 3, 4, 2, 64, 50
+    q, k = _randn(1, T, hq, d).to(gpu), _randn(2, B, hkv, L, d).to(gpu)
+    lens, cu = _i32(gpu, 50, 50, 50), _i32(gpu, 0, 20, 40, 64)
+    call = lambda: cross_attention(q, k, k, lens, cu_seqlens_q=cu, max_seqlen_q=24)
+    call()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = call()
+    for ends in ([20, 40, 64], [1, 2, 3], [5, 5, 9], [30, 40, 64], [9, 3, 4], [0, 0, 64]):
+        cu.copy_(torch.tensor([0] + ends, dtype=torch.int32))
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, call())
+        done = _computed([0] + ends, 24, T)
+        rest = torch.ones(T, dtype=torch.bool)
+        for a, b in done:
+            rest[a:b] = False
+        assert (out.cpu()[rest] == 0).all() and (out.cpu()[~rest] != 0).any(-1).all()
+
+
+def test_compiled_call_clears_its_rows(gpu):
+    q, k = _randn(1, 10, 4, 64).to(gpu), _randn(2, 2, 2, 20, 64).to(gpu)
+    lens, cu = _i32(gpu, 20, 20), _i32(gpu, 2, 3, 7)
+    step = torch.compile(lambda q: cross_attention(q, k, k, lens, cu_seqlens_q=cu) + 1, fullgraph=True,
+                         backend="aot_eager")
+    want = cross_attention(q, k, k, lens, cu_seqlens_q=cu) + 1
+    got = step(q)
+    assert torch.equal(want, got)
+    assert (got[:2] == 1).all() and (got[7:] == 1).all()

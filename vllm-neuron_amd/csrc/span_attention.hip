@@ -109,6 +109,7 @@ struct SpanParams {
   float scale_log2;
   SpanList list[2];
   int join;        // every piece goes to the workspace (rows have several spans)
+  int zero_rest;   // cross attention: rows that nothing computes are cleared
   float cost[2];   // time of a tall tile per workgroup, of a thin one per wave
   int over[2];     // cost of a segment's start in tiles (stores, query rows, table)
   int least[2];    // units of a share at least
@@ -252,19 +253,29 @@ MIA_DEV int plan(const SpanParams &p, PlanLds &lds, Share &sh) {
     q.units = kt ? (kt + p.over[l.thin]) * row_tiles(l, q.rows) * p.Hkv : 0;
     return q;
   };
-  // The tokens [x, y) of sequence u that this workgroup clears: those of a
-  // sequence without any key (cross attention) in equal runs over the launch,
-  // from workgroup `at` = u % grid on.
-  auto cleared = [&](int at, const Seq &q) {
+  // This workgroup's part of tokens [x, y): equal runs over the launch, from
+  // workgroup `at` (below grid) on.
+  auto part = [&](int x, int y, int at) {
+    const int n = max(y - x, 0);
+    const int each = n <= grid ? 1 : (n + grid - 1) / grid;
+    const int k = b < at ? b - at + grid : b - at;
+    return make_int2(x + min(k * each, n), x + min((k + 1) * each, n));
+  };
+  // The tokens of sequence u that it clears (cross attention): those of a
+  // sequence without any key and, with zero_rest, those up to the next sequence
+  // that nothing computes.
+  auto cleared = [&](int u, int at, const Seq &q) {
     int2 t = {0, 0};
-    if (q.len == 0 && q.rows > 0 && !p.join) {
-      const int n = (int)fdiv((uint32_t)q.rows, p.g_div);
-      const int each = n <= grid ? 1 : (n + grid - 1) / grid;
-      const int k = b < at ? b - at + grid : b - at;
-      t.x = q.tok0 + min(k * each, n);
-      t.y = q.tok0 + min((k + 1) * each, n);
+    if (p.join) return t;
+    const SpanList &l = p.list[1];
+    const int i = u - n0;
+    t.y = q.tok0 + (int)fdiv((uint32_t)q.rows, p.g_div);
+    t.x = q.len == 0 ? q.tok0 : t.y;
+    if (p.zero_rest) {
+      if (i == l.n - 1) t.y = p.num_tokens;
+      else if (l.cu) t.y = min(max(scalar_load(l.cu, i + 1), t.y), p.num_tokens);
     }
-    return t;
+    return t.x < t.y ? part(t.x, t.y, at) : t;
   };
   // (calls of up to 256 sequences: one per thread, kept)
   Seq mine = {0, 0, 0, 0, 0};
@@ -281,7 +292,7 @@ MIA_DEV int plan(const SpanParams &p, PlanLds &lds, Share &sh) {
     }
     sum[0] += mine.thin ? 0 : mine.units;
     sum[1] += mine.thin ? mine.units : 0;
-    const int2 t = cleared(at, mine);
+    const int2 t = cleared(u, at, mine);
     if (t.x < t.y) {
       more |= zero.x < zero.y;
       zero = t;
@@ -385,13 +396,19 @@ MIA_DEV int plan(const SpanParams &p, PlanLds &lds, Share &sh) {
       zero_rows(p, __builtin_amdgcn_readlane(t.x, src), __builtin_amdgcn_readlane(t.y, src));
     }
   };
+  if (p.zero_rest && wave == 0) {  // tokens before the first sequence, or all
+    const int head = bad ? p.num_tokens
+                         : p.list[1].cu ? min(max(scalar_load(p.list[1].cu, 0), 0), p.num_tokens) : 0;
+    const int2 t = part(0, head, 0);
+    if (t.x < t.y) zero_rows(p, t.x, t.y);
+  }
   if (!bad) {
     clear(zero);
     if (__builtin_amdgcn_ballot_w64(more)) {  // (a thread of several sequences)
       at = u0 < grid ? u0 : u0 % grid;
 #pragma nounroll
       for (int u = u0; u < u0 + per; ++u) {
-        clear(u < u1 ? cleared(at, seq_of(u)) : int2{0, 0});
+        clear(u < u1 ? cleared(u, at, seq_of(u)) : int2{0, 0});
         at = at + 1 == grid ? 0 : at + 1;
       }
     }
@@ -1810,6 +1827,7 @@ SpanParams cross_params(const mia_cross_args &a) {
   SpanParams p = {};
   set_cache(p, a);
   p.num_tokens = a.num_tokens, p.S = 1;
+  p.zero_rest = a.zero_rest;
   p.s_div = make_fastdiv(1);
   p.qs_b = a.q_stride[0], p.qs_s = 0, p.qs_h = a.q_stride[1];
   p.os_b = a.out_stride[0], p.os_s = 0, p.os_h = a.out_stride[1];

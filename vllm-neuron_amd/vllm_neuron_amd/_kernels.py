@@ -1141,8 +1141,9 @@ def _span_launch(a, query, launch, what, workspace, dev) -> None:
 
 def cross_attention(q, k_cache, v_cache, key_lens, out, *, softmax_scale, block_table=None,
                     cu_seqlens_q=None, max_seqlen_q=0, k_scales=None, v_scales=None,
-                    k_dequant=None, v_dequant=None, workspace=None) -> None:
-    """Attention of ``q [T, Hq, d]`` over ragged keys into ``out``."""
+                    k_dequant=None, v_dequant=None, workspace=None, zero_rest=False) -> None:
+    """Attention of ``q [T, Hq, d]`` over ragged keys into ``out``; rows of no
+    sequence stay as they were, or are cleared (``zero_rest``)."""
     dev = N.same_gpu(q, k_cache, v_cache, key_lens, out, block_table, cu_seqlens_q, k_scales,
                      v_scales, k_dequant, v_dequant, workspace)
     if q.dim() != 3:
@@ -1173,7 +1174,7 @@ def cross_attention(q, k_cache, v_cache, key_lens, out, *, softmax_scale, block_
         a, 0, q.data_ptr(), *q.stride(), out.data_ptr(), *out.stride(), T, n, cu, max_seqlen_q,
         hq, hkv, d, k_cache.data_ptr(), v_cache.data_ptr(), code, nb, *k_cache.stride(),
         *v_cache.stride(), bs, nblk, table, *bts, key_lens.data_ptr(), *scales, N.ptr(kd) or 0,
-        N.ptr(vd) or 0, softmax_scale, 0, 0, 0)
+        N.ptr(vd) or 0, softmax_scale, int(zero_rest), 0, 0)
     L = N.lib()
     _span_launch(a, L.mia_cross_workspace_bytes, L.mia_cross_attention, "cross_attention",
                  workspace, dev)

@@ -234,7 +234,7 @@ class CrossArgs(ctypes.Structure):
         ("block_size", c_i32), ("blocks_per_seq", c_i32), ("block_table", c_vp),
         ("bt_stride", c_i64 * 2), ("key_lens", c_vp), ("k_scales", c_vp), ("v_scales", c_vp),
         ("k_scale_stride", c_i64 * 3), ("v_scale_stride", c_i64 * 3),
-        ("k_dequant", c_vp), ("v_dequant", c_vp), ("softmax_scale", c_f32), ("_pad0", c_i32),
+        ("k_dequant", c_vp), ("v_dequant", c_vp), ("softmax_scale", c_f32), ("zero_rest", c_i32),
         ("workspace", c_vp), ("workspace_bytes", ctypes.c_size_t),
     ]
 

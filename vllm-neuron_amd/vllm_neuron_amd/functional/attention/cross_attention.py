@@ -39,9 +39,10 @@ def cross_attention(
     ``k``/``v`` are dense.  Lengths are read on the device (a captured call
     follows them) and clamped to what the table or ``L`` holds;
     ``max_seqlen_q`` bounds the query tokens of a sequence (default: T), those
-    past it are not computed.  A sequence without keys gives zeros; rows of
-    ``out`` that belong to no sequence are left as they were.  A
-    ``cu_seqlens_q`` that decreases somewhere computes nothing.
+    past it are not computed.  A sequence without keys gives zeros.  Rows that
+    nothing computes (past the maximum, or of no sequence) stay as they were in
+    a given ``out`` and are zeros in the returned tensor otherwise; a
+    ``cu_seqlens_q`` that decreases somewhere computes nothing at all.
 
     Caches: bf16; e4m3fn with static per-head scales; e4m3fn or int8 with the
     per-token scales of ``quant_kv_write``.  ``d`` is a multiple of 8 (8-bit

@@ -603,35 +603,41 @@ def _cross_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, key_lens: Tens
                      k_scales: Optional[Tensor], v_scales: Optional[Tensor],
                      k_dequant: Optional[Tensor], v_dequant: Optional[Tensor],
                      workspace: Optional[Tensor], max_seqlen_q: int,
-                     softmax_scale: float) -> None:
+                     softmax_scale: float, zero_rest: bool = False) -> None:
     K.cross_attention(q, k_cache, v_cache, key_lens, out, softmax_scale=softmax_scale,
                       block_table=block_table, cu_seqlens_q=cu_seqlens_q,
                       max_seqlen_q=max_seqlen_q, k_scales=k_scales, v_scales=v_scales,
-                      k_dequant=k_dequant, v_dequant=v_dequant, workspace=workspace)
+                      k_dequant=k_dequant, v_dequant=v_dequant, workspace=workspace,
+                      zero_rest=zero_rest)
 
 
 @_cross_attention.register_fake
 def _(q, k_cache, v_cache, key_lens, out, block_table, cu_seqlens_q, k_scales, v_scales,
-      k_dequant, v_dequant, workspace, max_seqlen_q, softmax_scale):
+      k_dequant, v_dequant, workspace, max_seqlen_q, softmax_scale, zero_rest=False):
     return None
 
 
 def cross_attention(q, k_cache, v_cache, key_lens, *, softmax_scale: float, block_table=None,
                     cu_seqlens_q=None, max_seqlen_q: int = 0, k_scales=None, v_scales=None,
                     k_dequant=None, v_dequant=None, out=None, workspace=None) -> Tensor:
-    if out is None:
-        out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+    # an output allocated here has no row of unknown memory: the launch clears
+    # those of no sequence (without any sequence there is no launch)
+    rest = out is None
+    if rest:
+        new = torch.empty if key_lens.numel() else torch.zeros
+        out = new(q.shape, dtype=torch.bfloat16, device=q.device)
     if _plain(q, k_cache, v_cache, key_lens, out, block_table, cu_seqlens_q, k_scales, v_scales,
               k_dequant, v_dequant, workspace):
         K.cross_attention(q, k_cache, v_cache, key_lens, out, softmax_scale=float(softmax_scale),
                           block_table=block_table, cu_seqlens_q=cu_seqlens_q,
                           max_seqlen_q=int(max_seqlen_q), k_scales=k_scales, v_scales=v_scales,
-                          k_dequant=k_dequant, v_dequant=v_dequant, workspace=workspace)
+                          k_dequant=k_dequant, v_dequant=v_dequant, workspace=workspace,
+                          zero_rest=rest)
         _written(out, workspace)
         return out
     _cross_attention(q, k_cache, v_cache, key_lens, out, block_table, cu_seqlens_q, k_scales,
                      v_scales, k_dequant, v_dequant, workspace, int(max_seqlen_q),
-                     float(softmax_scale))
+                     float(softmax_scale), rest)
     return out
 
 
