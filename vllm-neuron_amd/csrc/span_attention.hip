@@ -1758,10 +1758,7 @@ Layout span_layout(SpanParams &p, int D) {
   int64_t rows = 0, hdr = kHdr;
   for (int li = 0; li < 2; ++li) {
     SpanList &l = p.list[li];
-    if (l.n == 0) {
-      l.thin = p.list[1].thin;
-      continue;
-    }
+    if (l.n == 0) continue;
     const int64_t seq_rows = (int64_t)l.tok_max * p.G;
     l.thin = seq_rows <= 32;
     const int64_t units = (int64_t)w.grid * (l.thin ? kWaves : 1);
