@@ -66,9 +66,8 @@ constexpr int kThinKeys = 32;  // keys per thin tile
 constexpr int kAhead = 2;
 // Tall waves issue their products at a lower priority than the rest, so that
 // of a SIMD's two waves the one in its softmax is not held up by the other's
-// products: the same call 234 us at one priority, 226 with the products above
-// and 223 with them below.  (Products of one half of a tile between the
-// softmax of the other, at one priority: 245.)
+// products: the same call, eager on one box, 220 us at one priority, 211 with
+// the products above the rest and 210 with them below.
 
 enum CacheKind { kBf16 = 0, kFp8 = 1, kI8 = 2 };
 
@@ -1877,10 +1876,12 @@ void launch_span(const SpanParams &p, int grid, hipStream_t s) {
     else span_kernel<D, CT, SC, D, 2><<<grid, kThreads, 0, s>>>(p);
   }
   if (p.join) {
-    // Lane groups per row: as many as one round of resident waves (8 per SIMD)
-    // holds, since a row's pieces are loaded one after the other within a
-    // group.  128 rows of 64 heads, d = 64: 14.4 us by 8 groups, 7 by 2; 64
-    // rows of 32 heads, d = 128: 9 us by 8.
+    // Lane groups per row: more of them sum more of a row's pieces at once, as
+    // long as the launch has fewer waves than one resident round (8 per SIMD).
+    // By 2 / 4 / 8 groups, us: 4 rows of 32 heads (d = 64) 5.8 / 5.4 / 5.2; 64
+    // rows of 32 (d = 128, a round exactly by 8) 7.7 / 7.4 / 8.7; 64 int8 rows
+    // of 48 (d = 128) 14.0 / 12.3 / 16.0; 128 rows of 64 (d = 64, a round
+    // exactly by 4) 7.6 / 9.0 / 13.8.
     const int hq = p.Hkv * p.G;
     const int rows = p.num_tokens * hq;
     const int64_t waves = (int64_t)rows * (D / 4) / 64, resident = 32 * cu_count();
@@ -1888,8 +1889,8 @@ void launch_span(const SpanParams &p, int grid, hipStream_t s) {
       const int rpb = 256 / (D / 4) / groups;
       kernel<<<(rows + rpb - 1) / rpb, 256, 0, s>>>(p, make_fastdiv(hq));
     };
-    if (waves * 8 <= resident) join(span_join_kernel<D, CT, SC, 8>, 8);
-    else if (waves * 4 <= resident) join(span_join_kernel<D, CT, SC, 4>, 4);
+    if (waves * 8 < resident) join(span_join_kernel<D, CT, SC, 8>, 8);
+    else if (waves * 4 < resident) join(span_join_kernel<D, CT, SC, 4>, 4);
     else join(span_join_kernel<D, CT, SC, 2>, 2);
   }
 }
