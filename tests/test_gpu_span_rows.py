@@ -6,7 +6,12 @@ import pytest
 import torch
 
 from span_ref import attend, check
-from vllm_neuron_amd.functional import cross_attention
+from vllm_neuron_amd.functional import (
+    cross_attention,
+    quant_kv_read,
+    quant_kv_write,
+    shared_prefix_attention,
+)
 
 pytestmark = pytest.mark.gpu
 BF = torch.bfloat16
@@ -192,3 +197,28 @@ def test_compiled_call_clears_its_rows(gpu):
     got = step(q)
     assert torch.equal(want, got)
     assert (got[:2] == 1).all() and (got[7:] == 1).all()
+
+
+@pytest.mark.parametrize("code", [torch.int8, torch.float8_e4m3fn])
+@pytest.mark.parametrize("S", [1, 4])
+def test_decode_of_a_quantised_cache(gpu, code, S):
+    """An ordinary decode step: no prefix, and a prefix table of one entry that
+    is never read (out of the pool here)."""
+    B, hq, hkv, d, bs, nb = 5, 8, 2, 128, 16, 40
+    kc, vc = (torch.zeros(nb, hkv, bs, d, dtype=code, device=gpu) for _ in "kv")
+    ks, vs = (torch.zeros(nb, hkv, bs, device=gpu) for _ in "kv")
+    lens = [100, 4, 17, 64, 33]
+    t = torch.randperm(nb, generator=_gen(1))[:B * 7].view(B, 7).to(torch.int32)
+    slots = torch.cat([t[b].long().repeat_interleave(bs)[:n] * bs + torch.arange(n) % bs for b, n in enumerate(lens)])
+    quant_kv_write(_randn(2, len(slots), hkv, d).to(gpu), _randn(3, len(slots), hkv, d).to(gpu), slots.to(gpu),
+                   kc, vc, ks, vs)
+    q = _randn(4, B, S, hq, d)
+    out = shared_prefix_attention(q.to(gpu), kc, vc, _i32(gpu, 1 << 30), _i32(gpu, 0), t.to(gpu), _i32(gpu, *lens),
+                                  k_scales=ks, v_scales=vs)
+    k, v = (x.cpu().double() for x in quant_kv_read(kc, vc, ks, vs, slots.to(gpu), dtype=torch.float32))
+    at = 0
+    for b, n in enumerate(lens):
+        for s in range(S):
+            e = n - S + 1 + s
+            check(out[b, s:s + 1], *attend(q[b, s:s + 1], k[at:at + e], v[at:at + e], d ** -0.5), f"row {b}, token {s}")
+        at += n
