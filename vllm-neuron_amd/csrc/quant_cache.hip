@@ -20,10 +20,10 @@
 // Layout.  A row is read by LPR lanes with 16 bytes each (8 elements), the
 // maximum goes over those lanes with xor shuffles, and each lane stores its 8
 // codes; a thread takes K and V of its (token, head).  Bound by HBM for long
-// calls: 16383 tokens of 8 heads, d = 128, bf16 to int8 25.5 us (4.0 TB/s of
-// rows, codes and scales; a large device copy moves 4.9), read back 18.3 us
-// (5.6 TB/s); 2048 tokens 6.5 us each way.  A step's few rows take a launch and
-// three dependent loads: 3.7 and 2.5 us.  With K and V by separate threads the
+// calls: 16383 tokens of 8 heads, d = 128, bf16 to int8 25.9 us (3.9 TB/s of
+// rows, codes and scales; a large device copy moves 4.9), read back 18.6 us
+// (5.5 TB/s); 2048 tokens 6.4 us each way.  A step's few rows take a launch and
+// three dependent loads: 3.4 and 2.6 us.  With K and V by separate threads the
 // long calls took 28 and 23.6 us.
 #include <algorithm>
 

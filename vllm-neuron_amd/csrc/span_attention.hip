@@ -18,9 +18,9 @@
 //         through LDS and serve all four waves (v_mfma_f32_32x32x16_bf16).
 //         Bound by the MFMAs and exponentials.  K and V of the next tile arrive
 //         in the other of two LDS stages meanwhile.  2048 tokens of 32 heads
-//         over 6404 keys, d = 128: 205 us, 1.05 PFLOP/s; the matrix units are
-//         busy 53 % of the cycles, vector instructions issue in 50 %, at a
-//         clock that falls to 1.9 GHz.
+//         over 6404 keys, d = 128: 205-214 us by box, 1.0-1.05 PFLOP/s; the
+//         matrix units are busy 53 % of the cycles, vector instructions issue
+//         in 50 %, at a clock that falls to 1.9 GHz.
 //   thin  at most 16 or 32 rows: each wave streams 32-key tiles of its own, K
 //         straight into MFMA operands, V through a piece of LDS of the wave
 //         (v_mfma_f32_16x16x32_bf16).  Bound by HBM behind a start of 7 us
@@ -1773,7 +1773,8 @@ Layout span_layout(SpanParams &p, int D) {
     }
   }
   // Measured, side by side: a thin tile takes a wave 2.3 us and a tall one a
-  // workgroup 1.7 us at d = 64 (3.8 and 2.6 us at d = 128).  Thin costs of
+  // workgroup 1.7 us at d = 64 (3.8 and 2.6 us at d = 128): with four
+  // waves to a workgroup 0.34 and 0.37.  Calls differ little by it; thin costs of
   // 0.30 / 0.35 / 0.40 / 0.45: 64 rows behind 8192 keys (d = 128) 53.8 / 53.5 /
   // 53.1 / 53.2 us; 128 rows behind 4133 (d = 64) 44.9 / 44.2 / 44.1 / 44.7; 64
   // drafted int8 rows behind 32768 127.3 / 119.9 / 119.7 / 122.7.  A segment's
