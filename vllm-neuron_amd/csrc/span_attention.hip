@@ -18,7 +18,7 @@
 //         through LDS and serve all four waves (v_mfma_f32_32x32x16_bf16).
 //         Bound by the MFMAs and exponentials.  K and V of the next tile arrive
 //         in the other of two LDS stages meanwhile.  2048 tokens of 32 heads
-//         over 6404 keys, d = 128: 205-214 us by card, 1.0-1.05 PFLOP/s; the
+//         over 6404 keys, d = 128: 205-216 us by card, 1.0-1.05 PFLOP/s; the
 //         matrix units are busy 53 % of the cycles, vector instructions issue
 //         in 50 %, at a clock that falls to 1.9 GHz.
 //   thin  at most 16 or 32 rows: each wave streams 32-key tiles of its own, K
