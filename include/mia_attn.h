@@ -801,6 +801,59 @@ typedef struct {
 size_t mia_shared_prefix_workspace_bytes(const mia_shared_prefix_args *args);
 int mia_shared_prefix_attention(const mia_shared_prefix_args *args, mia_stream_t stream);
 
+/* ------------------------------------------------------------------------ */
+/* Rows quantised to int8 with one scale per row (no counterpart in the      */
+/* reference, whose weight quantisation lives in its compiler's library).    */
+/* x = in + add0 + add1 (bf16, each add rounded to bf16); with norm = 1      */
+/*   y = x * rsqrt(sum(x^2) / dim_actual + eps) * gamma, else y = x;         */
+/*   scales[row] = fl32(max|y| / 127), codes = rn(y * 127 / max|y|), ties to */
+/* even.  A row of zeros has scale 0; a row with a NaN or an infinity scale  */
+/* NaN and zero codes.                                                       */
+/* ------------------------------------------------------------------------ */
+typedef struct {
+  const void *x;    /* bf16 [rows, dim], contiguous channels */
+  const void *add0; /* optional, same shape and stride */
+  const void *add1;
+  int64_t x_stride; /* elements between rows */
+  void *codes;      /* int8 [rows, dim] */
+  int64_t codes_stride;
+  float *scales; /* [rows] */
+  int64_t rows;
+  int32_t dim;
+  int32_t dim_actual; /* divisor of the mean (0 = dim) */
+  int32_t norm;       /* 1: RMS norm */
+  float eps;
+  const void *gamma; /* [dim] fp32 (bf16 with gamma_bf16) or NULL (= 1) */
+  int32_t gamma_bf16;
+  int32_t _pad0;
+} mia_quant_rows_args;
+
+int mia_quant_rows(const mia_quant_rows_args *args, mia_stream_t stream);
+
+/* ------------------------------------------------------------------------ */
+/* Product of int8 rows and int8 weights (no counterpart in the reference):  */
+/*   out[m, n] = bf16(x_scales[m] w_scales[n] sum_k x[m, k] w[n, k] + b[n]), */
+/* integer sums exact in 32 bits (k <= 131072).  k is a multiple of 16, rows */
+/* of x and w 16-byte aligned.                                               */
+/* ------------------------------------------------------------------------ */
+typedef struct {
+  const void *x; /* int8 [rows, k] */
+  int64_t x_stride;
+  const float *x_scales; /* [rows] */
+  const void *w;         /* int8 [n, k] */
+  int64_t w_stride;
+  const float *w_scales; /* [n] */
+  const void *bias;      /* [n] fp32 (bf16 with bias_bf16) or NULL */
+  void *out;             /* bf16 [rows, n] */
+  int64_t out_stride;
+  int32_t rows;
+  int32_t n;
+  int32_t k;
+  int32_t bias_bf16;
+} mia_int8_linear_args;
+
+int mia_int8_linear(const mia_int8_linear_args *args, mia_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -125,6 +125,8 @@ size_t mia_args_size(int which) {
     case 13: return sizeof(mia_quant_kv_args);
     case 14: return sizeof(mia_cross_args);
     case 15: return sizeof(mia_shared_prefix_args);
+    case 16: return sizeof(mia_quant_rows_args);
+    case 17: return sizeof(mia_int8_linear_args);
     default: return 0;
   }
 }
@@ -813,6 +815,43 @@ int mia_shared_prefix_attention(const mia_shared_prefix_args *a, mia_stream_t st
                   a->workspace_bytes >= mia::shared_prefix_workspace(*a),
               MIA_ERR_VALUE, "shared_prefix: workspace missing, unaligned or too small");
   return mia::launch_shared_prefix(*a, (hipStream_t)stream);
+}
+
+int mia_quant_rows(const mia_quant_rows_args *a, mia_stream_t stream) {
+  mia::g_last_error.clear();
+  MIA_REQUIRE(a, MIA_ERR_VALUE, "quant_rows: null args");
+  MIA_REQUIRE(a->rows >= 0 && a->dim > 0, MIA_ERR_VALUE, "quant_rows: bad shape");
+  if (a->rows == 0) return MIA_OK;
+  MIA_REQUIRE(a->x && a->codes && a->scales, MIA_ERR_VALUE, "quant_rows: null tensor pointer");
+  MIA_REQUIRE(a->rows < (1ll << 31), MIA_ERR_VALUE, "quant_rows: 2^31 rows or more");
+  MIA_REQUIRE(a->norm == 0 || a->norm == 1, MIA_ERR_NOT_IMPLEMENTED,
+              "quant_rows: the norm is none or RMS");
+  MIA_REQUIRE(a->dim_actual >= 0 && a->dim_actual <= a->dim, MIA_ERR_VALUE,
+              "quant_rows: dim_actual out of range");
+  return mia::launch_quant_rows(*a, (hipStream_t)stream);
+}
+
+int mia_int8_linear(const mia_int8_linear_args *a, mia_stream_t stream) {
+  mia::g_last_error.clear();
+  MIA_REQUIRE(a, MIA_ERR_VALUE, "int8_linear: null args");
+  MIA_REQUIRE(a->rows >= 0 && a->n >= 0 && a->k > 0, MIA_ERR_VALUE, "int8_linear: bad shape");
+  if (a->rows == 0 || a->n == 0) return MIA_OK;
+  MIA_REQUIRE(a->x && a->x_scales && a->w && a->w_scales && a->out, MIA_ERR_VALUE,
+              "int8_linear: null tensor pointer");
+  MIA_REQUIRE(a->k <= 131072, MIA_ERR_NOT_IMPLEMENTED,
+              "int8_linear: k above 131072 (the 32-bit sums would overflow)");
+  MIA_REQUIRE(a->k % 16 == 0, MIA_ERR_NOT_IMPLEMENTED, "int8_linear: k must be a multiple of 16");
+  // a tile's 256 rows lie within 2^32 bytes
+  MIA_REQUIRE(a->x_stride >= 0 && a->x_stride < (1ll << 24) && a->w_stride >= 0 &&
+                  a->w_stride < (1ll << 24),
+              MIA_ERR_VALUE, "int8_linear: row stride out of range");
+  MIA_REQUIRE(aligned(a->x, 16) && aligned(a->w, 16) &&
+                  (a->x_stride % 16 == 0 || a->rows == 1) && (a->w_stride % 16 == 0 || a->n == 1),
+              MIA_ERR_VALUE, "int8_linear: rows must be 16-byte aligned");
+  // tiles along one grid axis, their threads within 2^32
+  MIA_REQUIRE((int64_t)(a->rows / 64 + 1) * (a->n / 64 + 1) < (1ll << 22), MIA_ERR_VALUE,
+              "int8_linear: rows * n beyond 2^34");
+  return mia::launch_int8_linear(*a, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -1215,3 +1215,89 @@ def shared_prefix_attention(q, k_cache, v_cache, prefix_table, prefix_len, block
     L = N.lib()
     _span_launch(a, L.mia_shared_prefix_workspace_bytes, L.mia_shared_prefix_attention,
                  "shared_prefix_attention", workspace, dev)
+
+
+# ---------------------------------------------------------------------------
+# int8 projections
+# ---------------------------------------------------------------------------
+def _vector(t, n, what, dev):
+    """A float32 or bf16 vector of ``n`` entries as the kernels read it (other
+    types as float32, other devices and strides copied)."""
+    if t.numel() != n:
+        raise ValueError(f"{what} has {t.numel()} entries, expected {n}")
+    t = t.detach().reshape(-1)
+    if t.dtype not in (torch.float32, torch.bfloat16):
+        t = t.float()
+    if t.device != dev:
+        t = t.to(dev)
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def quant_rows(x, norm, eps, gamma=None, add0=None, add1=None, dim_actual=0):
+    """Rows of ``x (+ add0) (+ add1) [..., dim]`` (bf16), RMS-normalised with
+    ``norm``, as int8 codes of the same shape and float32 scales ``[...]``."""
+    dev = N.same_gpu(x, add0, add1)
+    if x.dtype != torch.bfloat16:
+        raise NotImplementedError("quant_rows: bf16 input only")
+    shape = x.shape
+    if not shape or shape[-1] == 0:
+        raise ValueError(f"quant_rows: rows of no channels, {tuple(shape)}")
+    dim = shape[-1]
+    if gamma is not None and not norm:
+        raise ValueError("quant_rows: gamma belongs to a norm")
+    if not 0 <= dim_actual <= dim:
+        raise ValueError(f"quant_rows: dim_actual {dim_actual} of {dim} channels")
+    x2 = x if len(shape) == 2 else x.reshape(-1, dim)
+    adds = []
+    for t in (add0, add1):
+        if t is None:
+            continue
+        if t.dtype != torch.bfloat16 or t.shape != shape:
+            raise ValueError("residual adds must be bf16 with the input's shape")
+        adds.append(t if len(shape) == 2 else t.reshape(-1, dim))
+    if x2.stride(1) != 1 or any(t.stride() != x2.stride() for t in adds):
+        x2 = x2.contiguous()
+        adds = [t.contiguous() for t in adds]
+    if gamma is not None:
+        gamma = _vector(gamma, dim, "gamma", dev)
+    rows = x2.shape[0]
+    codes = torch.empty((rows, dim), dtype=torch.int8, device=dev)
+    scales = torch.empty((rows,), dtype=torch.float32, device=dev)
+    p = [t.data_ptr() for t in adds] + [0, 0]
+    a = N.QuantRowsArgs()
+    N.PACK_QUANT_ROWS.pack_into(
+        a, 0, x2.data_ptr(), p[0], p[1], x2.stride(0), codes.data_ptr(), dim, scales.data_ptr(),
+        rows, dim, dim_actual, int(norm), eps, 0 if gamma is None else gamma.data_ptr(),
+        int(gamma is not None and gamma.dtype == torch.bfloat16), 0)
+    N.launch(N.lib().mia_quant_rows, a, dev, "quant_rows")
+    if len(shape) != 2:
+        codes, scales = codes.reshape(shape), scales.reshape(shape[:-1])
+    return codes, scales
+
+
+def int8_linear(x, x_scales, w, w_scales, bias, out):
+    """``out [M, N] = bf16(x_scales w_scales (x [M, K] w [N, K]^T) + bias)``."""
+    dev = N.same_gpu(x, x_scales, w, w_scales, bias, out)
+    if x.dtype != torch.int8 or w.dtype != torch.int8 or x.dim() != 2 or w.dim() != 2:
+        raise ValueError(f"int8_linear: x and w must be int8 matrices, got {x.dtype} "
+                         f"{tuple(x.shape)} and {w.dtype} {tuple(w.shape)}")
+    (m, k), (n, wk) = x.shape, w.shape
+    if k != wk:
+        raise ValueError(f"int8_linear: x has {k} channels, w {wk}")
+    for s, c, what in ((x_scales, m, "x_scales"), (w_scales, n, "w_scales")):
+        if s.dtype != torch.float32 or s.dim() != 1 or s.shape[0] != c or (
+                c > 1 and s.stride(0) != 1):
+            raise ValueError(f"int8_linear: {what} must be a contiguous float32 vector of {c}, "
+                             f"got {s.dtype} {tuple(s.shape)}")
+    if out.shape != (m, n) or out.dtype != torch.bfloat16 or out.stride(1) != 1 and n > 1:
+        raise ValueError(f"int8_linear: out must be bf16 [{m}, {n}] with contiguous columns")
+    if bias is not None:
+        bias = _vector(bias, n, "bias", dev)
+    if (k > 1 and (x.stride(1) != 1 or w.stride(1) != 1)):
+        raise ValueError("int8_linear: the channels of x and w must be contiguous")
+    a = N.Int8LinearArgs()
+    N.PACK_INT8.pack_into(
+        a, 0, x.data_ptr(), x.stride(0), x_scales.data_ptr(), w.data_ptr(), w.stride(0),
+        w_scales.data_ptr(), 0 if bias is None else bias.data_ptr(), out.data_ptr(),
+        out.stride(0), m, n, k, int(bias is not None and bias.dtype == torch.bfloat16))
+    N.launch(N.lib().mia_int8_linear, a, dev, "int8_linear")

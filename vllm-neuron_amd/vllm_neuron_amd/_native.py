@@ -255,6 +255,23 @@ class SharedPrefixArgs(ctypes.Structure):
     ]
 
 
+class QuantRowsArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", c_vp), ("add0", c_vp), ("add1", c_vp), ("x_stride", c_i64),
+        ("codes", c_vp), ("codes_stride", c_i64), ("scales", c_vp), ("rows", c_i64),
+        ("dim", c_i32), ("dim_actual", c_i32), ("norm", c_i32), ("eps", c_f32),
+        ("gamma", c_vp), ("gamma_bf16", c_i32), ("_pad0", c_i32),
+    ]
+
+
+class Int8LinearArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", c_vp), ("x_stride", c_i64), ("x_scales", c_vp), ("w", c_vp), ("w_stride", c_i64),
+        ("w_scales", c_vp), ("bias", c_vp), ("out", c_vp), ("out_stride", c_i64),
+        ("rows", c_i32), ("n", c_i32), ("k", c_i32), ("bias_bf16", c_i32),
+    ]
+
+
 _CODES = {c_vp: "P", c_i32: "i", c_i64: "q", c_f32: "f", ctypes.c_size_t: "N"}
 
 
@@ -271,13 +288,15 @@ def _packer(st) -> struct.Struct:
 PACK_QUANT = _packer(QuantKvArgs)
 PACK_CROSS = _packer(CrossArgs)
 PACK_PREFIX = _packer(SharedPrefixArgs)
+PACK_QUANT_ROWS = _packer(QuantRowsArgs)
+PACK_INT8 = _packer(Int8LinearArgs)
 
 
 ARGS_STRUCTS = {
     0: KvWriteArgs, 1: GatherArgs, 2: MaskArgs, 3: DecodeArgs, 4: PrefillArgs,
     5: SlotMappingArgs, 6: PackedKArgs, 7: SwaTrimArgs, 8: ScatterRowsArgs, 9: StageArgs,
     10: QkvEpilogueArgs, 11: RowNormArgs, 12: SkinnyLinearArgs, 13: QuantKvArgs,
-    14: CrossArgs, 15: SharedPrefixArgs,
+    14: CrossArgs, 15: SharedPrefixArgs, 16: QuantRowsArgs, 17: Int8LinearArgs,
 }
 
 # Exported symbols (must match include/mia_attn.h).
@@ -290,6 +309,7 @@ EXPORTS = [
     "mia_row_norm", "mia_skinny_linear", "mia_paged_decode_noalloc",
     "mia_quant_kv_write", "mia_quant_kv_read", "mia_cross_workspace_bytes",
     "mia_cross_attention", "mia_shared_prefix_workspace_bytes", "mia_shared_prefix_attention",
+    "mia_quant_rows", "mia_int8_linear",
 ]
 
 # Static scratch capacity of mia_paged_decode_noalloc (include/mia_attn.h).
@@ -315,7 +335,8 @@ def _declare(lib: ctypes.CDLL) -> None:
                      ("mia_skinny_linear", SkinnyLinearArgs),
                      ("mia_quant_kv_write", QuantKvArgs), ("mia_quant_kv_read", QuantKvArgs),
                      ("mia_cross_attention", CrossArgs),
-                     ("mia_shared_prefix_attention", SharedPrefixArgs)):
+                     ("mia_shared_prefix_attention", SharedPrefixArgs),
+                     ("mia_quant_rows", QuantRowsArgs), ("mia_int8_linear", Int8LinearArgs)):
         fn = getattr(lib, name)
         fn.argtypes = [P(st), c_vp]
         fn.restype = c_i32

@@ -4,6 +4,7 @@ from .attention.attention_decode import attention_decode, scatter_packed_k
 from .attention.attention_decode_mask import gen_attention_decode_mask
 from .attention.attention_segmented_cte import segmented_attention
 from .attention.cross_attention import cross_attention
+from .attention.int8_linear import int8_linear, quant_rows
 from .attention.mixed_batch import mixed_batch_attention
 from .attention.qkv import qkv_proj
 from .attention.quant_cache import quant_kv_read, quant_kv_write
@@ -23,4 +24,6 @@ __all__ = [
     "quant_kv_read",
     "cross_attention",
     "shared_prefix_attention",
+    "quant_rows",
+    "int8_linear",
 ]

@@ -7,7 +7,10 @@ the reference signature (:672-730) and the semantics of its torch paths
 1. ``x = hidden (+ mlp_prev + attn_prev)`` and the optional RMS / LayerNorm
    / RMS-without-gamma row norm — ``mia_row_norm`` (fp32 statistics);
 2. ``qkv = x @ qkv_weights (+ bias)`` — a library GEMM (bf16 inputs, fp32
-   accumulation);
+   accumulation), or with ``QuantizationType.ROW`` the rows quantised to int8
+   as they are normalised and an integer product (``int8_linear``): int8
+   weights ``[H, fused]``, a transposed view of a ``[fused, H]`` tensor, and
+   their scales ``qkv_w_scale [fused]``;
 3. per-head RMS norm of the Q and K heads before / after RoPE, half-split
    RoPE (``cos[..., :d/2]`` on the first half, ``cos[..., d/2:]`` on the
    second, ``sin[..., :d/2]`` on both), and with ``use_block_kv`` the
@@ -22,7 +25,7 @@ bf16 for a bf16 ``cos_cache``, fp32 products and sum for an fp32 one.  With
 ``use_block_kv`` the reference's torch fallback drops the norm arguments;
 here they are applied, as on its kernel path.  Trainium placement hints
 (``use_dma_transpose``, ``store_output_in_sbuf``, ``sbm_*``,
-``use_auto_allocation``) have no meaning here and are ignored; weight
+``use_auto_allocation``) have no meaning here and are ignored; static weight
 quantisation, ``transpose_k_cache`` and gamma folded into the RoPE caches
 raise NotImplementedError.
 """
@@ -124,8 +127,9 @@ def qkv_proj(
             "num_q_heads and num_kv_heads must be specified when qk_norm is enabled")
     _validate_in_kernel_kv_cache_write_args(k_cache, v_cache, use_block_kv, slot_mapping,
                                             block_size)
-    if quantization_type != QuantizationType.NONE:
-        raise NotImplementedError("qkv_proj: weight quantisation is not supported")
+    int8 = quantization_type == QuantizationType.ROW
+    if quantization_type != QuantizationType.NONE and not int8:
+        raise NotImplementedError("qkv_proj: static weight quantisation is not supported")
     if weight_layout != QKVWeightLayout.CONTIGUOUS:
         raise NotImplementedError("qkv_proj: only the contiguous weight layout is supported")
     if transpose_k_cache:
@@ -147,6 +151,14 @@ def qkv_proj(
             f"and {tuple(qkv_weights.shape)}")
     if hidden.dtype != torch.bfloat16:
         raise NotImplementedError("qkv_proj: hidden must be bf16")
+    if int8:
+        if qkv_weights.dtype != torch.int8 or qkv_w_scale is None:
+            raise ValueError("qkv_proj: QuantizationType.ROW takes int8 weights and qkv_w_scale")
+        if qkv_in_scale is not None:
+            raise NotImplementedError("qkv_proj: static input scales are not supported")
+        if qkv_weights.stride(0) != 1:
+            raise ValueError("qkv_proj: int8 weights [H, fused] are the transposed view of a "
+                             "[fused, H] tensor (the H axis contiguous)")
     N.require_gpu(hidden, qkv_weights)
     B, S, H = hidden.shape
     T = B * S
@@ -156,22 +168,32 @@ def qkv_proj(
     # 1. residual add and row norm
     fused_add = mlp_prev is not None and attn_prev is not None
     adds = dict(add0=mlp_prev, add1=attn_prev) if fused_add else {}
-    if norm_type == NormType.RMS_NORM:
-        x = K.row_norm(hidden, K.NORM_RMS, eps, _vec(norm_weights), dim_actual=hidden_actual or 0,
-                       **adds)
-    elif norm_type == NormType.RMS_NORM_SKIP_GAMMA:
-        x = K.row_norm(hidden, K.NORM_RMS, eps, None, dim_actual=hidden_actual or 0, **adds)
-    elif norm_type == NormType.LAYER_NORM:
+    rms = norm_type in (NormType.RMS_NORM, NormType.RMS_NORM_SKIP_GAMMA)
+    gamma = _vec(norm_weights) if norm_type == NormType.RMS_NORM else None
+    if norm_type == NormType.LAYER_NORM:
         x = K.row_norm(hidden, K.NORM_LAYER, eps, _vec(norm_weights), _vec(norm_b), **adds)
+    elif int8:
+        x = hidden  # normalised where it is quantised
+    elif rms:
+        x = K.row_norm(hidden, K.NORM_RMS, eps, gamma, dim_actual=hidden_actual or 0, **adds)
     else:
         x = hidden + mlp_prev + attn_prev if fused_add else hidden
 
-    # 2. projection (library GEMM)
-    w = qkv_weights.to(bf)
-    if bias is not None:
-        out = torch.addmm(bias.reshape(1, -1).to(bf), x.reshape(T, H), w)
+    # 2. projection (library GEMM, or in 8-bit integers)
+    if int8:
+        if norm_type == NormType.LAYER_NORM:
+            adds = {}
+        code, scale = K.quant_rows(x.reshape(T, H), rms, eps, gamma,
+                                   dim_actual=(hidden_actual or 0) if rms else 0,
+                                   **{n: t.reshape(T, H) for n, t in adds.items()})
+        out = K.int8_linear(code, scale, qkv_weights.t(), qkv_w_scale.reshape(-1),
+                            None if bias is None else bias.reshape(-1))
     else:
-        out = torch.mm(x.reshape(T, H), w)
+        w = qkv_weights.to(bf)
+        if bias is not None:
+            out = torch.addmm(bias.reshape(1, -1).to(bf), x.reshape(T, H), w)
+        else:
+            out = torch.mm(x.reshape(T, H), w)
     out = out.reshape(B, S, fused)
 
     # 3. QK norm, RoPE, cache write: one pass, in place

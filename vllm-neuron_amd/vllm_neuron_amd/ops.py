@@ -679,10 +679,56 @@ def shared_prefix_attention(q, k_cache, v_cache, prefix_table, prefix_len, block
     return out
 
 
+# ---------------------------------------------------------------------------
+# int8 projections
+# ---------------------------------------------------------------------------
+@custom_op("mia::quant_rows", mutates_args=())
+def _quant_rows(x: Tensor, gamma: Optional[Tensor], add0: Optional[Tensor],
+                add1: Optional[Tensor], norm: bool, eps: float,
+                dim_actual: int) -> Tuple[Tensor, Tensor]:
+    return K.quant_rows(x, norm, eps, gamma, add0, add1, dim_actual)
+
+
+@_quant_rows.register_fake
+def _(x, gamma, add0, add1, norm, eps, dim_actual):
+    return (x.new_empty(x.shape, dtype=torch.int8),
+            x.new_empty(x.shape[:-1], dtype=torch.float32))
+
+
+def quant_rows(x, norm: bool = False, eps: float = 0.0, gamma=None, *, add0=None, add1=None,
+               dim_actual: int = 0) -> Tuple[Tensor, Tensor]:
+    if _plain(x, gamma, add0, add1):
+        return K.quant_rows(x, bool(norm), float(eps), gamma, add0, add1, int(dim_actual))
+    return _quant_rows(x, gamma, add0, add1, bool(norm), float(eps), int(dim_actual))
+
+
+@custom_op("mia::int8_linear", mutates_args=("out",))
+def _int8_linear(x: Tensor, x_scales: Tensor, w: Tensor, w_scales: Tensor,
+                 bias: Optional[Tensor], out: Tensor) -> None:
+    K.int8_linear(x, x_scales, w, w_scales, bias, out)
+
+
+@_int8_linear.register_fake
+def _(x, x_scales, w, w_scales, bias, out):
+    return None
+
+
+def int8_linear(x, x_scales, w, w_scales, bias=None, out=None) -> Tensor:
+    if out is None:
+        out = torch.empty((x.shape[0], w.shape[0]), dtype=torch.bfloat16, device=x.device)
+    if _plain(x, x_scales, w, w_scales, bias, out):
+        K.int8_linear(x, x_scales, w, w_scales, bias, out)
+        _written(out)
+        return out
+    _int8_linear(x, x_scales, w, w_scales, bias, out)
+    return out
+
+
 OPS: List[str] = [
     "kv_write", "gather_kv", "packed_k_convert", "scatter_rows", "stage_rows", "decode_mask",
     "slot_mapping", "remap_null_block", "swa_trim", "paged_decode", "paged_decode_write",
     "paged_prefill",
     "qkv_epilogue", "row_norm", "skinny_linear",
     "quant_kv_write", "quant_kv_read", "cross_attention", "shared_prefix_attention",
+    "quant_rows", "int8_linear",
 ]
