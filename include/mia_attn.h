@@ -854,6 +854,74 @@ typedef struct {
 
 int mia_int8_linear(const mia_int8_linear_args *args, mia_stream_t stream);
 
+/* ------------------------------------------------------------------------ */
+/* Rotation of Q and K by positions on one to four axes (text; time, height, */
+/* width), with K and V appended to the paged cache in the same pass (no     */
+/* counterpart in the reference, whose models expand cos and sin on the      */
+/* host side of the kernel and write the cache behind it).                   */
+/* Row x of head h and token t, optionally RMS-normalised over its head_dim  */
+/* channels (qk_norm; q_gamma / k_gamma, NULL = 1), has its first rot_dim    */
+/* channels rotated: pair i, (i, i + rot_dim / 2) or (2 i, 2 i + 1) with     */
+/* interleaved, by the angle positions[axis(i), t] * inv_freq[i]; cos and    */
+/* sin are multiplied by rope_scale.  axis(i): section[x] pairs of axis x    */
+/* one after the other, or with section_cycle axis i % axes where            */
+/* i < section[i % axes] * axes, else axis 0.                                */
+/* K and V go to slots[t] of a cache: bf16; e4m3fn of clamp(x / dequant[h])  */
+/* (NULL = 1); int8 or e4m3fn with per-token scales as mia_quant_kv_write    */
+/* forms them.  Q and K are rounded once, behind the rotation.  slots NULL:  */
+/* no cache (v unused).  Slots outside the pool are skipped; the others must */
+/* differ.  q_out may be q, k_out may be k.                                  */
+/* head_dim and rot_dim: multiples of 8, head_dim <= 256.                    */
+/* ------------------------------------------------------------------------ */
+typedef struct {
+  const void *q; /* bf16, element (t, h, e) at t*s0 + h*s1 + e */
+  int64_t q_stride[2];
+  const void *k;
+  int64_t k_stride[2];
+  const void *v;
+  int64_t v_stride[2];
+  void *q_out;
+  int64_t q_out_stride[2];
+  void *k_out; /* optional */
+  int64_t k_out_stride[2];
+  int64_t num_tokens;
+  int32_t num_q_heads;
+  int32_t num_kv_heads;
+  int32_t head_dim;
+  int32_t rot_dim;
+  const void *positions; /* I32 or I64 */
+  int64_t pos_stride[2]; /* axis, token */
+  int32_t pos_dtype;
+  int32_t axes;
+  const float *inv_freq; /* [rot_dim / 2] */
+  int32_t section[4];
+  int32_t section_cycle;
+  int32_t interleaved;
+  float rope_scale;
+  int32_t qk_norm;
+  const void *q_gamma; /* [head_dim] fp32 (bf16 with gamma_bf16) or NULL */
+  const void *k_gamma;
+  int32_t gamma_bf16;
+  float eps;
+  const void *slots; /* [num_tokens] or NULL */
+  int32_t slot_dtype; /* I32, I64 or U32 */
+  int32_t cache_dtype; /* BF16, FP8_E4M3FN or I8 */
+  void *k_cache;
+  void *v_cache;
+  int64_t k_cache_stride[4]; /* block, head, token, dim */
+  int64_t v_cache_stride[4];
+  float *k_scales; /* per token and head, or NULL */
+  float *v_scales;
+  int64_t k_scale_stride[3]; /* block, head, token */
+  int64_t v_scale_stride[3];
+  const float *k_dequant; /* [Hkv] or NULL */
+  const float *v_dequant;
+  int32_t num_blocks;
+  int32_t block_size;
+} mia_rope_append_args;
+
+int mia_rope_append(const mia_rope_append_args *args, mia_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -127,6 +127,7 @@ size_t mia_args_size(int which) {
     case 15: return sizeof(mia_shared_prefix_args);
     case 16: return sizeof(mia_quant_rows_args);
     case 17: return sizeof(mia_int8_linear_args);
+    case 18: return sizeof(mia_rope_append_args);
     default: return 0;
   }
 }
@@ -852,6 +853,79 @@ int mia_int8_linear(const mia_int8_linear_args *a, mia_stream_t stream) {
   MIA_REQUIRE((int64_t)(a->rows / 64 + 1) * (a->n / 64 + 1) < (1ll << 22), MIA_ERR_VALUE,
               "int8_linear: rows * n beyond 2^34");
   return mia::launch_int8_linear(*a, (hipStream_t)stream);
+}
+
+int mia_rope_append(const mia_rope_append_args *a, mia_stream_t stream) {
+  mia::g_last_error.clear();
+  MIA_REQUIRE(a, MIA_ERR_VALUE, "rope_append: null args");
+  MIA_REQUIRE(a->num_tokens >= 0, MIA_ERR_VALUE, "rope_append: num_tokens < 0");
+  if (a->num_tokens == 0) return MIA_OK;
+  MIA_REQUIRE(a->q && a->k && a->q_out && a->positions && a->inv_freq, MIA_ERR_VALUE,
+              "rope_append: null tensor pointer");
+  MIA_REQUIRE(a->num_q_heads > 0 && a->num_kv_heads > 0 && a->num_q_heads < (1 << 20) &&
+                  a->num_kv_heads < (1 << 20),
+              MIA_ERR_VALUE, "rope_append: bad head counts");
+  // a token's threads lie along one grid axis (2^32)
+  MIA_REQUIRE(a->num_tokens < (1ll << 24), MIA_ERR_VALUE, "rope_append: 2^24 tokens or more");
+  MIA_REQUIRE(a->head_dim > 0 && a->head_dim <= 256 && a->head_dim % 8 == 0,
+              MIA_ERR_NOT_IMPLEMENTED, "rope_append: head_dim must be a multiple of 8 up to 256");
+  MIA_REQUIRE(a->rot_dim > 0 && a->rot_dim % 8 == 0, MIA_ERR_NOT_IMPLEMENTED,
+              "rope_append: the rotated channels must be a multiple of 8");
+  MIA_REQUIRE(a->rot_dim <= a->head_dim, MIA_ERR_VALUE,
+              "rope_append: more rotated channels than head_dim");
+  MIA_REQUIRE(a->pos_dtype == MIA_DTYPE_I32 || a->pos_dtype == MIA_DTYPE_I64, MIA_ERR_VALUE,
+              "rope_append: positions must be int32 or int64");
+  MIA_REQUIRE(a->axes >= 1 && a->axes <= 4, MIA_ERR_NOT_IMPLEMENTED,
+              "rope_append: one to four position axes");
+  int64_t pairs = 0;
+  for (int i = 0; i < a->axes; ++i) {
+    MIA_REQUIRE(a->section[i] >= 0, MIA_ERR_VALUE, "rope_append: a negative section");
+    pairs += a->section[i];
+  }
+  MIA_REQUIRE(pairs == a->rot_dim / 2, MIA_ERR_VALUE,
+              "rope_append: the sections must hold every rotated channel pair");
+  auto rows = [&](const void *p, const int64_t *s, int heads) {
+    return aligned(p, 8) && (s[0] % 4 == 0 || a->num_tokens == 1) && (s[1] % 4 == 0 || heads == 1);
+  };
+  MIA_REQUIRE(rows(a->q, a->q_stride, a->num_q_heads) &&
+                  rows(a->k, a->k_stride, a->num_kv_heads) &&
+                  rows(a->q_out, a->q_out_stride, a->num_q_heads) &&
+                  rows(a->k_out, a->k_out_stride, a->num_kv_heads) &&
+                  rows(a->v, a->v_stride, a->num_kv_heads),
+              MIA_ERR_VALUE, "rope_append: rows must be 8-byte aligned");
+  if (!a->slots) {
+    MIA_REQUIRE(!a->v && a->k_out, MIA_ERR_VALUE,
+                "rope_append: without a cache K goes to k_out and there is no V");
+    return mia::launch_rope_append(*a, (hipStream_t)stream);
+  }
+  MIA_REQUIRE(a->v && a->k_cache && a->v_cache, MIA_ERR_VALUE, "rope_append: null tensor pointer");
+  MIA_REQUIRE(a->slot_dtype == MIA_DTYPE_I32 || a->slot_dtype == MIA_DTYPE_I64 ||
+                  a->slot_dtype == MIA_DTYPE_U32,
+              MIA_ERR_VALUE, "rope_append: slot dtype must be int32/int64/uint32");
+  MIA_REQUIRE(a->cache_dtype == MIA_DTYPE_BF16 || a->cache_dtype == MIA_DTYPE_FP8_E4M3FN ||
+                  a->cache_dtype == MIA_DTYPE_I8,
+              MIA_ERR_NOT_IMPLEMENTED, "rope_append: cache dtype must be bf16, fp8 or int8");
+  const bool bf = a->cache_dtype == MIA_DTYPE_BF16;
+  MIA_REQUIRE(!a->k_scales == !a->v_scales && !a->k_dequant == !a->v_dequant, MIA_ERR_VALUE,
+              "rope_append: the scales of K and V go together");
+  MIA_REQUIRE(!(bf && a->k_scales), MIA_ERR_VALUE,
+              "rope_append: a bf16 cache has no per-token scales");
+  MIA_REQUIRE(a->cache_dtype != MIA_DTYPE_I8 || a->k_scales, MIA_ERR_VALUE,
+              "rope_append: an int8 cache needs per-token scales");
+  MIA_REQUIRE(!a->k_dequant || (a->cache_dtype == MIA_DTYPE_FP8_E4M3FN && !a->k_scales),
+              MIA_ERR_VALUE, "rope_append: static scales belong to an fp8 cache");
+  MIA_REQUIRE(a->num_blocks > 0 && a->block_size > 0, MIA_ERR_VALUE, "rope_append: empty cache");
+  // 4 channels at a time: 8 bytes of bf16, 4 of codes
+  for (int i = 0; i < 2; ++i) {
+    const void *c = i ? a->v_cache : a->k_cache;
+    const int64_t *s = i ? a->v_cache_stride : a->k_cache_stride;
+    MIA_REQUIRE(s[3] == 1 && aligned(c, bf ? 8 : 4) && (s[0] % 4 == 0 || a->num_blocks == 1) &&
+                    (s[1] % 4 == 0 || a->num_kv_heads == 1) &&
+                    (s[2] % 4 == 0 || a->block_size == 1),
+                MIA_ERR_VALUE,
+                "rope_append: cache head_dim must be contiguous and its rows aligned to 4 elements");
+  }
+  return mia::launch_rope_append(*a, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -22,27 +22,6 @@ typedef __attribute__((address_space(3))) uint16_t lds_u16_t;
 // ---------------------------------------------------------------------------
 MIA_DEV float add_bf16(float a, float b) { return bf16lo(pack2_bf16(a + b, 0.f)); }
 
-// What a row's codes are formed with: amax of the (norm-weighted) row scaled
-// into [0.5, 1) by its exponent, and the reciprocal of that.
-struct RowScale {
-  float b, rc;
-  int e;
-  bool zero;
-  MIA_DEV void set(uint32_t mag) {
-    zero = mag == 0 || mag >= 0x7f800000u;  // a row of zeros, or with an inf or NaN
-    const float amax = __uint_as_float(mag);
-    e = __builtin_amdgcn_frexp_expf(amax);
-    b = zero ? 1.0f : ldexpf(amax, -e);
-    rc = __builtin_amdgcn_rcpf(b);
-    rc = fmaf(fmaf(-b, rc, 1.0f), rc, rc);
-  }
-  MIA_DEV uint32_t code(float x) const {
-    const float a = (zero ? 0.f : ldexpf(x, -e)) * 127.0f;
-    const float q = a * rc;
-    return (uint32_t)(int)rintf(fmaf(fmaf(-b, q, a), rc, q)) & 0xffu;
-  }
-};
-
 // The row's scale: fl32(amax / 127), of the normalised row.
 MIA_DEV float row_scale(uint32_t mag, float ss, const mia_quant_rows_args &a) {
   if (mag >= 0x7f800000u) return __uint_as_float(0x7fc00000u);
@@ -145,7 +124,7 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(mia_quant_rows_args a) 
     ss = (red[0].y + red[1].y) + (red[2].y + red[3].y);
   }
   if (!live) return;
-  RowScale rs;
+  RowCodes<127> rs;
   rs.set(mag);
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
@@ -153,7 +132,7 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(mia_quant_rows_args a) 
     if (c >= a.dim) continue;
     u32x2_t w = {0u, 0u};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w[i >> 2] |= rs.code(x[v][i]) << (8 * (i & 3));
+    for (int i = 0; i < 8; ++i) w[i >> 2] |= rs.int8(x[v][i]) << (8 * (i & 3));
     *reinterpret_cast<u32x2_t *>((uint8_t *)a.codes + row * a.codes_stride + c) = w;
   }
   if (tid == 0) a.scales[row] = row_scale(mag, ss, a);
@@ -185,10 +164,10 @@ __global__ __launch_bounds__(256) void quant_rows_any_kernel(mia_quant_rows_args
   mag = max(max(__float_as_uint(red[0].x), __float_as_uint(red[1].x)),
             max(__float_as_uint(red[2].x), __float_as_uint(red[3].x)));
   ss = (red[0].y + red[1].y) + (red[2].y + red[3].y);
-  RowScale rs;
+  RowCodes<127> rs;
   rs.set(mag);
   for (int c = threadIdx.x; c < a.dim; c += 256)
-    ((uint8_t *)a.codes)[row * a.codes_stride + c] = (uint8_t)rs.code(value(c, false));
+    ((uint8_t *)a.codes)[row * a.codes_stride + c] = (uint8_t)rs.int8(value(c, false));
   if (threadIdx.x == 0) a.scales[row] = row_scale(mag, ss, a);
 }
 

@@ -200,6 +200,33 @@ MIA_HD uint32_t quantize_e4m3fn(float x, float s, int mode) {
   return f32_to_e4m3fn_bits(y);
 }
 
+// Codes of a row by its largest magnitude `mag` (float bits; an infinity or NaN
+// is the largest): code(x) is x * Q / amax to fp32, for the caller to round.
+// x and amax are scaled by the power of two of amax (exact) and the quotient a
+// / b is q + (a - b q) / b with one fma for the remainder: right to the last
+// rounding, so a bf16 row gets the nearest code of the exact quotient.  Rows of
+// zeros, or with an infinity or NaN, get zero codes.
+template <int Q>
+struct RowCodes {
+  float b, rc;
+  int e;
+  bool zero;
+  MIA_DEV void set(uint32_t mag) {
+    zero = mag == 0 || mag >= 0x7f800000u;
+    const float amax = __uint_as_float(mag);
+    e = __builtin_amdgcn_frexp_expf(amax);
+    b = zero ? 1.0f : ldexpf(amax, -e);  // [0.5, 1)
+    rc = __builtin_amdgcn_rcpf(b);
+    rc = fmaf(fmaf(-b, rc, 1.0f), rc, rc);
+  }
+  MIA_DEV float code(float x) const {
+    const float a = (zero ? 0.f : ldexpf(x, -e)) * (float)Q;
+    const float q = a * rc;
+    return fmaf(fmaf(-b, q, a), rc, q);
+  }
+  MIA_DEV uint32_t int8(float x) const { return (uint32_t)(int)rintf(code(x)) & 0xffu; }
+};
+
 // ---------------------------------------------------------------------------
 // Division by an invariant positive integer d (Granlund & Montgomery 1994):
 // for 0 <= n < 2^31, n / d == umulhi(n, m) >> (s - 1) with s = ceil(log2 d),

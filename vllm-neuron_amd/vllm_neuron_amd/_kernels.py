@@ -1301,3 +1301,102 @@ def int8_linear(x, x_scales, w, w_scales, bias, out):
         w_scales.data_ptr(), 0 if bias is None else bias.data_ptr(), out.data_ptr(),
         out.stride(0), m, n, k, int(bias is not None and bias.dtype == torch.bfloat16))
     N.launch(N.lib().mia_int8_linear, a, dev, "int8_linear")
+
+
+# ---------------------------------------------------------------------------
+# rotation by several position axes, with the cache append
+# ---------------------------------------------------------------------------
+_NO_CACHE = (0,) * 25  # slots, dtypes, caches, scales and geometry
+
+
+def rope_append(q, k, v, positions, inv_freq, slots, k_cache, v_cache, q_out, k_out=None, *,
+                sections, cycle=False, interleaved=False, rope_scale=1.0, qk_norm=False,
+                q_gamma=None, k_gamma=None, eps=1e-6, k_scales=None, v_scales=None,
+                k_dequant=None, v_dequant=None) -> None:
+    """``q [T, Hq, d]`` and ``k [T, Hkv, d]`` rotated into ``q_out`` / ``k_out``,
+    K and ``v`` into ``slots [T]`` of a cache ``[nb, Hkv, bs, d]`` (None: no
+    cache)."""
+    dev = N.same_gpu(q, k, v, positions, inv_freq, slots, k_cache, v_cache, q_out, k_out,
+                     k_scales, v_scales, k_dequant, v_dequant, q_gamma, k_gamma)
+    if q.dim() != 3 or k.dim() != 3:
+        raise ValueError(f"q and k must be [T, heads, d], got {tuple(q.shape)} / "
+                         f"{tuple(k.shape)}")
+    T, hq, d = q.shape
+    hkv = k.shape[1]
+    if k.shape != (T, hkv, d) or (v is not None and v.shape != k.shape):
+        raise ValueError(f"K and V rows must be [{T}, Hkv, {d}], got {tuple(k.shape)} / "
+                         f"{None if v is None else tuple(v.shape)}")
+    rows = []
+    for t, like, what in ((q, q, "q"), (k, k, "k"), (v, k, "v"), (q_out, q, "q_out"),
+                          (k_out, k, "k_out")):
+        if t is None:
+            rows += (0, 0, 0)
+            continue
+        if t.dtype != torch.bfloat16:
+            raise NotImplementedError(f"rope_append: {what} must be bf16")
+        if t.shape != like.shape or t.stride(2) != 1:
+            raise ValueError(f"{what} must be a {tuple(like.shape)} view with contiguous d")
+        rows += (t.data_ptr(), t.stride(0), t.stride(1))
+    if inv_freq.dim() != 1 or inv_freq.dtype != torch.float32 or not inv_freq.is_contiguous():
+        raise ValueError("inv_freq must be a contiguous float32 vector of rot_dim / 2 entries")
+    half = inv_freq.shape[0]
+    if positions.dim() == 1:
+        positions = positions.unsqueeze(0)
+    axes = positions.shape[0] if positions.dim() == 2 else 0
+    if axes == 0 or positions.shape[1] != T:
+        raise ValueError(f"positions must be [T] or [axes, T] with T = {T}, got "
+                         f"{tuple(positions.shape)}")
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"positions must be int32 or int64, got {positions.dtype}")
+    sections = [half] if sections is None and axes == 1 else sections
+    if sections is None or len(sections) != axes or sum(sections) != half or min(sections) < 0:
+        raise ValueError(f"sections must split the {half} channel pairs over {axes} axes, got "
+                         f"{sections}")
+    if axes > 4:
+        raise NotImplementedError("rope_append: one to four position axes")
+    if not qk_norm and (q_gamma is not None or k_gamma is not None):
+        raise ValueError("q_gamma and k_gamma belong to qk_norm")
+    keep = []
+    for g, what in ((q_gamma, "q_gamma"), (k_gamma, "k_gamma")):
+        keep.append(None if g is None else _vector(g, d, what, dev))
+    if len({g.dtype for g in keep if g is not None}) > 1:
+        keep = [g.float() for g in keep]
+    gamma_bf16 = any(g is not None and g.dtype == torch.bfloat16 for g in keep)
+    cache = _NO_CACHE
+    if slots is not None:
+        if v is None or k_cache is None or v_cache is None:
+            raise ValueError("the cache append needs v, k_cache and v_cache")
+        shape = k_cache.shape
+        if len(shape) != 4 or v_cache.shape != shape or v_cache.dtype != k_cache.dtype:
+            raise ValueError(f"K and V caches must be [nb, Hkv, bs, d] of one dtype, got "
+                             f"{tuple(shape)} / {tuple(v_cache.shape)}")
+        if shape[1] != hkv or shape[3] != d:
+            raise ValueError(f"the cache has {shape[1]} heads of {shape[3]} channels, K "
+                             f"{hkv} of {d}")
+        if slots.dim() != 1 or slots.shape[0] != T:
+            raise ValueError(f"slots must be [T] = [{T}], got {tuple(slots.shape)}")
+        slots = slots if slots.is_contiguous() else slots.contiguous()
+        if (k_scales is None) != (v_scales is None) or (k_dequant is None) != (v_dequant is None):
+            raise ValueError("the scales of K and V go together")
+        scales = (0, 0, *_NO_STRIDES, *_NO_STRIDES)
+        if k_scales is not None:
+            _check_scales(shape, k_scales, v_scales)
+            scales = (k_scales.data_ptr(), v_scales.data_ptr(), *k_scales.stride(),
+                      *v_scales.stride())
+        dequant = (0, 0)
+        if k_dequant is not None:
+            keep += [_scale_f32(k_dequant, dev, hkv, "k_dequant_scale"),
+                     _scale_f32(v_dequant, dev, hkv, "v_dequant_scale")]
+            dequant = (keep[-2].data_ptr(), keep[-1].data_ptr())
+        cache = (slots.data_ptr(), N.mia_dtype(slots.dtype), N.mia_dtype(k_cache.dtype),
+                 k_cache.data_ptr(), v_cache.data_ptr(), *k_cache.stride(), *v_cache.stride(),
+                 *scales, *dequant, shape[0], shape[2])
+    elif k_cache is not None or v is not None:
+        raise ValueError("the cache append needs slots")
+    a = N.RopeAppendArgs()
+    N.PACK_ROPE.pack_into(
+        a, 0, *rows, T, hq, hkv, d, 2 * half, positions.data_ptr(), *positions.stride(),
+        N.mia_dtype(positions.dtype), axes, inv_freq.data_ptr(), *sections, *([0] * (4 - axes)),
+        int(cycle), int(interleaved), rope_scale, int(qk_norm), N.ptr(keep[0]) or 0,
+        N.ptr(keep[1]) or 0, int(gamma_bf16), eps, *cache)
+    N.launch(N.lib().mia_rope_append, a, dev, "rope_append")

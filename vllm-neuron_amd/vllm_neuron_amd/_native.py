@@ -272,6 +272,25 @@ class Int8LinearArgs(ctypes.Structure):
     ]
 
 
+class RopeAppendArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", c_vp), ("q_stride", c_i64 * 2), ("k", c_vp), ("k_stride", c_i64 * 2),
+        ("v", c_vp), ("v_stride", c_i64 * 2), ("q_out", c_vp), ("q_out_stride", c_i64 * 2),
+        ("k_out", c_vp), ("k_out_stride", c_i64 * 2), ("num_tokens", c_i64),
+        ("num_q_heads", c_i32), ("num_kv_heads", c_i32), ("head_dim", c_i32), ("rot_dim", c_i32),
+        ("positions", c_vp), ("pos_stride", c_i64 * 2), ("pos_dtype", c_i32), ("axes", c_i32),
+        ("inv_freq", c_vp), ("section", c_i32 * 4), ("section_cycle", c_i32),
+        ("interleaved", c_i32), ("rope_scale", c_f32), ("qk_norm", c_i32),
+        ("q_gamma", c_vp), ("k_gamma", c_vp), ("gamma_bf16", c_i32), ("eps", c_f32),
+        ("slots", c_vp), ("slot_dtype", c_i32), ("cache_dtype", c_i32),
+        ("k_cache", c_vp), ("v_cache", c_vp),
+        ("k_cache_stride", c_i64 * 4), ("v_cache_stride", c_i64 * 4),
+        ("k_scales", c_vp), ("v_scales", c_vp),
+        ("k_scale_stride", c_i64 * 3), ("v_scale_stride", c_i64 * 3),
+        ("k_dequant", c_vp), ("v_dequant", c_vp), ("num_blocks", c_i32), ("block_size", c_i32),
+    ]
+
+
 _CODES = {c_vp: "P", c_i32: "i", c_i64: "q", c_f32: "f", ctypes.c_size_t: "N"}
 
 
@@ -290,6 +309,7 @@ PACK_CROSS = _packer(CrossArgs)
 PACK_PREFIX = _packer(SharedPrefixArgs)
 PACK_QUANT_ROWS = _packer(QuantRowsArgs)
 PACK_INT8 = _packer(Int8LinearArgs)
+PACK_ROPE = _packer(RopeAppendArgs)
 
 
 ARGS_STRUCTS = {
@@ -297,6 +317,7 @@ ARGS_STRUCTS = {
     5: SlotMappingArgs, 6: PackedKArgs, 7: SwaTrimArgs, 8: ScatterRowsArgs, 9: StageArgs,
     10: QkvEpilogueArgs, 11: RowNormArgs, 12: SkinnyLinearArgs, 13: QuantKvArgs,
     14: CrossArgs, 15: SharedPrefixArgs, 16: QuantRowsArgs, 17: Int8LinearArgs,
+    18: RopeAppendArgs,
 }
 
 # Exported symbols (must match include/mia_attn.h).
@@ -309,7 +330,7 @@ EXPORTS = [
     "mia_row_norm", "mia_skinny_linear", "mia_paged_decode_noalloc",
     "mia_quant_kv_write", "mia_quant_kv_read", "mia_cross_workspace_bytes",
     "mia_cross_attention", "mia_shared_prefix_workspace_bytes", "mia_shared_prefix_attention",
-    "mia_quant_rows", "mia_int8_linear",
+    "mia_quant_rows", "mia_int8_linear", "mia_rope_append",
 ]
 
 # Static scratch capacity of mia_paged_decode_noalloc (include/mia_attn.h).
@@ -336,7 +357,8 @@ def _declare(lib: ctypes.CDLL) -> None:
                      ("mia_quant_kv_write", QuantKvArgs), ("mia_quant_kv_read", QuantKvArgs),
                      ("mia_cross_attention", CrossArgs),
                      ("mia_shared_prefix_attention", SharedPrefixArgs),
-                     ("mia_quant_rows", QuantRowsArgs), ("mia_int8_linear", Int8LinearArgs)):
+                     ("mia_quant_rows", QuantRowsArgs), ("mia_int8_linear", Int8LinearArgs),
+                     ("mia_rope_append", RopeAppendArgs)):
         fn = getattr(lib, name)
         fn.argtypes = [P(st), c_vp]
         fn.restype = c_i32

@@ -8,6 +8,7 @@ from .attention.int8_linear import int8_linear, quant_rows
 from .attention.mixed_batch import mixed_batch_attention
 from .attention.qkv import qkv_proj
 from .attention.quant_cache import quant_kv_read, quant_kv_write
+from .attention.rope_append import rope_kv_append, rope_rotate
 from .attention.shared_prefix import shared_prefix_attention
 from .attention.swa_fused import swa_fused_attention
 
@@ -26,4 +27,6 @@ __all__ = [
     "shared_prefix_attention",
     "quant_rows",
     "int8_linear",
+    "rope_kv_append",
+    "rope_rotate",
 ]

@@ -724,11 +724,57 @@ def int8_linear(x, x_scales, w, w_scales, bias=None, out=None) -> Tensor:
     return out
 
 
+# ---------------------------------------------------------------------------
+# rotation by several position axes, with the cache append
+# ---------------------------------------------------------------------------
+@custom_op("mia::rope_append", mutates_args=("q_out", "k_out", "k_cache", "v_cache", "k_scales",
+                                             "v_scales"))
+def _rope_append(q: Tensor, k: Tensor, v: Optional[Tensor], positions: Tensor, inv_freq: Tensor,
+                 slots: Optional[Tensor], k_cache: Optional[Tensor], v_cache: Optional[Tensor],
+                 q_out: Tensor, k_out: Optional[Tensor], k_scales: Optional[Tensor],
+                 v_scales: Optional[Tensor], k_dequant: Optional[Tensor],
+                 v_dequant: Optional[Tensor], q_gamma: Optional[Tensor],
+                 k_gamma: Optional[Tensor], sections: Optional[List[int]], cycle: bool,
+                 interleaved: bool, rope_scale: float, qk_norm: bool, eps: float) -> None:
+    K.rope_append(q, k, v, positions, inv_freq, slots, k_cache, v_cache, q_out, k_out,
+                  sections=sections, cycle=cycle, interleaved=interleaved,
+                  rope_scale=rope_scale, qk_norm=qk_norm, q_gamma=q_gamma, k_gamma=k_gamma,
+                  eps=eps, k_scales=k_scales, v_scales=v_scales, k_dequant=k_dequant,
+                  v_dequant=v_dequant)
+
+
+@_rope_append.register_fake
+def _(q, k, v, positions, inv_freq, slots, k_cache, v_cache, q_out, k_out, k_scales, v_scales,
+      k_dequant, v_dequant, q_gamma, k_gamma, sections, cycle, interleaved, rope_scale, qk_norm,
+      eps):
+    return None
+
+
+def rope_append(q, k, v, positions, inv_freq, slots, k_cache, v_cache, q_out, k_out=None, *,
+                sections=None, cycle: bool = False, interleaved: bool = False,
+                rope_scale: float = 1.0, qk_norm: bool = False, q_gamma=None, k_gamma=None,
+                eps: float = 1e-6, k_scales=None, v_scales=None, k_dequant=None,
+                v_dequant=None) -> None:
+    if _plain(q, k, v, positions, inv_freq, slots, k_cache, v_cache, q_out, k_out, k_scales,
+              v_scales, k_dequant, v_dequant, q_gamma, k_gamma):
+        K.rope_append(q, k, v, positions, inv_freq, slots, k_cache, v_cache, q_out, k_out,
+                      sections=sections, cycle=cycle, interleaved=interleaved,
+                      rope_scale=float(rope_scale), qk_norm=bool(qk_norm), q_gamma=q_gamma,
+                      k_gamma=k_gamma, eps=float(eps), k_scales=k_scales, v_scales=v_scales,
+                      k_dequant=k_dequant, v_dequant=v_dequant)
+        _written(q_out, k_out, k_cache, v_cache, k_scales, v_scales)
+        return
+    _rope_append(q, k, v, positions, inv_freq, slots, k_cache, v_cache, q_out, k_out, k_scales,
+                 v_scales, k_dequant, v_dequant, q_gamma, k_gamma,
+                 None if sections is None else [int(n) for n in sections], bool(cycle),
+                 bool(interleaved), float(rope_scale), bool(qk_norm), float(eps))
+
+
 OPS: List[str] = [
     "kv_write", "gather_kv", "packed_k_convert", "scatter_rows", "stage_rows", "decode_mask",
     "slot_mapping", "remap_null_block", "swa_trim", "paged_decode", "paged_decode_write",
     "paged_prefill",
     "qkv_epilogue", "row_norm", "skinny_linear",
     "quant_kv_write", "quant_kv_read", "cross_attention", "shared_prefix_attention",
-    "quant_rows", "int8_linear",
+    "quant_rows", "int8_linear", "rope_append",
 ]
