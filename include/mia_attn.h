@@ -922,6 +922,63 @@ typedef struct {
 
 int mia_rope_append(const mia_rope_append_args *args, mia_stream_t stream);
 
+/* ------------------------------------------------------------------------ */
+/* Attention over a paged cache with a sliding window and first tokens that  */
+/* stay visible (no counterpart in the reference, whose windows forget every */
+/* token behind them).                                                       */
+/* Sequence i has query tokens [cu_seqlens_q[i], cu_seqlens_q[i+1]) (token i */
+/* alone if cu_seqlens_q is NULL), the last of its seq_lens[i] tokens, all   */
+/* of them in the cache already.  The query at position p sees key t iff     */
+/* t <= p and (t < first_tokens or t > p - window).  The sink logit enters   */
+/* the denominator.  Rows without keys give 0.  seq_lens are clamped to what */
+/* the table holds; entries that no query sees are never used, others        */
+/* outside the pool read its first or last block.  cu_seqlens_q must not     */
+/* decrease (rows that two sequences claim get either's result); at most     */
+/* max_seqlen_q tokens of a sequence are computed.  Rows that nothing        */
+/* computes stay as they were, or give 0 with zero_rest.                     */
+/* Caches and heads as for mia_cross_attention with a table.                 */
+/* ------------------------------------------------------------------------ */
+typedef struct {
+  const void *q; /* bf16 */
+  int64_t q_stride[3]; /* token, hq, d */
+  void *out;           /* bf16 */
+  int64_t out_stride[3];
+  int32_t num_tokens;
+  int32_t num_seqs;
+  const int32_t *cu_seqlens_q; /* device, [num_seqs + 1], or NULL */
+  int32_t max_seqlen_q;
+  int32_t num_q_heads;
+  int32_t num_kv_heads;
+  int32_t head_dim;
+  const void *k_cache;
+  const void *v_cache;
+  int32_t cache_dtype; /* BF16, FP8_E4M3FN or I8 */
+  int32_t num_blocks;
+  int64_t k_cache_stride[4]; /* block, head, token, dim */
+  int64_t v_cache_stride[4];
+  int32_t block_size;
+  int32_t blocks_per_seq;
+  const int32_t *block_table; /* device */
+  int64_t bt_stride[2];       /* seq, j */
+  const int32_t *seq_lens;    /* device, [num_seqs] */
+  int32_t window;
+  int32_t first_tokens;
+  const float *k_scales; /* per token and head, or NULL */
+  const float *v_scales;
+  int64_t k_scale_stride[3]; /* block, head, token */
+  int64_t v_scale_stride[3];
+  const float *k_dequant; /* [Hkv] or NULL */
+  const float *v_dequant;
+  const float *sink; /* [Hq] or NULL */
+  float softmax_scale;
+  int32_t zero_rest;
+  void *workspace; /* mia_window_workspace_bytes() (may be 0), 256-byte aligned */
+  size_t workspace_bytes;
+} mia_window_args;
+
+size_t mia_window_workspace_bytes(const mia_window_args *args);
+int mia_window_attention(const mia_window_args *args, mia_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

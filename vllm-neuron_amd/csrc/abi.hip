@@ -128,6 +128,7 @@ size_t mia_args_size(int which) {
     case 16: return sizeof(mia_quant_rows_args);
     case 17: return sizeof(mia_int8_linear_args);
     case 18: return sizeof(mia_rope_append_args);
+    case 19: return sizeof(mia_window_args);
     default: return 0;
   }
 }
@@ -926,6 +927,51 @@ int mia_rope_append(const mia_rope_append_args *a, mia_stream_t stream) {
                 "rope_append: cache head_dim must be contiguous and its rows aligned to 4 elements");
   }
   return mia::launch_rope_append(*a, (hipStream_t)stream);
+}
+
+static int validate_window(const mia_window_args *a) {
+  MIA_REQUIRE(a, MIA_ERR_VALUE, "window_attention: null args");
+  MIA_REQUIRE(a->num_tokens >= 0 && a->num_seqs >= 0, MIA_ERR_VALUE,
+              "window_attention: bad shape");
+  if (a->num_tokens == 0 || a->num_seqs == 0) return MIA_OK;
+  MIA_REQUIRE(a->q && a->out && a->k_cache && a->v_cache && a->block_table && a->seq_lens,
+              MIA_ERR_VALUE, "window_attention: null tensor pointer");
+  MIA_REQUIRE(!a->cu_seqlens_q || a->max_seqlen_q > 0, MIA_ERR_VALUE,
+              "window_attention: max_seqlen_q must be positive");
+  MIA_REQUIRE(a->cu_seqlens_q || a->num_seqs <= a->num_tokens, MIA_ERR_VALUE,
+              "window_attention: fewer tokens than sequences of one token");
+  MIA_REQUIRE(a->window > 0 && a->window <= (1 << 30), MIA_ERR_VALUE,
+              "window_attention: the window must be in [1, 2^30]");
+  MIA_REQUIRE(a->first_tokens >= 0 && a->first_tokens <= (1 << 30), MIA_ERR_VALUE,
+              "window_attention: first_tokens must be in [0, 2^30]");
+  const int extents[2] = {a->num_tokens, a->num_q_heads};
+  const int rc = check_span(*a, a->q_stride, a->out_stride, extents, 2, a->num_tokens, true);
+  if (rc) return rc;
+  // the row tiles of all sequences lie along one grid axis, 32 pieces at most
+  const int64_t G = a->num_q_heads / a->num_kv_heads;
+  const int64_t most = a->cu_seqlens_q && a->max_seqlen_q < a->num_tokens ? a->max_seqlen_q
+                       : a->cu_seqlens_q ? a->num_tokens : 1;
+  MIA_REQUIRE((most * G / 128 + 1) * a->num_seqs < (1ll << 19) / a->num_kv_heads, MIA_ERR_VALUE,
+              "window_attention: row tiles * sequences * kv heads beyond 2^19");
+  return MIA_OK;
+}
+
+size_t mia_window_workspace_bytes(const mia_window_args *a) {
+  mia::g_last_error.clear();
+  if (validate_window(a) || a->num_tokens == 0 || a->num_seqs == 0) return 0;
+  return mia::window_workspace(*a);
+}
+
+int mia_window_attention(const mia_window_args *a, mia_stream_t stream) {
+  mia::g_last_error.clear();
+  const int rc = validate_window(a);
+  if (rc) return rc;
+  if (a->num_tokens == 0 || a->num_seqs == 0) return MIA_OK;
+  const size_t need = mia::window_workspace(*a);
+  MIA_REQUIRE(need == 0 || (a->workspace && aligned(a->workspace, 256) &&
+                            a->workspace_bytes >= need),
+              MIA_ERR_VALUE, "window_attention: workspace missing, unaligned or too small");
+  return mia::launch_window(*a, (hipStream_t)stream);
 }
 
 }  // extern "C"

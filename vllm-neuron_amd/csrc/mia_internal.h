@@ -36,6 +36,8 @@ int launch_skinny_linear(const mia_skinny_linear_args &a, hipStream_t s);
 int launch_quant_rows(const mia_quant_rows_args &a, hipStream_t s);
 int launch_int8_linear(const mia_int8_linear_args &a, hipStream_t s);
 int launch_rope_append(const mia_rope_append_args &a, hipStream_t s);
+size_t window_workspace(const mia_window_args &a);
+int launch_window(const mia_window_args &a, hipStream_t s);
 int launch_quant_kv(const mia_quant_kv_args &a, bool write, hipStream_t s);
 size_t cross_workspace(const mia_cross_args &a);
 int launch_cross(const mia_cross_args &a, hipStream_t s);

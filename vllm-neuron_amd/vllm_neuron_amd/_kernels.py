@@ -1400,3 +1400,49 @@ def rope_append(q, k, v, positions, inv_freq, slots, k_cache, v_cache, q_out, k_
         int(cycle), int(interleaved), rope_scale, int(qk_norm), N.ptr(keep[0]) or 0,
         N.ptr(keep[1]) or 0, int(gamma_bf16), eps, *cache)
     N.launch(N.lib().mia_rope_append, a, dev, "rope_append")
+
+
+# ---------------------------------------------------------------------------
+# sliding window with first tokens that stay visible
+# ---------------------------------------------------------------------------
+def window_attention(q, k_cache, v_cache, block_table, seq_lens, out, *, window, first_tokens,
+                     softmax_scale, cu_seqlens_q=None, max_seqlen_q=0, sink=None, k_scales=None,
+                     v_scales=None, k_dequant=None, v_dequant=None, workspace=None,
+                     zero_rest=False) -> None:
+    """Attention of ``q [T, Hq, d]`` over a window of a paged cache and its first
+    tokens into ``out``; rows of no sequence stay as they were, or are cleared
+    (``zero_rest``)."""
+    dev = N.same_gpu(q, k_cache, v_cache, block_table, seq_lens, out, cu_seqlens_q, sink, k_scales,
+                     v_scales, k_dequant, v_dequant, workspace)
+    if q.dim() != 3:
+        raise ValueError(f"q must be [T, Hq, d], got {tuple(q.shape)}")
+    _check_out(out, q)
+    if seq_lens.dim() != 1:
+        raise ValueError("seq_lens must be one int32 per sequence")
+    T, n = q.shape[0], seq_lens.shape[0]
+    seq_lens = _int32(seq_lens, n, "seq_lens")
+    (nb, hkv, bs, d), hq, code, scales, kd, vd = _span_cache(
+        q, k_cache, v_cache, k_scales, v_scales, k_dequant, v_dequant, dev)
+    cu = 0
+    if cu_seqlens_q is not None:
+        cu_seqlens_q = _int32(cu_seqlens_q, n + 1, "cu_seqlens_q")
+        cu = cu_seqlens_q.data_ptr()
+    if block_table.dim() != 2 or block_table.shape[0] != n or block_table.dtype != torch.int32:
+        raise ValueError(f"block table must be int32 [{n}, blocks], got {block_table.dtype} "
+                         f"{tuple(block_table.shape)}")
+    sk = _scale_f32(sink, dev, hq, "sink")
+    if sk is not None and sk.numel() != hq:
+        raise ValueError(f"sink must have {hq} entries, got {sk.numel()}")
+    for v, least, what in ((window, 1, "window"), (first_tokens, 0, "first_tokens")):
+        if not least <= v <= 1 << 30:
+            raise ValueError(f"{what} must be in [{least}, 2^30], got {v}")
+    a = N.WindowArgs()
+    N.PACK_WINDOW.pack_into(
+        a, 0, q.data_ptr(), *q.stride(), out.data_ptr(), *out.stride(), T, n, cu, max_seqlen_q,
+        hq, hkv, d, k_cache.data_ptr(), v_cache.data_ptr(), code, nb, *k_cache.stride(),
+        *v_cache.stride(), bs, block_table.shape[1], block_table.data_ptr(),
+        *block_table.stride(), seq_lens.data_ptr(), window, first_tokens, *scales,
+        N.ptr(kd) or 0, N.ptr(vd) or 0, N.ptr(sk) or 0, softmax_scale, int(zero_rest), 0, 0)
+    L = N.lib()
+    _span_launch(a, L.mia_window_workspace_bytes, L.mia_window_attention, "window_attention",
+                 workspace, dev)

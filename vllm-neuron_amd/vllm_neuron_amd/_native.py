@@ -291,6 +291,22 @@ class RopeAppendArgs(ctypes.Structure):
     ]
 
 
+class WindowArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", c_vp), ("q_stride", c_i64 * 3), ("out", c_vp), ("out_stride", c_i64 * 3),
+        ("num_tokens", c_i32), ("num_seqs", c_i32), ("cu_seqlens_q", c_vp),
+        ("max_seqlen_q", c_i32), ("num_q_heads", c_i32), ("num_kv_heads", c_i32),
+        ("head_dim", c_i32), ("k_cache", c_vp), ("v_cache", c_vp), ("cache_dtype", c_i32),
+        ("num_blocks", c_i32), ("k_cache_stride", c_i64 * 4), ("v_cache_stride", c_i64 * 4),
+        ("block_size", c_i32), ("blocks_per_seq", c_i32), ("block_table", c_vp),
+        ("bt_stride", c_i64 * 2), ("seq_lens", c_vp), ("window", c_i32),
+        ("first_tokens", c_i32), ("k_scales", c_vp), ("v_scales", c_vp),
+        ("k_scale_stride", c_i64 * 3), ("v_scale_stride", c_i64 * 3),
+        ("k_dequant", c_vp), ("v_dequant", c_vp), ("sink", c_vp), ("softmax_scale", c_f32),
+        ("zero_rest", c_i32), ("workspace", c_vp), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 _CODES = {c_vp: "P", c_i32: "i", c_i64: "q", c_f32: "f", ctypes.c_size_t: "N"}
 
 
@@ -310,6 +326,7 @@ PACK_PREFIX = _packer(SharedPrefixArgs)
 PACK_QUANT_ROWS = _packer(QuantRowsArgs)
 PACK_INT8 = _packer(Int8LinearArgs)
 PACK_ROPE = _packer(RopeAppendArgs)
+PACK_WINDOW = _packer(WindowArgs)
 
 
 ARGS_STRUCTS = {
@@ -317,7 +334,7 @@ ARGS_STRUCTS = {
     5: SlotMappingArgs, 6: PackedKArgs, 7: SwaTrimArgs, 8: ScatterRowsArgs, 9: StageArgs,
     10: QkvEpilogueArgs, 11: RowNormArgs, 12: SkinnyLinearArgs, 13: QuantKvArgs,
     14: CrossArgs, 15: SharedPrefixArgs, 16: QuantRowsArgs, 17: Int8LinearArgs,
-    18: RopeAppendArgs,
+    18: RopeAppendArgs, 19: WindowArgs,
 }
 
 # Exported symbols (must match include/mia_attn.h).
@@ -331,6 +348,7 @@ EXPORTS = [
     "mia_quant_kv_write", "mia_quant_kv_read", "mia_cross_workspace_bytes",
     "mia_cross_attention", "mia_shared_prefix_workspace_bytes", "mia_shared_prefix_attention",
     "mia_quant_rows", "mia_int8_linear", "mia_rope_append",
+    "mia_window_workspace_bytes", "mia_window_attention",
 ]
 
 # Static scratch capacity of mia_paged_decode_noalloc (include/mia_attn.h).
@@ -358,7 +376,8 @@ def _declare(lib: ctypes.CDLL) -> None:
                      ("mia_cross_attention", CrossArgs),
                      ("mia_shared_prefix_attention", SharedPrefixArgs),
                      ("mia_quant_rows", QuantRowsArgs), ("mia_int8_linear", Int8LinearArgs),
-                     ("mia_rope_append", RopeAppendArgs)):
+                     ("mia_rope_append", RopeAppendArgs),
+                     ("mia_window_attention", WindowArgs)):
         fn = getattr(lib, name)
         fn.argtypes = [P(st), c_vp]
         fn.restype = c_i32
@@ -370,6 +389,8 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.mia_cross_workspace_bytes.restype = ctypes.c_size_t
     lib.mia_shared_prefix_workspace_bytes.argtypes = [P(SharedPrefixArgs)]
     lib.mia_shared_prefix_workspace_bytes.restype = ctypes.c_size_t
+    lib.mia_window_workspace_bytes.argtypes = [P(WindowArgs)]
+    lib.mia_window_workspace_bytes.restype = ctypes.c_size_t
     lib.mia_slot_mapping_host.argtypes = [P(SlotMappingArgs)]
     lib.mia_slot_mapping_host.restype = c_i32
     lib.mia_remap_null_block.argtypes = [c_vp, c_vp, c_i64, c_i32, c_vp]

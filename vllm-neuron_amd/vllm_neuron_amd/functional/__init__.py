@@ -11,6 +11,7 @@ from .attention.quant_cache import quant_kv_read, quant_kv_write
 from .attention.rope_append import rope_kv_append, rope_rotate
 from .attention.shared_prefix import shared_prefix_attention
 from .attention.swa_fused import swa_fused_attention
+from .attention.window_attention import window_attention
 
 __all__ = [
     "flash_attention",
@@ -29,4 +30,5 @@ __all__ = [
     "int8_linear",
     "rope_kv_append",
     "rope_rotate",
+    "window_attention",
 ]

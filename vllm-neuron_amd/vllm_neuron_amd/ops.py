@@ -770,11 +770,61 @@ def rope_append(q, k, v, positions, inv_freq, slots, k_cache, v_cache, q_out, k_
                  bool(interleaved), float(rope_scale), bool(qk_norm), float(eps))
 
 
+# ---------------------------------------------------------------------------
+# sliding window with first tokens that stay visible
+# ---------------------------------------------------------------------------
+@custom_op("mia::window_attention", mutates_args=("out", "workspace"))
+def _window_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Tensor,
+                      seq_lens: Tensor, out: Tensor, cu_seqlens_q: Optional[Tensor],
+                      sink: Optional[Tensor], k_scales: Optional[Tensor],
+                      v_scales: Optional[Tensor], k_dequant: Optional[Tensor],
+                      v_dequant: Optional[Tensor], workspace: Optional[Tensor], window: int,
+                      first_tokens: int, max_seqlen_q: int, softmax_scale: float,
+                      zero_rest: bool) -> None:
+    K.window_attention(q, k_cache, v_cache, block_table, seq_lens, out, window=window,
+                       first_tokens=first_tokens, softmax_scale=softmax_scale,
+                       cu_seqlens_q=cu_seqlens_q, max_seqlen_q=max_seqlen_q, sink=sink,
+                       k_scales=k_scales, v_scales=v_scales, k_dequant=k_dequant,
+                       v_dequant=v_dequant, workspace=workspace, zero_rest=zero_rest)
+
+
+@_window_attention.register_fake
+def _(q, k_cache, v_cache, block_table, seq_lens, out, cu_seqlens_q, sink, k_scales, v_scales,
+      k_dequant, v_dequant, workspace, window, first_tokens, max_seqlen_q, softmax_scale,
+      zero_rest):
+    return None
+
+
+def window_attention(q, k_cache, v_cache, block_table, seq_lens, *, window: int,
+                     first_tokens: int = 0, softmax_scale: float, cu_seqlens_q=None,
+                     max_seqlen_q: int = 0, sink=None, k_scales=None, v_scales=None,
+                     k_dequant=None, v_dequant=None, out=None, workspace=None) -> Tensor:
+    # an output allocated here has no row of unknown memory: the launch clears
+    # those of no sequence (without any sequence there is no launch)
+    rest = out is None
+    if rest:
+        new = torch.empty if seq_lens.numel() else torch.zeros
+        out = new(q.shape, dtype=torch.bfloat16, device=q.device)
+    if _plain(q, k_cache, v_cache, block_table, seq_lens, out, cu_seqlens_q, sink, k_scales,
+              v_scales, k_dequant, v_dequant, workspace):
+        K.window_attention(q, k_cache, v_cache, block_table, seq_lens, out, window=int(window),
+                           first_tokens=int(first_tokens), softmax_scale=float(softmax_scale),
+                           cu_seqlens_q=cu_seqlens_q, max_seqlen_q=int(max_seqlen_q), sink=sink,
+                           k_scales=k_scales, v_scales=v_scales, k_dequant=k_dequant,
+                           v_dequant=v_dequant, workspace=workspace, zero_rest=rest)
+        _written(out, workspace)
+        return out
+    _window_attention(q, k_cache, v_cache, block_table, seq_lens, out, cu_seqlens_q, sink,
+                      k_scales, v_scales, k_dequant, v_dequant, workspace, int(window),
+                      int(first_tokens), int(max_seqlen_q), float(softmax_scale), rest)
+    return out
+
+
 OPS: List[str] = [
     "kv_write", "gather_kv", "packed_k_convert", "scatter_rows", "stage_rows", "decode_mask",
     "slot_mapping", "remap_null_block", "swa_trim", "paged_decode", "paged_decode_write",
     "paged_prefill",
     "qkv_epilogue", "row_norm", "skinny_linear",
     "quant_kv_write", "quant_kv_read", "cross_attention", "shared_prefix_attention",
-    "quant_rows", "int8_linear", "rope_append",
+    "quant_rows", "int8_linear", "rope_append", "window_attention",
 ]
