@@ -272,3 +272,22 @@ def test_calls_on_other_streams_and_in_graphs(gpu):
         assert torch.equal(out, step(fresh))
     compiled = torch.compile(step, fullgraph=True, backend="aot_eager")
     assert torch.equal(compiled(x), want)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 700, 4096), (16, 5000, 1040), (30, 9000, 272), (40, 2500, 4112), (64, 6144, 144),
+                                   (100, 17000, 80), (150, 4100, 2064), (260, 3000, 3088), (600, 2050, 400),
+                                   (513, 520, 8208), (1300, 5200, 656), (4100, 2570, 336), (5000, 7000, 64),
+                                   (2049, 8193, 16)])
+def test_products_whatever_form_is_taken(gpu, m, n, k):
+    """Sizes across the forms' ranges, with ragged last tiles in every axis."""
+    g = torch.Generator(device=gpu).manual_seed(m)
+    x = torch.randint(-127, 128, (m, k), generator=g, device=gpu, dtype=torch.int32).to(torch.int8)
+    w = torch.randint(-127, 128, (n, k), generator=g, device=gpu, dtype=torch.int32).to(torch.int8)
+    xs = torch.rand(m, generator=g, device=gpu) + 0.1
+    ws = torch.rand(n, generator=g, device=gpu) * 0.01
+    y = int8_linear(x, xs, w, ws)
+    acc = torch.zeros(m, n, dtype=torch.float64, device=gpu)
+    for i in range(0, k, 1024):  # exact in float32: 1024 products of at most 127 * 127 are below 2^24
+        acc += (x[:, i:i + 1024].float() @ w[:, i:i + 1024].float().t()).double()
+    ref = acc * xs.double()[:, None] * ws.double()
+    assert ((y.double() - ref).abs() <= 2.0 ** -8 * ref.abs() + 2.0 ** -21 * ref.abs()).all()

@@ -1,20 +1,16 @@
 // int8_linear.hip — rows quantised to int8 with one scale per token, and their
 // product with int8 weights of one scale per output channel.
 #include <algorithm>
+#include <atomic>
 
-#include "mia_device.h"
-#include "mia_internal.h"
+#include "attn_tile.h"
 
 namespace mia {
 namespace {
 
 typedef int i32x4_t __attribute__((ext_vector_type(4)));
 typedef int i32x16_t __attribute__((ext_vector_type(16)));
-typedef __attribute__((address_space(3))) uint8_t lds_u8_t;
-typedef __attribute__((address_space(3))) u32x4_t lds_u32x4_t;
 typedef __attribute__((address_space(3))) u32x2_t lds_u32x2_t;
-typedef __attribute__((address_space(3))) f32x4_t lds_f32x4_t;
-typedef __attribute__((address_space(3))) float lds_f32_t;
 typedef __attribute__((address_space(3))) uint16_t lds_u16_t;
 
 // ---------------------------------------------------------------------------
@@ -192,166 +188,37 @@ MIA_DEV float bias_at(const GemmParams &p, int n) {
   return p.bias_bf16 ? bf16_bits_to_f32(((const uint16_t *)p.bias)[n]) : ((const float *)p.bias)[n];
 }
 
-// One 16-byte-per-lane copy HBM -> LDS: lane l's lands at lds_dst + 16 l.
-// Inline assembly, so that the compiler adds no waits before reads of other
-// stages; the wait for the copies is explicit.
-MIA_DEV void copy1(const uint8_t *src, uint32_t off, uint32_t lds_dst) {
-  const uint32_t m0 = readfirstlane((int)lds_dst);
-  asm volatile(
-      "s_mov_b32 m0, %0\n\t"
-      "s_nop 0\n\t"
-      "global_load_lds_dwordx4 %2, %1\n\t"
-      :: "s"(m0), "s"(src), "v"(off) : "memory", "m0");
+// The workgroup's tile (column, row).  Each XCD (workgroups go round robin over
+// 8) takes a contiguous run of the tiles, in groups of 8 row tiles, so that its
+// L2 holds what they share.
+MIA_DEV int2 tile_of(const GemmParams &p) {
+  const int total = p.mt * p.nt;
+  const int full = total / 8, rem = total % 8, xcd = blockIdx.x % 8;
+  const int id = xcd * full + min(xcd, rem) + blockIdx.x / 8;
+  const int gsz = 8 * p.nt;
+  const int g = id / gsz, first = g * 8, rows = min(p.mt - first, 8);
+  const int r = id - g * gsz;
+  return make_int2(r / rows, first + r % rows);
 }
 
-constexpr int kBK = 128;  // bytes of k per tile
-
-// Tiled form.  WN x WM waves, each TN x TM products of 32 x 32.
-template <int WN, int WM, int TN, int TM, int STAGES>
-__global__ __launch_bounds__(WN *WM * 64) void gemm_kernel(GemmParams p) {
-  constexpr int WAVES = WN * WM;
-  constexpr int BN = WN * TN * 32, BM = WM * TM * 32;
-  constexpr int NC = BN / 8 / WAVES, MC = BM / 8 / WAVES;  // copies per wave and tile
-  static_assert(BN % (8 * WAVES) == 0 && BM % (8 * WAVES) == 0, "whole copies");
-  constexpr int STAGE = (BN + BM) * kBK;
-  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
-  lds_u8_t *const lds = (lds_u8_t *)smem;
-  const uint32_t lds0 = (uint32_t)(uintptr_t)lds;
-
-  const int tid = threadIdx.x;
-  const int wave = readfirstlane(tid >> 6);
-  const int lane = tid & 63;
-  const int wn = wave % WN, wm = wave / WN;
-  const int rl = lane & 31, half = lane >> 5;
-
-  // tiles: each XCD (workgroups go round robin over 8) takes a contiguous run
-  // of them, in groups of 8 row tiles, so that its L2 holds what they share
-  int tn, tm;
-  {
-    const int total = p.mt * p.nt;
-    const int per = (total + 7) / 8;
-    const int b = blockIdx.x;
-    const int full = total / 8, rem = total % 8, xcd = b % 8;
-    (void)per;
-    const int id = xcd * full + min(xcd, rem) + b / 8;
-    const int gsz = 8 * p.nt;
-    const int g = id / gsz, first = g * 8, rows = min(p.mt - first, 8);
-    const int r = id - g * gsz;
-    tm = first + r % rows;
-    tn = r / rows;
-  }
-  const int n0 = tn * BN, m0 = tm * BM;
-
-  // row and chunk of a lane in copy j: lane l fills slot l % 8 of row l / 8;
-  // chunk c of a row lies in slot c ^ ((row >> 1) & 7) (reads of 16 rows at
-  // one chunk then touch all banks)
-  const uint8_t *wsrc = p.w + (int64_t)n0 * p.w_ld;
-  const uint8_t *xsrc = p.x + (int64_t)m0 * p.x_ld;
-  uint32_t won[NC], xom[MC];
-  const int chunk_e = (lane & 7) ^ (lane >> 4);  // even row groups; odd ones: ^ 4
-#pragma unroll
-  for (int j = 0; j < NC; ++j) {
-    const int g = wave * NC + j, row = g * 8 + (lane >> 3);
-    won[j] = (uint32_t)min(row, p.n - 1 - n0) * (uint32_t)p.w_ld + (chunk_e ^ ((g & 1) * 4)) * 16;
-  }
-#pragma unroll
-  for (int j = 0; j < MC; ++j) {
-    const int g = wave * MC + j, row = g * 8 + (lane >> 3);
-    xom[j] = (uint32_t)min(row, p.m - 1 - m0) * (uint32_t)p.x_ld + (chunk_e ^ ((g & 1) * 4)) * 16;
-  }
-  const int steps = (p.k + kBK - 1) / kBK, full = p.k / kBK;
-  auto load = [&](int t) {
-    const uint32_t dst = lds0 + (uint32_t)(t % STAGES) * STAGE;
-    const int k0 = t * kBK;
-    if (t < full) {
-#pragma unroll
-      for (int j = 0; j < NC; ++j) copy1(wsrc + k0, won[j], dst + (wave * NC + j) * 1024);
-#pragma unroll
-      for (int j = 0; j < MC; ++j)
-        copy1(xsrc + k0, xom[j], dst + BN * kBK + (wave * MC + j) * 1024);
-    } else {
-      // chunks past k keep what the stage held: those of x are cleared below
-#pragma unroll
-      for (int j = 0; j < NC; ++j)
-        if (k0 + (chunk_e ^ (((wave * NC + j) & 1) * 4)) * 16 < p.k)
-          copy1(wsrc + k0, won[j], dst + (wave * NC + j) * 1024);
-#pragma unroll
-      for (int j = 0; j < MC; ++j)
-        if (k0 + (chunk_e ^ (((wave * MC + j) & 1) * 4)) * 16 < p.k)
-          copy1(xsrc + k0, xom[j], dst + BN * kBK + (wave * MC + j) * 1024);
-    }
-  };
-
-  i32x16_t acc[TN][TM] = {};
-  const int swz = (rl >> 1) & 7;  // (rows of a fragment start at multiples of 32)
-  const lds_u8_t *const wrow = lds + (wn * TN * 32 + rl) * kBK;
-  const lds_u8_t *const xrow = lds + BN * kBK + (wm * TM * 32 + rl) * kBK;
-  auto compute = [&](int t) {
-    const uint32_t st = (uint32_t)(t % STAGES) * STAGE;
-    i32x4_t wf[2][TN], xf[2][TM];
-    auto read = [&](int s) {
-      const uint32_t c = (uint32_t)(((2 * s + half) ^ swz) << 4) + st;
-#pragma unroll
-      for (int i = 0; i < TN; ++i)
-        wf[s & 1][i] = __builtin_bit_cast(i32x4_t, *(const lds_u32x4_t *)(wrow + c + i * 32 * kBK));
-#pragma unroll
-      for (int i = 0; i < TM; ++i)
-        xf[s & 1][i] = __builtin_bit_cast(i32x4_t, *(const lds_u32x4_t *)(xrow + c + i * 32 * kBK));
-    };
-    read(0);
-#pragma unroll
-    for (int s = 0; s < kBK / 32; ++s) {
-      if (s + 1 < kBK / 32) read(s + 1);
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int i = 0; i < TN; ++i)
-#pragma unroll
-        for (int j = 0; j < TM; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wf[s & 1][i], xf[s & 1][j], acc[i][j],
-                                                            0, 0, 0);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-  };
-
-#pragma unroll
-  for (int t = 0; t < STAGES - 1; ++t)
-    if (t < steps) load(t);
-  for (int t = 0; t < steps; ++t) {
-    // this tile's own copies have landed (those of later whole tiles may be
-    // under way); the barrier makes every wave's visible and the stage of the
-    // tile before free
-    if (STAGES > 2 && t + STAGES - 2 < full)
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 2) * (NC + MC)) : "memory");
-    else
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    if (t + STAGES - 1 < steps) load(t + STAGES - 1);
-    if (t >= full) {
-      // rows of x past k count nothing (whatever w's hold there)
-      lds_u8_t *const xb = lds + (t % STAGES) * STAGE + BN * kBK;
-      const int left = (p.k - t * kBK) / 16;
-      for (int i = tid; i < BM * 8; i += WAVES * 64)
-        if ((i & 7) >= left)
-          *(lds_u32x4_t *)(xb + (i >> 3) * kBK + (((i & 7) ^ ((i >> 4) & 7)) << 4)) =
-              u32x4_t{0u, 0u, 0u, 0u};
-      __syncthreads();
-    }
-    compute(t);
-  }
-
-  // ---- epilogue: out = acc xs ws + bias, rounded to bf16 through LDS so that
-  // rows are stored whole
-  __syncthreads();
-  lds_f32_t *const wsl = (lds_f32_t *)lds;  // [BN] scales, [BN] bias
-  for (int i = tid; i < BN; i += WAVES * 64) {
+// out = acc xs ws + bias of the workgroup's tile, rounded to bf16 through LDS so
+// that rows are stored whole.  acc: TN x TM products of 32 x 32 of wave (wn, wm),
+// lane: row (token) lane % 32, channels 8 g + 4 (lane / 32) ...  Every thread
+// calls it, those with `has` hold sums.  LDS is free.
+template <int TN, int TM, int BN, int THREADS>
+MIA_DEV void store_tile(const GemmParams &p, lds_u8_t *all, const i32x16_t (&acc)[TN][TM], int n0,
+                        int m0, int wn, int wm, int wave, bool has) {
+  const int tid = threadIdx.x, lane = tid & 63, rl = lane & 31, half = lane >> 5;
+  lds_f32_t *const wsl = (lds_f32_t *)all;  // [BN] scales, [BN] bias
+  for (int i = tid; i < BN; i += THREADS) {
     const int n = min(n0 + i, p.n - 1);
     wsl[i] = p.ws[n];
     wsl[BN + i] = bias_at(p, n);
   }
   __syncthreads();
+  if (!has) return;
   constexpr int ROWB = TN * 64 + 16;
-  lds_u8_t *const stage = lds + BN * 8 + wave * 32 * ROWB;
+  lds_u8_t *const stage = all + BN * 8 + wave * 32 * ROWB;
   const int nw = wn * TN * 32, mw = m0 + wm * TM * 32;
 #pragma unroll
   for (int j = 0; j < TM; ++j) {
@@ -394,87 +261,402 @@ __global__ __launch_bounds__(WN *WM * 64) void gemm_kernel(GemmParams p) {
   }
 }
 
-// Streaming form, at most 16 MT rows: a workgroup takes 16 NT columns, its
-// waves shares of k, operands straight from memory.
+
+constexpr int kBK = 128;  // bytes of k per tile
+
+// WN x WM waves, each TN x TM products of 32 x 32, KS such groups with a share
+// of k and a ring of tiles each.
+template <int WN, int WM, int TN, int TM, int STAGES, int KS>
+__global__ __launch_bounds__(WN *WM *KS * 64) void gemm_kernel(GemmParams p) {
+  constexpr int WAVES = WN * WM;  // of a group
+  constexpr int THREADS = WAVES * KS * 64;
+  constexpr int BN = WN * TN * 32, BM = WM * TM * 32;
+  constexpr int NC = BN / 8 / WAVES, MC = BM / 8 / WAVES;  // copies per wave and tile
+  static_assert(BN % (8 * WAVES) == 0 && BM % (8 * WAVES) == 0, "whole copies");
+  constexpr int STAGE = (BN + BM) * kBK;
+  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+  const int tid = threadIdx.x;
+  const int group = KS == 1 ? 0 : readfirstlane(tid / (WAVES * 64));
+  const int wave = readfirstlane(tid >> 6) - group * WAVES;
+  const int lane = tid & 63;
+  lds_u8_t *const all = (lds_u8_t *)smem;
+  lds_u8_t *const lds = all + group * STAGES * STAGE;  // the group's ring
+  const uint32_t lds0 = (uint32_t)(uintptr_t)lds;
+  const int wn = wave % WN, wm = wave / WN;
+  const int rl = lane & 31, half = lane >> 5;
+
+  const int2 tile = tile_of(p);
+  const int n0 = tile.x * BN, m0 = tile.y * BM;
+
+  // row and chunk of a lane in copy j: lane l fills slot l % 8 of row l / 8;
+  // chunk c of a row lies in slot c ^ ((row >> 1) & 7) (reads of 16 rows at
+  // one chunk then touch all banks)
+  const uint8_t *wsrc = p.w + (int64_t)n0 * p.w_ld;
+  const uint8_t *xsrc = p.x + (int64_t)m0 * p.x_ld;
+  uint32_t won[NC], xom[MC];
+  const int chunk_e = (lane & 7) ^ (lane >> 4);  // even row groups; odd ones: ^ 4
+#pragma unroll
+  for (int j = 0; j < NC; ++j) {
+    const int g = wave * NC + j, row = g * 8 + (lane >> 3);
+    won[j] = (uint32_t)min(row, p.n - 1 - n0) * (uint32_t)p.w_ld + (chunk_e ^ ((g & 1) * 4)) * 16;
+  }
+#pragma unroll
+  for (int j = 0; j < MC; ++j) {
+    const int g = wave * MC + j, row = g * 8 + (lane >> 3);
+    xom[j] = (uint32_t)min(row, p.m - 1 - m0) * (uint32_t)p.x_ld + (chunk_e ^ ((g & 1) * 4)) * 16;
+  }
+  // the group's tiles [t0, t1); every group takes `rounds` steps of the loop
+  const int steps = (p.k + kBK - 1) / kBK, full = p.k / kBK;
+  const int t0 = steps * group / KS, t1 = steps * (group + 1) / KS;
+  const int rounds = (steps + KS - 1) / KS;
+  auto load = [&](int t) {
+    const uint32_t dst = lds0 + (uint32_t)(t % STAGES) * STAGE;
+    const int k0 = t * kBK;
+    if (t < full) {
+#pragma unroll
+      for (int j = 0; j < NC; ++j) copy1(wsrc + k0, won[j], dst + (wave * NC + j) * 1024);
+#pragma unroll
+      for (int j = 0; j < MC; ++j)
+        copy1(xsrc + k0, xom[j], dst + BN * kBK + (wave * MC + j) * 1024);
+    } else {
+      // chunks past k: zeros for x, so that they count nothing whatever w's hold
+      // there; the stage's last readers are behind the barrier as for a copy
+#pragma unroll
+      for (int j = 0; j < NC; ++j)
+        if (k0 + (chunk_e ^ (((wave * NC + j) & 1) * 4)) * 16 < p.k)
+          copy1(wsrc + k0, won[j], dst + (wave * NC + j) * 1024);
+#pragma unroll
+      for (int j = 0; j < MC; ++j) {
+        const uint32_t at = BN * kBK + (wave * MC + j) * 1024;
+        if (k0 + (chunk_e ^ (((wave * MC + j) & 1) * 4)) * 16 < p.k)
+          copy1(xsrc + k0, xom[j], dst + at);
+        else
+          *(lds_u32x4_t *)(lds + (t % STAGES) * STAGE + at + lane * 16) = u32x4_t{0u, 0u, 0u, 0u};
+      }
+    }
+  };
+
+  i32x16_t acc[TN][TM] = {};
+  const int swz = (rl >> 1) & 7;  // (rows of a fragment start at multiples of 32)
+  const lds_u8_t *const wrow = lds + (wn * TN * 32 + rl) * kBK;
+  const lds_u8_t *const xrow = lds + BN * kBK + (wm * TM * 32 + rl) * kBK;
+  auto compute = [&](int t) {
+    const uint32_t st = (uint32_t)(t % STAGES) * STAGE;
+    i32x4_t wf[2][TN], xf[2][TM];
+    auto read = [&](int s) {
+      const uint32_t c = (uint32_t)(((2 * s + half) ^ swz) << 4) + st;
+#pragma unroll
+      for (int i = 0; i < TN; ++i)
+        wf[s & 1][i] = __builtin_bit_cast(i32x4_t, *(const lds_u32x4_t *)(wrow + c + i * 32 * kBK));
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+        xf[s & 1][i] = __builtin_bit_cast(i32x4_t, *(const lds_u32x4_t *)(xrow + c + i * 32 * kBK));
+    };
+    read(0);
+#pragma unroll
+    for (int s = 0; s < kBK / 32; ++s) {
+      if (s + 1 < kBK / 32) read(s + 1);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int j = 0; j < TM; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wf[s & 1][i], xf[s & 1][j], acc[i][j],
+                                                            0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+
+#pragma unroll
+  for (int i = 0; i < STAGES - 1; ++i)
+    if (t0 + i < t1) load(t0 + i);
+  for (int i = 0; i < rounds; ++i) {
+    const int t = t0 + i;
+    // this tile's own copies have landed (those of later whole tiles may be
+    // under way); the barrier makes every wave's visible and the stage of the
+    // tile before free
+    if (STAGES > 2 && t + STAGES - 2 < min(t1, full))
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((STAGES - 2) * (NC + MC)) : "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (t + STAGES - 1 < t1) load(t + STAGES - 1);
+    if (KS == 1 || t < t1) compute(t);
+  }
+
+  // ---- epilogue: out = acc xs ws + bias, rounded to bf16 through LDS so that
+  // rows are stored whole
+  __syncthreads();
+  if constexpr (KS > 1) {
+    // the groups' sums meet in the first group's registers
+    typedef __attribute__((address_space(3))) i32x4_t lds_i32x4_t;
+    constexpr int SUMS = WAVES * 64 * TN * TM * 16;  // of a group
+    lds_i32x4_t *const sums = (lds_i32x4_t *)all;
+    static_assert((KS - 1) * SUMS * 4 <= KS * STAGES * STAGE, "sums fit");
+    const int at = (wave * 64 + lane) * 4;
+    if (group > 0) {
+#pragma unroll
+      for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int j = 0; j < TM; ++j)
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+            sums[((group - 1) * TN * TM * 4 + (i * TM + j) * 4 + g) * WAVES * 64 + at / 4] =
+                i32x4_t{acc[i][j][g * 4], acc[i][j][g * 4 + 1], acc[i][j][g * 4 + 2],
+                        acc[i][j][g * 4 + 3]};
+    }
+    __syncthreads();
+    if (group == 0) {
+#pragma unroll
+      for (int k = 1; k < KS; ++k)
+#pragma unroll
+        for (int i = 0; i < TN; ++i)
+#pragma unroll
+          for (int j = 0; j < TM; ++j)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const i32x4_t v =
+                  sums[((k - 1) * TN * TM * 4 + (i * TM + j) * 4 + g) * WAVES * 64 + at / 4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[i][j][g * 4 + e] += v[e];
+            }
+    }
+    __syncthreads();
+  }
+  store_tile<TN, TM, BN, THREADS>(p, all, acc, n0, m0, wn, wm, wave, group == 0);
+}
+
+// Tiles of 256 x 256 by eight waves in two groups that take turns: while one
+// group's waves issue their 16 products, the other's (one of each to a SIMD) read
+// their fragments and copy a tile ahead, so that the matrix units do not wait for
+// LDS, copies or barriers.  Four stages of 64 bytes of k.
+template <int WN, int WM, int TN, int TM>
+__global__ __launch_bounds__(WN *WM * 64) void gemm_turns_kernel(GemmParams p) {
+  constexpr int WAVES = WN * WM, STAGES = 4, BK = 64;
+  constexpr int BN = WN * TN * 32, BM = WM * TM * 32;
+  constexpr int NC = BN / 16 / WAVES, MC = BM / 16 / WAVES;  // copies per wave and tile
+  static_assert(BN % (16 * WAVES) == 0 && BM % (16 * WAVES) == 0, "whole copies");
+  constexpr int STAGE = (BN + BM) * BK;
+  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+  lds_u8_t *const lds = (lds_u8_t *)smem;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)lds;
+  const int tid = threadIdx.x;
+  const int wave = readfirstlane(tid >> 6);
+  const int lane = tid & 63;
+  const int wn = wave % WN, wm = wave / WN;
+  const int rl = lane & 31, half = lane >> 5;
+  const int2 tile = tile_of(p);
+  const int n0 = tile.x * BN, m0 = tile.y * BM;
+
+  // lane l of a copy fills slot l % 4 of row l / 4; chunk c of a row lies in slot
+  // c ^ ((row >> 2) & 3)
+  const uint8_t *wsrc = p.w + (int64_t)n0 * p.w_ld;
+  const uint8_t *xsrc = p.x + (int64_t)m0 * p.x_ld;
+  const int chunk = (lane & 3) ^ ((lane >> 4) & 3);
+  uint32_t won[NC], xom[MC];
+#pragma unroll
+  for (int j = 0; j < NC; ++j) {
+    const int row = (wave * NC + j) * 16 + (lane >> 2);
+    won[j] = (uint32_t)min(row, p.n - 1 - n0) * (uint32_t)p.w_ld + chunk * 16;
+  }
+#pragma unroll
+  for (int j = 0; j < MC; ++j) {
+    const int row = (wave * MC + j) * 16 + (lane >> 2);
+    xom[j] = (uint32_t)min(row, p.m - 1 - m0) * (uint32_t)p.x_ld + chunk * 16;
+  }
+  const int steps = (p.k + BK - 1) / BK, full = p.k / BK;
+  auto load = [&](int t) {
+    const uint32_t st = (uint32_t)(t % STAGES) * STAGE;
+    const int k0 = t * BK;
+    auto copies = [&]() {
+#pragma unroll
+      for (int j = 0; j < NC; ++j) copy1(wsrc + k0, won[j], lds0 + st + (wave * NC + j) * 1024);
+#pragma unroll
+      for (int j = 0; j < MC; ++j)
+        copy1(xsrc + k0, xom[j], lds0 + st + BN * BK + (wave * MC + j) * 1024);
+    };
+    if (t < full) {
+      copies();
+    } else if (k0 + chunk * 16 < p.k) {
+      copies();
+    } else {
+      // chunks past k: zeros for x, so that they count nothing whatever w's hold
+#pragma unroll
+      for (int j = 0; j < MC; ++j)
+        *(lds_u32x4_t *)(lds + st + BN * BK + (wave * MC + j) * 1024 + lane * 16) =
+            u32x4_t{0u, 0u, 0u, 0u};
+    }
+  };
+
+  i32x16_t acc[TN][TM] = {};
+  const int swz = (rl >> 2) & 3;
+  const lds_u8_t *const wrow = lds + (wn * TN * 32 + rl) * BK;
+  const lds_u8_t *const xrow = lds + BN * BK + (wm * TM * 32 + rl) * BK;
+  i32x4_t wf[2][TN], xf[2][TM];
+  auto read = [&](int t, int s) {
+    const uint32_t c = (uint32_t)(((2 * s + half) ^ swz) << 4) + (uint32_t)(t % STAGES) * STAGE;
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+      wf[s][i] = __builtin_bit_cast(i32x4_t, *(const lds_u32x4_t *)(wrow + c + i * 32 * BK));
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+      xf[s][i] = __builtin_bit_cast(i32x4_t, *(const lds_u32x4_t *)(xrow + c + i * 32 * BK));
+  };
+  auto multiply = [&](int s) {
+#pragma unroll
+    for (int j = 0; j < TM; ++j)
+#pragma unroll
+      for (int i = 0; i < TN; ++i)
+        acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wf[s][i], xf[s][j], acc[i][j], 0, 0, 0);
+  };
+  auto barrier = [&]() {
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+  };
+#pragma unroll
+  for (int t = 0; t < STAGES - 1; ++t)
+    if (t < steps) load(t);
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  barrier();
+  // the second group runs one barrier behind the first: in step t a group copies
+  // into the stage of tile t - 1, which the other has read before its last
+  // barrier, and waits for its own copies of tile t + 1, so that two barriers on
+  // both groups' have landed
+  const bool second = wave >= WAVES / 2;
+  if (second) barrier();
+  for (int t = 0; t < steps; ++t) {
+    read(t, 0);
+    read(t, 1);
+    if (t + 3 < steps) load(t + 3);
+    if (t + 3 < full)
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * (NC + MC)) : "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    barrier();
+    __builtin_amdgcn_s_setprio(1);
+    multiply(0);
+    multiply(1);
+    __builtin_amdgcn_s_setprio(0);
+    barrier();
+  }
+  if (!second) barrier();
+  __syncthreads();
+  store_tile<TN, TM, BN, WAVES * 64>(p, lds, acc, n0, m0, wn, wm, wave, true);
+}
+// Streaming form, at most 16 rows: a workgroup takes 16 columns, its waves
+// shares of k, operands straight from memory (v_mfma_i32_16x16x64_i8).
 constexpr int kStreamWaves = 8;
 constexpr int kStreamAhead = 4;  // k steps loaded together
 
-template <int MT, int NT>
 __global__ __launch_bounds__(kStreamWaves * 64) void stream_kernel(GemmParams p) {
-  __shared__ __attribute__((aligned(16))) int red[kStreamWaves][NT * 16][MT * 16 + 1];
+  __shared__ int red[kStreamWaves][16][17];
   const int tid = threadIdx.x;
   const int wave = readfirstlane(tid >> 6);
   const int lane = tid & 63;
   const int r = lane & 15, g = lane >> 4;
-  const int n0 = blockIdx.x * NT * 16;
+  const int n0 = blockIdx.x * 16;
   const int steps = (p.k + 63) / 64;
   const int s0 = steps * wave / kStreamWaves, s1 = steps * (wave + 1) / kStreamWaves;
-  const uint8_t *wp[NT], *xp[MT];
-#pragma unroll
-  for (int i = 0; i < NT; ++i) wp[i] = p.w + (int64_t)min(n0 + i * 16 + r, p.n - 1) * p.w_ld;
-#pragma unroll
-  for (int j = 0; j < MT; ++j) xp[j] = p.x + (int64_t)min(j * 16 + r, p.m - 1) * p.x_ld;
-  i32x4_t acc[NT][MT] = {};
+  const uint8_t *wp = p.w + (int64_t)min(n0 + r, p.n - 1) * p.w_ld;
+  const uint8_t *xp = p.x + (int64_t)min(r, p.m - 1) * p.x_ld;
+  i32x4_t acc = {};
   constexpr int U = kStreamAhead;
   for (int s = s0; s < s1; s += U) {
-    i32x4_t wf[U][NT], xf[U][MT];
+    i32x4_t wf[U], xf[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       // past the share or k: a place that is there, cleared below
       const int k = min(s + u, s1 - 1) * 64 + g * 16;
       const int kk = k < p.k ? k : 0;
-#pragma unroll
-      for (int i = 0; i < NT; ++i) wf[u][i] = *reinterpret_cast<const i32x4_t *>(wp[i] + kk);
-#pragma unroll
-      for (int j = 0; j < MT; ++j) xf[u][j] = *reinterpret_cast<const i32x4_t *>(xp[j] + kk);
+      wf[u] = *reinterpret_cast<const i32x4_t *>(wp + kk);
+      xf[u] = *reinterpret_cast<const i32x4_t *>(xp + kk);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const bool in = s + u < s1 && (s + u) * 64 + g * 16 < p.k;
-#pragma unroll
-      for (int j = 0; j < MT; ++j) {
-        const i32x4_t b = in ? xf[u][j] : i32x4_t{0, 0, 0, 0};
-#pragma unroll
-        for (int i = 0; i < NT; ++i)
-          acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[u][i], b, acc[i][j], 0, 0, 0);
-      }
+      acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[u], in ? xf[u] : i32x4_t{0, 0, 0, 0}, acc, 0,
+                                                  0, 0);
     }
   }
   // lane (r, g): column (token) r, rows (channels) 4 g ..
 #pragma unroll
-  for (int i = 0; i < NT; ++i)
-#pragma unroll
-    for (int j = 0; j < MT; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) red[wave][i * 16 + g * 4 + e][j * 16 + r] = acc[i][j][e];
+  for (int e = 0; e < 4; ++e) red[wave][g * 4 + e][r] = acc[e];
   __syncthreads();
-  for (int q = tid; q < NT * 16 * MT * 16; q += kStreamWaves * 64) {
-    const int c = q % (NT * 16), t = q / (NT * 16);
-    if (t >= p.m || n0 + c >= p.n) continue;
-    int v = 0;
+  const int c = tid % 16, t = tid / 16;
+  if (t >= p.m || n0 + c >= p.n) return;
+  int v = 0;
 #pragma unroll
-    for (int i = 0; i < kStreamWaves; ++i) v += red[i][c][t];
-    const float y = fmaf((float)v * p.xs[t], p.ws[n0 + c], bias_at(p, n0 + c));
-    p.out[(int64_t)t * p.out_ld + n0 + c] = (uint16_t)(pack2_bf16(y, 0.f) & 0xffffu);
-  }
+  for (int i = 0; i < kStreamWaves; ++i) v += red[i][c][t];
+  const float y = fmaf((float)v * p.xs[t], p.ws[n0 + c], bias_at(p, n0 + c));
+  p.out[(int64_t)t * p.out_ld + n0 + c] = (uint16_t)(pack2_bf16(y, 0.f) & 0xffffu);
 }
 
-template <int WN, int WM, int TN, int TM, int STAGES>
+template <auto kernel>
+int launch_tiles(const GemmParams &p, int threads, int bytes, hipStream_t s) {
+  // (said once per device: the call takes a few us)
+  static std::atomic<uint64_t> said{0};
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess) dev = 64;
+  if (bytes > 65536 && (dev >= 64 || !(said.load(std::memory_order_relaxed) >> dev & 1))) {
+    const hipError_t e = hipFuncSetAttribute((const void *)kernel,
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != hipSuccess) return check_hip(e, "int8_linear");
+    if (dev < 64) said.fetch_or(1ull << dev, std::memory_order_relaxed);
+  }
+  kernel<<<p.mt * p.nt, threads, bytes, s>>>(p);
+  return check_hip(hipGetLastError(), "int8_linear");
+}
+
+template <int WN, int WM, int TN, int TM, int STAGES, int KS = 1>
 int launch_gemm(GemmParams &p, hipStream_t s) {
   constexpr int BN = WN * TN * 32, BM = WM * TM * 32;
   p.nt = (p.n + BN - 1) / BN;
   p.mt = (p.m + BM - 1) / BM;
-  constexpr int bytes = (BN + BM) * kBK * STAGES;
+  constexpr int bytes = (BN + BM) * kBK * STAGES * KS;
   static_assert(bytes >= BN * 8 + WN * WM * 32 * (TN * 64 + 16), "epilogue fits");
-  auto kernel = gemm_kernel<WN, WM, TN, TM, STAGES>;
-  if (bytes > 65536) {
-    const hipError_t e = hipFuncSetAttribute((const void *)kernel,
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e != hipSuccess) return check_hip(e, "int8_linear");
-  }
-  kernel<<<p.mt * p.nt, WN * WM * 64, bytes, s>>>(p);
+  return launch_tiles<gemm_kernel<WN, WM, TN, TM, STAGES, KS>>(p, WN * WM * KS * 64, bytes, s);
+}
+
+int launch_turns(GemmParams &p, hipStream_t s) {
+  p.nt = (p.n + 255) / 256;
+  p.mt = (p.m + 255) / 256;
+  return launch_tiles<gemm_turns_kernel<4, 2, 2, 4>>(p, 512, 512 * 64 * 4, s);
+}
+
+int launch_stream(GemmParams &p, hipStream_t s) {
+  stream_kernel<<<(p.n + 15) / 16, kStreamWaves * 64, 0, s>>>(p);
   return check_hip(hipGetLastError(), "int8_linear");
 }
+
+// The forms of the product: tile, workgroups that a CU holds, and the time of a
+// call, once + rounds (round + step k / 128) us, where a round is a tile on
+// every CU.  The constants are least squares over measurements at 1 to 8191 rows
+// of k = 256 to 14336 and 512 to 10240 columns (weights rotated through 256 MB);
+// the form chosen by them took 0.3 % longer than the fastest one on the
+// geometric mean, 18 % at most (8191 x 2880 x 5120).  Of 64 x 4096 x 6144, us, by
+// form in the table's order from the third on: 18.5, 13.3, 11.4, 8.3, 12.1, 8.1;
+// 517 x 2880 x 5120 from the first on: 34.5, 19.4, 18.0, 24.7, 27.5, 38.5, 53.2,
+// 38.7; 8191 x 8192 x 10240: 691, 806; 4 x 2048 x 2048 from the third on: 10.6, 8.0,
+// 7.1, 5.2, 4.8, 5.1, 3.2.
+struct Form {
+  int bm, bn, per_cu, rows;  // rows: at most (0: any number)
+  float once, round, step;
+  int (*launch)(GemmParams &, hipStream_t);
+};
+const Form kForms[] = {
+    {256, 256, 1, 0, -16.2f, 23.5f, 1.126f, launch_turns},
+    {128, 128, 2, 0, -7.0f, 10.8f, 0.707f, launch_gemm<2, 2, 2, 2, 2, 1>},
+    {128, 128, 1, 0, -2.8f, 7.3f, 0.478f, launch_gemm<2, 2, 2, 2, 2, 2>},
+    {64, 128, 1, 0, -0.5f, 4.1f, 0.322f, launch_gemm<2, 2, 2, 1, 3, 2>},
+    {64, 64, 1, 0, 0.7f, 3.0f, 0.242f, launch_gemm<2, 1, 1, 2, 3, 2>},
+    {64, 32, 1, 0, 1.0f, 2.3f, 0.139f, launch_gemm<1, 2, 1, 1, 3, 4>},
+    {32, 32, 1, 0, 1.5f, 1.8f, 0.114f, launch_gemm<1, 1, 1, 1, 3, 4>},
+    {32, 64, 1, 0, 0.9f, 2.4f, 0.140f, launch_gemm<2, 1, 1, 1, 3, 4>},
+    {16, 16, 1, 16, 2.0f, 0.8f, 0.071f, launch_stream},
+};
 
 }  // namespace
 
@@ -503,16 +685,20 @@ int launch_int8_linear(const mia_int8_linear_args &a, hipStream_t s) {
   p.out = (uint16_t *)a.out, p.out_ld = a.out_stride;
   p.m = a.rows, p.n = a.n, p.k = a.k;
   p.vec = a.n % 8 == 0 && a.out_stride % 8 == 0 && (uintptr_t)a.out % 16 == 0;
-  if (p.m <= 64) {
-    const int c16 = (p.n + 15) / 16, c32 = (p.n + 31) / 32;
-    if (p.m <= 16) stream_kernel<1, 1><<<c16, kStreamWaves * 64, 0, s>>>(p);
-    else if (p.m <= 32) stream_kernel<2, 1><<<c16, kStreamWaves * 64, 0, s>>>(p);
-    else stream_kernel<4, 2><<<c32, kStreamWaves * 64, 0, s>>>(p);
-    return check_hip(hipGetLastError(), "int8_linear");
+  // The form that the measured costs below say is the fastest.
+  const float steps = (float)p.k / kBK;
+  const int cus = cu_count();
+  int best = 0;
+  float least = 0.f;
+  for (int i = 0; i < (int)(sizeof(kForms) / sizeof(kForms[0])); ++i) {
+    const Form &f = kForms[i];
+    if (f.rows < p.m && f.rows) continue;
+    const int64_t tiles = (int64_t)((p.m + f.bm - 1) / f.bm) * ((p.n + f.bn - 1) / f.bn);
+    const int64_t rounds = (tiles + f.per_cu * cus - 1) / (f.per_cu * cus);
+    const float cost = f.once + (float)rounds * (f.round + steps * f.step);
+    if (i == 0 || cost < least) least = cost, best = i;
   }
-  const int64_t big = (int64_t)((p.n + 255) / 256) * ((p.m + 255) / 256);
-  if (big >= 192) return launch_gemm<4, 2, 2, 4, 2>(p, s);
-  return launch_gemm<2, 2, 2, 2, 2>(p, s);
+  return kForms[best].launch(p, s);
 }
 
 }  // namespace mia

@@ -283,14 +283,27 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void window_tall_kernel(
     g.set(p, keys, k0, ent);
     if constexpr (DMA) {
       const uint32_t dst = (uint32_t)(uintptr_t)base + (st * 2) * TILEB + wave * 16 * ROWB;
+      const int kt = k0 - wave * 16;
       if (p.d == D) {
         copy16<NP>(g.k, ko, dst);
-        copy16<NP>(g.v, vo, dst + TILEB);
       } else {
 #pragma unroll
-        for (int jj = 0; jj < NP; ++jj) {
+        for (int jj = 0; jj < NP; ++jj)
           if (k_chunk(jj) * CE < p.d) copy1(g.k, ko[jj], dst + jj * 1024);
-          if (v_chunk(jj) * CE < p.d) copy1(g.v, vo[jj], dst + TILEB + jj * 1024);
+      }
+      const bool edge = kt + kTallKeys > tl.hi || (kt < tl.lo && kt + kTallKeys > p.first);
+      if (p.d == D && !edge) {
+        copy16<NP>(g.v, vo, dst + TILEB);
+      } else {
+        // values that no row sees are zeros: 0 * NaN would reach the sums (and
+        // channels past d stay the zeros they are)
+#pragma unroll
+        for (int jj = 0; jj < NP; ++jj) {
+          if (!tl.any(k0 + jj * RPW + lr, p.first))
+            *(lds_u32x4_t *)(base + (st * 2 + 1) * TILEB + wave * 16 * ROWB + jj * 1024 +
+                             lane * 16) = u32x4_t{0u, 0u, 0u, 0u};
+          else if (v_chunk(jj) * CE < p.d)
+            copy1(g.v, vo[jj], dst + TILEB + jj * 1024);
         }
       }
     } else {
@@ -353,9 +366,14 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void window_tall_kernel(
   const int tr_col = ((lane >> 4) & 1) * 16 + 4 * (tr_k & 3);
   const int tr_row = half * 4 + (tr_k >> 2);
 
+  // positions of the wave's first and last row
+  const int w_lo = tl.pos0 + (int)fdiv((uint32_t)min(r0 + wave * 32, tl.rows - 1), p.g_div);
+  const int w_hi = tl.pos0 + (int)fdiv((uint32_t)min(r0 + wave * 32 + 31, tl.rows - 1), p.g_div);
   auto compute = [&](int x, int st) {
+    const int kt = tl.tile(x) * kTallKeys;
+    if (kt > w_hi || (kt >= p.first && kt + kTallKeys - 1 <= w_lo - p.window)) return;
     const lds_u8_t *kb = base + (st * 2) * TILEB;
-    const lds_u8_t *vb = base + (st * 2 + 1) * TILEB;
+    const lds_u8_t *vb = kb + TILEB;
     const lds_f32_t *ksb = scb + (st * 2) * kTallKeys;
     const lds_f32_t *vsb = ksb + kTallKeys;
     // S^T = K . Q^T: lane = row rl, value e of block b: key b*32 + (e/4)*8 +
@@ -408,10 +426,9 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void window_tall_kernel(
           for (int i = 0; i < 4; ++i) s[b][g * 4 + i] *= ks4[i];
         }
     }
-    const int kt = tl.tile(x) * kTallKeys;
-    if (!tl.every(kt, kt + kTallKeys, p.window, p.first)) {
-      // keys behind the row (negative distances are large as unsigned) and,
-      // but for the first ones, before its window
+    if (kt + kTallKeys - 1 > w_lo || (kt <= w_hi - p.window && kt + kTallKeys > p.first)) {
+      // keys behind the row (negative distances are large as unsigned) and, but
+      // for the first ones, before its window
       const int dist = pos - kt - half * 4, first = p.first - kt - half * 4;
       const bool some = p.first > kt;
 #pragma unroll
@@ -516,17 +533,6 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void window_tall_kernel(
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         if (x + 1 < x1) load_tile(x + 1, st ^ 1);
-        const int kt = tl.tile(x) * kTallKeys;
-        if (kt + kTallKeys > tl.hi || (kt < tl.lo && kt + kTallKeys > p.first)) {
-          // values that no row sees are cleared: 0 * NaN would reach the sums
-          lds_u8_t *const vb = base + (st * 2 + 1) * TILEB;
-          for (int o = tid * 16; o < TILEB; o += kThreads * 16)
-            if (!tl.any(kt + o / ROWB, p.first))
-              *(lds_u32x4_t *)(vb + o) = u32x4_t{0u, 0u, 0u, 0u};
-          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-          __builtin_amdgcn_s_barrier();
-          asm volatile("" ::: "memory");
-        }
         if (live) compute(x, st);
         st ^= 1;
       }
@@ -624,8 +630,15 @@ __global__ __launch_bounds__(kThreads, 2) void window_thin_kernel(WindowParams p
 
   auto k_chan = [](int j, int g) { return CT == kBf16 ? j * 32 + g * 8 : j * 64 + g * 16; };
   const int vds = lane % DS, vtl = lane / DS;
-  u32x4_t kr[2][NK], vr[NV];
-  float sr = 0.f;
+  // A tile's loads are in flight while the tile before is computed.  (Two tiles
+  // ahead take registers that cost a resident workgroup: 128 x 528 int8 keys,
+  // d = 64, 24.6 against 22.6 us, bf16 37 against 31.)
+  struct Slot {
+    u32x4_t k[2][NK], v[NV];
+    float s;
+    Group g[2];
+    int ent[2];  // the table entries of the tile behind
+  } slot;
   // bytes of a lane's chunks in a row; past the head dim the first chunk: K is
   // cleared at its use, what V gives there is stored nowhere
   uint32_t kch[NK];
@@ -636,40 +649,41 @@ __global__ __launch_bounds__(kThreads, 2) void window_thin_kernel(WindowParams p
   const bool narrow = p.d < D;
   Keys keys;
   keys.set(p, wk.i, wk.h);
-  Group g[2];
-  int ent[2];  // table entries of a tile, loaded one tile ahead
-  auto load_entries = [&](int x) {
+  auto load_entries = [&](Slot &t, int x) {
     const int k0 = tl.tile(x) * kThinKeys;
-    ent[0] = keys.entry(p, k0);
-    ent[1] = keys.entry(p, k0 + 16);
+    t.ent[0] = keys.entry(p, k0);
+    t.ent[1] = keys.entry(p, k0 + 16);
   };
-  auto locate = [&](int x) {
+  // the places of tile x (its entries are loaded), and the entries of the tile
+  // behind
+  auto locate = [&](Slot &t, int x) {
     const int k0 = tl.tile(x) * kThinKeys;
-    g[0].set(p, keys, k0, ent[0]);
-    g[1].set(p, keys, k0 + 16, ent[1]);
-    if (x + kWaves < x1) load_entries(x + kWaves);
+    t.g[0].set(p, keys, k0, t.ent[0]);
+    t.g[1].set(p, keys, k0 + 16, t.ent[1]);
+    if (x + kWaves < x1) load_entries(t, x + kWaves);
   };
-  auto load_k = [&]() {
+  auto load_k = [&](Slot &t) {
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
-      for (int j = 0; j < NK; ++j) kr[b][j] = *reinterpret_cast<const u32x4_t *>(g[b].k + kch[j]);
+      for (int j = 0; j < NK; ++j)
+        t.k[b][j] = *reinterpret_cast<const u32x4_t *>(t.g[b].k + kch[j]);
   };
-  auto load_v = [&]() {
+  auto load_v = [&](Slot &t) {
 #pragma unroll
     for (int j = 0; j < NV; ++j)
-      vr[j] = *reinterpret_cast<const u32x4_t *>(
-          g[j * TL / 16].v + ((uint32_t)(j * TL % 16 + vtl) * p.vc_t + vch));
+      t.v[j] = *reinterpret_cast<const u32x4_t *>(
+          t.g[j * TL / 16].v + ((uint32_t)(j * TL % 16 + vtl) * p.vc_t + vch));
   };
   // lane l: scale of key l (K), of key l - 32 (V)
-  auto load_s = [&]() {
+  auto load_s = [&](Slot &t) {
     if constexpr (SC) {
       const int k = lane & 31;
       const bool up = k >= 16;
-      const float *ks = up ? g[1].ks(p, keys) : g[0].ks(p, keys);
-      const float *vs = up ? g[1].vs(p, keys) : g[0].vs(p, keys);
+      const float *ks = up ? t.g[1].ks(p, keys) : t.g[0].ks(p, keys);
+      const float *vs = up ? t.g[1].vs(p, keys) : t.g[0].vs(p, keys);
       const float *sp = lane < 32 ? ks : vs;
-      sr = sp[(uint64_t)(k & 15) * (lane < 32 ? p.ks_t : p.vs_t)];
+      t.s = sp[(uint64_t)(k & 15) * (lane < 32 ? p.ks_t : p.vs_t)];
     }
   };
 
@@ -709,7 +723,17 @@ __global__ __launch_bounds__(kThreads, 2) void window_thin_kernel(WindowParams p
   const int tr_x = tr_row & (VNCH - 1);
 
   f32x4_t s[NC][2];
-  auto scores = [&]() {
+  // (the conversions of codes stay behind this: drawn to the loads, over the
+  // loop's edge, four registers would be held for each)
+  auto here = [](u32x4_t &x) {
+    if constexpr (CT == kI8) asm volatile("" : "+v"(x));
+  };
+  auto scores = [&](Slot &t) {
+    auto &kr = t.k;
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int j = 0; j < NK; ++j) here(kr[b][j]);
     if (narrow) {
 #pragma unroll
       for (int b = 0; b < 2; ++b)
@@ -734,12 +758,13 @@ __global__ __launch_bounds__(kThreads, 2) void window_thin_kernel(WindowParams p
       }
     }
   };
-  auto store_v = [&](int kt, bool whole) {
+  auto store_v = [&](Slot &sl, int kt, bool whole) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int t = j * TL + vtl;
+      here(sl.v[j]);
       // values that no row sees are cleared: 0 * NaN would reach the sums
-      const u32x4_t v = whole || tl.any(kt + t, p.first) ? vr[j] : u32x4_t{0u, 0u, 0u, 0u};
+      const u32x4_t v = whole || tl.any(kt + t, p.first) ? sl.v[j] : u32x4_t{0u, 0u, 0u, 0u};
       if constexpr (CT == kBf16) {
         *(lds_u32x4_t *)(vw + t * ROWB + ((vds ^ (t & (VNCH - 1))) << 4)) = v;
       } else {
@@ -751,7 +776,10 @@ __global__ __launch_bounds__(kThreads, 2) void window_thin_kernel(WindowParams p
       }
     }
   };
-  u32x4_t pk[NC];
+  // probabilities as the sum of two bf16 values (2^-17 of each is left): the
+  // products are few beside the keys' bytes, and one alone would be the largest
+  // error of the output but its own rounding
+  u32x4_t pk[NC], pl[NC];
   auto softmax = [&](int kt, bool whole) {
     f32x4_t ks4[2], vs4[2];
     if constexpr (SC) {
@@ -808,9 +836,12 @@ __global__ __launch_bounds__(kThreads, 2) void window_thin_kernel(WindowParams p
           l_run[n] += pr[i];
           if constexpr (SC) pr[i] *= vs4[b][i];
         }
-        // rounded to bf16 for the MFMA; the sum keeps the unrounded ones
-        pk[n][2 * b] = pack2_bf16(pr[0], pr[1]);
-        pk[n][2 * b + 1] = pack2_bf16(pr[2], pr[3]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t w = pack2_bf16(pr[2 * i], pr[2 * i + 1]);
+          pk[n][2 * b + i] = w;
+          pl[n][2 * b + i] = pack2_bf16(pr[2 * i] - bf16lo(w), pr[2 * i + 1] - bf16hi(w));
+        }
       }
     }
   };
@@ -827,10 +858,14 @@ __global__ __launch_bounds__(kThreads, 2) void window_thin_kernel(WindowParams p
           __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t *)(vw + off + 16 * ROWB)));
       const u32x4_t v = {t0[0], t0[1], t1[0], t1[1]};
 #pragma unroll
-      for (int n = 0; n < NC; ++n)
+      for (int n = 0; n < NC; ++n) {
         acc[n][blk] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
             __builtin_bit_cast(bf16x8_t, v), __builtin_bit_cast(bf16x8_t, pk[n]), acc[n][blk], 0,
             0, 0);
+        acc[n][blk] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+            __builtin_bit_cast(bf16x8_t, v), __builtin_bit_cast(bf16x8_t, pl[n]), acc[n][blk], 0,
+            0, 0);
+      }
     }
   };
 
@@ -838,29 +873,27 @@ __global__ __launch_bounds__(kThreads, 2) void window_thin_kernel(WindowParams p
   // product (copy to LDS) has freed the registers
   int x = x0 + wave;
   if (x < x1) {
-    load_entries(x);
-    locate(x);
-    load_k();
-    load_s();
-    load_v();
-    while (true) {
-      const int kt = tl.tile(x) * kThinKeys;
-      const bool whole = tl.every(kt, kt + kThinKeys, p.window, p.first);
-      const bool go = x + kWaves < x1;
-      if (go) locate(x + kWaves);
-      scores();
-      if constexpr (SC) sw[lane] = whole || tl.any(kt + (lane & 31), p.first) ? sr : 0.f;
-      if (go) {
-        load_k();
-        load_s();
-      }
-      softmax(kt, whole);
-      store_v(kt, whole);
-      if (go) load_v();
-      values();
-      if (!go) break;
-      x += kWaves;
+    load_entries(slot, x);
+    locate(slot, x);
+    load_k(slot);
+    load_s(slot);
+    load_v(slot);
+  }
+  for (; x < x1; x += kWaves) {
+    const int kt = tl.tile(x) * kThinKeys;
+    const bool whole = tl.every(kt, kt + kThinKeys, p.window, p.first);
+    const bool go = x + kWaves < x1;
+    if (go) locate(slot, x + kWaves);
+    scores(slot);
+    if constexpr (SC) sw[lane] = whole || tl.any(kt + (lane & 31), p.first) ? slot.s : 0.f;
+    if (go) {
+      load_k(slot);
+      load_s(slot);
     }
+    softmax(kt, whole);
+    store_v(slot, kt, whole);
+    if (go) load_v(slot);
+    values();
   }
 
   // ---- the waves' sums joined, thread -> rows and four channels
@@ -954,7 +987,7 @@ int64_t up(int64_t x, int64_t a) { return (x + a - 1) / a * a; }
 
 struct Plan {
   bool thin;
-  int cols;  // thin: 16-row groups
+  int tile_rows;  // rows of a workgroup
   int64_t blocks;
   size_t o, total;  // byte offset of the sums, size
 };
@@ -964,8 +997,7 @@ Plan plan_window(WindowParams &p) {
   const int D = p.d <= 64 ? 64 : 128;
   const int64_t seq_rows = (int64_t)p.tok_max * p.G;
   w.thin = seq_rows <= 32;
-  w.cols = seq_rows <= 16 ? 1 : 2;
-  const int tile_rows = w.thin ? w.cols * 16 : kRows;
+  const int tile_rows = w.tile_rows = seq_rows <= 16 ? 16 : seq_rows <= 32 ? 32 : kRows;
   p.rt_max = (int)((seq_rows + tile_rows - 1) / tile_rows);
   p.part_rows = (int)std::min<int64_t>(seq_rows, tile_rows);
   // tiles of a row tile at most, row tiles that have rows at most
@@ -1029,7 +1061,7 @@ template <int D, int CT, bool SC, int DU>
 void launch_form(const WindowParams &p, const Plan &w, hipStream_t s) {
   const unsigned n = (unsigned)w.blocks;
   if (!w.thin) window_tall_kernel<D, CT, SC, DU><<<n, kThreads, 0, s>>>(p);
-  else if (w.cols == 1) window_thin_kernel<D, CT, SC, DU, 1><<<n, kThreads, 0, s>>>(p);
+  else if (w.tile_rows == 16) window_thin_kernel<D, CT, SC, DU, 1><<<n, kThreads, 0, s>>>(p);
   else window_thin_kernel<D, CT, SC, DU, 2><<<n, kThreads, 0, s>>>(p);
 }
 
@@ -1059,9 +1091,8 @@ int launch_window(const mia_window_args &a, hipStream_t s) {
   if (p.split > 1) {
     const int D = p.d <= 64 ? 64 : 128, rpb = 256 / (D / 4);
     const unsigned n = (unsigned)(w.blocks / p.split * ((p.part_rows + rpb - 1) / rpb));
-    const int tile_rows = w.thin ? w.cols * 16 : kRows;
-    if (D == 64) window_join_kernel<64><<<n, 256, 0, s>>>(p, tile_rows);
-    else window_join_kernel<128><<<n, 256, 0, s>>>(p, tile_rows);
+    if (D == 64) window_join_kernel<64><<<n, 256, 0, s>>>(p, w.tile_rows);
+    else window_join_kernel<128><<<n, 256, 0, s>>>(p, w.tile_rows);
   }
   return check_hip(hipGetLastError(), "window_attention");
 }
