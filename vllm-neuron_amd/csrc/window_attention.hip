@@ -44,6 +44,7 @@ struct WindowParams {
   float scale_log2;
   int rt_max;     // row tiles of a sequence at most
   int split;      // pieces of a row tile's keys
+  FastDiv rt_div, split_div, seq_div;
   int part_rows;  // rows of a partial
   float *part_o;  // [piece][part_rows][D]
   float2 *part_ml;
@@ -51,12 +52,15 @@ struct WindowParams {
 
 // The keys that a row tile sees: those of a sequence's rows [r0, r1), whose
 // first and last query stand at p_lo and p_hi: [0, min(first, hi)) and [lo, hi).
-// In tiles of T keys: n_first tiles from 0 on, then those from tile t_lo on.
+// They are taken in groups of 16, the first tokens' and then the window's, end to
+// end, and a tile is the next 2 or 4 groups of that list: 128 keys behind 4 first
+// ones fill three tiles of 64, where tiles that start at multiples of 64 are five.
 struct Tiles {
   int tok0, rows;      // first query token, rows of the sequence
   int pos0;            // position of its first query
   int p_lo, p_hi, lo, hi;
-  int n_first, t_lo, n;
+  int n_first, g_lo;   // groups of first tokens, first group of the window
+  int n;               // tiles
 
   template <int T>
   MIA_DEV bool set(const WindowParams &p, int i, int r0, int rows_tile) {
@@ -75,19 +79,24 @@ struct Tiles {
     p_hi = pos0 + (int)fdiv((uint32_t)(r1 - 1), p.g_div);
     hi = max(p_hi + 1, 0);
     lo = min(max(p_lo - p.window + 1, 0), hi);
-    t_lo = lo / T;
-    n_first = min((min(p.first, hi) + T - 1) / T, t_lo);
-    n = n_first + (hi + T - 1) / T - t_lo;
+    g_lo = lo / 16;
+    n_first = min((min(p.first, hi) + 15) / 16, g_lo);
+    n = (n_first + (hi + 15) / 16 - g_lo + T / 16 - 1) / (T / 16);
     return true;
   }
-  MIA_DEV int tile(int x) const { return x < n_first ? x : x - n_first + t_lo; }
+  // first key of group g of the list (past its end: keys that no row sees)
+  MIA_DEV int key(int g) const { return (g < n_first ? g : g - n_first + g_lo) * 16; }
   // does any row of the tile see key k?
   MIA_DEV bool any(int k, int first) const { return k < hi && (k < first || k >= lo); }
-  // does every row of the tile see every key of [k0, k1)?
-  MIA_DEV bool every(int k0, int k1, int window, int first) const {
-    return k1 - 1 <= p_lo && (k1 <= first || k0 > p_hi - window);
+  // are there keys among the 16 from k on that none sees?
+  MIA_DEV bool edge(int k, int first) const {
+    return k + 16 > hi || (k < lo && k + 16 > first);
   }
 };
+// Do the rows from position lo to hi all see every key of [k0, k1)?
+MIA_DEV bool see_all(const WindowParams &p, int lo, int hi, int k0, int k1) {
+  return k1 - 1 <= lo && (k1 <= p.first || k0 > hi - p.window);
+}
 
 // Where a head's keys lie (wave-uniform).
 struct Keys {
@@ -127,6 +136,29 @@ struct Group {
     return s.vs + (uint64_t)blk * p.vs_blk + (uint64_t)off * p.vs_t;
   }
 };
+
+// Keys that a lane's row does not see, a bit for each of its scores.  A lane
+// holds four consecutive keys of every STEP, from its first one on, N in all, in
+// the order of the keys: those at a distance of at most d behind the first are
+// its first count(d) scores.
+template <int STEP, int N>
+MIA_DEV uint32_t hidden(const WindowParams &p, int pos, int k0) {
+  auto count = [](int d) {
+    d = min(max(d, -1), N / 4 * STEP - 1);
+    constexpr int SH = STEP == 8 ? 3 : 4;
+    return (d >> SH) * 4 + min((d & (STEP - 1)) + 1, 4);
+  };
+  auto bits = [](int n) { return n >= 32 ? 0xffffffffu : (1u << n) - 1u; };
+  const int dist = pos - k0;
+  const uint32_t behind = bits(count(dist));  // at or before the row's position
+  const uint32_t old = bits(count(dist - p.window));
+  const uint32_t first = bits(count(p.first - 1 - k0));
+  return ~(behind & (~old | first));
+}
+MIA_DEV float hide(float x, uint32_t hid, int bit) {
+  const uint32_t t = (uint32_t)__builtin_amdgcn_sbfe((int)hid, bit, 1);
+  return __uint_as_float((t & 0xff800000u) | (~t & __float_as_uint(x)));
+}
 
 // log2(e) x softmax scale x per-head scale of K: its magnitude; a negative
 // factor goes to q (sign bits), so that the largest product is the largest
@@ -184,12 +216,19 @@ struct Work {
     const int full = total / 8, rem = total % 8, x = b % 8;
     int id = x * full + min(x, rem) + b / 8;
     piece = id;
-    s = id % p.split;
-    id /= p.split;
-    rt = id % p.rt_max;
-    id /= p.rt_max;
-    i = id % p.n_seq;
-    h = id / p.n_seq;
+    int next = (int)fdiv((uint32_t)id, p.split_div);
+    s = id - next * p.split;
+    id = next;
+    next = (int)fdiv((uint32_t)id, p.rt_div);
+    rt = id - next * p.rt_max;
+    h = (int)fdiv((uint32_t)next, p.seq_div);
+    i = next - h * p.n_seq;
+  }
+  // the piece's tiles [x, y) of n (at most 2^25, of at most 32 pieces)
+  MIA_DEV int2 share(const WindowParams &p, int n) const {
+    if (p.split == 1) return make_int2(0, n);
+    return make_int2((int)fdiv((uint32_t)(n * s), p.split_div),
+                     (int)fdiv((uint32_t)(n * (s + 1)), p.split_div));
   }
 };
 
@@ -233,8 +272,15 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void window_tall_kernel(
   Tiles tl;
   const int r0 = wk.rt * kRows;
   if (!tl.set<kTallKeys>(p, wk.i, r0, kRows)) return;
-  const int x0 = (int)((int64_t)tl.n * wk.s / p.split);
-  const int x1 = (int)((int64_t)tl.n * (wk.s + 1) / p.split);
+  const int2 share = wk.share(p, tl.n);
+  const int x0 = share.x, x1 = share.y;
+
+  // (the first table entry is under way while the rows are loaded)
+  Keys keys;
+  keys.set(p, wk.i, wk.h);
+  int ent = 0;  // the wave's table entry of a tile, loaded one tile ahead
+  auto load_entry = [&](int x) { ent = keys.entry(p, tl.key(4 * x + wave)); };
+  if (x0 < x1) load_entry(x0);
 
   // ---- the rows
   const int rloc = wave * 32 + rl;
@@ -263,10 +309,6 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void window_tall_kernel(
   constexpr int NR = DMA ? 1 : NP;
   u32x4_t kr[NR], vr[NR];
   float sr[NR];
-  Keys keys;
-  keys.set(p, wk.i, wk.h);
-  int ent = 0;  // the wave's table entry of a tile, loaded one tile ahead
-  auto load_entry = [&](int x) { ent = keys.entry(p, tl.tile(x) * kTallKeys + wave * 16); };
   // the chunk a lane loads: for copies the one that the swizzle puts in its
   // slot, else its own (past the head dim: the first, stored nowhere)
   auto k_chunk = [&](int jj) { return DMA ? lc ^ k_swz<D>(jj * RPW + lr) : ch_ok ? lc : 0; };
@@ -278,12 +320,11 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void window_tall_kernel(
     vo[jj] = (uint32_t)(jj * RPW + lr) * p.vc_t + v_chunk(jj) * 16;
   }
   auto load_tile = [&](int x, int st) {
-    const int k0 = tl.tile(x) * kTallKeys + wave * 16;
+    const int k0 = tl.key(4 * x + wave);
     Group g;
     g.set(p, keys, k0, ent);
     if constexpr (DMA) {
       const uint32_t dst = (uint32_t)(uintptr_t)base + (st * 2) * TILEB + wave * 16 * ROWB;
-      const int kt = k0 - wave * 16;
       if (p.d == D) {
         copy16<NP>(g.k, ko, dst);
       } else {
@@ -291,8 +332,7 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void window_tall_kernel(
         for (int jj = 0; jj < NP; ++jj)
           if (k_chunk(jj) * CE < p.d) copy1(g.k, ko[jj], dst + jj * 1024);
       }
-      const bool edge = kt + kTallKeys > tl.hi || (kt < tl.lo && kt + kTallKeys > p.first);
-      if (p.d == D && !edge) {
+      if (p.d == D && !tl.edge(k0, p.first)) {
         copy16<NP>(g.v, vo, dst + TILEB);
       } else {
         // values that no row sees are zeros: 0 * NaN would reach the sums (and
@@ -322,14 +362,14 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void window_tall_kernel(
   };
   // 8-bit caches: the loaded tile widened into stage st
   auto store_tile = [&](int x, int st) {
-    const int kt = tl.tile(x) * kTallKeys;
+    const int k0 = tl.key(4 * x + wave);
     lds_u8_t *const kb = base + (st * 2) * TILEB;
     lds_u8_t *const vb = base + (st * 2 + 1) * TILEB;
 #pragma unroll
     for (int jj = 0; jj < NR; ++jj) {
       const int row = wave * 16 + jj * RPW + lr;
       // values that no row sees are cleared: 0 * NaN would reach the sums
-      const bool in = tl.any(kt + row, p.first);
+      const bool in = tl.any(k0 + jj * RPW + lr, p.first);
       const u32x4_t v = in ? vr[jj] : u32x4_t{0u, 0u, 0u, 0u};
       if (ch_ok)
 #pragma unroll
@@ -370,8 +410,10 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void window_tall_kernel(
   const int w_lo = tl.pos0 + (int)fdiv((uint32_t)min(r0 + wave * 32, tl.rows - 1), p.g_div);
   const int w_hi = tl.pos0 + (int)fdiv((uint32_t)min(r0 + wave * 32 + 31, tl.rows - 1), p.g_div);
   auto compute = [&](int x, int st) {
-    const int kt = tl.tile(x) * kTallKeys;
-    if (kt > w_hi || (kt >= p.first && kt + kTallKeys - 1 <= w_lo - p.window)) return;
+    // first key of the tile, and whether its groups follow each other
+    const int kt = tl.key(4 * x);
+    const bool row = 4 * x >= tl.n_first || 4 * x + 4 <= tl.n_first;
+    if (row && (kt > w_hi || (kt >= p.first && kt + kTallKeys - 1 <= w_lo - p.window))) return;
     const lds_u8_t *kb = base + (st * 2) * TILEB;
     const lds_u8_t *vb = kb + TILEB;
     const lds_f32_t *ksb = scb + (st * 2) * kTallKeys;
@@ -426,20 +468,19 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void window_tall_kernel(
           for (int i = 0; i < 4; ++i) s[b][g * 4 + i] *= ks4[i];
         }
     }
-    if (kt + kTallKeys - 1 > w_lo || (kt <= w_hi - p.window && kt + kTallKeys > p.first)) {
-      // keys behind the row (negative distances are large as unsigned) and, but
-      // for the first ones, before its window
-      const int dist = pos - kt - half * 4, first = p.first - kt - half * 4;
-      const bool some = p.first > kt;
+    if (!row || !see_all(p, w_lo, w_hi, kt, kt + kTallKeys)) {
+      uint32_t hid = 0;
+      if (row) {
+        hid = hidden<8, 32>(p, pos, kt + half * 4);
+      } else {
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          hid |= (hidden<8, 8>(p, pos, tl.key(4 * x + g) + half * 4) & 0xffu) << (8 * g);
+      }
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int k = b * 32 + (e >> 2) * 8 + (e & 3);
-          bool see = (uint32_t)(dist - k) < (uint32_t)p.window;
-          if (some) see |= k < first && k <= dist;
-          s[b][e] = see ? s[b][e] : -INFINITY;
-        }
+        for (int e = 0; e < 16; ++e) s[b][e] = hide(s[b][e], hid, b * 16 + e);
     }
     // online softmax; the maximum moves only when a score passes it by more
     // than 8 (log2 units): probabilities stay below 2^8, the accumulators are
@@ -522,7 +563,6 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void window_tall_kernel(
         *(lds_u32x4_t *)(base + o) = u32x4_t{0u, 0u, 0u, 0u};
       __syncthreads();
     }
-    load_entry(x0);
     load_tile(x0, 0);
     int st = 0;
     if constexpr (DMA) {
@@ -625,8 +665,8 @@ __global__ __launch_bounds__(kThreads, 2) void window_thin_kernel(WindowParams p
   Tiles tl;
   if (!tl.set<kThinKeys>(p, wk.i, 0, NC * 16)) return;
   // the piece's tiles, of which every wave takes each fourth
-  const int x0 = (int)((int64_t)tl.n * wk.s / p.split);
-  const int x1 = (int)((int64_t)tl.n * (wk.s + 1) / p.split);
+  const int2 share = wk.share(p, tl.n);
+  const int x0 = share.x, x1 = share.y;
 
   auto k_chan = [](int j, int g) { return CT == kBf16 ? j * 32 + g * 8 : j * 64 + g * 16; };
   const int vds = lane % DS, vtl = lane / DS;
@@ -650,16 +690,14 @@ __global__ __launch_bounds__(kThreads, 2) void window_thin_kernel(WindowParams p
   Keys keys;
   keys.set(p, wk.i, wk.h);
   auto load_entries = [&](Slot &t, int x) {
-    const int k0 = tl.tile(x) * kThinKeys;
-    t.ent[0] = keys.entry(p, k0);
-    t.ent[1] = keys.entry(p, k0 + 16);
+    t.ent[0] = keys.entry(p, tl.key(2 * x));
+    t.ent[1] = keys.entry(p, tl.key(2 * x + 1));
   };
   // the places of tile x (its entries are loaded), and the entries of the tile
   // behind
   auto locate = [&](Slot &t, int x) {
-    const int k0 = tl.tile(x) * kThinKeys;
-    t.g[0].set(p, keys, k0, t.ent[0]);
-    t.g[1].set(p, keys, k0 + 16, t.ent[1]);
+    t.g[0].set(p, keys, tl.key(2 * x), t.ent[0]);
+    t.g[1].set(p, keys, tl.key(2 * x + 1), t.ent[1]);
     if (x + kWaves < x1) load_entries(t, x + kWaves);
   };
   auto load_k = [&](Slot &t) {
@@ -758,13 +796,14 @@ __global__ __launch_bounds__(kThreads, 2) void window_thin_kernel(WindowParams p
       }
     }
   };
-  auto store_v = [&](Slot &sl, int kt, bool whole) {
+  auto store_v = [&](Slot &sl, const int (&k0)[2], bool whole) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int t = j * TL + vtl;
       here(sl.v[j]);
       // values that no row sees are cleared: 0 * NaN would reach the sums
-      const u32x4_t v = whole || tl.any(kt + t, p.first) ? sl.v[j] : u32x4_t{0u, 0u, 0u, 0u};
+      const u32x4_t v =
+          whole || tl.any(k0[j * TL / 16] + (t & 15), p.first) ? sl.v[j] : u32x4_t{0u, 0u, 0u, 0u};
       if constexpr (CT == kBf16) {
         *(lds_u32x4_t *)(vw + t * ROWB + ((vds ^ (t & (VNCH - 1))) << 4)) = v;
       } else {
@@ -780,7 +819,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_thin_kernel(WindowParams p
   // products are few beside the keys' bytes, and one alone would be the largest
   // error of the output but its own rounding
   u32x4_t pk[NC], pl[NC];
-  auto softmax = [&](int kt, bool whole) {
+  auto softmax = [&](const int (&k0)[2], bool whole) {
     f32x4_t ks4[2], vs4[2];
     if constexpr (SC) {
 #pragma unroll
@@ -798,15 +837,12 @@ __global__ __launch_bounds__(kThreads, 2) void window_thin_kernel(WindowParams p
           for (int i = 0; i < 4; ++i) s[n][b][i] *= ks4[b][i];
       }
       if (!whole) {
-        const int dist = pos[n] - kt - kg * 4, first = p.first - kt - kg * 4;
+        const uint32_t hid = (hidden<16, 4>(p, pos[n], k0[0] + kg * 4) & 15u) |
+                             hidden<16, 4>(p, pos[n], k0[1] + kg * 4) << 4;
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int k = b * 16 + i;
-            const bool see = (uint32_t)(dist - k) < (uint32_t)p.window || (k < first && k <= dist);
-            s[n][b][i] = see ? s[n][b][i] : -INFINITY;
-          }
+          for (int i = 0; i < 4; ++i) s[n][b][i] = hide(s[n][b][i], hid, b * 4 + i);
       }
       float mx = -INFINITY;
 #pragma unroll
@@ -880,18 +916,22 @@ __global__ __launch_bounds__(kThreads, 2) void window_thin_kernel(WindowParams p
     load_v(slot);
   }
   for (; x < x1; x += kWaves) {
-    const int kt = tl.tile(x) * kThinKeys;
-    const bool whole = tl.every(kt, kt + kThinKeys, p.window, p.first);
+    const int k0[2] = {tl.key(2 * x), tl.key(2 * x + 1)};
+    const bool whole = see_all(p, tl.p_lo, tl.p_hi, k0[0], k0[0] + 16) &&
+                       see_all(p, tl.p_lo, tl.p_hi, k0[1], k0[1] + 16);
     const bool go = x + kWaves < x1;
     if (go) locate(slot, x + kWaves);
     scores(slot);
-    if constexpr (SC) sw[lane] = whole || tl.any(kt + (lane & 31), p.first) ? slot.s : 0.f;
+    if constexpr (SC) {
+      const int k = (lane & 16 ? k0[1] : k0[0]) + (lane & 15);
+      sw[lane] = whole || tl.any(k, p.first) ? slot.s : 0.f;
+    }
     if (go) {
       load_k(slot);
       load_s(slot);
     }
-    softmax(kt, whole);
-    store_v(slot, kt, whole);
+    softmax(k0, whole);
+    store_v(slot, k0, whole);
     if (go) load_v(slot);
     values();
   }
@@ -1003,8 +1043,8 @@ Plan plan_window(WindowParams &p) {
   // tiles of a row tile at most, row tiles that have rows at most
   const int T = w.thin ? kThinKeys : kTallKeys;
   const int64_t span = (int64_t)p.window + tile_rows / p.G + 1;
-  const int64_t tiles = std::min<int64_t>((p.cap + T - 1) / T,
-                                          (p.first + T - 1) / T + (span + T - 1) / T + 1);
+  const int64_t tiles =
+      std::min<int64_t>((p.cap + T - 1) / T, ((p.first + 15) / 16 + (span + 30) / 16) * 16 / T + 1);
   const int64_t busy =
       std::min<int64_t>((int64_t)p.n_seq * p.rt_max,
                         (int64_t)p.num_tokens * p.G / tile_rows + p.n_seq) * p.Hkv;
@@ -1017,6 +1057,9 @@ Plan plan_window(WindowParams &p) {
   const int64_t piece = (int64_t)p.part_rows * (D * 4 + 8);
   p.split = (int)std::max<int64_t>(1, std::min<int64_t>(p.split, (128 << 20) / (tiles_all * piece)));
   w.blocks = tiles_all * p.split;
+  p.rt_div = make_fastdiv(p.rt_max);
+  p.split_div = make_fastdiv(p.split);
+  p.seq_div = make_fastdiv(p.n_seq);
   w.o = w.total = 0;
   if (p.split > 1) {
     w.o = (size_t)up(w.blocks * p.part_rows * 8, 256);
