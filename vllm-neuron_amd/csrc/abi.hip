@@ -894,6 +894,8 @@ int mia_rope_append(const mia_rope_append_args *a, mia_stream_t stream) {
                   rows(a->k_out, a->k_out_stride, a->num_kv_heads) &&
                   rows(a->v, a->v_stride, a->num_kv_heads),
               MIA_ERR_VALUE, "rope_append: rows must be 8-byte aligned");
+  MIA_REQUIRE(aligned(a->q_gamma, 16) && aligned(a->k_gamma, 16), MIA_ERR_VALUE,
+              "rope_append: q_gamma and k_gamma must be 16-byte aligned");
   if (!a->slots) {
     MIA_REQUIRE(!a->v && a->k_out, MIA_ERR_VALUE,
                 "rope_append: without a cache K goes to k_out and there is no V");

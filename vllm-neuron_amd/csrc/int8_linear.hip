@@ -34,104 +34,117 @@ MIA_DEV float gamma_at(const mia_quant_rows_args &a, int c) {
   return ((const float *)a.gamma)[c];
 }
 
-// LANES threads per row, NV vectors of 8 channels each, held in registers.
-template <int LANES, int NV>
+// LANES threads per row, NV vectors of 8 channels each, held in registers.  With
+// NORM a workgroup takes rows row0, row0 + stride, ...: gamma, twice the bytes of
+// a row where it is fp32, is loaded once for all of them.
+template <int LANES, int NV, bool NORM>
 __global__ __launch_bounds__(256) void quant_rows_kernel(mia_quant_rows_args a) {
   constexpr int RPB = 256 / LANES;
-  __shared__ float2 red[4];
+  __shared__ float2 red[2][4];
   const int tid = threadIdx.x % LANES;
-  const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / LANES;
-  const bool live = row < a.rows;
-  const int64_t at = (live ? row : 0) * a.x_stride;
-  float x[NV][8];
+  f32x4_t gamma[NORM ? NV : 1][2];
+  if (NORM) {
 #pragma unroll
-  for (int v = 0; v < NV; ++v) {
-    const int c = (v * LANES + tid) * 8;
-    u32x4_t w = {0u, 0u, 0u, 0u}, w0 = w, w1 = w;
-    if (c < a.dim) {
-      w = *reinterpret_cast<const u32x4_t *>((const uint16_t *)a.x + at + c);
-      if (a.add0) w0 = *reinterpret_cast<const u32x4_t *>((const uint16_t *)a.add0 + at + c);
-      if (a.add1) w1 = *reinterpret_cast<const u32x4_t *>((const uint16_t *)a.add1 + at + c);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[v][2 * i] = bf16lo(w[i]);
-      x[v][2 * i + 1] = bf16hi(w[i]);
-    }
-    if (a.add0)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[v][2 * i] = add_bf16(x[v][2 * i], bf16lo(w0[i]));
-        x[v][2 * i + 1] = add_bf16(x[v][2 * i + 1], bf16hi(w0[i]));
+    for (int v = 0; v < NV; ++v) {
+      const int c = (v * LANES + tid) * 8;
+      gamma[v][0] = gamma[v][1] = f32x4_t{1.f, 1.f, 1.f, 1.f};
+      if (c >= a.dim || !a.gamma) continue;
+      if (a.gamma_bf16) {
+        const u32x4_t g = *reinterpret_cast<const u32x4_t *>((const uint16_t *)a.gamma + c);
+        gamma[v][0] = f32x4_t{bf16lo(g[0]), bf16hi(g[0]), bf16lo(g[1]), bf16hi(g[1])};
+        gamma[v][1] = f32x4_t{bf16lo(g[2]), bf16hi(g[2]), bf16lo(g[3]), bf16hi(g[3])};
+      } else {
+        gamma[v][0] = *reinterpret_cast<const f32x4_t *>((const float *)a.gamma + c);
+        gamma[v][1] = *reinterpret_cast<const f32x4_t *>((const float *)a.gamma + c + 4);
       }
-    if (a.add1)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[v][2 * i] = add_bf16(x[v][2 * i], bf16lo(w1[i]));
-        x[v][2 * i + 1] = add_bf16(x[v][2 * i + 1], bf16hi(w1[i]));
-      }
+    }
   }
-  float ss = 0.f;
-  if (a.norm) {
+  const int64_t stride = (int64_t)gridDim.x * RPB;
+  int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / LANES;
+  u32x4_t raw[NV];
+  auto load = [&](int64_t r) {
+    const int64_t at = (r < a.rows ? r : 0) * a.x_stride;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int c = (v * LANES + tid) * 8;
+      raw[v] = u32x4_t{0u, 0u, 0u, 0u};
+      if (c < a.dim) raw[v] = *reinterpret_cast<const u32x4_t *>((const uint16_t *)a.x + at + c);
+    }
+  };
+  load(row);
+  // (every thread of a workgroup takes as many turns)
+  for (int64_t first = (int64_t)blockIdx.x * RPB, turn = 0; first < a.rows;
+       first += stride, row += stride, ++turn) {
+    const bool live = row < a.rows;
+    float x[NV][8];
 #pragma unroll
     for (int v = 0; v < NV; ++v)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) ss = fmaf(x[v][i], x[v][i], ss);
-    if (a.gamma) {
+      for (int i = 0; i < 4; ++i) {
+        x[v][2 * i] = bf16lo(raw[v][i]);
+        x[v][2 * i + 1] = bf16hi(raw[v][i]);
+      }
+    if (first + stride < a.rows) load(row + stride);
+    auto add = [&](const void *t) {
+      if (!t) return;
+      const int64_t at = (live ? row : 0) * a.x_stride;
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
         const int c = (v * LANES + tid) * 8;
         if (c >= a.dim) continue;
-        if (a.gamma_bf16) {
-          const u32x4_t g = *reinterpret_cast<const u32x4_t *>((const uint16_t *)a.gamma + c);
+        const u32x4_t w = *reinterpret_cast<const u32x4_t *>((const uint16_t *)t + at + c);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            x[v][2 * i] *= bf16lo(g[i]);
-            x[v][2 * i + 1] *= bf16hi(g[i]);
-          }
-        } else {
-          const f32x4_t g0 = *reinterpret_cast<const f32x4_t *>((const float *)a.gamma + c);
-          const f32x4_t g1 = *reinterpret_cast<const f32x4_t *>((const float *)a.gamma + c + 4);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            x[v][i] *= g0[i];
-            x[v][4 + i] *= g1[i];
-          }
+        for (int i = 0; i < 4; ++i) {
+          x[v][2 * i] = add_bf16(x[v][2 * i], bf16lo(w[i]));
+          x[v][2 * i + 1] = add_bf16(x[v][2 * i + 1], bf16hi(w[i]));
         }
       }
+    };
+    add(a.add0);
+    add(a.add1);
+    float ss = 0.f;
+    if constexpr (NORM) {
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          ss = fmaf(x[v][i], x[v][i], ss);
+          x[v][i] *= gamma[v][i >> 2][i & 3];
+        }
     }
+    // magnitudes as integers: an infinity or NaN is the largest
+    uint32_t mag = 0;
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mag = max(mag, __float_as_uint(x[v][i]) & 0x7fffffffu);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      mag = max(mag, (uint32_t)__shfl_xor((int)mag, o, 64));
+      if (NORM) ss += __shfl_xor(ss, o, 64);
+    }
+    if constexpr (LANES == 256) {
+      float2 *const rd = red[turn & 1];
+      if ((threadIdx.x & 63) == 0) rd[threadIdx.x >> 6] = make_float2(__uint_as_float(mag), ss);
+      __syncthreads();
+      mag = max(max(__float_as_uint(rd[0].x), __float_as_uint(rd[1].x)),
+                max(__float_as_uint(rd[2].x), __float_as_uint(rd[3].x)));
+      ss = (rd[0].y + rd[1].y) + (rd[2].y + rd[3].y);
+    }
+    if (!live) continue;
+    RowCodes<127> rs;
+    rs.set(mag);
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int c = (v * LANES + tid) * 8;
+      if (c >= a.dim) continue;
+      u32x2_t w = {0u, 0u};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i >> 2] |= rs.int8(x[v][i]) << (8 * (i & 3));
+      *reinterpret_cast<u32x2_t *>((uint8_t *)a.codes + row * a.codes_stride + c) = w;
+    }
+    if (tid == 0) a.scales[row] = row_scale(mag, ss, a);
   }
-  // magnitudes as integers: an infinity or NaN is the largest
-  uint32_t mag = 0;
-#pragma unroll
-  for (int v = 0; v < NV; ++v)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) mag = max(mag, __float_as_uint(x[v][i]) & 0x7fffffffu);
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    mag = max(mag, (uint32_t)__shfl_xor((int)mag, o, 64));
-    if (a.norm) ss += __shfl_xor(ss, o, 64);
-  }
-  if constexpr (LANES == 256) {
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = make_float2(__uint_as_float(mag), ss);
-    __syncthreads();
-    mag = max(max(__float_as_uint(red[0].x), __float_as_uint(red[1].x)),
-              max(__float_as_uint(red[2].x), __float_as_uint(red[3].x)));
-    ss = (red[0].y + red[1].y) + (red[2].y + red[3].y);
-  }
-  if (!live) return;
-  RowCodes<127> rs;
-  rs.set(mag);
-#pragma unroll
-  for (int v = 0; v < NV; ++v) {
-    const int c = (v * LANES + tid) * 8;
-    if (c >= a.dim) continue;
-    u32x2_t w = {0u, 0u};
-#pragma unroll
-    for (int i = 0; i < 8; ++i) w[i >> 2] |= rs.int8(x[v][i]) << (8 * (i & 3));
-    *reinterpret_cast<u32x2_t *>((uint8_t *)a.codes + row * a.codes_stride + c) = w;
-  }
-  if (tid == 0) a.scales[row] = row_scale(mag, ss, a);
 }
 
 // Any width, alignment and length: a workgroup per row, read twice.
@@ -658,6 +671,26 @@ const Form kForms[] = {
     {16, 16, 1, 16, 2.0f, 0.8f, 0.071f, launch_stream},
 };
 
+template <int LANES, int NV, bool NORM>
+void launch_rows_form(const mia_quant_rows_args &a, hipStream_t s) {
+  constexpr int RPB = 256 / LANES;
+  const int64_t groups = (a.rows + RPB - 1) / RPB;
+  // with gamma in registers as many workgroups as are resident at once
+  constexpr int RESIDENT = NV == 1 ? 8 : NV == 2 ? 6 : NV == 4 ? 4 : 2;
+  const int64_t most = NORM ? (int64_t)cu_count() * RESIDENT : groups;
+  quant_rows_kernel<LANES, NV, NORM><<<(unsigned)std::min(groups, most), 256, 0, s>>>(a);
+}
+
+template <bool NORM>
+void launch_rows(const mia_quant_rows_args &a, hipStream_t s) {
+  if (a.dim <= 512) launch_rows_form<64, 1, NORM>(a, s);
+  else if (a.dim <= 1024) launch_rows_form<64, 2, NORM>(a, s);
+  else if (a.dim <= 2048) launch_rows_form<256, 1, NORM>(a, s);
+  else if (a.dim <= 4096) launch_rows_form<256, 2, NORM>(a, s);
+  else if (a.dim <= 8192) launch_rows_form<256, 4, NORM>(a, s);
+  else launch_rows_form<256, 8, NORM>(a, s);
+}
+
 }  // namespace
 
 int launch_quant_rows(const mia_quant_rows_args &a, hipStream_t s) {
@@ -665,14 +698,9 @@ int launch_quant_rows(const mia_quant_rows_args &a, hipStream_t s) {
   const bool vec = a.dim % 8 == 0 && a.dim <= 16384 && a.x_stride % 8 == 0 &&
                    a.codes_stride % 8 == 0 && ok(a.x, 16) && ok(a.add0, 16) && ok(a.add1, 16) &&
                    ok(a.gamma, 16) && ok(a.codes, 8);
-  const unsigned rows = (unsigned)a.rows, rows4 = (unsigned)((a.rows + 3) / 4);
-  if (!vec) quant_rows_any_kernel<<<rows, 256, 0, s>>>(a);
-  else if (a.dim <= 512) quant_rows_kernel<64, 1><<<rows4, 256, 0, s>>>(a);
-  else if (a.dim <= 1024) quant_rows_kernel<64, 2><<<rows4, 256, 0, s>>>(a);
-  else if (a.dim <= 2048) quant_rows_kernel<256, 1><<<rows, 256, 0, s>>>(a);
-  else if (a.dim <= 4096) quant_rows_kernel<256, 2><<<rows, 256, 0, s>>>(a);
-  else if (a.dim <= 8192) quant_rows_kernel<256, 4><<<rows, 256, 0, s>>>(a);
-  else quant_rows_kernel<256, 8><<<rows, 256, 0, s>>>(a);
+  if (!vec) quant_rows_any_kernel<<<(unsigned)a.rows, 256, 0, s>>>(a);
+  else if (a.norm) launch_rows<true>(a, s);
+  else launch_rows<false>(a, s);
   return check_hip(hipGetLastError(), "quant_rows");
 }
 

@@ -35,11 +35,16 @@ MIA_DEV int axis_of(const mia_rope_append_args &a, int i) {
   return x;
 }
 
+// v_rsq_f32 (1 ulp); it takes numbers below the least normal one for zeros.
+MIA_DEV float inverse_root(float x) {
+  return x < 1e-30f ? 1.0f / sqrtf(x) : __builtin_amdgcn_rsqf(x);
+}
+
 constexpr int kMaxRows = 4;  // head rows per lane group at most
 
 // Workgroup (token t, head range): L lanes of 8 channels per head row (head
 // dim <= 8 L); the G lane groups take rows g, g + G, ....
-template <int L, int KIND>
+template <int L, int KIND, bool NORM>
 __global__ __launch_bounds__(256) void rope_append_kernel(mia_rope_append_args a, int rows) {
   constexpr int G = 256 / L;
   __shared__ __attribute__((aligned(16))) float cs[2][8 * L / 2];
@@ -52,6 +57,7 @@ __global__ __launch_bounds__(256) void rope_append_kernel(mia_rope_append_args a
   // rotated ones are pairs (e0 + i, e1 + i)
   const bool split = rot && !a.interleaved;
   const int e0 = split ? 4 * j : 8 * j, e1 = split ? R / 2 + 4 * j : 8 * j + 4;
+  const float inv_d = 1.0f / (float)d;
   const int h0 = blockIdx.y * G * rows + grp;
   auto source = [&](int hh) {
     const uint16_t *p;
@@ -72,6 +78,20 @@ __global__ __launch_bounds__(256) void rope_append_kernel(mia_rope_append_args a
       const u32x2_t y = *reinterpret_cast<const u32x2_t *>(p + e1);
       raw[r] = u32x4_t{x[0], x[1], y[0], y[1]};
     }
+  }
+  // the lane's norm weights of Q and K
+  f32x4_t gq[2], gk[2];
+  if (NORM && act) {
+    auto four = [&](const void *g, int e) {
+      if (!g) return f32x4_t{1.f, 1.f, 1.f, 1.f};
+      if (a.gamma_bf16) {
+        const u32x2_t w = *reinterpret_cast<const u32x2_t *>((const uint16_t *)g + e);
+        return f32x4_t{bf16lo(w[0]), bf16hi(w[0]), bf16lo(w[1]), bf16hi(w[1])};
+      }
+      return *reinterpret_cast<const f32x4_t *>((const float *)g + e);
+    };
+    gq[0] = four(a.q_gamma, e0), gq[1] = four(a.q_gamma, e1);
+    gk[0] = four(a.k_gamma, e0), gk[1] = four(a.k_gamma, e1);
   }
   int64_t slot = -1, blk = 0, off = 0;
   if constexpr (KIND != kRows) {
@@ -109,25 +129,17 @@ __global__ __launch_bounds__(256) void rope_append_kernel(mia_rope_append_args a
       x[2 * i] = bf16lo(w[i]);
       x[2 * i + 1] = bf16hi(w[i]);
     }
-    if (a.qk_norm) {  // uniform: every lane takes part in the sum
+    if constexpr (NORM) {  // (every lane takes part in the sum)
       float ss = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
 #pragma unroll
       for (int m = L / 2; m >= 1; m >>= 1) ss += __shfl_xor(ss, m, 64);
       if (kind != 2) {
-        const float rinv = 1.0f / sqrtf(ss / (float)d + a.eps);
-        const void *g = kind == 0 ? a.q_gamma : a.k_gamma;
+        const float rinv = inverse_root(ss * inv_d + a.eps);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] *= rinv;
-        if (g && act) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int e = i < 4 ? e0 + i : e1 + i - 4;
-            x[i] *= a.gamma_bf16 ? bf16_bits_to_f32(((const uint16_t *)g)[e])
-                                 : ((const float *)g)[e];
-          }
-        }
+        for (int i = 0; i < 8; ++i)
+          x[i] *= rinv * (kind == 0 ? gq[i >> 2][i & 3] : gk[i >> 2][i & 3]);
       }
     }
     if (kind != 2 && rot) {
@@ -219,21 +231,33 @@ __global__ __launch_bounds__(256) void rope_append_kernel(mia_rope_append_args a
   }
 }
 
-template <int L>
+template <int L, bool NORM>
 void launch_lanes(const mia_rope_append_args &a, int kind, hipStream_t s) {
   constexpr int G = 256 / L;
   const int heads = a.num_q_heads + (a.v ? 2 : 1) * a.num_kv_heads;
   const int sets = (heads + G - 1) / G;  // rows per group in one workgroup per token
-  const int parts = a.num_tokens < 512 ? sets : (sets + kMaxRows - 1) / kMaxRows;
+  // Few tokens need workgroups, many of them fewer repeated angles and loads in
+  // flight: rows of 1 / 2 / 3 / 4 per group, 64 heads of d = 128 with norms, 100
+  // tokens 4.4 / 4.4 / 4.5 / 4.5 us, 512 8.9 / 7.6 / 7.6 / 8.4, 2047 22 / 18.3 / 18.2
+  // / 18.0; 48 heads, 16383 tokens 106 / 93 / 79 / 79.
+  const int most = a.num_tokens < 256 ? 1 : a.num_tokens < 1024 ? 2 : kMaxRows;
+  const int parts = (sets + most - 1) / most;
   const int rows = (sets + parts - 1) / parts;
   const dim3 grid((unsigned)a.num_tokens, (sets + rows - 1) / rows);
   switch (kind) {
-    case kRows: rope_append_kernel<L, kRows><<<grid, 256, 0, s>>>(a, rows); break;
-    case kBf16: rope_append_kernel<L, kBf16><<<grid, 256, 0, s>>>(a, rows); break;
-    case kFp8Static: rope_append_kernel<L, kFp8Static><<<grid, 256, 0, s>>>(a, rows); break;
-    case kFp8: rope_append_kernel<L, kFp8><<<grid, 256, 0, s>>>(a, rows); break;
-    default: rope_append_kernel<L, kI8><<<grid, 256, 0, s>>>(a, rows);
+    case kRows: rope_append_kernel<L, kRows, NORM><<<grid, 256, 0, s>>>(a, rows); break;
+    case kBf16: rope_append_kernel<L, kBf16, NORM><<<grid, 256, 0, s>>>(a, rows); break;
+    case kFp8Static: rope_append_kernel<L, kFp8Static, NORM><<<grid, 256, 0, s>>>(a, rows); break;
+    case kFp8: rope_append_kernel<L, kFp8, NORM><<<grid, 256, 0, s>>>(a, rows); break;
+    default: rope_append_kernel<L, kI8, NORM><<<grid, 256, 0, s>>>(a, rows);
   }
+}
+
+template <bool NORM>
+void launch_norm(const mia_rope_append_args &a, int kind, hipStream_t s) {
+  if (a.head_dim <= 64) launch_lanes<8, NORM>(a, kind, s);
+  else if (a.head_dim <= 128) launch_lanes<16, NORM>(a, kind, s);
+  else launch_lanes<32, NORM>(a, kind, s);
 }
 
 }  // namespace
@@ -243,9 +267,8 @@ int launch_rope_append(const mia_rope_append_args &a, hipStream_t s) {
                    : a.cache_dtype == MIA_DTYPE_BF16 ? kBf16
                    : a.cache_dtype == MIA_DTYPE_I8 ? kI8
                    : a.k_scales ? kFp8 : kFp8Static;
-  if (a.head_dim <= 64) launch_lanes<8>(a, kind, s);
-  else if (a.head_dim <= 128) launch_lanes<16>(a, kind, s);
-  else launch_lanes<32>(a, kind, s);
+  if (a.qk_norm) launch_norm<true>(a, kind, s);
+  else launch_norm<false>(a, kind, s);
   return check_hip(hipGetLastError(), "rope_kv_append");
 }
 
