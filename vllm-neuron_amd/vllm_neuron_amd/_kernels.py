@@ -1222,15 +1222,16 @@ def shared_prefix_attention(q, k_cache, v_cache, prefix_table, prefix_len, block
 # ---------------------------------------------------------------------------
 def _vector(t, n, what, dev):
     """A float32 or bf16 vector of ``n`` entries as the kernels read it (other
-    types as float32, other devices and strides copied)."""
+    types as float32, other devices, strides and alignments copied)."""
     if t.numel() != n:
         raise ValueError(f"{what} has {t.numel()} entries, expected {n}")
-    t = t.detach().reshape(-1)
     if t.dtype not in (torch.float32, torch.bfloat16):
-        t = t.float()
+        t = t.detach().float()
     if t.device != dev:
-        t = t.to(dev)
-    return t if t.is_contiguous() else t.contiguous()
+        t = t.detach().to(dev)
+    if not t.is_contiguous():
+        t = t.detach().contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.detach().clone()
 
 
 def quant_rows(x, norm, eps, gamma=None, add0=None, add1=None, dim_actual=0):
@@ -1243,63 +1244,67 @@ def quant_rows(x, norm, eps, gamma=None, add0=None, add1=None, dim_actual=0):
     if not shape or shape[-1] == 0:
         raise ValueError(f"quant_rows: rows of no channels, {tuple(shape)}")
     dim = shape[-1]
-    if gamma is not None and not norm:
-        raise ValueError("quant_rows: gamma belongs to a norm")
+    if gamma is not None:
+        if not norm:
+            raise ValueError("quant_rows: gamma belongs to a norm")
+        gamma = _vector(gamma, dim, "gamma", dev)
     if not 0 <= dim_actual <= dim:
         raise ValueError(f"quant_rows: dim_actual {dim_actual} of {dim} channels")
-    x2 = x if len(shape) == 2 else x.reshape(-1, dim)
-    adds = []
-    for t in (add0, add1):
-        if t is None:
-            continue
-        if t.dtype != torch.bfloat16 or t.shape != shape:
+    flat = len(shape) == 2
+    x2 = x if flat else x.reshape(-1, dim)
+    adds = ()
+    if add0 is not None or add1 is not None:
+        adds = [t for t in (add0, add1) if t is not None]
+        if any(t.dtype != torch.bfloat16 or t.shape != shape for t in adds):
             raise ValueError("residual adds must be bf16 with the input's shape")
-        adds.append(t if len(shape) == 2 else t.reshape(-1, dim))
-    if x2.stride(1) != 1 or any(t.stride() != x2.stride() for t in adds):
+        adds = [t.reshape(-1, dim) for t in adds]
+    stride = x2.stride()
+    if stride[1] != 1 or any(t.stride() != stride for t in adds):
         x2 = x2.contiguous()
         adds = [t.contiguous() for t in adds]
-    if gamma is not None:
-        gamma = _vector(gamma, dim, "gamma", dev)
+        stride = x2.stride()
     rows = x2.shape[0]
     codes = torch.empty((rows, dim), dtype=torch.int8, device=dev)
     scales = torch.empty((rows,), dtype=torch.float32, device=dev)
-    p = [t.data_ptr() for t in adds] + [0, 0]
     a = N.QuantRowsArgs()
     N.PACK_QUANT_ROWS.pack_into(
-        a, 0, x2.data_ptr(), p[0], p[1], x2.stride(0), codes.data_ptr(), dim, scales.data_ptr(),
-        rows, dim, dim_actual, int(norm), eps, 0 if gamma is None else gamma.data_ptr(),
-        int(gamma is not None and gamma.dtype == torch.bfloat16), 0)
+        a, 0, x2.data_ptr(), adds[0].data_ptr() if adds else 0,
+        adds[1].data_ptr() if len(adds) > 1 else 0, stride[0], codes.data_ptr(), dim,
+        scales.data_ptr(), rows, dim, dim_actual, norm, eps,
+        0 if gamma is None else gamma.data_ptr(),
+        gamma is not None and gamma.dtype == torch.bfloat16, 0)
     N.launch(N.lib().mia_quant_rows, a, dev, "quant_rows")
-    if len(shape) != 2:
-        codes, scales = codes.reshape(shape), scales.reshape(shape[:-1])
+    if not flat:
+        return codes.reshape(shape), scales.reshape(shape[:-1])
     return codes, scales
 
 
 def int8_linear(x, x_scales, w, w_scales, bias, out):
     """``out [M, N] = bf16(x_scales w_scales (x [M, K] w [N, K]^T) + bias)``."""
     dev = N.same_gpu(x, x_scales, w, w_scales, bias, out)
-    if x.dtype != torch.int8 or w.dtype != torch.int8 or x.dim() != 2 or w.dim() != 2:
+    xs, wshape = x.shape, w.shape
+    if x.dtype != torch.int8 or w.dtype != torch.int8 or len(xs) != 2 or len(wshape) != 2:
         raise ValueError(f"int8_linear: x and w must be int8 matrices, got {x.dtype} "
-                         f"{tuple(x.shape)} and {w.dtype} {tuple(w.shape)}")
-    (m, k), (n, wk) = x.shape, w.shape
-    if k != wk:
-        raise ValueError(f"int8_linear: x has {k} channels, w {wk}")
+                         f"{tuple(xs)} and {w.dtype} {tuple(wshape)}")
+    (m, k), n = xs, wshape[0]
+    if k != wshape[1]:
+        raise ValueError(f"int8_linear: x has {k} channels, w {wshape[1]}")
     for s, c, what in ((x_scales, m, "x_scales"), (w_scales, n, "w_scales")):
-        if s.dtype != torch.float32 or s.dim() != 1 or s.shape[0] != c or (
-                c > 1 and s.stride(0) != 1):
+        if s.dtype != torch.float32 or s.dim() != 1 or s.shape[0] != c or not s.is_contiguous():
             raise ValueError(f"int8_linear: {what} must be a contiguous float32 vector of {c}, "
                              f"got {s.dtype} {tuple(s.shape)}")
-    if out.shape != (m, n) or out.dtype != torch.bfloat16 or out.stride(1) != 1 and n > 1:
+    x_st, w_st, o_st = x.stride(), w.stride(), out.stride()
+    if out.shape != (m, n) or out.dtype != torch.bfloat16 or (o_st[1] != 1 and n > 1):
         raise ValueError(f"int8_linear: out must be bf16 [{m}, {n}] with contiguous columns")
+    if k > 1 and (x_st[1] != 1 or w_st[1] != 1):
+        raise ValueError("int8_linear: the channels of x and w must be contiguous")
     if bias is not None:
         bias = _vector(bias, n, "bias", dev)
-    if (k > 1 and (x.stride(1) != 1 or w.stride(1) != 1)):
-        raise ValueError("int8_linear: the channels of x and w must be contiguous")
     a = N.Int8LinearArgs()
     N.PACK_INT8.pack_into(
-        a, 0, x.data_ptr(), x.stride(0), x_scales.data_ptr(), w.data_ptr(), w.stride(0),
-        w_scales.data_ptr(), 0 if bias is None else bias.data_ptr(), out.data_ptr(),
-        out.stride(0), m, n, k, int(bias is not None and bias.dtype == torch.bfloat16))
+        a, 0, x.data_ptr(), x_st[0], x_scales.data_ptr(), w.data_ptr(), w_st[0],
+        w_scales.data_ptr(), 0 if bias is None else bias.data_ptr(), out.data_ptr(), o_st[0],
+        m, n, k, bias is not None and bias.dtype == torch.bfloat16)
     N.launch(N.lib().mia_int8_linear, a, dev, "int8_linear")
 
 
@@ -1307,6 +1312,20 @@ def int8_linear(x, x_scales, w, w_scales, bias, out):
 # rotation by several position axes, with the cache append
 # ---------------------------------------------------------------------------
 _NO_CACHE = (0,) * 25  # slots, dtypes, caches, scales and geometry
+_NO_SCALES = (0, 0, *_NO_STRIDES, *_NO_STRIDES)
+_PAD = ((), (0, 0, 0), (0, 0), (0,), ())  # sections of the axes that are not there
+
+
+def _head_rows(t, shape, what):
+    """Address and strides of bf16 rows ``[T, heads, d]`` (None: zeros)."""
+    if t is None:
+        return _NO_STRIDES
+    if t.dtype != torch.bfloat16:
+        raise NotImplementedError(f"rope_append: {what} must be bf16")
+    st = t.stride()
+    if t.shape != shape or st[2] != 1:
+        raise ValueError(f"{what} must be a {tuple(shape)} view with contiguous d")
+    return t.data_ptr(), st[0], st[1]
 
 
 def rope_append(q, k, v, positions, inv_freq, slots, k_cache, v_cache, q_out, k_out=None, *,
@@ -1318,50 +1337,44 @@ def rope_append(q, k, v, positions, inv_freq, slots, k_cache, v_cache, q_out, k_
     cache)."""
     dev = N.same_gpu(q, k, v, positions, inv_freq, slots, k_cache, v_cache, q_out, k_out,
                      k_scales, v_scales, k_dequant, v_dequant, q_gamma, k_gamma)
-    if q.dim() != 3 or k.dim() != 3:
-        raise ValueError(f"q and k must be [T, heads, d], got {tuple(q.shape)} / "
-                         f"{tuple(k.shape)}")
-    T, hq, d = q.shape
-    hkv = k.shape[1]
-    if k.shape != (T, hkv, d) or (v is not None and v.shape != k.shape):
-        raise ValueError(f"K and V rows must be [{T}, Hkv, {d}], got {tuple(k.shape)} / "
+    qs, ks = q.shape, k.shape
+    if len(qs) != 3 or len(ks) != 3:
+        raise ValueError(f"q and k must be [T, heads, d], got {tuple(qs)} / {tuple(ks)}")
+    T, hq, d = qs
+    hkv = ks[1]
+    if ks[0] != T or ks[2] != d or (v is not None and v.shape != ks):
+        raise ValueError(f"K and V rows must be [{T}, Hkv, {d}], got {tuple(ks)} / "
                          f"{None if v is None else tuple(v.shape)}")
-    rows = []
-    for t, like, what in ((q, q, "q"), (k, k, "k"), (v, k, "v"), (q_out, q, "q_out"),
-                          (k_out, k, "k_out")):
-        if t is None:
-            rows += (0, 0, 0)
-            continue
-        if t.dtype != torch.bfloat16:
-            raise NotImplementedError(f"rope_append: {what} must be bf16")
-        if t.shape != like.shape or t.stride(2) != 1:
-            raise ValueError(f"{what} must be a {tuple(like.shape)} view with contiguous d")
-        rows += (t.data_ptr(), t.stride(0), t.stride(1))
+    rows = (*_head_rows(q, qs, "q"), *_head_rows(k, ks, "k"), *_head_rows(v, ks, "v"),
+            *_head_rows(q_out, qs, "q_out"), *_head_rows(k_out, ks, "k_out"))
     if inv_freq.dim() != 1 or inv_freq.dtype != torch.float32 or not inv_freq.is_contiguous():
         raise ValueError("inv_freq must be a contiguous float32 vector of rot_dim / 2 entries")
     half = inv_freq.shape[0]
-    if positions.dim() == 1:
-        positions = positions.unsqueeze(0)
-    axes = positions.shape[0] if positions.dim() == 2 else 0
-    if axes == 0 or positions.shape[1] != T:
+    ps, p_st = positions.shape, positions.stride()
+    if len(ps) == 1:
+        ps, p_st = (1, *ps), (0, *p_st)
+    if len(ps) != 2 or ps[0] == 0 or ps[1] != T:
         raise ValueError(f"positions must be [T] or [axes, T] with T = {T}, got "
                          f"{tuple(positions.shape)}")
+    axes = ps[0]
     if positions.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"positions must be int32 or int64, got {positions.dtype}")
-    sections = [half] if sections is None and axes == 1 else sections
-    if sections is None or len(sections) != axes or sum(sections) != half or min(sections) < 0:
+    if sections is None and axes == 1:
+        sections = (half,)
+    elif sections is None or len(sections) != axes or sum(sections) != half or min(sections) < 0:
         raise ValueError(f"sections must split the {half} channel pairs over {axes} axes, got "
                          f"{sections}")
     if axes > 4:
         raise NotImplementedError("rope_append: one to four position axes")
-    if not qk_norm and (q_gamma is not None or k_gamma is not None):
-        raise ValueError("q_gamma and k_gamma belong to qk_norm")
-    keep = []
-    for g, what in ((q_gamma, "q_gamma"), (k_gamma, "k_gamma")):
-        keep.append(None if g is None else _vector(g, d, what, dev))
-    if len({g.dtype for g in keep if g is not None}) > 1:
-        keep = [g.float() for g in keep]
-    gamma_bf16 = any(g is not None and g.dtype == torch.bfloat16 for g in keep)
+    bf16 = False
+    if q_gamma is not None or k_gamma is not None:
+        if not qk_norm:
+            raise ValueError("q_gamma and k_gamma belong to qk_norm")
+        q_gamma = None if q_gamma is None else _vector(q_gamma, d, "q_gamma", dev)
+        k_gamma = None if k_gamma is None else _vector(k_gamma, d, "k_gamma", dev)
+        if q_gamma is not None and k_gamma is not None and q_gamma.dtype != k_gamma.dtype:
+            q_gamma, k_gamma = q_gamma.float(), k_gamma.float()
+        bf16 = (k_gamma if q_gamma is None else q_gamma).dtype == torch.bfloat16
     cache = _NO_CACHE
     if slots is not None:
         if v is None or k_cache is None or v_cache is None:
@@ -1375,19 +1388,20 @@ def rope_append(q, k, v, positions, inv_freq, slots, k_cache, v_cache, q_out, k_
                              f"{hkv} of {d}")
         if slots.dim() != 1 or slots.shape[0] != T:
             raise ValueError(f"slots must be [T] = [{T}], got {tuple(slots.shape)}")
-        slots = slots if slots.is_contiguous() else slots.contiguous()
+        if not slots.is_contiguous():
+            slots = slots.contiguous()
         if (k_scales is None) != (v_scales is None) or (k_dequant is None) != (v_dequant is None):
             raise ValueError("the scales of K and V go together")
-        scales = (0, 0, *_NO_STRIDES, *_NO_STRIDES)
+        scales = _NO_SCALES
         if k_scales is not None:
             _check_scales(shape, k_scales, v_scales)
             scales = (k_scales.data_ptr(), v_scales.data_ptr(), *k_scales.stride(),
                       *v_scales.stride())
         dequant = (0, 0)
         if k_dequant is not None:
-            keep += [_scale_f32(k_dequant, dev, hkv, "k_dequant_scale"),
-                     _scale_f32(v_dequant, dev, hkv, "v_dequant_scale")]
-            dequant = (keep[-2].data_ptr(), keep[-1].data_ptr())
+            k_dequant = _scale_f32(k_dequant, dev, hkv, "k_dequant_scale")
+            v_dequant = _scale_f32(v_dequant, dev, hkv, "v_dequant_scale")
+            dequant = (k_dequant.data_ptr(), v_dequant.data_ptr())
         cache = (slots.data_ptr(), N.mia_dtype(slots.dtype), N.mia_dtype(k_cache.dtype),
                  k_cache.data_ptr(), v_cache.data_ptr(), *k_cache.stride(), *v_cache.stride(),
                  *scales, *dequant, shape[0], shape[2])
@@ -1395,10 +1409,10 @@ def rope_append(q, k, v, positions, inv_freq, slots, k_cache, v_cache, q_out, k_
         raise ValueError("the cache append needs slots")
     a = N.RopeAppendArgs()
     N.PACK_ROPE.pack_into(
-        a, 0, *rows, T, hq, hkv, d, 2 * half, positions.data_ptr(), *positions.stride(),
-        N.mia_dtype(positions.dtype), axes, inv_freq.data_ptr(), *sections, *([0] * (4 - axes)),
-        int(cycle), int(interleaved), rope_scale, int(qk_norm), N.ptr(keep[0]) or 0,
-        N.ptr(keep[1]) or 0, int(gamma_bf16), eps, *cache)
+        a, 0, *rows, T, hq, hkv, d, 2 * half, positions.data_ptr(), *p_st,
+        N.mia_dtype(positions.dtype), axes, inv_freq.data_ptr(), *sections, *_PAD[axes], cycle,
+        interleaved, rope_scale, qk_norm, N.ptr(q_gamma) or 0, N.ptr(k_gamma) or 0, bf16, eps,
+        *cache)
     N.launch(N.lib().mia_rope_append, a, dev, "rope_append")
 
 
