@@ -274,12 +274,7 @@ def test_calls_on_other_streams_and_in_graphs(gpu):
     assert torch.equal(compiled(x), want)
 
 
-@pytest.mark.parametrize("m,n,k", [(1, 700, 4096), (16, 5000, 1040), (30, 9000, 272), (40, 2500, 4112), (64, 6144, 144),
-                                   (100, 17000, 80), (150, 4100, 2064), (260, 3000, 3088), (600, 2050, 400),
-                                   (513, 520, 8208), (1300, 5200, 656), (4100, 2570, 336), (5000, 7000, 64),
-                                   (2049, 8193, 16)])
-def test_products_whatever_form_is_taken(gpu, m, n, k):
-    """Sizes across the forms' ranges, with ragged last tiles in every axis."""
+def _exact_product(gpu, m, n, k):
     g = torch.Generator(device=gpu).manual_seed(m)
     x = torch.randint(-127, 128, (m, k), generator=g, device=gpu, dtype=torch.int32).to(torch.int8)
     w = torch.randint(-127, 128, (n, k), generator=g, device=gpu, dtype=torch.int32).to(torch.int8)
@@ -291,3 +286,19 @@ def test_products_whatever_form_is_taken(gpu, m, n, k):
         acc += (x[:, i:i + 1024].float() @ w[:, i:i + 1024].float().t()).double()
     ref = acc * xs.double()[:, None] * ws.double()
     assert ((y.double() - ref).abs() <= 2.0 ** -8 * ref.abs() + 2.0 ** -21 * ref.abs()).all()
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 700, 4096), (16, 5000, 1040), (30, 9000, 272), (40, 2500, 4112), (64, 6144, 144),
+                                   (100, 17000, 80), (150, 4100, 2064), (260, 3000, 3088), (600, 2050, 400),
+                                   (513, 520, 8208), (1300, 5200, 656), (4100, 2570, 336), (5000, 7000, 64),
+                                   (2049, 8193, 16)])
+def test_products_whatever_form_is_taken(gpu, m, n, k):
+    """Sizes across the forms' ranges, with ragged last tiles in every axis."""
+    _exact_product(gpu, m, n, k)
+
+
+@pytest.mark.parametrize("k", [16, 112, 128, 144, 240, 256, 272, 384, 400, 512, 528, 640, 656, 768, 784, 1024, 1040])
+@pytest.mark.parametrize("m,n", [(129, 12000), (129, 4100), (70, 9000), (300, 12000), (5, 4100)])
+def test_few_tiles_of_k(gpu, m, n, k):
+    """Fewer tiles along k than a ring holds, as many, and more, whole and not."""
+    _exact_product(gpu, m, n, k)

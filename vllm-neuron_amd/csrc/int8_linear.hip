@@ -274,6 +274,48 @@ MIA_DEV void store_tile(const GemmParams &p, lds_u8_t *all, const i32x16_t (&acc
   }
 }
 
+// The sums of G groups of WAVES waves meet in the first group's registers, through
+// LDS, which is free; at: the lane's place in its group.  Every thread calls it.
+template <int G, int WAVES, int TN, int TM>
+MIA_DEV void join_sums(lds_u8_t *all, i32x16_t (&acc)[TN][TM], int group, int at) {
+  if constexpr (G > 1) {
+    typedef __attribute__((address_space(3))) i32x4_t lds_i32x4_t;
+    lds_i32x4_t *const sums = (lds_i32x4_t *)all + at;
+    constexpr int PER = TN * TM * 4;
+    if (group > 0) {
+#pragma unroll
+      for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int j = 0; j < TM; ++j)
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+            sums[((group - 1) * PER + (i * TM + j) * 4 + g) * WAVES * 64] =
+                i32x4_t{acc[i][j][g * 4], acc[i][j][g * 4 + 1], acc[i][j][g * 4 + 2],
+                        acc[i][j][g * 4 + 3]};
+    }
+    __syncthreads();
+    if (group == 0) {
+#pragma unroll
+      for (int k = 1; k < G; ++k)
+#pragma unroll
+        for (int i = 0; i < TN; ++i)
+#pragma unroll
+          for (int j = 0; j < TM; ++j)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const i32x4_t v = sums[((k - 1) * PER + (i * TM + j) * 4 + g) * WAVES * 64];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[i][j][g * 4 + e] += v[e];
+            }
+    }
+    __syncthreads();
+  }
+}
+
+// LDS that join_sums needs
+constexpr int join_bytes(int g, int waves, int products) {
+  return (g - 1) * waves * 64 * products * 16 * 4;
+}
 
 constexpr int kBK = 128;  // bytes of k per tile
 
@@ -401,43 +443,154 @@ __global__ __launch_bounds__(WN *WM *KS * 64) void gemm_kernel(GemmParams p) {
   // ---- epilogue: out = acc xs ws + bias, rounded to bf16 through LDS so that
   // rows are stored whole
   __syncthreads();
-  if constexpr (KS > 1) {
-    // the groups' sums meet in the first group's registers
-    typedef __attribute__((address_space(3))) i32x4_t lds_i32x4_t;
-    constexpr int SUMS = WAVES * 64 * TN * TM * 16;  // of a group
-    lds_i32x4_t *const sums = (lds_i32x4_t *)all;
-    static_assert((KS - 1) * SUMS * 4 <= KS * STAGES * STAGE, "sums fit");
-    const int at = (wave * 64 + lane) * 4;
-    if (group > 0) {
-#pragma unroll
-      for (int i = 0; i < TN; ++i)
-#pragma unroll
-        for (int j = 0; j < TM; ++j)
-#pragma unroll
-          for (int g = 0; g < 4; ++g)
-            sums[((group - 1) * TN * TM * 4 + (i * TM + j) * 4 + g) * WAVES * 64 + at / 4] =
-                i32x4_t{acc[i][j][g * 4], acc[i][j][g * 4 + 1], acc[i][j][g * 4 + 2],
-                        acc[i][j][g * 4 + 3]};
-    }
-    __syncthreads();
-    if (group == 0) {
-#pragma unroll
-      for (int k = 1; k < KS; ++k)
-#pragma unroll
-        for (int i = 0; i < TN; ++i)
-#pragma unroll
-          for (int j = 0; j < TM; ++j)
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              const i32x4_t v =
-                  sums[((k - 1) * TN * TM * 4 + (i * TM + j) * 4 + g) * WAVES * 64 + at / 4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e) acc[i][j][g * 4 + e] += v[e];
-            }
-    }
-    __syncthreads();
-  }
+  join_sums<KS, WAVES>(all, acc, group, wave * 64 + lane);
   store_tile<TN, TM, BN, THREADS>(p, all, acc, n0, m0, wn, wm, wave, group == 0);
+}
+
+// WN x WM x KG waves, each TN x TM products of 32 x 32 over its KG-th part of a
+// tile's k.  One ring of tiles for the worgrouproup; a wave reads its fragments of
+// tile t + 1 and copies its part of tile t + STAGES - 1 between the products of
+// tile t, so that neither LDS, nor the copies' issue, nor the barrier stands between
+// two products.  A CU alone takes 0.34 us per 128 x 128 x 128 so (0.21 at the matrix
+// units' rate), where rings whose waves copy, read and then multiply take 0.48 with
+// eight waves and 0.57 with four: waiting for memory was none of it (the same with
+// every byte in L2 and with 2 to 5 stages).
+template <int WN, int WM, int TN, int TM, int STAGES, int KG>
+__global__ __launch_bounds__(WN *WM *KG * 64) void gemm_pipe_kernel(GemmParams p) {
+  constexpr int WAVES = WN * WM * KG, THREADS = WAVES * 64;
+  constexpr int NS = kBK / 32 / KG;  // fragments of a tile that a wave reads
+  constexpr int BN = WN * TN * 32, BM = WM * TM * 32;
+  constexpr int NC = BN / 8 / WAVES, MC = BM / 8 / WAVES;  // copies per wave and tile
+  static_assert(BN % (8 * WAVES) == 0 && BM % (8 * WAVES) == 0, "whole copies");
+  static_assert(NS >= 2 && STAGES >= 3, "read and copied ahead");
+  constexpr int STAGE = (BN + BM) * kBK;
+  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+  const int tid = threadIdx.x;
+  const int wave = readfirstlane(tid >> 6);
+  const int lane = tid & 63;
+  lds_u8_t *const lds = (lds_u8_t *)smem;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)lds;
+  const int wn = wave % WN, wm = wave / WN % WM, group = wave / (WN * WM);
+  const int rl = lane & 31, half = lane >> 5;
+
+  const int2 tile = tile_of(p);
+  const int n0 = tile.x * BN, m0 = tile.y * BM;
+  const uint8_t *wsrc = p.w + (int64_t)n0 * p.w_ld;
+  const uint8_t *xsrc = p.x + (int64_t)m0 * p.x_ld;
+  uint32_t won[NC], xom[MC];
+  const int chunk_e = (lane & 7) ^ (lane >> 4);  // even row groups; odd ones: ^ 4
+#pragma unroll
+  for (int j = 0; j < NC; ++j) {
+    const int g = wave * NC + j, row = g * 8 + (lane >> 3);
+    won[j] = (uint32_t)min(row, p.n - 1 - n0) * (uint32_t)p.w_ld + (chunk_e ^ ((g & 1) * 4)) * 16;
+  }
+#pragma unroll
+  for (int j = 0; j < MC; ++j) {
+    const int g = wave * MC + j, row = g * 8 + (lane >> 3);
+    xom[j] = (uint32_t)min(row, p.m - 1 - m0) * (uint32_t)p.x_ld + (chunk_e ^ ((g & 1) * 4)) * 16;
+  }
+  const int steps = (p.k + kBK - 1) / kBK, full = p.k / kBK;
+  // copy j of tile t, to the stage at dst
+  auto copy = [&](int t, uint32_t dst, int j) {
+    if (j < NC)
+      copy1(wsrc + t * kBK, won[j], lds0 + dst + (wave * NC + j) * 1024);
+    else
+      copy1(xsrc + t * kBK, xom[j - NC], lds0 + dst + BN * kBK + (wave * MC + j - NC) * 1024);
+  };
+  // the last tile where k ends inside it: chunks past k are zeros for x, so that
+  // they count nothing whatever w's hold there
+  auto load_part = [&](int t, uint32_t dst) {
+    const int k0 = t * kBK;
+#pragma unroll
+    for (int j = 0; j < NC + MC; ++j) {
+      const int g = j < NC ? wave * NC + j : wave * MC + j - NC;
+      if (k0 + (chunk_e ^ ((g & 1) * 4)) * 16 < p.k)
+        copy(t, dst, j);
+      else if (j >= NC)
+        *(lds_u32x4_t *)(lds + dst + BN * kBK + g * 1024 + lane * 16) = u32x4_t{0u, 0u, 0u, 0u};
+    }
+  };
+
+  i32x16_t acc[TN][TM] = {};
+  const int swz = (rl >> 1) & 7;  // (rows of a fragment start at multiples of 32)
+  const lds_u8_t *const wrow = lds + (wn * TN * 32 + rl) * kBK;
+  const lds_u8_t *const xrow = lds + BN * kBK + (wm * TM * 32 + rl) * kBK;
+  i32x4_t wf[NS][TN], xf[NS][TM];
+  auto read = [&](uint32_t st, int s) {
+    const uint32_t c = (uint32_t)(((2 * (group * NS + s) + half) ^ swz) << 4) + st;
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+      wf[s][i] = __builtin_bit_cast(i32x4_t, *(const lds_u32x4_t *)(wrow + c + i * 32 * kBK));
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+      xf[s][i] = __builtin_bit_cast(i32x4_t, *(const lds_u32x4_t *)(xrow + c + i * 32 * kBK));
+  };
+  auto multiply = [&](int s) {  // (in its place: reads before it, copies after it)
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+#pragma unroll
+      for (int j = 0; j < TM; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wf[s][i], xf[s][j], acc[i][j], 0, 0, 0);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+#pragma unroll
+  for (int i = 0; i < STAGES - 1; ++i)
+    if (i < full) {
+#pragma unroll
+      for (int j = 0; j < NC + MC; ++j) copy(i, i * STAGE, j);
+    } else if (i < steps) {
+      load_part(i, i * STAGE);
+    }
+  if (STAGES - 1 <= full)
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 2) * (NC + MC)) : "memory");
+  else
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  uint32_t st = 0, prev = (STAGES - 1) * STAGE;  // stages of this tile and of the one before
+#pragma unroll
+  for (int s = 0; s < NS - 1; ++s) read(0, s);
+  for (int t = 0; t < steps; ++t) {
+    // tile t - 1 + STAGES goes to the stage that tile t - 1 left
+    const int next = t - 1 + STAGES;
+    const bool whole = next < full;
+    auto some = [&](int c) {
+      if (whole) {
+#pragma unroll
+        for (int j = 0; j < NC + MC; ++j)
+          if (j * NS / (NC + MC) == c) copy(next, prev, j);
+      }
+    };
+    const uint32_t following = st + STAGE == STAGES * STAGE ? 0 : st + STAGE;
+    read(st, NS - 1);
+    multiply(0);
+    // tile t + 1 has landed, and every wave has read tile t - 1 (past the last
+    // tile what is read counts nothing)
+    if (next - 1 < full)
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 3) * (NC + MC)) : "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      if (s + 1 < NS) {
+        read(following, s);
+        multiply(s + 1);
+      }
+      some(s);
+      if (s == 0 && !whole && next < steps) {
+        load_part(next, prev);
+        __builtin_amdgcn_s_waitcnt(0xC07F);
+      }
+    }
+    prev = st, st = following;
+  }
+  __syncthreads();
+  join_sums<KG, WN * WM>(lds, acc, group, wave % (WN * WM) * 64 + lane);
+  store_tile<TN, TM, BN, THREADS>(p, lds, acc, n0, m0, wn, wm, wave, group == 0);
 }
 
 // Tiles of 256 x 256 by eight waves in two groups that take turns: while one
@@ -629,8 +782,20 @@ int launch_gemm(GemmParams &p, hipStream_t s) {
   p.nt = (p.n + BN - 1) / BN;
   p.mt = (p.m + BM - 1) / BM;
   constexpr int bytes = (BN + BM) * kBK * STAGES * KS;
-  static_assert(bytes >= BN * 8 + WN * WM * 32 * (TN * 64 + 16), "epilogue fits");
+  static_assert(bytes >= BN * 8 + WN * WM * KS * 32 * (TN * 64 + 16), "epilogue fits");
+  static_assert(bytes >= join_bytes(KS, WN * WM, TN * TM), "sums fit");
   return launch_tiles<gemm_kernel<WN, WM, TN, TM, STAGES, KS>>(p, WN * WM * KS * 64, bytes, s);
+}
+
+template <int WN, int WM, int TN, int TM, int STAGES, int KG>
+int launch_pipe(GemmParams &p, hipStream_t s) {
+  constexpr int BN = WN * TN * 32, BM = WM * TM * 32;
+  p.nt = (p.n + BN - 1) / BN;
+  p.mt = (p.m + BM - 1) / BM;
+  constexpr int bytes = (BN + BM) * kBK * STAGES;
+  static_assert(bytes >= BN * 8 + WN * WM * KG * 32 * (TN * 64 + 16), "epilogue fits");
+  static_assert(bytes >= join_bytes(KG, WN * WM, TN * TM), "sums fit");
+  return launch_tiles<gemm_pipe_kernel<WN, WM, TN, TM, STAGES, KG>>(p, WN * WM * KG * 64, bytes, s);
 }
 
 int launch_turns(GemmParams &p, hipStream_t s) {
@@ -649,26 +814,26 @@ int launch_stream(GemmParams &p, hipStream_t s) {
 // every CU.  The constants are least squares over measurements at 1 to 8191 rows
 // of k = 256 to 14336 and 512 to 10240 columns (weights rotated through 256 MB);
 // the form chosen by them took 0.3 % longer than the fastest one on the
-// geometric mean, 18 % at most (8191 x 2880 x 5120).  Of 64 x 4096 x 6144, us, by
-// form in the table's order from the third on: 18.5, 13.3, 11.4, 8.3, 12.1, 8.1;
-// 517 x 2880 x 5120 from the first on: 34.5, 19.4, 18.0, 24.7, 27.5, 38.5, 53.2,
-// 38.7; 8191 x 8192 x 10240: 691, 806; 4 x 2048 x 2048 from the third on: 10.6, 8.0,
-// 7.1, 5.2, 4.8, 5.1, 3.2.
+// geometric mean, 16 % at most (8191 x 2880 x 5120: 150 against 129 us).  Examples,
+// us, by form in the table's order:
+//   64 x 4096 x 6144, from the third on: 15.2, 12.1, 10.2, 12.1, 8.1
+//   517 x 2880 x 5120, from the first on: 34.3, 19.3, 15.3, 22.7, 24.2, 53.4, 38.9
+//   8191 x 8192 x 10240, the first two: 682, 803
+//   4 x 2048 x 2048, from the third on: 8.9, 7.5, 6.5, 4.7, 5.1, 3.3
 struct Form {
   int bm, bn, per_cu, rows;  // rows: at most (0: any number)
   float once, round, step;
   int (*launch)(GemmParams &, hipStream_t);
 };
 const Form kForms[] = {
-    {256, 256, 1, 0, -16.2f, 23.5f, 1.126f, launch_turns},
-    {128, 128, 2, 0, -7.0f, 10.8f, 0.707f, launch_gemm<2, 2, 2, 2, 2, 1>},
-    {128, 128, 1, 0, -2.8f, 7.3f, 0.478f, launch_gemm<2, 2, 2, 2, 2, 2>},
-    {64, 128, 1, 0, -0.5f, 4.1f, 0.322f, launch_gemm<2, 2, 2, 1, 3, 2>},
-    {64, 64, 1, 0, 0.7f, 3.0f, 0.242f, launch_gemm<2, 1, 1, 2, 3, 2>},
-    {64, 32, 1, 0, 1.0f, 2.3f, 0.139f, launch_gemm<1, 2, 1, 1, 3, 4>},
-    {32, 32, 1, 0, 1.5f, 1.8f, 0.114f, launch_gemm<1, 1, 1, 1, 3, 4>},
-    {32, 64, 1, 0, 0.9f, 2.4f, 0.140f, launch_gemm<2, 1, 1, 1, 3, 4>},
-    {16, 16, 1, 16, 2.0f, 0.8f, 0.071f, launch_stream},
+    {256, 256, 1, 0, -12.9f, 20.0f, 1.158f, launch_turns},
+    {128, 128, 2, 0, -5.9f, 9.7f, 0.698f, launch_gemm<2, 2, 2, 2, 2, 1>},
+    {128, 128, 1, 0, -2.7f, 6.4f, 0.394f, launch_pipe<2, 4, 2, 1, 4, 1>},
+    {64, 128, 1, 0, -0.6f, 3.8f, 0.303f, launch_pipe<4, 2, 1, 1, 5, 1>},
+    {64, 64, 1, 0, 0.6f, 2.7f, 0.224f, launch_pipe<2, 2, 1, 1, 6, 2>},
+    {32, 32, 1, 0, 1.3f, 1.8f, 0.115f, launch_gemm<1, 1, 1, 1, 3, 4>},
+    {32, 64, 1, 0, 0.8f, 2.4f, 0.142f, launch_gemm<2, 1, 1, 1, 3, 4>},
+    {16, 16, 1, 16, 1.7f, 0.9f, 0.077f, launch_stream},
 };
 
 template <int LANES, int NV, bool NORM>
