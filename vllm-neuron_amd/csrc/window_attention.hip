@@ -200,7 +200,7 @@ struct Work {
     auto clear = [&](int t0, int t1) {
       const int c4 = p.d / 4, row = p.G * c4;
       for (int t = t0 + rt; t < t1; t += p.rt_max)
-        for (int x = threadIdx.x; x < row; x += kThreads) {
+        for (int x = threadIdx.x; x < row; x += blockDim.x) {
           const int g = x / c4;
           *reinterpret_cast<u32x2_t *>(p.out + (int64_t)t * p.os_t +
                                        (int64_t)(h * p.G + g) * p.os_h + (x - g * c4) * 4) =
@@ -622,20 +622,21 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void window_tall_kernel(
 // ---------------------------------------------------------------------------
 // thin form: at most 16 NC rows, each wave streams tiles of its own
 // ---------------------------------------------------------------------------
-template <int D, bool SC, int NC>
+template <int D, bool SC, int NC, int WAVES>
 struct ThinLds {
   union {
     struct {
-      uint8_t v[kWaves][kThinKeys * D * 2];
-      float sc[kWaves][SC ? 2 * kThinKeys : 4];
+      uint8_t v[WAVES][kThinKeys * D * 2];
+      float sc[WAVES][SC ? 2 * kThinKeys : 4];
     };
-    float o[kWaves][NC * 16][D + 4];  // the waves' sums, joined at the end
+    float o[WAVES][NC * 16][D + 4];  // the waves' sums, joined at the end
   };
-  float2 ml[kWaves][NC * 16];
+  float2 ml[WAVES][NC * 16];
 };
 
-template <int D, int CT, bool SC, int DU, int NC>
-__global__ __launch_bounds__(kThreads, 2) void window_thin_kernel(WindowParams p) {
+template <int D, int CT, bool SC, int DU, int NC, int WAVES>
+__global__ __launch_bounds__(WAVES * 64, 2) void window_thin_kernel(WindowParams p) {
+  constexpr int THREADS = WAVES * 64;
   // (8-bit k-steps come in pairs: all of D)
   constexpr int EB = CT == kBf16 ? 2 : 1;
   constexpr int KSTEPS = (CT == kBf16 ? DU : D) / 32;
@@ -650,7 +651,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_thin_kernel(WindowParams p
   constexpr int ROWB = D * 2;
   constexpr int VNCH = D / 8;
   constexpr int DB16 = DU / 16;
-  __shared__ __attribute__((aligned(1024))) ThinLds<D, SC, NC> lds;
+  __shared__ __attribute__((aligned(1024))) ThinLds<D, SC, NC, WAVES> lds;
 
   const int wave = readfirstlane((int)threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
@@ -664,7 +665,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_thin_kernel(WindowParams p
   wk.clear_rest(p);
   Tiles tl;
   if (!tl.set<kThinKeys>(p, wk.i, 0, NC * 16)) return;
-  // the piece's tiles, of which every wave takes each fourth
+  // the piece's tiles, which the waves take in turn
   const int2 share = wk.share(p, tl.n);
   const int x0 = share.x, x1 = share.y;
 
@@ -698,7 +699,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_thin_kernel(WindowParams p
   auto locate = [&](Slot &t, int x) {
     t.g[0].set(p, keys, tl.key(2 * x), t.ent[0]);
     t.g[1].set(p, keys, tl.key(2 * x + 1), t.ent[1]);
-    if (x + kWaves < x1) load_entries(t, x + kWaves);
+    if (x + WAVES < x1) load_entries(t, x + WAVES);
   };
   auto load_k = [&](Slot &t) {
 #pragma unroll
@@ -915,12 +916,12 @@ __global__ __launch_bounds__(kThreads, 2) void window_thin_kernel(WindowParams p
     load_s(slot);
     load_v(slot);
   }
-  for (; x < x1; x += kWaves) {
+  for (; x < x1; x += WAVES) {
     const int k0[2] = {tl.key(2 * x), tl.key(2 * x + 1)};
     const bool whole = see_all(p, tl.p_lo, tl.p_hi, k0[0], k0[0] + 16) &&
                        see_all(p, tl.p_lo, tl.p_hi, k0[1], k0[1] + 16);
-    const bool go = x + kWaves < x1;
-    if (go) locate(slot, x + kWaves);
+    const bool go = x + WAVES < x1;
+    if (go) locate(slot, x + WAVES);
     scores(slot);
     if constexpr (SC) {
       const int k = (lane & 16 ? k0[1] : k0[0]) + (lane & 15);
@@ -951,13 +952,13 @@ __global__ __launch_bounds__(kThreads, 2) void window_thin_kernel(WindowParams p
   const int c = threadIdx.x % C4 * 4;
   if (c >= p.d) return;
 #pragma unroll
-  for (int k = 0; k < NC * 16 * C4 / kThreads; ++k) {
-    const int r = k * (kThreads / C4) + (int)threadIdx.x / C4;
+  for (int k = 0; k < (NC * 16 * C4 + THREADS - 1) / THREADS; ++k) {
+    const int r = k * (THREADS / C4) + (int)threadIdx.x / C4;
     if (r >= tl.rows) return;
     float m = -INFINITY, l = 0.f;
     f32x4_t o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
+    for (int w = 0; w < WAVES; ++w) {
       const f32x4_t v = *reinterpret_cast<const f32x4_t *>(&lds.o[w][r][c]);
       add_piece(m, l, o, lds.ml[w][r].x, lds.ml[w][r].y, v);
     }
@@ -1028,6 +1029,7 @@ int64_t up(int64_t x, int64_t a) { return (x + a - 1) / a * a; }
 struct Plan {
   bool thin;
   int tile_rows;  // rows of a workgroup
+  int waves;      // of a thin workgroup
   int64_t blocks;
   size_t o, total;  // byte offset of the sums, size
 };
@@ -1048,9 +1050,21 @@ Plan plan_window(WindowParams &p) {
   const int64_t busy =
       std::min<int64_t>((int64_t)p.n_seq * p.rt_max,
                         (int64_t)p.num_tokens * p.G / tile_rows + p.n_seq) * p.Hkv;
-  const int64_t slots = (int64_t)cu_count() * 2;
-  const int64_t least = w.thin ? 8 : 6;  // tiles of a piece at least
+  // Thin workgroups of eight waves where every CU has one at most (and there is more
+  // than a tile for each of four): half the tiles one after the other.  us at 1024
+  // keys, d = 128, bf16, 4 / 8 waves: 256 workgroups 32.5 / 28.9, int8 22.7 / 18.6;
+  // 320 workgroups 41.0 / 43.8, 512 52.3 / 54.9.
+  w.waves = w.thin && busy <= cu_count() && tiles > 4 ? 8 : 4;
+  // Keys are cut where workgroups are few, to pieces of `least` tiles at least.  A
+  // cut costs a second launch (2 us, 4 of host time where calls are not captured),
+  // which up to 40 tiles at d = 64 (20 at 128) it does not earn back: us uncut / cut,
+  // captured, bf16, 4 x 8 heads, d = 64: 512 keys 7.4 / 8.5, 1024 10.6 / 10.3, 2048
+  // 15.4 / 12.1; 16 x 8 heads: 1024 11.1 / 13.0, 2048 17.2 / 17.9; d = 128, 8 x 8
+  // heads: 512 11.2 / 12.0, 1024 15.9 / 14.0.
+  const int64_t slots = (int64_t)cu_count() * 8 / w.waves;
+  const int64_t least = w.thin ? 8 : 6;
   p.split = (int)std::max<int64_t>(1, std::min<int64_t>({slots / busy, tiles / least, 32}));
+  if (w.waves == 8 && tiles * D <= 40 * 64) p.split = 1;
   // (slots for partials are by the longest sequence: many short ones beside it
   // would take gigabytes that nothing writes)
   const int64_t tiles_all = (int64_t)p.n_seq * p.rt_max * p.Hkv;
@@ -1100,12 +1114,18 @@ WindowParams window_params(const mia_window_args &a) {
   return p;
 }
 
+template <int D, int CT, bool SC, int DU, int NC>
+void launch_thin(const WindowParams &p, const Plan &w, hipStream_t s) {
+  const unsigned n = (unsigned)w.blocks;
+  if (w.waves == 8) window_thin_kernel<D, CT, SC, DU, NC, 8><<<n, 512, 0, s>>>(p);
+  else window_thin_kernel<D, CT, SC, DU, NC, 4><<<n, 256, 0, s>>>(p);
+}
+
 template <int D, int CT, bool SC, int DU>
 void launch_form(const WindowParams &p, const Plan &w, hipStream_t s) {
-  const unsigned n = (unsigned)w.blocks;
-  if (!w.thin) window_tall_kernel<D, CT, SC, DU><<<n, kThreads, 0, s>>>(p);
-  else if (w.tile_rows == 16) window_thin_kernel<D, CT, SC, DU, 1><<<n, kThreads, 0, s>>>(p);
-  else window_thin_kernel<D, CT, SC, DU, 2><<<n, kThreads, 0, s>>>(p);
+  if (!w.thin) window_tall_kernel<D, CT, SC, DU><<<(unsigned)w.blocks, kThreads, 0, s>>>(p);
+  else if (w.tile_rows == 16) launch_thin<D, CT, SC, DU, 1>(p, w, s);
+  else launch_thin<D, CT, SC, DU, 2>(p, w, s);
 }
 
 template <int D, int DU>
