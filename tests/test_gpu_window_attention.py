@@ -150,6 +150,21 @@ def test_keys_cut_into_pieces(gpu, cache, batch, Hkv, new, lens, window):
     c.check()
 
 
+@pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("Hq,Hkv,d", [(4, 1, 64), (20, 1, 128), (2, 1, 96)])
+def test_more_sequences_than_compute_units(gpu, cache, Hq, Hkv, d):
+    lens = [1 + 37 * i % 310 for i in range(300)]
+    Call(gpu, [1] * len(lens), lens, Hq, Hkv, d, 16, 170, 5, cache).check()
+
+
+@pytest.mark.parametrize("cache", ["bf16", "int8", "fp8s"])
+@pytest.mark.parametrize("Hq,d,window", [(4, 64, 500), (4, 64, 1200), (4, 64, 1290), (24, 64, 2500), (8, 128, 560),
+                                         (8, 128, 660), (30, 128, 1500)])
+def test_long_windows_of_one_token(gpu, cache, Hq, d, window):
+    """Keys that one workgroup takes whole and keys that are cut."""
+    Call(gpu, [1, 1], [window + 300, window - 100], Hq, 1, d, 32, window, 4, cache, sink=True).check()
+
+
 def test_token_per_sequence_without_a_list(gpu):
     c = Call(gpu, [1] * 6, [1, 5, 64, 80, 200, 0], 8, 2, 64, 16, 48, 2)
     a = c.run()

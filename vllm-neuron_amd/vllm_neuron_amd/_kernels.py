@@ -1264,8 +1264,8 @@ def quant_rows(x, norm, eps, gamma=None, add0=None, add1=None, dim_actual=0):
         adds = [t.contiguous() for t in adds]
         stride = x2.stride()
     rows = x2.shape[0]
-    codes = torch.empty((rows, dim), dtype=torch.int8, device=dev)
-    scales = torch.empty((rows,), dtype=torch.float32, device=dev)
+    codes = x2.new_empty((rows, dim), dtype=torch.int8)
+    scales = x2.new_empty((rows,), dtype=torch.float32)
     a = N.QuantRowsArgs()
     N.PACK_QUANT_ROWS.pack_into(
         a, 0, x2.data_ptr(), adds[0].data_ptr() if adds else 0,

@@ -715,8 +715,11 @@ def _(x, x_scales, w, w_scales, bias, out):
 
 def int8_linear(x, x_scales, w, w_scales, bias=None, out=None) -> Tensor:
     if out is None:
-        out = torch.empty((x.shape[0], w.shape[0]), dtype=torch.bfloat16, device=x.device)
-    if _plain(x, x_scales, w, w_scales, bias, out):
+        out = x_scales.new_empty((x.shape[0], w.shape[0]), dtype=torch.bfloat16)
+        if _plain(x, x_scales, w, w_scales, bias):
+            K.int8_linear(x, x_scales, w, w_scales, bias, out)
+            return out
+    elif _plain(x, x_scales, w, w_scales, bias, out):
         K.int8_linear(x, x_scales, w, w_scales, bias, out)
         _written(out)
         return out
@@ -812,7 +815,8 @@ def window_attention(q, k_cache, v_cache, block_table, seq_lens, *, window: int,
                            cu_seqlens_q=cu_seqlens_q, max_seqlen_q=int(max_seqlen_q), sink=sink,
                            k_scales=k_scales, v_scales=v_scales, k_dequant=k_dequant,
                            v_dequant=v_dequant, workspace=workspace, zero_rest=rest)
-        _written(out, workspace)
+        if not rest or workspace is not None:
+            _written(out, workspace)
         return out
     _window_attention(q, k_cache, v_cache, block_table, seq_lens, out, cu_seqlens_q, sink,
                       k_scales, v_scales, k_dequant, v_dequant, workspace, int(window),
