@@ -155,7 +155,7 @@ def test_products_of_layer_sizes(gpu, m, n, k):
 @pytest.mark.parametrize("m", [3, 100])
 def test_largest_sums(gpu, m):
     """Every code at an end of its range, k at the limit."""
-    k = 131072
+    k = 131056
     x = torch.full((m, k), 127, dtype=torch.int8, device=gpu)
     w = torch.full((20, k), 127, dtype=torch.int8, device=gpu)
     w[1] = -127
@@ -166,6 +166,8 @@ def test_largest_sums(gpu, m):
     # (-128 is a code that a weight may have)
     y = int8_linear(torch.full_like(x, -128), one, torch.full_like(w, 127), torch.ones(20, device=gpu))
     assert (y == torch.tensor([-128.0 * 127 * k]).to(torch.bfloat16).item()).all()
+    y = int8_linear(torch.full_like(x, -128), one, torch.full_like(w, -128), torch.ones(20, device=gpu))
+    assert (y == torch.tensor([128.0 * 128 * k]).to(torch.bfloat16).item()).all()
 
 
 @pytest.mark.parametrize("m", [5, 90])

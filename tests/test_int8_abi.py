@@ -55,7 +55,7 @@ def test_quant_rows_refusals(over, err, text):
     (dict(rows=-1), ValueError, "shape"),
     (dict(k=0), ValueError, "shape"),
     (dict(k=24), NotImplementedError, "multiple of 16"),
-    (dict(k=131088, x_stride=131088, w_stride=131088), NotImplementedError, "131072"),
+    (dict(k=131072, x_stride=131072, w_stride=131072), NotImplementedError, "131072"),
     (dict(x=FAKE + 8), ValueError, "16-byte"),
     (dict(w=FAKE + 4), ValueError, "16-byte"),
     (dict(x_stride=264), ValueError, "16-byte"),

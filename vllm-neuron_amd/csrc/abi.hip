@@ -840,8 +840,8 @@ int mia_int8_linear(const mia_int8_linear_args *a, mia_stream_t stream) {
   if (a->rows == 0 || a->n == 0) return MIA_OK;
   MIA_REQUIRE(a->x && a->x_scales && a->w && a->w_scales && a->out, MIA_ERR_VALUE,
               "int8_linear: null tensor pointer");
-  MIA_REQUIRE(a->k <= 131072, MIA_ERR_NOT_IMPLEMENTED,
-              "int8_linear: k above 131072 (the 32-bit sums would overflow)");
+  MIA_REQUIRE(a->k < 131072, MIA_ERR_NOT_IMPLEMENTED,
+              "int8_linear: k of 131072 or more (the 32-bit sums could overflow)");
   MIA_REQUIRE(a->k % 16 == 0, MIA_ERR_NOT_IMPLEMENTED, "int8_linear: k must be a multiple of 16");
   // a tile's 256 rows lie within 2^32 bytes
   MIA_REQUIRE(a->x_stride >= 0 && a->x_stride < (1ll << 24) && a->w_stride >= 0 &&

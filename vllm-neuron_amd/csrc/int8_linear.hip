@@ -1,5 +1,36 @@
 // int8_linear.hip — rows quantised to int8 with one scale per token, and their
 // product with int8 weights of one scale per output channel.
+//
+// Mathematics.  y[m, n] = xs[m] ws[n] sum_k xc[m, k] wc[n, k] + b[n], xs = max|x| /
+// 127, xc = rn(127 x / max|x|) (ties to even, the rounding of the exact quotient; of
+// a row with gamma that of fp32 products, so that a code next to a border may be its
+// neighbour).  Of an RMS-normalised row x r gamma, r = 1 / sqrt(mean x^2 + eps), the
+// codes do not depend on r: they are those of x gamma, and r multiplies the scale.  So one
+// pass over the row gives maximum and sum of squares together, and nothing is rounded
+// between norm and code.  The sums are exact in 32-bit integers: 128^2 k < 2^31
+// for k < 131072.  What follows is fp32, rounded to bf16 once.
+//
+// Rows are held in registers between the pass for the maximum and the codes: 2 bytes
+// read and 1 written per value, bound by HBM for many rows (8191 x 8192 with a norm
+// 41-45 us, 4.5-4.9 TB/s; a large copy moves 4.97), by launch and two dependent loads
+// for few (64 x 4096: 4.0 us).  The next row is under way while one is reduced.
+//
+// Products.  The larger a tile, the less is copied to LDS and read from it per
+// product (a CU copies up to 140 KB/us of what lies in L2); but there are 256 CUs to
+// fill.  Hence forms of many tile sizes, chosen by measured costs (kForms), all with
+// v_mfma_i32_32x32x32_i8 but the one that streams the weights for 16 rows or fewer:
+//   256 x 256, waves that take turns: bound by power.  8191 x 8192 x 10240: 565-580 us,
+//     2.4 POP/s, the matrix units busy 69 % of the cycles at a clock that falls to 1.7
+//     GHz; the library's product of two 8192^3 int8 matrices reaches 2.15.
+//   128 x 128, 64 x 128 and 64 x 64, ring of tiles read and copied ahead: 517 x 2880 x
+//     5120 15.3 us (1.0 POP/s), bound by the 200 tiles' 23 steps and the start.
+//   32 x 64, 32 x 32, four groups of waves with a quarter of k each: latency of the copies.
+//     64 x 4096 x 6144 8.0 us, 3.3 TB/s of weights.
+//   16 rows or fewer, operands straight to registers: 4 x 2048 x 2048 3.3 us (launch
+//     and one load); 16 x 4096 x 4096 6.4 us.
+// LDS tiles hold rows of 128 (256 x 256: 64) bytes of k in 16-byte chunks, exchanged
+// within a row so that the 16 rows that a fragment read touches at once lie in all
+// banks (conflicts: 3 % of the LDS cycles).
 #include <algorithm>
 #include <atomic>
 

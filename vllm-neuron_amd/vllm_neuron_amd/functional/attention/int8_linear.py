@@ -52,7 +52,7 @@ def int8_linear(
     """``x_scales * w_scales * (x @ w.T) + bias`` in bf16 ``[..., N]``: the sums
     exact in 32-bit integers, the rest in float32, rounded once.
 
-    ``K`` is a multiple of 16 (at most 131072), the rows of ``x`` and ``w`` are
+    ``K`` is a multiple of 16 (below 131072), the rows of ``x`` and ``w`` are
     contiguous and 16-byte aligned.  A row with scale NaN gives NaN.
     """
     if x.dim() == 2:
