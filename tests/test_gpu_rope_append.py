@@ -121,6 +121,29 @@ def test_quantised_caches(gpu, code, norm, T, hq, hkv, d, rot):
     assert not torch.isnan(quant_kv_read(K, V, ks, vs, slots.to(gpu))[0]).any()
 
 
+@pytest.mark.parametrize("code", [torch.int8, torch.float8_e4m3fn])
+@pytest.mark.parametrize("d", [8, 24, 40, 72, 80, 104, 120, 136, 200, 248])
+def test_normalised_heads_narrower_than_their_lanes(gpu, code, d):
+    """Lanes past the head dim hold zeros, whatever their registers held: they
+    enter the row's maximum.  Behind kernels that leave NaN in registers."""
+    T, hkv, bs = 300, 3, 16
+    x = _rows(T, 1, hkv, d, d)
+    pos, inv, slots = torch.arange(T), _inv(d), torch.arange(T)
+    g = 1 + 0.1 * torch.randn(d, generator=torch.Generator().manual_seed(4))
+    k, v = x[:, 1:1 + hkv], x[:, 1 + hkv:]
+    K = torch.zeros((20, hkv, bs, d), dtype=torch.uint8, device=gpu).view(code)
+    V, ks = K.clone(), torch.zeros((20, hkv, bs), device=gpu)
+    vs = ks.clone()
+    junk = torch.full((256, 1 << 14), math.nan, device=gpu)
+    for _ in range(3):
+        junk = torch.tanh(junk) * junk
+        rope_kv_append(x[:, :1].to(gpu), k.to(gpu), v.to(gpu), pos.to(gpu), inv.to(gpu), slots.to(gpu), K, V, qk_norm=True,
+                       q_gamma=g.to(gpu), k_gamma=g.to(gpu), eps=1e-5, k_scales=ks, v_scales=vs)
+        at = slots.to(gpu)
+        rows = K.view(torch.uint8)[at // bs, :, at % bs].view(code).float()
+        _codes_close(rows, ks[at // bs, :, at % bs], *rotate(rms(k, g, 1e-5), pos, inv, None, "blocks", "half"), code, "k")
+
+
 @pytest.mark.parametrize("factors", [False, True])
 def test_static_fp8_cache(gpu, factors):
     T, hq, hkv, d, bs = 9, 4, 2, 64, 16

@@ -95,8 +95,10 @@ __global__ __launch_bounds__(256) void rope_append_kernel(mia_rope_append_args a
       raw[r] = u32x4_t{x[0], x[1], y[0], y[1]};
     }
   }
-  // the lane's norm weights of Q and K
-  f32x4_t gq[2], gk[2];
+  // the lane's norm weights of Q and K (of lanes past the head dim too: their zeros
+  // stay zeros and enter the row's maximum)
+  const f32x4_t ones = {1.f, 1.f, 1.f, 1.f};
+  f32x4_t gq[2] = {ones, ones}, gk[2] = {ones, ones};
   if (NORM && act) {
     auto four = [&](const void *g, int e) {
       if (!g) return f32x4_t{1.f, 1.f, 1.f, 1.f};
