@@ -276,6 +276,17 @@ def test_calls_on_other_streams_and_in_graphs(gpu):
     assert torch.equal(compiled(x), want)
 
 
+@pytest.mark.parametrize("rows,dim", [((1 << 24) + 3, 7), ((1 << 25) + 5, 8)])
+@pytest.mark.parametrize("norm", [NormType.NO_NORM, RMS])
+def test_more_rows_than_a_grid_holds(gpu, rows, dim, norm):
+    x = torch.randint(-1000, 1000, (rows, dim), device=gpu, dtype=torch.int16).to(torch.bfloat16)
+    g = torch.ones(dim, device=gpu) if norm == RMS else None
+    code, scale = quant_rows(x, norm_type=norm, norm_weights=g)
+    for i in range(0, rows, 1 << 22):
+        c, s = quant_rows(x[i:i + (1 << 22)], norm_type=norm, norm_weights=g)
+        assert torch.equal(code[i:i + (1 << 22)], c) and torch.equal(scale[i:i + (1 << 22)], s)
+
+
 def _exact_product(gpu, m, n, k):
     g = torch.Generator(device=gpu).manual_seed(m)
     x = torch.randint(-127, 128, (m, k), generator=g, device=gpu, dtype=torch.int32).to(torch.int8)

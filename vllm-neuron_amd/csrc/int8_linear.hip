@@ -178,37 +178,40 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(mia_quant_rows_args a) 
   }
 }
 
-// Any width, alignment and length: a workgroup per row, read twice.
+// Any width, alignment and length: a workgroup takes a row at a time, read twice.
 __global__ __launch_bounds__(256) void quant_rows_any_kernel(mia_quant_rows_args a) {
-  __shared__ float2 red[4];
-  const int64_t row = blockIdx.x;
-  const int64_t at = row * a.x_stride;
-  float ss = 0.f;
-  auto value = [&](int c, bool sum) {
-    float x = bf16_bits_to_f32(((const uint16_t *)a.x)[at + c]);
-    if (a.add0) x = add_bf16(x, bf16_bits_to_f32(((const uint16_t *)a.add0)[at + c]));
-    if (a.add1) x = add_bf16(x, bf16_bits_to_f32(((const uint16_t *)a.add1)[at + c]));
-    if (sum) ss = fmaf(x, x, ss);
-    return a.norm && a.gamma ? x * gamma_at(a, c) : x;
-  };
-  uint32_t mag = 0;
-  for (int c = threadIdx.x; c < a.dim; c += 256)
-    mag = max(mag, __float_as_uint(value(c, true)) & 0x7fffffffu);
+  __shared__ float2 red[2][4];
+  int turn = 0;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
+    const int64_t at = row * a.x_stride;
+    float ss = 0.f;
+    auto value = [&](int c, bool sum) {
+      float x = bf16_bits_to_f32(((const uint16_t *)a.x)[at + c]);
+      if (a.add0) x = add_bf16(x, bf16_bits_to_f32(((const uint16_t *)a.add0)[at + c]));
+      if (a.add1) x = add_bf16(x, bf16_bits_to_f32(((const uint16_t *)a.add1)[at + c]));
+      if (sum) ss = fmaf(x, x, ss);
+      return a.norm && a.gamma ? x * gamma_at(a, c) : x;
+    };
+    uint32_t mag = 0;
+    for (int c = threadIdx.x; c < a.dim; c += 256)
+      mag = max(mag, __float_as_uint(value(c, true)) & 0x7fffffffu);
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    mag = max(mag, (uint32_t)__shfl_xor((int)mag, o, 64));
-    ss += __shfl_xor(ss, o, 64);
+    for (int o = 1; o < 64; o <<= 1) {
+      mag = max(mag, (uint32_t)__shfl_xor((int)mag, o, 64));
+      ss += __shfl_xor(ss, o, 64);
+    }
+    float2 *const rd = red[turn];
+    if ((threadIdx.x & 63) == 0) rd[threadIdx.x >> 6] = make_float2(__uint_as_float(mag), ss);
+    __syncthreads();
+    mag = max(max(__float_as_uint(rd[0].x), __float_as_uint(rd[1].x)),
+              max(__float_as_uint(rd[2].x), __float_as_uint(rd[3].x)));
+    ss = (rd[0].y + rd[1].y) + (rd[2].y + rd[3].y);
+    RowCodes<127> rs;
+    rs.set(mag);
+    for (int c = threadIdx.x; c < a.dim; c += 256)
+      ((uint8_t *)a.codes)[row * a.codes_stride + c] = (uint8_t)rs.int8(value(c, false));
+    if (threadIdx.x == 0) a.scales[row] = row_scale(mag, ss, a);
   }
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = make_float2(__uint_as_float(mag), ss);
-  __syncthreads();
-  mag = max(max(__float_as_uint(red[0].x), __float_as_uint(red[1].x)),
-            max(__float_as_uint(red[2].x), __float_as_uint(red[3].x)));
-  ss = (red[0].y + red[1].y) + (red[2].y + red[3].y);
-  RowCodes<127> rs;
-  rs.set(mag);
-  for (int c = threadIdx.x; c < a.dim; c += 256)
-    ((uint8_t *)a.codes)[row * a.codes_stride + c] = (uint8_t)rs.int8(value(c, false));
-  if (threadIdx.x == 0) a.scales[row] = row_scale(mag, ss, a);
 }
 
 // ---------------------------------------------------------------------------
@@ -867,13 +870,15 @@ const Form kForms[] = {
     {16, 16, 1, 16, 1.7f, 0.9f, 0.077f, launch_stream},
 };
 
+constexpr int64_t kMostGroups = 1 << 23;  // a grid's threads stay below 2^32
+
 template <int LANES, int NV, bool NORM>
 void launch_rows_form(const mia_quant_rows_args &a, hipStream_t s) {
   constexpr int RPB = 256 / LANES;
   const int64_t groups = (a.rows + RPB - 1) / RPB;
   // with gamma in registers as many workgroups as are resident at once
   constexpr int RESIDENT = NV == 1 ? 8 : NV == 2 ? 6 : NV == 4 ? 4 : 2;
-  const int64_t most = NORM ? (int64_t)cu_count() * RESIDENT : groups;
+  const int64_t most = NORM ? (int64_t)cu_count() * RESIDENT : kMostGroups;
   quant_rows_kernel<LANES, NV, NORM><<<(unsigned)std::min(groups, most), 256, 0, s>>>(a);
 }
 
@@ -894,7 +899,7 @@ int launch_quant_rows(const mia_quant_rows_args &a, hipStream_t s) {
   const bool vec = a.dim % 8 == 0 && a.dim <= 16384 && a.x_stride % 8 == 0 &&
                    a.codes_stride % 8 == 0 && ok(a.x, 16) && ok(a.add0, 16) && ok(a.add1, 16) &&
                    ok(a.gamma, 16) && ok(a.codes, 8);
-  if (!vec) quant_rows_any_kernel<<<(unsigned)a.rows, 256, 0, s>>>(a);
+  if (!vec) quant_rows_any_kernel<<<(unsigned)std::min(a.rows, kMostGroups), 256, 0, s>>>(a);
   else if (a.norm) launch_rows<true>(a, s);
   else launch_rows<false>(a, s);
   return check_hip(hipGetLastError(), "quant_rows");
