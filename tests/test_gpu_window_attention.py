@@ -165,6 +165,14 @@ def test_long_windows_of_one_token(gpu, cache, Hq, d, window):
     Call(gpu, [1, 1], [window + 300, window - 100], Hq, 1, d, 32, window, 4, cache, sink=True).check()
 
 
+def test_many_prompts_without_a_bound(gpu):
+    """max_seqlen_q is all tokens where it is not given: most workgroups have no
+    rows."""
+    new = [1 + 7 * i % 41 for i in range(300)]
+    c = Call(gpu, new, [n + 11 * i % 50 for i, n in enumerate(new)], 64, 8, 64, 16, 20, 3)
+    c.check(max_seqlen_q=None)
+
+
 def test_token_per_sequence_without_a_list(gpu):
     c = Call(gpu, [1] * 6, [1, 5, 64, 80, 200, 0], 8, 2, 64, 16, 48, 2)
     a = c.run()

@@ -103,7 +103,7 @@ def test_rope_refusals(over, err, text):
     (dict(block_size=24), NotImplementedError, "block_size"),
     (dict(k_cache=FAKE + 8), ValueError, "16-byte"),
     (dict(q=FAKE + 2), ValueError, "q rows"),
-    (dict(num_tokens=1 << 20, num_seqs=1 << 12, max_seqlen_q=1 << 20), ValueError, "2\\^19"),
+    (dict(num_tokens=1 << 20, num_seqs=1 << 12, max_seqlen_q=1 << 20), ValueError, "2\\^23"),
     (dict(num_seqs=1, num_tokens=1, max_seqlen_q=1, num_q_heads=4, num_kv_heads=1, blocks_per_seq=1000,
           window=1 << 20), ValueError, "workspace"),
 ])

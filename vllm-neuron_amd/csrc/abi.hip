@@ -949,12 +949,14 @@ static int validate_window(const mia_window_args *a) {
   const int extents[2] = {a->num_tokens, a->num_q_heads};
   const int rc = check_span(*a, a->q_stride, a->out_stride, extents, 2, a->num_tokens, true);
   if (rc) return rc;
-  // the row tiles of all sequences lie along one grid axis, 32 pieces at most
+  // the row tiles of all sequences lie along one grid axis, 256 threads each below
+  // 2^32 (those that are cut or have 512 threads are far fewer)
   const int64_t G = a->num_q_heads / a->num_kv_heads;
   const int64_t most = a->cu_seqlens_q && a->max_seqlen_q < a->num_tokens ? a->max_seqlen_q
                        : a->cu_seqlens_q ? a->num_tokens : 1;
-  MIA_REQUIRE((most * G / 128 + 1) * a->num_seqs < (1ll << 19) / a->num_kv_heads, MIA_ERR_VALUE,
-              "window_attention: row tiles * sequences * kv heads beyond 2^19");
+  MIA_REQUIRE((most * G / 128 + 1) * a->num_seqs < (1ll << 23) / a->num_kv_heads, MIA_ERR_VALUE,
+              "window_attention: row tiles * sequences * kv heads beyond 2^23 (max_seqlen_q "
+              "too large)");
   return MIA_OK;
 }
 

@@ -47,7 +47,8 @@ def window_attention(
 
     Lengths are read on the device (a captured call follows them) and clamped to
     what the table holds; ``max_seqlen_q`` bounds the query tokens of a sequence
-    (default: T), those past it are not computed; ``cu_seqlens_q`` must not
+    (default: T, at the cost of a workgroup for every row tile that a sequence of
+    T tokens would have), those past it are not computed; ``cu_seqlens_q`` must not
     decrease.  A query without keys gives zeros.  Rows that nothing computes stay
     as they were in a given ``out`` and are zeros in the returned tensor
     otherwise.  A NaN or infinity in a value row reaches the queries that see it,
