@@ -28,7 +28,7 @@
 //     64 x 4096 x 6144 8.0 us, 3.3 TB/s of weights.
 //   16 rows or fewer, operands straight to registers: 4 x 2048 x 2048 3.3 us (launch
 //     and one load); 16 x 4096 x 4096 6.4 us.
-// LDS tiles hold rows of 128 (256 x 256: 64) bytes of k in 16-byte chunks, exchanged
+// LDS tiles hold rows of 128 (256 x 256: 64, 64 x 64: 256) bytes of k in 16-byte chunks, exchanged
 // within a row so that the 16 rows that a fragment read touches at once lie in all
 // banks (conflicts: 3 % of the LDS cycles).
 #include <algorithm>
@@ -482,22 +482,24 @@ __global__ __launch_bounds__(WN *WM *KS * 64) void gemm_kernel(GemmParams p) {
 }
 
 // WN x WM x KG waves, each TN x TM products of 32 x 32 over its KG-th part of a
-// tile's k.  One ring of tiles for the worgrouproup; a wave reads its fragments of
+// tile's k.  One ring of tiles for the workgroup; a wave reads its fragments of
 // tile t + 1 and copies its part of tile t + STAGES - 1 between the products of
 // tile t, so that neither LDS, nor the copies' issue, nor the barrier stands between
 // two products.  A CU alone takes 0.34 us per 128 x 128 x 128 so (0.21 at the matrix
 // units' rate), where rings whose waves copy, read and then multiply take 0.48 with
 // eight waves and 0.57 with four: waiting for memory was none of it (the same with
-// every byte in L2 and with 2 to 5 stages).
-template <int WN, int WM, int TN, int TM, int STAGES, int KG>
+// every byte in L2 and with 2 to 5 stages).  Tiles of 64 x 64 take 256 bytes of k at
+// a time, half the barriers: 200 x 4096 x 4096 9.4 against 10.7 us.
+template <int WN, int WM, int TN, int TM, int STAGES, int KG, int BK>
 __global__ __launch_bounds__(WN *WM *KG * 64) void gemm_pipe_kernel(GemmParams p) {
   constexpr int WAVES = WN * WM * KG, THREADS = WAVES * 64;
-  constexpr int NS = kBK / 32 / KG;  // fragments of a tile that a wave reads
+  constexpr int NS = BK / 32 / KG;  // fragments of a tile that a wave reads
   constexpr int BN = WN * TN * 32, BM = WM * TM * 32;
-  constexpr int NC = BN / 8 / WAVES, MC = BM / 8 / WAVES;  // copies per wave and tile
-  static_assert(BN % (8 * WAVES) == 0 && BM % (8 * WAVES) == 0, "whole copies");
+  constexpr int CPR = BK / 16, RPC = 64 / CPR;  // chunks per row, rows per copy
+  constexpr int NC = BN / RPC / WAVES, MC = BM / RPC / WAVES;  // copies per wave and tile
+  static_assert(BN % (RPC * WAVES) == 0 && BM % (RPC * WAVES) == 0, "whole copies");
   static_assert(NS >= 2 && STAGES >= 3, "read and copied ahead");
-  constexpr int STAGE = (BN + BM) * kBK;
+  constexpr int STAGE = (BN + BM) * BK;
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   const int tid = threadIdx.x;
   const int wave = readfirstlane(tid >> 6);
@@ -512,52 +514,57 @@ __global__ __launch_bounds__(WN *WM *KG * 64) void gemm_pipe_kernel(GemmParams p
   const uint8_t *wsrc = p.w + (int64_t)n0 * p.w_ld;
   const uint8_t *xsrc = p.x + (int64_t)m0 * p.x_ld;
   uint32_t won[NC], xom[MC];
-  const int chunk_e = (lane & 7) ^ (lane >> 4);  // even row groups; odd ones: ^ 4
+  // chunk c of a row lies in slot c ^ swz(row): reads of 16 rows at one chunk touch
+  // all banks
+  auto swz = [](int row) { return BK == 128 ? (row >> 1) & 7 : row & 15; };
+  // row and chunk of the lane in copy g of an operand
+  const int crow = lane / CPR;
+  auto chunk = [&](int g) { return (lane % CPR) ^ swz(g * RPC + crow); };
 #pragma unroll
   for (int j = 0; j < NC; ++j) {
-    const int g = wave * NC + j, row = g * 8 + (lane >> 3);
-    won[j] = (uint32_t)min(row, p.n - 1 - n0) * (uint32_t)p.w_ld + (chunk_e ^ ((g & 1) * 4)) * 16;
+    const int g = wave * NC + j;
+    won[j] = (uint32_t)min(g * RPC + crow, p.n - 1 - n0) * (uint32_t)p.w_ld + chunk(g) * 16;
   }
 #pragma unroll
   for (int j = 0; j < MC; ++j) {
-    const int g = wave * MC + j, row = g * 8 + (lane >> 3);
-    xom[j] = (uint32_t)min(row, p.m - 1 - m0) * (uint32_t)p.x_ld + (chunk_e ^ ((g & 1) * 4)) * 16;
+    const int g = wave * MC + j;
+    xom[j] = (uint32_t)min(g * RPC + crow, p.m - 1 - m0) * (uint32_t)p.x_ld + chunk(g) * 16;
   }
-  const int steps = (p.k + kBK - 1) / kBK, full = p.k / kBK;
+  const int steps = (p.k + BK - 1) / BK, full = p.k / BK;
   // copy j of tile t, to the stage at dst
   auto copy = [&](int t, uint32_t dst, int j) {
     if (j < NC)
-      copy1(wsrc + t * kBK, won[j], lds0 + dst + (wave * NC + j) * 1024);
+      copy1(wsrc + t * BK, won[j], lds0 + dst + (wave * NC + j) * 1024);
     else
-      copy1(xsrc + t * kBK, xom[j - NC], lds0 + dst + BN * kBK + (wave * MC + j - NC) * 1024);
+      copy1(xsrc + t * BK, xom[j - NC], lds0 + dst + BN * BK + (wave * MC + j - NC) * 1024);
   };
   // the last tile where k ends inside it: chunks past k are zeros for x, so that
   // they count nothing whatever w's hold there
   auto load_part = [&](int t, uint32_t dst) {
-    const int k0 = t * kBK;
+    const int k0 = t * BK;
 #pragma unroll
     for (int j = 0; j < NC + MC; ++j) {
       const int g = j < NC ? wave * NC + j : wave * MC + j - NC;
-      if (k0 + (chunk_e ^ ((g & 1) * 4)) * 16 < p.k)
+      if (k0 + chunk(g) * 16 < p.k)
         copy(t, dst, j);
       else if (j >= NC)
-        *(lds_u32x4_t *)(lds + dst + BN * kBK + g * 1024 + lane * 16) = u32x4_t{0u, 0u, 0u, 0u};
+        *(lds_u32x4_t *)(lds + dst + BN * BK + g * 1024 + lane * 16) = u32x4_t{0u, 0u, 0u, 0u};
     }
   };
 
   i32x16_t acc[TN][TM] = {};
-  const int swz = (rl >> 1) & 7;  // (rows of a fragment start at multiples of 32)
-  const lds_u8_t *const wrow = lds + (wn * TN * 32 + rl) * kBK;
-  const lds_u8_t *const xrow = lds + BN * kBK + (wm * TM * 32 + rl) * kBK;
+  const int mine = swz(rl);  // (rows of a fragment start at multiples of 32)
+  const lds_u8_t *const wrow = lds + (wn * TN * 32 + rl) * BK;
+  const lds_u8_t *const xrow = lds + BN * BK + (wm * TM * 32 + rl) * BK;
   i32x4_t wf[NS][TN], xf[NS][TM];
   auto read = [&](uint32_t st, int s) {
-    const uint32_t c = (uint32_t)(((2 * (group * NS + s) + half) ^ swz) << 4) + st;
+    const uint32_t c = (uint32_t)(((2 * (group * NS + s) + half) ^ mine) << 4) + st;
 #pragma unroll
     for (int i = 0; i < TN; ++i)
-      wf[s][i] = __builtin_bit_cast(i32x4_t, *(const lds_u32x4_t *)(wrow + c + i * 32 * kBK));
+      wf[s][i] = __builtin_bit_cast(i32x4_t, *(const lds_u32x4_t *)(wrow + c + i * 32 * BK));
 #pragma unroll
     for (int i = 0; i < TM; ++i)
-      xf[s][i] = __builtin_bit_cast(i32x4_t, *(const lds_u32x4_t *)(xrow + c + i * 32 * kBK));
+      xf[s][i] = __builtin_bit_cast(i32x4_t, *(const lds_u32x4_t *)(xrow + c + i * 32 * BK));
   };
   auto multiply = [&](int s) {  // (in its place: reads before it, copies after it)
     __builtin_amdgcn_sched_barrier(0);
@@ -821,15 +828,15 @@ int launch_gemm(GemmParams &p, hipStream_t s) {
   return launch_tiles<gemm_kernel<WN, WM, TN, TM, STAGES, KS>>(p, WN * WM * KS * 64, bytes, s);
 }
 
-template <int WN, int WM, int TN, int TM, int STAGES, int KG>
+template <int WN, int WM, int TN, int TM, int STAGES, int KG, int BK>
 int launch_pipe(GemmParams &p, hipStream_t s) {
   constexpr int BN = WN * TN * 32, BM = WM * TM * 32;
   p.nt = (p.n + BN - 1) / BN;
   p.mt = (p.m + BM - 1) / BM;
-  constexpr int bytes = (BN + BM) * kBK * STAGES;
+  constexpr int bytes = (BN + BM) * BK * STAGES;
   static_assert(bytes >= BN * 8 + WN * WM * KG * 32 * (TN * 64 + 16), "epilogue fits");
   static_assert(bytes >= join_bytes(KG, WN * WM, TN * TM), "sums fit");
-  return launch_tiles<gemm_pipe_kernel<WN, WM, TN, TM, STAGES, KG>>(p, WN * WM * KG * 64, bytes, s);
+  return launch_tiles<gemm_pipe_kernel<WN, WM, TN, TM, STAGES, KG, BK>>(p, WN * WM * KG * 64, bytes, s);
 }
 
 int launch_turns(GemmParams &p, hipStream_t s) {
@@ -847,27 +854,28 @@ int launch_stream(GemmParams &p, hipStream_t s) {
 // call, once + rounds (round + step k / 128) us, where a round is a tile on
 // every CU.  The constants are least squares over measurements at 1 to 8191 rows
 // of k = 256 to 14336 and 512 to 10240 columns (weights rotated through 256 MB);
-// the form chosen by them took 0.3 % longer than the fastest one on the
-// geometric mean, 16 % at most (8191 x 2880 x 5120: 150 against 129 us).  Examples,
+// the form chosen by them took 0.6 % longer than the fastest one on the
+// geometric mean, 20 % at most (8191 x 2880 x 5120: 150 against 126 us).  Examples,
 // us, by form in the table's order:
-//   64 x 4096 x 6144, from the third on: 15.2, 12.1, 10.2, 12.1, 8.1
-//   517 x 2880 x 5120, from the first on: 34.3, 19.3, 15.3, 22.7, 24.2, 53.4, 38.9
-//   8191 x 8192 x 10240, the first two: 682, 803
-//   4 x 2048 x 2048, from the third on: 8.9, 7.5, 6.5, 4.7, 5.1, 3.3
+//   64 x 4096 x 6144, from the third on: 15.4, 12.1, 9.4, 11.9, 7.9
+//   200 x 4096 x 4096, from the first on: 37.8, 22.6, 15.7, 12.5, 9.6, 21.7, 13.7
+//   517 x 2880 x 5120: 34.1, 18.6, 15.2, 22.5, 24.1, 53.2, 38.4
+//   8191 x 8192 x 10240, the first two: 667.9, 782.8
+//   4 x 2048 x 2048, from the third on: 9.1, 7.4, 6.0, 4.8, 5.2, 3.6
 struct Form {
   int bm, bn, per_cu, rows;  // rows: at most (0: any number)
   float once, round, step;
   int (*launch)(GemmParams &, hipStream_t);
 };
 const Form kForms[] = {
-    {256, 256, 1, 0, -12.9f, 20.0f, 1.158f, launch_turns},
-    {128, 128, 2, 0, -5.9f, 9.7f, 0.698f, launch_gemm<2, 2, 2, 2, 2, 1>},
-    {128, 128, 1, 0, -2.7f, 6.4f, 0.394f, launch_pipe<2, 4, 2, 1, 4, 1>},
-    {64, 128, 1, 0, -0.6f, 3.8f, 0.303f, launch_pipe<4, 2, 1, 1, 5, 1>},
-    {64, 64, 1, 0, 0.6f, 2.7f, 0.224f, launch_pipe<2, 2, 1, 1, 6, 2>},
-    {32, 32, 1, 0, 1.3f, 1.8f, 0.115f, launch_gemm<1, 1, 1, 1, 3, 4>},
-    {32, 64, 1, 0, 0.8f, 2.4f, 0.142f, launch_gemm<2, 1, 1, 1, 3, 4>},
-    {16, 16, 1, 16, 1.7f, 0.9f, 0.077f, launch_stream},
+    {256, 256, 1, 0, -12.7f, 19.8f, 1.166f, launch_turns},
+    {128, 128, 2, 0, -6.2f, 9.9f, 0.698f, launch_gemm<2, 2, 2, 2, 2, 1>},
+    {128, 128, 1, 0, -2.1f, 5.8f, 0.401f, launch_pipe<2, 4, 2, 1, 4, 1, 128>},
+    {64, 128, 1, 0, -0.3f, 3.6f, 0.301f, launch_pipe<4, 2, 1, 1, 5, 1, 128>},
+    {64, 64, 1, 0, 0.6f, 2.8f, 0.183f, launch_pipe<2, 2, 1, 1, 5, 2, 256>},
+    {32, 32, 1, 0, 1.3f, 1.8f, 0.114f, launch_gemm<1, 1, 1, 1, 3, 4>},
+    {32, 64, 1, 0, 0.8f, 2.4f, 0.140f, launch_gemm<2, 1, 1, 1, 3, 4>},
+    {16, 16, 1, 16, 1.7f, 0.9f, 0.078f, launch_stream},
 };
 
 constexpr int64_t kMostGroups = 1 << 23;  // a grid's threads stay below 2^32
