@@ -1264,7 +1264,9 @@ def quant_rows(x, norm, eps, gamma=None, add0=None, add1=None, dim_actual=0):
         adds = [t.contiguous() for t in adds]
         stride = x2.stride()
     rows = x2.shape[0]
-    codes = x2.new_empty((rows, dim), dtype=torch.int8)
+    # (the cheaper call where it gives whole rows)
+    codes = (torch.empty_like(x2, dtype=torch.int8) if stride[0] == dim
+             else x2.new_empty((rows, dim), dtype=torch.int8))
     scales = x2.new_empty((rows,), dtype=torch.float32)
     a = N.QuantRowsArgs()
     N.PACK_QUANT_ROWS.pack_into(

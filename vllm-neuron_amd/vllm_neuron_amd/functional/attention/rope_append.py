@@ -69,7 +69,7 @@ def rope_kv_append(
     """
     cycle, interleaved = _options(section_order, pairs)
     if q_out is None:
-        q_out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+        q_out = q.new_empty(q.shape, dtype=torch.bfloat16)
     K.rope_append(q, k, v, positions, inv_freq, slots, k_cache, v_cache, q_out, k_out,
                   sections=sections, cycle=cycle, interleaved=interleaved,
                   rope_scale=rope_scale, qk_norm=qk_norm, q_gamma=q_gamma, k_gamma=k_gamma,

@@ -806,8 +806,8 @@ def window_attention(q, k_cache, v_cache, block_table, seq_lens, *, window: int,
     # those of no sequence (without any sequence there is no launch)
     rest = out is None
     if rest:
-        new = torch.empty if seq_lens.numel() else torch.zeros
-        out = new(q.shape, dtype=torch.bfloat16, device=q.device)
+        new = q.new_empty if seq_lens.numel() else q.new_zeros
+        out = new(q.shape, dtype=torch.bfloat16)
     if _plain(q, k_cache, v_cache, block_table, seq_lens, out, cu_seqlens_q, sink, k_scales,
               v_scales, k_dequant, v_dequant, workspace):
         K.window_attention(q, k_cache, v_cache, block_table, seq_lens, out, window=int(window),
