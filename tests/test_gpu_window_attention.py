@@ -234,6 +234,17 @@ def test_strides(gpu):
     assert torch.equal(got, want) and got.data_ptr() == out.data_ptr()
 
 
+@pytest.mark.parametrize("cache", ["bf16", "int8"])
+@pytest.mark.parametrize("d", [16, 64, 80, 96, 128])
+def test_outputs_that_start_at_eight_bytes(gpu, d, cache):
+    c = Call(gpu, [1, 70, 130], [50, 170, 131], 6, 2, d, 16, 40, 5, cache, poison=False)
+    want = c.check()
+    room = torch.full((c.q.shape[0], 6, d + 12), 3.0, dtype=BF, device=gpu)
+    out = room[..., 4:4 + d]
+    c.run(out=out)
+    assert torch.equal(out, want) and (room[..., :4] == 3.0).all() and (room[..., 4 + d:] == 3.0).all()
+
+
 def test_scales_and_signs(gpu):
     c = Call(gpu, [1, 90], [70, 130], 4, 2, 64, 16, 50, 3, "fp8s")
     for s in (-0.3, 0.0, 2.0):

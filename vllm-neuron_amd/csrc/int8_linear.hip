@@ -41,7 +41,6 @@ namespace {
 
 typedef int i32x4_t __attribute__((ext_vector_type(4)));
 typedef int i32x16_t __attribute__((ext_vector_type(16)));
-typedef __attribute__((address_space(3))) u32x2_t lds_u32x2_t;
 typedef __attribute__((address_space(3))) uint16_t lds_u16_t;
 
 // ---------------------------------------------------------------------------

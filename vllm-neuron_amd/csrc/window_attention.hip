@@ -20,7 +20,7 @@
 //         cycles each, the clock at 1.8 GHz.  Eight waves in two groups, one in its
 //         products while the other is in its softmax, took 294; the next tile's scores between
 //         this one's exponentials 345; fragments read 4 or 6 ahead instead of 2 the same.
-//         Short windows: 2183 tokens of 64 heads, d = 64, window 128: 24 us, two
+//         Short windows: 2183 tokens of 64 heads, d = 64, window 128: 23.4 us, two
 //         thirds of it start, loads' latency and stores.
 //   thin  16 or 32 rows: each wave streams 32-key tiles of its own, K straight to
 //         operands, V through LDS (v_mfma_f32_16x16x32_bf16).  Probabilities go in two
@@ -620,22 +620,39 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void window_tall_kernel(
 
   // ---- final rows, or a partial
   const float l = sum32(l_run);
-  if (!ok) return;
   if (p.split == 1) {
-    uint16_t *op = p.out + (int64_t)(tl.tok0 + j) * p.os_t + (int64_t)hq * p.os_h;
-    const float f = row_factor(p, wk.h, hq, m_run, l);
+    // Through LDS, so that rows are stored in whole lines: a lane's own channels
+    // come in pieces of 8 bytes, 16 of a row at a time, and L2 takes a request for
+    // each (2183 tokens of 64 heads, d = 64, window 128: 24.8 against 23.4 us; 8191 of
+    // 32 heads, d = 128: 73 against 67).
+    const float f = ok ? row_factor(p, wk.h, hq, m_run, l) : 0.f;
+    constexpr int PITCH = ROWB + 16, CPR = DU / 8, RPS = 64 / CPR;  // chunks of a row, rows a store
+    static_assert(kWaves * 32 * PITCH <= 4 * TILEB, "the rows fit");
+    __syncthreads();  // (the last tile has been read)
+    lds_u8_t *const rows = base + wave * 32 * PITCH;
 #pragma unroll
     for (int i = 0; i < DBLK; ++i)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int d0 = i * 32 + g * 8 + half * 4;
-        if (d0 < p.d)
-          *reinterpret_cast<u32x2_t *>(op + d0) =
-              u32x2_t{pack2_bf16(acc[i][g * 4] * f, acc[i][g * 4 + 1] * f),
-                      pack2_bf16(acc[i][g * 4 + 2] * f, acc[i][g * 4 + 3] * f)};
-      }
+      for (int g = 0; g < 4; ++g)
+        *(lds_u32x2_t *)(rows + rl * PITCH + (i * 32 + g * 8 + half * 4) * 2) =
+            u32x2_t{pack2_bf16(acc[i][g * 4] * f, acc[i][g * 4 + 1] * f),
+                    pack2_bf16(acc[i][g * 4 + 2] * f, acc[i][g * 4 + 3] * f)};
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+    typedef u32x4_t __attribute__((aligned(8))) u32x4_a8;  // (rows of out start at 8 bytes)
+    const int c = lane % CPR;
+    for (int y = lane / CPR; y < 32; y += RPS) {
+      const int ro = r0 + wave * 32 + y;
+      if (ro >= tl.rows) break;
+      const int jo = (int)fdiv((uint32_t)ro, p.g_div);
+      uint16_t *op = p.out + (int64_t)(tl.tok0 + jo) * p.os_t +
+                     (int64_t)(wk.h * p.G + ro - jo * p.G) * p.os_h + c * 8;
+      const u32x4_t v = *(const lds_u32x4_t *)(rows + y * PITCH + c * 16);
+      if (lane < CPR * RPS && c * 8 < p.d) *reinterpret_cast<u32x4_a8 *>(op) = v;
+    }
     return;
   }
+  if (!ok) return;
   const int64_t pr = wk.piece * p.part_rows + rloc;
   float *po = p.part_o + pr * D;
 #pragma unroll
