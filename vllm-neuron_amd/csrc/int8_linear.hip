@@ -19,8 +19,8 @@
 // product (a CU copies up to 140 KB/us of what lies in L2); but there are 256 CUs to
 // fill.  Hence forms of many tile sizes, chosen by measured costs (kForms), all with
 // v_mfma_i32_32x32x32_i8 but the one that streams the weights for 16 rows or fewer:
-//   256 x 256, waves that take turns: bound by power.  8191 x 8192 x 10240: 565-580 us,
-//     2.4 POP/s, the matrix units busy 69 % of the cycles at a clock that falls to 1.7
+//   256 x 256, waves that take turns: bound by power.  8191 x 8192 x 10240: 565-595 us by card,
+//     2.3-2.4 POP/s, the matrix units busy 70 % of the cycles at a clock that falls to 1.7
 //     GHz; the library's product of two 8192^3 int8 matrices reaches 2.15.
 //   128 x 128, 64 x 128 and 64 x 64, ring of tiles read and copied ahead: 517 x 2880 x
 //     5120 15.3 us (1.0 POP/s), bound by the 200 tiles' 23 steps and the start.
