@@ -13,7 +13,7 @@
 // takes no exchange, and a head row lies in 8, 16 or 32 lanes, which reduce norm and
 // maximum among themselves.  Bound by HBM: every value is read and written once.
 // 16383 tokens of 32 + 8 + 8 heads, d = 128, 75 us (403 MB, 5.4 TB/s; a large copy moves
-// 4.97); 2047 tokens of 48 + 8 + 8 heads with norms 17.4 us (67 MB, 3.9 TB/s: 2047
+// 4.97); 2047 tokens of 48 + 8 + 8 heads with norms 16.2 us (67 MB, 4.1 TB/s: 2047
 // workgroups' start); a decode step's 8 tokens to an int8 cache 4.5 us, launch
 // and the chain position, angle, row.
 #include <algorithm>
@@ -60,8 +60,10 @@ constexpr int kMaxRows = 4;  // head rows per lane group at most
 
 // Workgroup (token t, head range): L lanes of 8 channels per head row (head
 // dim <= 8 L); the G lane groups take rows g, g + G, ....
+// Eight waves per SIMD (64 registers): 2047 tokens of 64 heads with norms 16.2 us, 17.4
+// with the seven that 68 leave; quantised rows with norms would spill.
 template <int L, int KIND, bool NORM>
-__global__ __launch_bounds__(256) void rope_append_kernel(mia_rope_append_args a, int rows) {
+__global__ __launch_bounds__(256, KIND <= kBf16 || !NORM ? 8 : 6) void rope_append_kernel(mia_rope_append_args a, int rows) {
   constexpr int G = 256 / L;
   __shared__ __attribute__((aligned(16))) float cs[2][8 * L / 2];
   const int64_t t = blockIdx.x;
@@ -256,8 +258,8 @@ void launch_lanes(const mia_rope_append_args &a, int kind, hipStream_t s) {
   const int sets = (heads + G - 1) / G;  // rows per group in one workgroup per token
   // Few tokens need workgroups, many of them fewer repeated angles and loads in
   // flight: rows of 1 / 2 / 3 / 4 per group, 64 heads of d = 128 with norms, 100
-  // tokens 4.4 / 4.4 / 4.5 / 4.5 us, 512 8.9 / 7.6 / 7.6 / 8.4, 2047 22 / 18.3 / 18.2
-  // / 18.0; 48 heads, 16383 tokens 106 / 93 / 79 / 79.
+  // tokens 4.4 / 4.8 / 4.8 / 6.0 us, 512 7.7 / 7.6 / 7.7 / 8.1, 2047 20.3 / 17.8 / 17.5
+  // / 16.4; 48 heads, 16383 tokens 98 / 91 / 78 / 76.
   const int most = a.num_tokens < 256 ? 1 : a.num_tokens < 1024 ? 2 : kMaxRows;
   const int parts = (sets + most - 1) / most;
   const int rows = (sets + parts - 1) / parts;
