@@ -312,7 +312,7 @@ def test_products_whatever_form_is_taken(gpu, m, n, k):
 
 @pytest.mark.parametrize("k", [16, 112, 128, 144, 240, 256, 272, 384, 400, 512, 528, 640, 656, 768, 784, 1024, 1040, 1264,
                                1280, 1296, 1536, 1552])
-@pytest.mark.parametrize("m,n", [(129, 12000), (129, 4100), (70, 9000), (300, 12000), (5, 4100)])
+@pytest.mark.parametrize("m,n", [(129, 12000), (129, 4100), (70, 9000), (300, 12000), (400, 10200), (500, 10200), (5, 4100)])
 def test_few_tiles_of_k(gpu, m, n, k):
     """Fewer tiles along k than a ring holds, as many, and more, whole and not."""
     _exact_product(gpu, m, n, k)

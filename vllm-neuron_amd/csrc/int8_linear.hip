@@ -22,7 +22,7 @@
 //   256 x 256, waves that take turns: bound by power.  8191 x 8192 x 10240: 565-595 us by card,
 //     2.3-2.4 POP/s, the matrix units busy 70 % of the cycles at a clock that falls to 1.7
 //     GHz; the library's product of two 8192^3 int8 matrices reaches 2.15.
-//   128 x 128, 64 x 128 and 64 x 64, ring of tiles read and copied ahead: 517 x 2880 x
+//   192, 160, 128 and 64 x 128, 64 x 64, ring of tiles read and copied ahead: 517 x 2880 x
 //     5120 15.3 us (1.0 POP/s), bound by the 200 tiles' 23 steps and the start.
 //   32 x 64, 32 x 32, four groups of waves with a quarter of k each: latency of the copies.
 //     64 x 4096 x 6144 8.0 us, 3.3 TB/s of weights.
@@ -495,8 +495,11 @@ __global__ __launch_bounds__(WN *WM *KG * 64) void gemm_pipe_kernel(GemmParams p
   constexpr int NS = BK / 32 / KG;  // fragments of a tile that a wave reads
   constexpr int BN = WN * TN * 32, BM = WM * TM * 32;
   constexpr int CPR = BK / 16, RPC = 64 / CPR;  // chunks per row, rows per copy
-  constexpr int NC = BN / RPC / WAVES, MC = BM / RPC / WAVES;  // copies per wave and tile
-  static_assert(BN % (RPC * WAVES) == 0 && BM % (RPC * WAVES) == 0, "whole copies");
+  // copies of a tile and per wave; where they are no multiple of the waves, the last
+  // ones are made again (the same bytes to the same place)
+  constexpr int CN = BN / RPC, CM = BM / RPC;
+  constexpr int NC = (CN + WAVES - 1) / WAVES, MC = (CM + WAVES - 1) / WAVES;
+  static_assert(BN % RPC == 0 && BM % RPC == 0, "whole copies");
   static_assert(NS >= 2 && STAGES >= 3, "read and copied ahead");
   constexpr int STAGE = (BN + BM) * BK;
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
@@ -519,23 +522,27 @@ __global__ __launch_bounds__(WN *WM *KG * 64) void gemm_pipe_kernel(GemmParams p
   // row and chunk of the lane in copy g of an operand
   const int crow = lane / CPR;
   auto chunk = [&](int g) { return (lane % CPR) ^ swz(g * RPC + crow); };
+  auto nth = [&](int j) {  // the wave's copy j: its number in W (X)
+    if (j < NC) return CN % WAVES ? min(wave * NC + j, CN - 1) : wave * NC + j;
+    return CM % WAVES ? min(wave * MC + j - NC, CM - 1) : wave * MC + j - NC;
+  };
 #pragma unroll
   for (int j = 0; j < NC; ++j) {
-    const int g = wave * NC + j;
+    const int g = nth(j);
     won[j] = (uint32_t)min(g * RPC + crow, p.n - 1 - n0) * (uint32_t)p.w_ld + chunk(g) * 16;
   }
 #pragma unroll
   for (int j = 0; j < MC; ++j) {
-    const int g = wave * MC + j;
+    const int g = nth(NC + j);
     xom[j] = (uint32_t)min(g * RPC + crow, p.m - 1 - m0) * (uint32_t)p.x_ld + chunk(g) * 16;
   }
   const int steps = (p.k + BK - 1) / BK, full = p.k / BK;
   // copy j of tile t, to the stage at dst
   auto copy = [&](int t, uint32_t dst, int j) {
     if (j < NC)
-      copy1(wsrc + t * BK, won[j], lds0 + dst + (wave * NC + j) * 1024);
+      copy1(wsrc + t * BK, won[j], lds0 + dst + nth(j) * 1024);
     else
-      copy1(xsrc + t * BK, xom[j - NC], lds0 + dst + BN * BK + (wave * MC + j - NC) * 1024);
+      copy1(xsrc + t * BK, xom[j - NC], lds0 + dst + BN * BK + nth(j) * 1024);
   };
   // the last tile where k ends inside it: chunks past k are zeros for x, so that
   // they count nothing whatever w's hold there
@@ -543,7 +550,7 @@ __global__ __launch_bounds__(WN *WM *KG * 64) void gemm_pipe_kernel(GemmParams p
     const int k0 = t * BK;
 #pragma unroll
     for (int j = 0; j < NC + MC; ++j) {
-      const int g = j < NC ? wave * NC + j : wave * MC + j - NC;
+      const int g = nth(j);
       if (k0 + chunk(g) * 16 < p.k)
         copy(t, dst, j);
       else if (j >= NC)
@@ -853,28 +860,33 @@ int launch_stream(GemmParams &p, hipStream_t s) {
 // call, once + rounds (round + step k / 128) us, where a round is a tile on
 // every CU.  The constants are least squares over measurements at 1 to 8191 rows
 // of k = 256 to 14336 and 512 to 10240 columns (weights rotated through 256 MB);
-// the form chosen by them took 0.6 % longer than the fastest one on the
-// geometric mean, 20 % at most (8191 x 2880 x 5120: 150 against 126 us).  Examples,
-// us, by form in the table's order:
-//   64 x 4096 x 6144, from the third on: 15.4, 12.1, 9.4, 11.9, 7.9
-//   200 x 4096 x 4096, from the first on: 37.8, 22.6, 15.7, 12.5, 9.6, 21.7, 13.7
-//   517 x 2880 x 5120: 34.1, 18.6, 15.2, 22.5, 24.1, 53.2, 38.4
-//   8191 x 8192 x 10240, the first two: 667.9, 782.8
-//   4 x 2048 x 2048, from the third on: 9.1, 7.4, 6.0, 4.8, 5.2, 3.6
+// the form chosen by them took 0.3 % longer than the fastest one on the
+// geometric mean, 22 % at most (8191 x 2880 x 5120: 155 against 127 us).  Heights of
+// 160 and 192 rows are for sizes that would take a round more at 128.  Examples, us,
+// by form in the table's order:
+//   64 x 4096 x 6144, the last four but one: 12.2, 9.3, 11.9, 8.0
+//   180 x 4096 x 4096: 37.8, 22.5, 20.8, 19.8, 15.9, 12.5, 9.4, 17.1, 13.8
+//   517 x 2880 x 5120: 34.5, 18.9, 19.6, 18.6, 15.3, 22.8, 24.5, 53.5, 38.6
+//   600 x 8192 x 10240, the first five: 92.3, 65.5, 92.8, 87.2, 75.9
+//   850 x 4096 x 6144, the first five: 42.5, 28.7, 28.7, 43.9, 35.9
+//   8191 x 8192 x 10240, the first two: 688.3, 783.0
+//   4 x 2048 x 2048, the last five: 7.4, 6.0, 4.7, 5.1, 3.2
 struct Form {
   int bm, bn, per_cu, rows;  // rows: at most (0: any number)
   float once, round, step;
   int (*launch)(GemmParams &, hipStream_t);
 };
 const Form kForms[] = {
-    {256, 256, 1, 0, -12.7f, 19.8f, 1.166f, launch_turns},
-    {128, 128, 2, 0, -6.2f, 9.9f, 0.698f, launch_gemm<2, 2, 2, 2, 2, 1>},
-    {128, 128, 1, 0, -2.1f, 5.8f, 0.401f, launch_pipe<2, 4, 2, 1, 4, 1, 128>},
+    {256, 256, 1, 0, -15.0f, 22.2f, 1.149f, launch_turns},
+    {128, 128, 2, 0, -6.5f, 10.3f, 0.685f, launch_gemm<2, 2, 2, 2, 2, 1>},
+    {192, 128, 1, 0, -3.5f, 8.0f, 0.574f, launch_pipe<2, 6, 2, 1, 4, 1, 128>},
+    {160, 128, 1, 0, -2.0f, 6.3f, 0.545f, launch_pipe<2, 5, 2, 1, 4, 1, 128>},
+    {128, 128, 1, 0, -2.0f, 5.8f, 0.417f, launch_pipe<2, 4, 2, 1, 4, 1, 128>},
     {64, 128, 1, 0, -0.3f, 3.6f, 0.301f, launch_pipe<4, 2, 1, 1, 5, 1, 128>},
-    {64, 64, 1, 0, 0.6f, 2.8f, 0.183f, launch_pipe<2, 2, 1, 1, 5, 2, 256>},
-    {32, 32, 1, 0, 1.3f, 1.8f, 0.114f, launch_gemm<1, 1, 1, 1, 3, 4>},
-    {32, 64, 1, 0, 0.8f, 2.4f, 0.140f, launch_gemm<2, 1, 1, 1, 3, 4>},
-    {16, 16, 1, 16, 1.7f, 0.9f, 0.078f, launch_stream},
+    {64, 64, 1, 0, 0.5f, 2.9f, 0.188f, launch_pipe<2, 2, 1, 1, 5, 2, 256>},
+    {32, 32, 1, 0, 1.4f, 1.8f, 0.113f, launch_gemm<1, 1, 1, 1, 3, 4>},
+    {32, 64, 1, 0, 0.9f, 2.4f, 0.139f, launch_gemm<2, 1, 1, 1, 3, 4>},
+    {16, 16, 1, 16, 1.9f, 0.8f, 0.073f, launch_stream},
 };
 
 constexpr int64_t kMostGroups = 1 << 23;  // a grid's threads stay below 2^32
