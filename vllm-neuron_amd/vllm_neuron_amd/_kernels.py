@@ -1281,22 +1281,30 @@ def quant_rows(x, norm, eps, gamma=None, add0=None, add1=None, dim_actual=0):
     return codes, scales
 
 
-def int8_linear(x, x_scales, w, w_scales, bias, out):
-    """``out [M, N] = bf16(x_scales w_scales (x [M, K] w [N, K]^T) + bias)``."""
+def _scale_vector(s, n, what):
+    raise ValueError(f"int8_linear: {what} must be a contiguous float32 vector of {n}, "
+                     f"got {s.dtype} {tuple(s.shape)}")
+
+
+def int8_linear(x, x_scales, w, w_scales, bias, out, fresh=False):
+    """``out [M, N] = bf16(x_scales w_scales (x [M, K] w [N, K]^T) + bias)``;
+    ``fresh``: ``out`` was made for this call."""
     dev = N.same_gpu(x, x_scales, w, w_scales, bias, out)
     xs, wshape = x.shape, w.shape
-    if x.dtype != torch.int8 or w.dtype != torch.int8 or len(xs) != 2 or len(wshape) != 2:
+    i8, f32 = torch.int8, torch.float32
+    if x.dtype is not i8 or w.dtype is not i8 or len(xs) != 2 or len(wshape) != 2:
         raise ValueError(f"int8_linear: x and w must be int8 matrices, got {x.dtype} "
                          f"{tuple(xs)} and {w.dtype} {tuple(wshape)}")
-    (m, k), n = xs, wshape[0]
-    if k != wshape[1]:
-        raise ValueError(f"int8_linear: x has {k} channels, w {wshape[1]}")
-    for s, c, what in ((x_scales, m, "x_scales"), (w_scales, n, "w_scales")):
-        if s.dtype != torch.float32 or s.dim() != 1 or s.shape[0] != c or not s.is_contiguous():
-            raise ValueError(f"int8_linear: {what} must be a contiguous float32 vector of {c}, "
-                             f"got {s.dtype} {tuple(s.shape)}")
+    (m, k), (n, kw) = xs, wshape
+    if k != kw:
+        raise ValueError(f"int8_linear: x has {k} channels, w {kw}")
+    if x_scales.dtype is not f32 or x_scales.shape != (m,) or not x_scales.is_contiguous():
+        _scale_vector(x_scales, m, "x_scales")
+    if w_scales.dtype is not f32 or w_scales.shape != (n,) or not w_scales.is_contiguous():
+        _scale_vector(w_scales, n, "w_scales")
     x_st, w_st, o_st = x.stride(), w.stride(), out.stride()
-    if out.shape != (m, n) or out.dtype != torch.bfloat16 or (o_st[1] != 1 and n > 1):
+    if not fresh and (out.shape != (m, n) or out.dtype is not torch.bfloat16
+                      or (o_st[1] != 1 and n > 1)):
         raise ValueError(f"int8_linear: out must be bf16 [{m}, {n}] with contiguous columns")
     if k > 1 and (x_st[1] != 1 or w_st[1] != 1):
         raise ValueError("int8_linear: the channels of x and w must be contiguous")

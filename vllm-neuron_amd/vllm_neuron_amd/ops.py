@@ -717,7 +717,7 @@ def int8_linear(x, x_scales, w, w_scales, bias=None, out=None) -> Tensor:
     if out is None:
         out = x_scales.new_empty((x.shape[0], w.shape[0]), dtype=torch.bfloat16)
         if _plain(x, x_scales, w, w_scales, bias):
-            K.int8_linear(x, x_scales, w, w_scales, bias, out)
+            K.int8_linear(x, x_scales, w, w_scales, bias, out, True)
             return out
     elif _plain(x, x_scales, w, w_scales, bias, out):
         K.int8_linear(x, x_scales, w, w_scales, bias, out)
