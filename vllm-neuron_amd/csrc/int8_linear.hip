@@ -48,8 +48,10 @@ typedef __attribute__((address_space(3))) uint16_t lds_u16_t;
 // ---------------------------------------------------------------------------
 MIA_DEV float add_bf16(float a, float b) { return bf16lo(pack2_bf16(a + b, 0.f)); }
 
-// The row's scale: fl32(amax / 127), of the normalised row.
+// The row's scale: fl32(amax / 127), of the normalised row.  (Of zeros without an
+// eps it would be 0 times an infinity.)
 MIA_DEV float row_scale(uint32_t mag, float ss, const mia_quant_rows_args &a) {
+  if (mag == 0) return 0.f;
   if (mag >= 0x7f800000u) return __uint_as_float(0x7fc00000u);
   float amax = __uint_as_float(mag);
   if (a.norm) {
