@@ -808,7 +808,9 @@ int mia_shared_prefix_attention(const mia_shared_prefix_args *args, mia_stream_t
 /*   y = x * rsqrt(sum(x^2) / dim_actual + eps) * gamma, else y = x;         */
 /*   scales[row] = fl32(max|y| / 127), codes = rn(y * 127 / max|y|), ties to */
 /* even.  A row of zeros has scale 0; a row with a NaN or an infinity scale  */
-/* NaN and zero codes.                                                       */
+/* NaN and zero codes (with gamma: one where a product x gamma in fp32 is    */
+/* either).  The sum of squares does not leave fp32, however large or small  */
+/* the row.                                                                  */
 /* ------------------------------------------------------------------------ */
 typedef struct {
   const void *x;    /* bf16 [rows, dim], contiguous channels */

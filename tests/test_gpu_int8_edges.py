@@ -26,3 +26,34 @@ def test_normalised_rows_of_zeros(gpu, dim, eps):
         assert (codes[[1, 4]] == 0).all() and (scales[[1, 4]] == 0).all()
         assert not torch.isnan(scales).any()
     assert (codes == 0).all() and (scales == 0).all()
+
+
+@pytest.mark.parametrize("dim", DIMS)
+@pytest.mark.parametrize("eps", [0.0, 1e-6])
+@pytest.mark.parametrize("adds", [False, True])
+def test_normalised_rows_whose_squares_leave_float32(gpu, dim, eps, adds):
+    """The definition in float64, whatever the row's size.  Scales as for
+    ordinary rows: fp32 but for the sum; a code may be the neighbour where the
+    quotient lies within 2^-20 of a border.  The powers of two keep the values at
+    bf16's steps, so that sums and products with gamma round as ordinary ones do."""
+    gen = torch.Generator().manual_seed(dim)
+    size = torch.tensor([0, 60, 63, 64, 70, 120, -55, -60, -63, -75, -100, 0, 126])
+    x = (torch.rand(len(size), dim, generator=gen) - 0.5).double() * torch.exp2(size.double())[:, None]
+    x = x.to(BF)
+    x[11] = 0
+    x[11, dim // 2] = 2.0 ** 100  # one value alone
+    gamma = torch.exp2(torch.randint(-1, 1, (dim,), generator=gen).float())
+    more = {}
+    if adds:
+        a, b = x / 4, x.flip(1) / 4
+        more, (x, base) = dict(mlp_prev=a.to(gpu), attn_prev=b.to(gpu)), ((x / 2 + a) + b, x / 2)
+    else:
+        base = x
+    codes, scales = quant_rows(base.to(gpu), norm_type=RMS, norm_weights=gamma.to(gpu), eps=eps, **more)
+    r = x.double()
+    y = r / torch.sqrt(r.square().mean(-1, keepdim=True) + eps) * gamma.double()
+    amax = y.abs().amax(-1, keepdim=True)
+    q = y * 127.0 / amax
+    assert ((codes.cpu().double() - q).abs() <= 0.5 + q.abs() * 2.0 ** -20).all()
+    want = amax[:, 0] / 127.0
+    assert ((scales.cpu().double() - want).abs() <= want * 2.0 ** -20).all(), scales.cpu().double() / want

@@ -48,15 +48,28 @@ typedef __attribute__((address_space(3))) uint16_t lds_u16_t;
 // ---------------------------------------------------------------------------
 MIA_DEV float add_bf16(float a, float b) { return bf16lo(pack2_bf16(a + b, 0.f)); }
 
-// The row's scale: fl32(amax / 127), of the normalised row.  (Of zeros without an
-// eps it would be 0 times an infinity.)
-MIA_DEV float row_scale(uint32_t mag, float ss, const mia_quant_rows_args &a) {
-  if (mag == 0) return 0.f;
+// The squares of a row have left fp32 where their sum is an infinity (values from
+// 2^60 on or so), or so small that what it lost counts: an eps from 2^-75 on is
+// 2^25 times it and more.
+MIA_DEV bool squares_left(float ss, const mia_quant_rows_args &a) {
+  return !(ss <= 3.402823466e38f && ss >= (a.eps < 0x1p-75f ? 0x1p-100f : 0.f));
+}
+
+// 1 / rms, times f, of squares of the values times f.
+MIA_DEV float inverse_rms(float ss, float f, const mia_quant_rows_args &a) {
+  const float n = (float)(a.dim_actual > 0 ? a.dim_actual : a.dim);
+  return 1.0f / sqrtf(ss / n + a.eps * f * f);
+}
+
+// The row's scale: fl32(amax / 127), of the normalised row; -amax where its squares
+// have left fp32 (`left`).
+MIA_DEV float row_scale(uint32_t mag, float ss, bool left, const mia_quant_rows_args &a) {
   if (mag >= 0x7f800000u) return __uint_as_float(0x7fc00000u);
   float amax = __uint_as_float(mag);
   if (a.norm) {
-    const float n = (float)(a.dim_actual > 0 ? a.dim_actual : a.dim);
-    amax *= 1.0f / sqrtf(ss / n + a.eps);
+    if (mag == 0) return 0.f;  // (without an eps it would be 0 times an infinity)
+    if (left) return -amax;
+    amax *= inverse_rms(ss, 1.0f, a);
   }
   return amax / 127.0f;
 }
@@ -66,6 +79,50 @@ MIA_DEV float gamma_at(const mia_quant_rows_args &a, int c) {
   return ((const float *)a.gamma)[c];
 }
 
+// Channel c of the row at `at`, with its residual adds.
+MIA_DEV float row_value(const mia_quant_rows_args &a, int64_t at, int c) {
+  float x = bf16_bits_to_f32(((const uint16_t *)a.x)[at + c]);
+  if (a.add0) x = add_bf16(x, bf16_bits_to_f32(((const uint16_t *)a.add0)[at + c]));
+  if (a.add1) x = add_bf16(x, bf16_bits_to_f32(((const uint16_t *)a.add1)[at + c]));
+  return x;
+}
+
+// The scale of a row whose squares have left fp32, -amax so far, by a second read:
+// squares of the values times 2^-80 (at most 2^96 each, 2^-32 of a sum that was an
+// infinity) or 2^80 (2^-106 to 2^60).  The row's LANES threads call it; sums: their
+// waves'.  No part of the rows' own loop, which it would cost registers and 2 to 14 %.
+template <int LANES>
+MIA_DEV void scale_again(const mia_quant_rows_args &a, int64_t row, int tid, float2 *sums) {
+  float lo = 0.f, hi = 0.f;
+  int c = tid;
+  asm volatile("" : "+v"(c));  // (addresses are formed here, not before the rows' loop)
+#pragma nounroll
+  for (; c < a.dim; c += LANES) {
+    const float x = row_value(a, row * a.x_stride, c);
+    lo = fmaf(x * 0x1p-80f, x * 0x1p-80f, lo);
+    hi = fmaf(x * 0x1p80f, x * 0x1p80f, hi);
+  }
+#pragma nounroll
+  for (int o = 1; o < 64; o <<= 1) {
+    lo += __shfl_xor(lo, o, 64);
+    hi += __shfl_xor(hi, o, 64);
+  }
+  if constexpr (LANES == 256) {
+    __syncthreads();  // (those of the row before have been read)
+    if ((tid & 63) == 0) sums[tid >> 6] = make_float2(lo, hi);
+    __syncthreads();
+    lo = (sums[0].x + sums[1].x) + (sums[2].x + sums[3].x);
+    hi = (sums[0].y + sums[1].y) + (sums[2].y + sums[3].y);
+  }
+  if (tid != 0) return;
+  const float amax = -a.scales[row];
+  if (!(amax > 0.f)) return;  // (another row's squares have)
+  // (small values' sum is below 2^60 of them, large ones' an infinity or beyond)
+  const bool small = hi < 0x1p100f;
+  const float f = small ? 0x1p80f : 0x1p-80f;
+  a.scales[row] = amax * f * inverse_rms(small ? hi : lo, f, a) / 127.0f;
+}
+
 // LANES threads per row, NV vectors of 8 channels each, held in registers.  With
 // NORM a workgroup takes rows row0, row0 + stride, ...: gamma, twice the bytes of
 // a row where it is fp32, is loaded once for all of them.
@@ -73,7 +130,9 @@ template <int LANES, int NV, bool NORM>
 __global__ __launch_bounds__(256) void quant_rows_kernel(mia_quant_rows_args a) {
   constexpr int RPB = 256 / LANES;
   __shared__ float2 red[2][4];
+  __shared__ float2 sums[4];
   const int tid = threadIdx.x % LANES;
+  bool left = false;  // has a row to be scaled again?
   f32x4_t gamma[NORM ? NV : 1][2];
   if (NORM) {
 #pragma unroll
@@ -92,7 +151,8 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(mia_quant_rows_args a) 
     }
   }
   const int64_t stride = (int64_t)gridDim.x * RPB;
-  int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / LANES;
+  const int own = LANES == 256 ? 0 : threadIdx.x / LANES;  // (0: a row of all threads is uniform)
+  int64_t row = (int64_t)blockIdx.x * RPB + own;
   u32x4_t raw[NV];
   auto load = [&](int64_t r) {
     const int64_t at = (r < a.rows ? r : 0) * a.x_stride;
@@ -175,21 +235,25 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(mia_quant_rows_args a) 
       for (int i = 0; i < 8; ++i) w[i >> 2] |= rs.int8(x[v][i]) << (8 * (i & 3));
       *reinterpret_cast<u32x2_t *>((uint8_t *)a.codes + row * a.codes_stride + c) = w;
     }
-    if (tid == 0) a.scales[row] = row_scale(mag, ss, a);
+    const bool again = NORM && mag - 1u < 0x7f7fffffu && squares_left(ss, a);
+    if (tid == 0) a.scales[row] = row_scale(mag, ss, again, a);
+    left |= again;
   }
+  if (NORM && left)  // (the same for a row's threads)
+    for (row = (int64_t)blockIdx.x * RPB + own; row < a.rows; row += stride)
+      scale_again<LANES>(a, row, tid, sums);
 }
 
 // Any width, alignment and length: a workgroup takes a row at a time, read twice.
 __global__ __launch_bounds__(256) void quant_rows_any_kernel(mia_quant_rows_args a) {
   __shared__ float2 red[2][4];
+  __shared__ float2 sums[4];
   int turn = 0;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
     const int64_t at = row * a.x_stride;
     float ss = 0.f;
     auto value = [&](int c, bool sum) {
-      float x = bf16_bits_to_f32(((const uint16_t *)a.x)[at + c]);
-      if (a.add0) x = add_bf16(x, bf16_bits_to_f32(((const uint16_t *)a.add0)[at + c]));
-      if (a.add1) x = add_bf16(x, bf16_bits_to_f32(((const uint16_t *)a.add1)[at + c]));
+      const float x = row_value(a, at, c);
       if (sum) ss = fmaf(x, x, ss);
       return a.norm && a.gamma ? x * gamma_at(a, c) : x;
     };
@@ -211,7 +275,9 @@ __global__ __launch_bounds__(256) void quant_rows_any_kernel(mia_quant_rows_args
     rs.set(mag);
     for (int c = threadIdx.x; c < a.dim; c += 256)
       ((uint8_t *)a.codes)[row * a.codes_stride + c] = (uint8_t)rs.int8(value(c, false));
-    if (threadIdx.x == 0) a.scales[row] = row_scale(mag, ss, a);
+    const bool again = a.norm && squares_left(ss, a);
+    if (threadIdx.x == 0) a.scales[row] = row_scale(mag, ss, again, a);
+    if (again) scale_again<256>(a, row, threadIdx.x, sums);
   }
 }
 

@@ -29,7 +29,8 @@ def quant_rows(
     ``scale = max|y| / 127`` and ``code = round(y * 127 / max|y|)`` (ties to
     even) of ``y = x (+ mlp_prev) (+ attn_prev)`` or its RMS norm, which is not
     rounded in between.  A row of zeros has scale 0; a row that holds a NaN or
-    an infinity scale NaN and zero codes.  The rows of a weight ``[N, K]`` give
+    an infinity (or, in fp32, a product with ``norm_weights`` that is one) scale
+    NaN and zero codes.  The rows of a weight ``[N, K]`` give
     what ``int8_linear`` takes.
     """
     if norm_type not in (NormType.NO_NORM, NormType.RMS_NORM, NormType.RMS_NORM_SKIP_GAMMA):
