@@ -867,7 +867,8 @@ int mia_int8_linear(const mia_int8_linear_args *args, mia_stream_t stream);
 /* interleaved, by the angle positions[axis(i), t] * inv_freq[i]; cos and    */
 /* sin are multiplied by rope_scale.  axis(i): section[x] pairs of axis x    */
 /* one after the other, or with section_cycle axis i % axes where            */
-/* i < section[i % axes] * axes, else axis 0.                                */
+/* i < section[i % axes] * axes, else axis 0 (sections that hold more pairs  */
+/* than fall to their axis so are cut).                                      */
 /* K and V go to slots[t] of a cache: bf16; e4m3fn of clamp(x / dequant[h])  */
 /* (NULL = 1); int8 or e4m3fn with per-token scales as mia_quant_kv_write    */
 /* forms them.  Q and K are rounded once, behind the rotation.  slots NULL:  */

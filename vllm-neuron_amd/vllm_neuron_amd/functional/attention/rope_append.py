@@ -55,10 +55,13 @@ def rope_kv_append(
     The first ``rot`` channels of a head are rotated; pair ``i`` is ``(i, i +
     rot / 2)`` (``pairs="half"``) or ``(2 i, 2 i + 1)`` (``"interleaved"``), its
     angle ``positions[axis(i)] * inv_freq[i]``, cos and sin times ``rope_scale``.
-    ``sections`` says how many pairs each axis has: one axis after the other
-    (``section_order="blocks"``), or the axes in turn while their pairs last and
-    axis 0 elsewhere (``"cycle"``).  Angles are formed in 64 bits, so far
-    positions rotate as near ones do.  With ``qk_norm`` the heads of Q and K are
+    ``sections`` says how many pairs each axis has, one axis after the other
+    (``section_order="blocks"``); or, with ``"cycle"``, how many turns each axis
+    takes: pair ``i`` is of axis ``i % axes`` where ``i < sections[i % axes] *
+    axes``, else of axis 0.  Of ``n`` pairs no axis past the first can have more than
+    every ``axes``-th so; a larger section is cut, and axis 0 has what is left
+    (``[1, 1, 6]`` of 8 pairs is 0 1 2 0 0 2 0 0).  Angles are formed in 64 bits, so
+    far positions rotate as near ones do.  With ``qk_norm`` the heads of Q and K are
     RMS-normalised first.  Q, and K in a bf16 cache, are rounded once.
 
     Caches: bf16; int8 or e4m3fn with per-token scales, as ``quant_kv_write``
