@@ -57,3 +57,17 @@ def test_normalised_rows_whose_squares_leave_float32(gpu, dim, eps, adds):
     assert ((codes.cpu().double() - q).abs() <= 0.5 + q.abs() * 2.0 ** -20).all()
     want = amax[:, 0] / 127.0
     assert ((scales.cpu().double() - want).abs() <= want * 2.0 ** -20).all(), scales.cpu().double() / want
+
+
+def test_scales_of_leading_axes(gpu):
+    x = torch.randint(-127, 128, (2, 3, 64), device=gpu, dtype=torch.int32).to(torch.int8)
+    w, ws = x.view(6, 64)[:5].contiguous(), torch.ones(5, device=gpu)
+    xs = torch.rand(2, 3, device=gpu)
+    want = int8_linear(x.view(6, 64), xs.view(6), w, ws)
+    assert torch.equal(int8_linear(x, xs, w, ws).view(6, 5), want)
+    assert torch.equal(int8_linear(x[0, 0], xs[0, 0], w, ws), want[0])
+    for same in (xs.view(6), xs[..., None], xs[None]):
+        assert torch.equal(int8_linear(x, same, w, ws).view(6, 5), want)
+    for bad in (xs.t(), xs.view(3, 2), xs.view(1, 6), xs[:1]):
+        with pytest.raises(ValueError, match="x_scales"):
+            int8_linear(x, bad, w, ws)

@@ -58,7 +58,11 @@ def int8_linear(
     """
     if x.dim() == 2:
         return K.int8_linear(x, x_scales, w, w_scales, bias, out)
-    shape = (*x.shape[:-1], w.shape[0])
+    lead = x.shape[:-1]
+    if x_scales.dim() != 1 and [n for n in x_scales.shape if n != 1] != [n for n in lead if n != 1]:
+        raise ValueError(f"int8_linear: x_scales must be {tuple(lead)}, one per row of x, got "
+                         f"{tuple(x_scales.shape)}")
+    shape = (*lead, w.shape[0])
     if out is not None:
         if tuple(out.shape) != shape:
             raise ValueError(f"int8_linear: out must be {shape}, got {tuple(out.shape)}")
