@@ -836,7 +836,7 @@ int mia_quant_rows(const mia_quant_rows_args *args, mia_stream_t stream);
 /* Product of int8 rows and int8 weights (no counterpart in the reference):  */
 /*   out[m, n] = bf16(x_scales[m] w_scales[n] sum_k x[m, k] w[n, k] + b[n]), */
 /* integer sums exact in 32 bits (k < 131072).  k is a multiple of 16, rows */
-/* of x and w 16-byte aligned.                                               */
+/* of x and w 16-byte aligned and less than 2^24 bytes apart.                */
 /* ------------------------------------------------------------------------ */
 typedef struct {
   const void *x; /* int8 [rows, k] */

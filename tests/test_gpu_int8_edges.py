@@ -71,3 +71,21 @@ def test_scales_of_leading_axes(gpu):
     for bad in (xs.t(), xs.view(3, 2), xs.view(1, 6), xs[:1]):
         with pytest.raises(ValueError, match="x_scales"):
             int8_linear(x, bad, w, ws)
+
+
+@pytest.mark.parametrize("m", [1, 3, 40])
+def test_rows_far_apart(gpu, m):
+    """The last token of each sequence: rows 2^24 bytes apart and more."""
+    k, n = 256, 48
+    g = torch.Generator().manual_seed(m)
+    codes = torch.randint(-127, 128, (m, k), generator=g, dtype=torch.int32).to(torch.int8).to(gpu)
+    w = torch.randint(-127, 128, (n, k), generator=g, dtype=torch.int32).to(torch.int8).to(gpu)
+    xs, ws = torch.rand(m, generator=g).to(gpu), torch.rand(n, generator=g).to(gpu)
+    pool = torch.zeros(m, (1 << 24) // k + 1, k, dtype=torch.int8, device=gpu)
+    pool[:, -1] = codes
+    x = pool[:, -1]
+    assert x.stride(0) > 1 << 24
+    assert torch.equal(int8_linear(x, xs, w, ws), int8_linear(codes, xs, w, ws))
+    if m == 1:  # one channel: the stride of its axis is never used
+        one = pool[:, -1]
+        assert torch.equal(int8_linear(codes, xs, one, ws[:1]), int8_linear(codes, xs, one.contiguous(), ws[:1]))

@@ -844,8 +844,9 @@ int mia_int8_linear(const mia_int8_linear_args *a, mia_stream_t stream) {
               "int8_linear: k of 131072 or more (the 32-bit sums could overflow)");
   MIA_REQUIRE(a->k % 16 == 0, MIA_ERR_NOT_IMPLEMENTED, "int8_linear: k must be a multiple of 16");
   // a tile's 256 rows lie within 2^32 bytes
-  MIA_REQUIRE(a->x_stride >= 0 && a->x_stride < (1ll << 24) && a->w_stride >= 0 &&
-                  a->w_stride < (1ll << 24),
+  // (the stride of an axis of one row is never used)
+  MIA_REQUIRE((a->rows == 1 || (a->x_stride >= 0 && a->x_stride < (1ll << 24))) &&
+                  (a->n == 1 || (a->w_stride >= 0 && a->w_stride < (1ll << 24))),
               MIA_ERR_VALUE, "int8_linear: row stride out of range");
   MIA_REQUIRE(aligned(a->x, 16) && aligned(a->w, 16) &&
                   (a->x_stride % 16 == 0 || a->rows == 1) && (a->w_stride % 16 == 0 || a->n == 1),

@@ -995,7 +995,7 @@ int launch_quant_rows(const mia_quant_rows_args &a, hipStream_t s) {
 int launch_int8_linear(const mia_int8_linear_args &a, hipStream_t s) {
   GemmParams p = {};
   p.x = (const uint8_t *)a.x, p.w = (const uint8_t *)a.w;
-  p.x_ld = a.x_stride, p.w_ld = a.w_stride;
+  p.x_ld = a.rows == 1 ? 0 : a.x_stride, p.w_ld = a.n == 1 ? 0 : a.w_stride;
   p.xs = a.x_scales, p.ws = a.w_scales;
   p.bias = a.bias, p.bias_bf16 = a.bias_bf16;
   p.out = (uint16_t *)a.out, p.out_ld = a.out_stride;

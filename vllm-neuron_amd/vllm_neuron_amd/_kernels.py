@@ -1308,6 +1308,10 @@ def int8_linear(x, x_scales, w, w_scales, bias, out, fresh=False):
         raise ValueError(f"int8_linear: out must be bf16 [{m}, {n}] with contiguous columns")
     if k > 1 and (x_st[1] != 1 or w_st[1] != 1):
         raise ValueError("int8_linear: the channels of x and w must be contiguous")
+    if x_st[0] >= 1 << 24 and m > 1:
+        # (a tile's rows lie within 2^32 bytes; such rows are a token of each sequence)
+        x = x.contiguous()
+        x_st = x.stride()
     if bias is not None:
         bias = _vector(bias, n, "bias", dev)
     a = N.Int8LinearArgs()

@@ -54,7 +54,8 @@ def int8_linear(
     exact in 32-bit integers, the rest in float32, rounded once.
 
     ``K`` is a multiple of 16 (below 131072), the rows of ``x`` and ``w`` are
-    contiguous and 16-byte aligned.  A row with scale NaN gives NaN.
+    contiguous and 16-byte aligned, those of ``w`` less than 2^24 bytes apart.  A row
+    with scale NaN gives NaN.
     """
     if x.dim() == 2:
         return K.int8_linear(x, x_scales, w, w_scales, bias, out)
