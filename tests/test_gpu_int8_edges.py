@@ -89,3 +89,9 @@ def test_rows_far_apart(gpu, m):
     if m == 1:  # one channel: the stride of its axis is never used
         one = pool[:, -1]
         assert torch.equal(int8_linear(codes, xs, one, ws[:1]), int8_linear(codes, xs, one.contiguous(), ws[:1]))
+
+
+def test_vectors_of_another_device_are_refused(gpu):
+    x = torch.ones(4, 64, dtype=BF, device=gpu)
+    with pytest.raises(RuntimeError, match="GPU tensors only"):
+        quant_rows(x, norm_type=RMS, norm_weights=torch.ones(64))

@@ -1220,15 +1220,13 @@ def shared_prefix_attention(q, k_cache, v_cache, prefix_table, prefix_len, block
 # ---------------------------------------------------------------------------
 # int8 projections
 # ---------------------------------------------------------------------------
-def _vector(t, n, what, dev):
+def _vector(t, n, what):
     """A float32 or bf16 vector of ``n`` entries as the kernels read it (other
-    types as float32, other devices, strides and alignments copied)."""
+    types as float32, other strides and alignments copied)."""
     if t.numel() != n:
         raise ValueError(f"{what} has {t.numel()} entries, expected {n}")
     if t.dtype not in (torch.float32, torch.bfloat16):
         t = t.detach().float()
-    if t.device != dev:
-        t = t.detach().to(dev)
     if not t.is_contiguous():
         t = t.detach().contiguous()
     return t if t.data_ptr() % 16 == 0 else t.detach().clone()
@@ -1237,7 +1235,7 @@ def _vector(t, n, what, dev):
 def quant_rows(x, norm, eps, gamma=None, add0=None, add1=None, dim_actual=0):
     """Rows of ``x (+ add0) (+ add1) [..., dim]`` (bf16), RMS-normalised with
     ``norm``, as int8 codes of the same shape and float32 scales ``[...]``."""
-    dev = N.same_gpu(x, add0, add1)
+    dev = N.same_gpu(x, add0, add1, gamma)
     if x.dtype != torch.bfloat16:
         raise NotImplementedError("quant_rows: bf16 input only")
     shape = x.shape
@@ -1247,7 +1245,7 @@ def quant_rows(x, norm, eps, gamma=None, add0=None, add1=None, dim_actual=0):
     if gamma is not None:
         if not norm:
             raise ValueError("quant_rows: gamma belongs to a norm")
-        gamma = _vector(gamma, dim, "gamma", dev)
+        gamma = _vector(gamma, dim, "gamma")
     if not 0 <= dim_actual <= dim:
         raise ValueError(f"quant_rows: dim_actual {dim_actual} of {dim} channels")
     flat = len(shape) == 2
@@ -1313,7 +1311,7 @@ def int8_linear(x, x_scales, w, w_scales, bias, out, fresh=False):
         x = x.contiguous()
         x_st = x.stride()
     if bias is not None:
-        bias = _vector(bias, n, "bias", dev)
+        bias = _vector(bias, n, "bias")
     a = N.Int8LinearArgs()
     N.PACK_INT8.pack_into(
         a, 0, x.data_ptr(), x_st[0], x_scales.data_ptr(), w.data_ptr(), w_st[0],
@@ -1384,8 +1382,8 @@ def rope_append(q, k, v, positions, inv_freq, slots, k_cache, v_cache, q_out, k_
     if q_gamma is not None or k_gamma is not None:
         if not qk_norm:
             raise ValueError("q_gamma and k_gamma belong to qk_norm")
-        q_gamma = None if q_gamma is None else _vector(q_gamma, d, "q_gamma", dev)
-        k_gamma = None if k_gamma is None else _vector(k_gamma, d, "k_gamma", dev)
+        q_gamma = None if q_gamma is None else _vector(q_gamma, d, "q_gamma")
+        k_gamma = None if k_gamma is None else _vector(k_gamma, d, "k_gamma")
         if q_gamma is not None and k_gamma is not None and q_gamma.dtype != k_gamma.dtype:
             q_gamma, k_gamma = q_gamma.float(), k_gamma.float()
         bf16 = (k_gamma if q_gamma is None else q_gamma).dtype == torch.bfloat16
