@@ -95,3 +95,14 @@ def test_vectors_of_another_device_are_refused(gpu):
     x = torch.ones(4, 64, dtype=BF, device=gpu)
     with pytest.raises(RuntimeError, match="GPU tensors only"):
         quant_rows(x, norm_type=RMS, norm_weights=torch.ones(64))
+
+
+def test_sizes_past_32_bits_are_refused(gpu):
+    x, one = torch.zeros(1, 16, dtype=torch.int8, device=gpu), torch.ones(1, device=gpu)
+    out, many = torch.zeros(1, 1, dtype=BF, device=gpu), torch.empty(1 << 31, device=gpu)
+    with pytest.raises(ValueError):
+        ops.int8_linear(x.expand(1 << 31, 16), many, x, one, out=out.expand(1 << 31, 1))
+    with pytest.raises(ValueError):
+        ops.int8_linear(x, one, x.expand(1 << 31, 16), many, out=out.expand(1, 1 << 31))
+    with pytest.raises(ValueError):
+        quant_rows(torch.empty(0, 1 << 31, dtype=BF, device=gpu))

@@ -1267,12 +1267,15 @@ def quant_rows(x, norm, eps, gamma=None, add0=None, add1=None, dim_actual=0):
              else x2.new_empty((rows, dim), dtype=torch.int8))
     scales = x2.new_empty((rows,), dtype=torch.float32)
     a = N.QuantRowsArgs()
-    N.PACK_QUANT_ROWS.pack_into(
-        a, 0, x2.data_ptr(), adds[0].data_ptr() if adds else 0,
-        adds[1].data_ptr() if len(adds) > 1 else 0, stride[0], codes.data_ptr(), dim,
-        scales.data_ptr(), rows, dim, dim_actual, norm, eps,
-        0 if gamma is None else gamma.data_ptr(),
-        gamma is not None and gamma.dtype == torch.bfloat16, 0)
+    try:
+        N.PACK_QUANT_ROWS.pack_into(
+            a, 0, x2.data_ptr(), adds[0].data_ptr() if adds else 0,
+            adds[1].data_ptr() if len(adds) > 1 else 0, stride[0], codes.data_ptr(), dim,
+            scales.data_ptr(), rows, dim, dim_actual, norm, eps,
+            0 if gamma is None else gamma.data_ptr(),
+            gamma is not None and gamma.dtype == torch.bfloat16, 0)
+    except N.PACK_ERRORS as e:
+        raise N.out_of_range("quant_rows", e) from e
     N.launch(N.lib().mia_quant_rows, a, dev, "quant_rows")
     if not flat:
         return codes.reshape(shape), scales.reshape(shape[:-1])
@@ -1313,10 +1316,13 @@ def int8_linear(x, x_scales, w, w_scales, bias, out, fresh=False):
     if bias is not None:
         bias = _vector(bias, n, "bias")
     a = N.Int8LinearArgs()
-    N.PACK_INT8.pack_into(
-        a, 0, x.data_ptr(), x_st[0], x_scales.data_ptr(), w.data_ptr(), w_st[0],
-        w_scales.data_ptr(), 0 if bias is None else bias.data_ptr(), out.data_ptr(), o_st[0],
-        m, n, k, bias is not None and bias.dtype == torch.bfloat16)
+    try:
+        N.PACK_INT8.pack_into(
+            a, 0, x.data_ptr(), x_st[0], x_scales.data_ptr(), w.data_ptr(), w_st[0],
+            w_scales.data_ptr(), 0 if bias is None else bias.data_ptr(), out.data_ptr(), o_st[0],
+            m, n, k, bias is not None and bias.dtype == torch.bfloat16)
+    except N.PACK_ERRORS as e:
+        raise N.out_of_range("int8_linear", e) from e
     N.launch(N.lib().mia_int8_linear, a, dev, "int8_linear")
 
 
@@ -1420,11 +1426,14 @@ def rope_append(q, k, v, positions, inv_freq, slots, k_cache, v_cache, q_out, k_
     elif k_cache is not None or v is not None:
         raise ValueError("the cache append needs slots")
     a = N.RopeAppendArgs()
-    N.PACK_ROPE.pack_into(
-        a, 0, *rows, T, hq, hkv, d, 2 * half, positions.data_ptr(), *p_st,
-        N.mia_dtype(positions.dtype), axes, inv_freq.data_ptr(), *sections, *_PAD[axes], cycle,
-        interleaved, rope_scale, qk_norm, N.ptr(q_gamma) or 0, N.ptr(k_gamma) or 0, bf16, eps,
-        *cache)
+    try:
+        N.PACK_ROPE.pack_into(
+            a, 0, *rows, T, hq, hkv, d, 2 * half, positions.data_ptr(), *p_st,
+            N.mia_dtype(positions.dtype), axes, inv_freq.data_ptr(), *sections, *_PAD[axes], cycle,
+            interleaved, rope_scale, qk_norm, N.ptr(q_gamma) or 0, N.ptr(k_gamma) or 0, bf16, eps,
+            *cache)
+    except N.PACK_ERRORS as e:
+        raise N.out_of_range("rope_append", e) from e
     N.launch(N.lib().mia_rope_append, a, dev, "rope_append")
 
 
@@ -1462,13 +1471,17 @@ def window_attention(q, k_cache, v_cache, block_table, seq_lens, out, *, window,
     for v, least, what in ((window, 1, "window"), (first_tokens, 0, "first_tokens")):
         if not least <= v <= 1 << 30:
             raise ValueError(f"{what} must be in [{least}, 2^30], got {v}")
+    most = min(max_seqlen_q, T)  # (any larger bound is none)
     a = N.WindowArgs()
-    N.PACK_WINDOW.pack_into(
-        a, 0, q.data_ptr(), *q.stride(), out.data_ptr(), *out.stride(), T, n, cu, max_seqlen_q,
-        hq, hkv, d, k_cache.data_ptr(), v_cache.data_ptr(), code, nb, *k_cache.stride(),
-        *v_cache.stride(), bs, block_table.shape[1], block_table.data_ptr(),
-        *block_table.stride(), seq_lens.data_ptr(), window, first_tokens, *scales,
-        N.ptr(kd) or 0, N.ptr(vd) or 0, N.ptr(sk) or 0, softmax_scale, int(zero_rest), 0, 0)
+    try:
+        N.PACK_WINDOW.pack_into(
+            a, 0, q.data_ptr(), *q.stride(), out.data_ptr(), *out.stride(), T, n, cu, most,
+            hq, hkv, d, k_cache.data_ptr(), v_cache.data_ptr(), code, nb, *k_cache.stride(),
+            *v_cache.stride(), bs, block_table.shape[1], block_table.data_ptr(),
+            *block_table.stride(), seq_lens.data_ptr(), window, first_tokens, *scales,
+            N.ptr(kd) or 0, N.ptr(vd) or 0, N.ptr(sk) or 0, softmax_scale, int(zero_rest), 0, 0)
+    except N.PACK_ERRORS as e:
+        raise N.out_of_range("window_attention", e) from e
     L = N.lib()
     _span_launch(a, L.mia_window_workspace_bytes, L.mia_window_attention, "window_attention",
                  workspace, dev)

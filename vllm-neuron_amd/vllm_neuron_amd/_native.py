@@ -320,6 +320,15 @@ def _packer(st) -> struct.Struct:
     return struct.Struct("@" + code)
 
 
+PACK_ERRORS = (struct.error, OverflowError)
+
+
+def out_of_range(what: str, e: Exception) -> ValueError:
+    """The error of a call with a number that its argument struct cannot hold (a
+    size of 2^31 and more where the kernels count in 32 bits)."""
+    return ValueError(f"{what}: a size or number out of range ({e})")
+
+
 PACK_QUANT = _packer(QuantKvArgs)
 PACK_CROSS = _packer(CrossArgs)
 PACK_PREFIX = _packer(SharedPrefixArgs)
