@@ -856,6 +856,14 @@ typedef struct {
 
 int mia_int8_linear(const mia_int8_linear_args *args, mia_stream_t stream);
 
+/* The product is written in several forms (tiles); the call above takes the */
+/* one that the measured costs say is the fastest.  Their number, the one    */
+/* taken for a size (-1: none), and the product by a given one, the same     */
+/* numbers to the last bit: for measurements and tests.                      */
+int mia_int8_linear_forms(void);
+int mia_int8_linear_choice(const mia_int8_linear_args *args);
+int mia_int8_linear_form(const mia_int8_linear_args *args, int32_t form, mia_stream_t stream);
+
 /* ------------------------------------------------------------------------ */
 /* Rotation of Q and K by positions on one to four axes (text; time, height, */
 /* width), with K and V appended to the paged cache in the same pass (no     */

@@ -833,8 +833,7 @@ int mia_quant_rows(const mia_quant_rows_args *a, mia_stream_t stream) {
   return mia::launch_quant_rows(*a, (hipStream_t)stream);
 }
 
-int mia_int8_linear(const mia_int8_linear_args *a, mia_stream_t stream) {
-  mia::g_last_error.clear();
+static int validate_int8(const mia_int8_linear_args *a) {
   MIA_REQUIRE(a, MIA_ERR_VALUE, "int8_linear: null args");
   MIA_REQUIRE(a->rows >= 0 && a->n >= 0 && a->k > 0, MIA_ERR_VALUE, "int8_linear: bad shape");
   if (a->rows == 0 || a->n == 0) return MIA_OK;
@@ -854,7 +853,32 @@ int mia_int8_linear(const mia_int8_linear_args *a, mia_stream_t stream) {
   // tiles along one grid axis, their threads within 2^32
   MIA_REQUIRE((int64_t)(a->rows / 64 + 1) * (a->n / 64 + 1) < (1ll << 22), MIA_ERR_VALUE,
               "int8_linear: rows * n beyond 2^34");
-  return mia::launch_int8_linear(*a, (hipStream_t)stream);
+  return MIA_OK;
+}
+
+int mia_int8_linear(const mia_int8_linear_args *a, mia_stream_t stream) {
+  mia::g_last_error.clear();
+  const int rc = validate_int8(a);
+  if (rc || a->rows == 0 || a->n == 0) return rc;
+  return mia::launch_int8_linear(*a, mia::int8_linear_choice(*a), (hipStream_t)stream);
+}
+
+int mia_int8_linear_forms(void) { return mia::int8_linear_forms(); }
+
+int mia_int8_linear_choice(const mia_int8_linear_args *a) {
+  mia::g_last_error.clear();
+  if (validate_int8(a) || a->rows == 0 || a->n == 0) return -1;
+  return mia::int8_linear_choice(*a);
+}
+
+int mia_int8_linear_form(const mia_int8_linear_args *a, int32_t form, mia_stream_t stream) {
+  mia::g_last_error.clear();
+  const int rc = validate_int8(a);
+  if (rc) return rc;
+  MIA_REQUIRE(form >= 0 && form < mia::int8_linear_forms(), MIA_ERR_VALUE,
+              "int8_linear: no such form");
+  if (a->rows == 0 || a->n == 0) return MIA_OK;
+  return mia::launch_int8_linear(*a, form, (hipStream_t)stream);
 }
 
 int mia_rope_append(const mia_rope_append_args *a, mia_stream_t stream) {

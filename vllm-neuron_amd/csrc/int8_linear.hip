@@ -875,6 +875,12 @@ __global__ __launch_bounds__(kStreamWaves * 64) void stream_kernel(GemmParams p)
   p.out[(int64_t)t * p.out_ld + n0 + c] = (uint16_t)(pack2_bf16(y, 0.f) & 0xffffu);
 }
 
+// (a grid of 2^32 threads and more would be cut without an error)
+int check_grid(int64_t groups, int threads) {
+  if (groups * threads < (1ll << 32)) return MIA_OK;
+  return set_error(MIA_ERR_VALUE, "int8_linear: more tiles than a grid holds");
+}
+
 template <auto kernel>
 int launch_tiles(const GemmParams &p, int threads, int bytes, hipStream_t s) {
   // (said once per device: the call takes a few us)
@@ -887,6 +893,7 @@ int launch_tiles(const GemmParams &p, int threads, int bytes, hipStream_t s) {
     if (e != hipSuccess) return check_hip(e, "int8_linear");
     if (dev < 64) said.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
+  if (const int rc = check_grid((int64_t)p.mt * p.nt, threads)) return rc;
   kernel<<<p.mt * p.nt, threads, bytes, s>>>(p);
   return check_hip(hipGetLastError(), "int8_linear");
 }
@@ -920,6 +927,7 @@ int launch_turns(GemmParams &p, hipStream_t s) {
 }
 
 int launch_stream(GemmParams &p, hipStream_t s) {
+  if (const int rc = check_grid(((int64_t)p.n + 15) / 16, kStreamWaves * 64)) return rc;
   stream_kernel<<<(p.n + 15) / 16, kStreamWaves * 64, 0, s>>>(p);
   return check_hip(hipGetLastError(), "int8_linear");
 }
@@ -992,7 +1000,29 @@ int launch_quant_rows(const mia_quant_rows_args &a, hipStream_t s) {
   return check_hip(hipGetLastError(), "quant_rows");
 }
 
-int launch_int8_linear(const mia_int8_linear_args &a, hipStream_t s) {
+int int8_linear_forms() { return (int)(sizeof(kForms) / sizeof(kForms[0])); }
+
+// The form that the measured costs say is the fastest.
+int int8_linear_choice(const mia_int8_linear_args &a) {
+  const float steps = (float)a.k / kBK;
+  const int cus = cu_count();
+  int best = 0;
+  float least = 0.f;
+  for (int i = 0; i < int8_linear_forms(); ++i) {
+    const Form &f = kForms[i];
+    if (f.rows < a.rows && f.rows) continue;
+    const int64_t tiles = (int64_t)((a.rows + f.bm - 1) / f.bm) * ((a.n + f.bn - 1) / f.bn);
+    const int64_t rounds = (tiles + f.per_cu * cus - 1) / (f.per_cu * cus);
+    const float cost = f.once + (float)rounds * (f.round + steps * f.step);
+    if (i == 0 || cost < least) least = cost, best = i;
+  }
+  return best;
+}
+
+int launch_int8_linear(const mia_int8_linear_args &a, int form, hipStream_t s) {
+  const Form &f = kForms[form];
+  if (f.rows && f.rows < a.rows)
+    return set_error(MIA_ERR_VALUE, "int8_linear: more rows than the form takes");
   GemmParams p = {};
   p.x = (const uint8_t *)a.x, p.w = (const uint8_t *)a.w;
   p.x_ld = a.rows == 1 ? 0 : a.x_stride, p.w_ld = a.n == 1 ? 0 : a.w_stride;
@@ -1001,20 +1031,7 @@ int launch_int8_linear(const mia_int8_linear_args &a, hipStream_t s) {
   p.out = (uint16_t *)a.out, p.out_ld = a.out_stride;
   p.m = a.rows, p.n = a.n, p.k = a.k;
   p.vec = a.n % 8 == 0 && a.out_stride % 8 == 0 && (uintptr_t)a.out % 16 == 0;
-  // The form that the measured costs below say is the fastest.
-  const float steps = (float)p.k / kBK;
-  const int cus = cu_count();
-  int best = 0;
-  float least = 0.f;
-  for (int i = 0; i < (int)(sizeof(kForms) / sizeof(kForms[0])); ++i) {
-    const Form &f = kForms[i];
-    if (f.rows < p.m && f.rows) continue;
-    const int64_t tiles = (int64_t)((p.m + f.bm - 1) / f.bm) * ((p.n + f.bn - 1) / f.bn);
-    const int64_t rounds = (tiles + f.per_cu * cus - 1) / (f.per_cu * cus);
-    const float cost = f.once + (float)rounds * (f.round + steps * f.step);
-    if (i == 0 || cost < least) least = cost, best = i;
-  }
-  return kForms[best].launch(p, s);
+  return f.launch(p, s);
 }
 
 }  // namespace mia

@@ -34,7 +34,9 @@ int launch_qkv_epilogue(const mia_qkv_epilogue_args &a, hipStream_t s);
 int launch_row_norm(const mia_row_norm_args &a, hipStream_t s);
 int launch_skinny_linear(const mia_skinny_linear_args &a, hipStream_t s);
 int launch_quant_rows(const mia_quant_rows_args &a, hipStream_t s);
-int launch_int8_linear(const mia_int8_linear_args &a, hipStream_t s);
+int int8_linear_forms();
+int int8_linear_choice(const mia_int8_linear_args &a);
+int launch_int8_linear(const mia_int8_linear_args &a, int form, hipStream_t s);
 int launch_rope_append(const mia_rope_append_args &a, hipStream_t s);
 size_t window_workspace(const mia_window_args &a);
 int launch_window(const mia_window_args &a, hipStream_t s);

@@ -356,7 +356,8 @@ EXPORTS = [
     "mia_row_norm", "mia_skinny_linear", "mia_paged_decode_noalloc",
     "mia_quant_kv_write", "mia_quant_kv_read", "mia_cross_workspace_bytes",
     "mia_cross_attention", "mia_shared_prefix_workspace_bytes", "mia_shared_prefix_attention",
-    "mia_quant_rows", "mia_int8_linear", "mia_rope_append",
+    "mia_quant_rows", "mia_int8_linear", "mia_int8_linear_forms", "mia_int8_linear_choice",
+    "mia_int8_linear_form", "mia_rope_append",
     "mia_window_workspace_bytes", "mia_window_attention",
 ]
 
@@ -398,6 +399,12 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.mia_cross_workspace_bytes.restype = ctypes.c_size_t
     lib.mia_shared_prefix_workspace_bytes.argtypes = [P(SharedPrefixArgs)]
     lib.mia_shared_prefix_workspace_bytes.restype = ctypes.c_size_t
+    lib.mia_int8_linear_forms.argtypes = []
+    lib.mia_int8_linear_forms.restype = c_i32
+    lib.mia_int8_linear_choice.argtypes = [P(Int8LinearArgs)]
+    lib.mia_int8_linear_choice.restype = c_i32
+    lib.mia_int8_linear_form.argtypes = [P(Int8LinearArgs), c_i32, c_vp]
+    lib.mia_int8_linear_form.restype = c_i32
     lib.mia_window_workspace_bytes.argtypes = [P(WindowArgs)]
     lib.mia_window_workspace_bytes.restype = ctypes.c_size_t
     lib.mia_slot_mapping_host.argtypes = [P(SlotMappingArgs)]
