@@ -227,6 +227,16 @@ struct RowCodes {
   MIA_DEV uint32_t int8(float x) const { return (uint32_t)(int)rintf(code(x)) & 0xffu; }
 };
 
+// The scale that a cache keeps beside such codes: fl32(amax / Q), or the next
+// smaller number where code Q would read back as an infinity (the largest fp32
+// values); NaN of a row with a NaN or an infinity.
+template <int Q>
+MIA_DEV float cache_scale(uint32_t mag) {
+  if (mag >= 0x7f800000u) return __uint_as_float(0x7fc00000u);
+  const float s = __uint_as_float(mag) / (float)Q;
+  return s * (float)Q > 3.402823466e38f ? __uint_as_float(__float_as_uint(s) - 1u) : s;
+}
+
 // ---------------------------------------------------------------------------
 // Division by an invariant positive integer d (Granlund & Montgomery 1994):
 // for 0 <= n < 2^31, n / d == umulhi(n, m) >> (s - 1) with s = ceil(log2 d),

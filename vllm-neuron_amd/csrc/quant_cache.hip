@@ -143,7 +143,7 @@ __global__ __launch_bounds__(256) void quant_write_kernel(QuantKParams p) {
   const RowPos r = row_pos(p, in ? row : 0);
   const bool act = c0 < p.d;
   constexpr int SB = SRC == MIA_DTYPE_F32 ? 4 : 2;
-  constexpr float Q = I8 ? 127.0f : 448.0f;
+  constexpr int Q = I8 ? 127 : 448;
   float x[2][8];
 #pragma unroll
   for (int y = 0; y < 2; ++y) {
@@ -162,33 +162,18 @@ __global__ __launch_bounds__(256) void quant_write_kernel(QuantKParams p) {
 #pragma unroll
     for (int o = 1; o < LPR; o <<= 1) mag = max(mag, (uint32_t)__shfl_xor((int)mag, o, 64));
     if (!in || r.slot < 0) continue;
-    const float amax = __uint_as_float(mag);
-    const bool bad = mag >= 0x7f800000u;
-    const bool zero = bad || mag == 0;
-    const int e = __builtin_amdgcn_frexp_expf(amax);
-    const float b = zero ? 1.0f : ldexpf(amax, -e);  // [0.5, 1)
-    float rc = __builtin_amdgcn_rcpf(b);
-    rc = fmaf(fmaf(-b, rc, 1.0f), rc, rc);
-    float y8[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float a = (zero ? 0.f : ldexpf(x[y][i], -e)) * Q;
-      const float q = a * rc;
-      y8[i] = fmaf(fmaf(-b, q, a), rc, q);
-    }
+    RowCodes<Q> rc;
+    rc.set(mag);
     u32x2_t w;
     if constexpr (I8) {
+      w = u32x2_t{0u, 0u};
 #pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        uint32_t v = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          v |= ((uint32_t)(int)rintf(y8[4 * g + i]) & 0xffu) << (8 * i);
-        w[g] = v;
-      }
+      for (int i = 0; i < 8; ++i) w[i >> 2] |= rc.int8(x[y][i]) << (8 * (i & 3));
     } else {
-      w[0] = e4m3fn_x4(y8[0], y8[1], y8[2], y8[3]);
-      w[1] = e4m3fn_x4(y8[4], y8[5], y8[6], y8[7]);
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+        w[g] = e4m3fn_x4(rc.code(x[y][4 * g]), rc.code(x[y][4 * g + 1]), rc.code(x[y][4 * g + 2]),
+                         rc.code(x[y][4 * g + 3]));
     }
     uint8_t *dst = p.cache[y] + r.blk * p.c_blk[y] + (int64_t)r.h * p.c_h[y] + r.off * p.c_t[y];
     if constexpr (VEC) {
@@ -200,12 +185,8 @@ __global__ __launch_bounds__(256) void quant_write_kernel(QuantKParams p) {
           dst[(int64_t)(c0 + i) * p.c_d[y]] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
     }
     if (threadIdx.x % LPR == 0) {
-      float sc = amax / Q;
-      // the largest fp32 values: code Q must not read back as an infinity
-      if (SRC == MIA_DTYPE_F32 && sc * Q > 3.402823466e38f)
-        sc = __uint_as_float(__float_as_uint(sc) - 1u);
       p.scales[y][r.blk * p.s_blk[y] + (int64_t)r.h * p.s_h[y] + r.off * p.s_t[y]] =
-          bad ? __uint_as_float(0x7fc00000u) : sc;
+          cache_scale<Q>(mag);
     }
   }
 }

@@ -231,11 +231,7 @@ __global__ __launch_bounds__(256, KIND <= kBf16 || !NORM ? 8 : 6) void rope_appe
         if (j == 0) {
           const int64_t *ss = kind == 1 ? a.k_scale_stride : a.v_scale_stride;
           float *sc = kind == 1 ? a.k_scales : a.v_scales;
-          float s = __uint_as_float(mag) / (float)Q;
-          // the largest fp32 values: code Q must not read back as an infinity
-          if (s * (float)Q > 3.402823466e38f) s = __uint_as_float(__float_as_uint(s) - 1u);
-          sc[blk * ss[0] + h * ss[1] + off * ss[2]] =
-              mag >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : s;
+          sc[blk * ss[0] + h * ss[1] + off * ss[2]] = cache_scale<Q>(mag);
         }
       }
     }
