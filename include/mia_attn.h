@@ -835,6 +835,7 @@ int mia_quant_rows(const mia_quant_rows_args *args, mia_stream_t stream);
 /* ------------------------------------------------------------------------ */
 /* Product of int8 rows and int8 weights (no counterpart in the reference):  */
 /*   out[m, n] = bf16(x_scales[m] w_scales[n] sum_k x[m, k] w[n, k] + b[n]), */
+/* fp32 behind the sum, (sum x_scales[m]) w_scales[n] + b[n] in this order;  */
 /* integer sums exact in 32 bits (k < 131072).  k is a multiple of 16, rows */
 /* of x and w 16-byte aligned and less than 2^24 bytes apart.                */
 /* ------------------------------------------------------------------------ */
@@ -941,7 +942,10 @@ int mia_rope_append(const mia_rope_append_args *args, mia_stream_t stream);
 /* alone if cu_seqlens_q is NULL), the last of its seq_lens[i] tokens, all   */
 /* of them in the cache already.  The query at position p sees key t iff     */
 /* t <= p and (t < first_tokens or t > p - window).  The sink logit enters   */
-/* the denominator.  Rows without keys give 0.  seq_lens are clamped to what */
+/* the denominator.  Rows without keys give 0.  Probabilities meet V as one  */
+/* bf16 number, as two where max_seqlen_q (at most num_tokens; 1 without     */
+/* cu_seqlens_q) times the heads of a kv head is at most 32, whatever the    */
+/* sequences' own lengths.  seq_lens are clamped to what                     */
 /* the table holds; entries that no query sees are never used, others        */
 /* outside the pool read its first or last block.  cu_seqlens_q must not     */
 /* decrease (rows that two sequences claim get either's result); at most     */

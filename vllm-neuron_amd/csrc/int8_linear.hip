@@ -18,16 +18,18 @@
 // Products.  The larger a tile, the less is copied to LDS and read from it per
 // product (a CU copies up to 140 KB/us of what lies in L2); but there are 256 CUs to
 // fill.  Hence forms of many tile sizes, chosen by measured costs (kForms), all with
-// v_mfma_i32_32x32x32_i8 but the one that streams the weights for 16 rows or fewer:
+// v_mfma_i32_32x32x32_i8 but the one that streams the weights for 16 rows or fewer.
+// Two times: weights from memory (a model's, more than the 256 MB that the memory-side
+// cache holds), in brackets weights found there:
 //   256 x 256, waves that take turns: bound by power.  8191 x 8192 x 10240: 565-595 us by card,
 //     2.3-2.4 POP/s, the matrix units busy 70 % of the cycles at a clock that falls to 1.7
 //     GHz; the library's product of two 8192^3 int8 matrices reaches 2.15.
 //   192, 160, 128 and 64 x 128, 64 x 64, ring of tiles read and copied ahead: 517 x 2880 x
-//     5120 15.3 us (1.0 POP/s), bound by the 200 tiles' 23 steps and the start.
+//     5120 17.3 us (14.2-15.3), bound by the 200 tiles' 23 steps and the start.
 //   32 x 64, 32 x 32, four groups of waves with a quarter of k each: latency of the copies.
-//     64 x 4096 x 6144 8.0 us, 3.3 TB/s of weights.
-//   16 rows or fewer, operands straight to registers: 4 x 2048 x 2048 3.3 us (launch
-//     and one load); 16 x 4096 x 4096 6.4 us.
+//     64 x 4096 x 6144 11.3 us (8.1), 2.2 TB/s of weights.
+//   16 rows or fewer, operands straight to registers: 4 x 2048 x 2048 3.9 us (3.4:
+//     launch and one load); 16 x 4096 x 4096 7.1 us (6.2).
 // LDS tiles hold rows of 128 (256 x 256: 64, 64 x 64: 256) bytes of k in 16-byte chunks, exchanged
 // within a row so that the 16 rows that a fragment read touches at once lie in all
 // banks (conflicts: 3 % of the LDS cycles).
@@ -935,18 +937,25 @@ int launch_stream(GemmParams &p, hipStream_t s) {
 // The forms of the product: tile, workgroups that a CU holds, and the time of a
 // call, once + rounds (round + step k / 128) us, where a round is a tile on
 // every CU.  The constants are least squares over measurements at 1 to 8191 rows
-// of k = 256 to 14336 and 512 to 10240 columns (weights rotated through 256 MB);
-// the form chosen by them took 0.3 % longer than the fastest one on the
-// geometric mean, 22 % at most (8191 x 2880 x 5120: 155 against 127 us).  Heights of
-// 160 and 192 rows are for sizes that would take a round more at 128.  Examples, us,
-// by form in the table's order:
-//   64 x 4096 x 6144, the last four but one: 12.2, 9.3, 11.9, 8.0
-//   180 x 4096 x 4096: 37.8, 22.5, 20.8, 19.8, 15.9, 12.5, 9.4, 17.1, 13.8
-//   517 x 2880 x 5120: 34.5, 18.9, 19.6, 18.6, 15.3, 22.8, 24.5, 53.5, 38.6
-//   600 x 8192 x 10240, the first five: 92.3, 65.5, 92.8, 87.2, 75.9
-//   850 x 4096 x 6144, the first five: 42.5, 28.7, 28.7, 43.9, 35.9
-//   8191 x 8192 x 10240, the first two: 688.3, 783.0
-//   4 x 2048 x 2048, the last five: 7.4, 6.0, 4.7, 5.1, 3.2
+// of k = 256 to 14336 and 512 to 10240 columns, weights rotated through 256 MB, of
+// which the memory-side cache holds a part: weights from memory take longer, the
+// fewer the rows the more, with the same forms ahead.  The form chosen by them took
+// 0.3 % longer than the fastest one on the geometric mean, 22 % at most (8191 x 2880 x
+// 5120: 155 against 127 us with a few weights in turn, 157 against 152 from memory; a
+// clock that falls under load is no part of the model).  Heights of 160 and 192
+// rows are for sizes that would take a round more at 128.  Examples, us, by form in
+// the table's order, weights rotated through 1.6 GB; in brackets that of the form
+// taken at 240 MB:
+//   4 x 2048 x 2048, the last five: 9.1, 7.2, 5.4, 6.5, 3.9 (3.6)
+//   16 x 4096 x 4096, the last five: 14.8, 10.7, 7.8, 9.9, 7.1 (6.4)
+//   64 x 2880 x 5120, four before the last: 17.8, 12.1, 13.8, 10.8 (9.1)
+//   64 x 4096 x 6144, four before the last: 17.8, 13.3, 14.7, 11.3 (8.1)
+//   180 x 4096 x 4096: 52.6, 30.9, 26.0, 21.7, 19.8, 16.5, 12.2, 19.5, 17.7 (9.3)
+//   517 x 2880 x 5120: 35.6, 23.6, 24.0, 20.6, 17.3, 27.7, 27.9, 62.5, 46.1 (18.0-19.7)
+//   600 x 8192 x 10240, the first five: 89.8, 69.2, 93.4, 87.4, 76.8 (55.3)
+//   850 x 4096 x 6144, the first five: 48.8, 33.9, 31.6, 44.0, 42.7 (29.1)
+//   8191 x 2880 x 5120, the first five: 152, 157, 162, 178, 194 (156)
+//   8191 x 8192 x 10240, the first five, 400 MB: 575-581, 679-698, 715-737, 764, 781
 struct Form {
   int bm, bn, per_cu, rows;  // rows: at most (0: any number)
   float once, round, step;

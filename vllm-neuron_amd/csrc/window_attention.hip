@@ -15,8 +15,8 @@
 // Forms, by the rows of a sequence and kv head (query tokens x heads of the group):
 //   tall  128 rows a workgroup, 32 per wave, 64-key tiles of K and V through two LDS
 //         stages (v_mfma_f32_32x32x16_bf16), probabilities rounded to bf16.  Bound by power
-//         and issue: 8191 tokens, 32 heads of d = 128, window 2048: 277-290 us by card,
-//         850-890 TFLOP/s, matrix units and vector instructions busy 45 % of the
+//         and issue: 8191 tokens, 32 heads of d = 128, window 2048: 277-293 us by card,
+//         840-890 TFLOP/s, matrix units and vector instructions busy 45 % of the
 //         cycles each, the clock at 1.8 GHz.  Eight waves in two groups, one in its
 //         products while the other is in its softmax, took 294; the next tile's scores between
 //         this one's exponentials 345; fragments read 4 or 6 ahead instead of 2 the same.
@@ -26,8 +26,9 @@
 //         operands, V through LDS (v_mfma_f32_16x16x32_bf16).  Probabilities go in two
 //         bf16 parts (the second product is free here), so that the result is as exact
 //         as the bf16 output.  Bound by HBM: 64 tokens over 4100 keys, 32 heads, d = 128:
-//         178 us, 5.8 TB/s; 128 over 528 int8 keys, d = 64: 20.6 us, 3.5 TB/s.  Few rows: by
-//         the chain lengths, table, keys, values, join (4 tokens over 1028 keys 10.5 us).
+//         178 us, 5.8 TB/s; 128 over 528 int8 keys, d = 64: 19.3-20.6 us, 3.5-3.7 TB/s.
+//         Few rows: by the chain lengths, table, keys, values, join (4 tokens over 1028 keys
+//         9.8-10.5 us).
 #include <algorithm>
 
 #include "attn_tile.h"

@@ -25,7 +25,7 @@ def _options(section_order: str, pairs: str) -> Tuple[bool, bool]:
 
 
 def rope_kv_append(
-    q: Tensor,                              # [T, Hq, d] bf16, any token / head strides
+    q: Tensor,                              # [T, Hq, d] bf16, rows 8-byte aligned, any strides
     k: Tensor,                              # [T, Hkv, d]
     v: Tensor,
     positions: Tensor,                      # [T] or [axes, T] int32 / int64

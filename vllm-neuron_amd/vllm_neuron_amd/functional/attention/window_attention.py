@@ -6,6 +6,10 @@ attention_decode_mask.py:94-236); its sinks are logits, not tokens.  Here the
 first tokens of a sequence stay in view however far the window has moved, over
 the paged cache and for prompts and single tokens alike, so that a sequence of
 any length keeps the blocks of its first tokens and of its window alone.
+
+Keys are taken as they were stored.  Rotated ones keep the positions that they
+were rotated by, so the distance of a query from the first tokens grows with the
+sequence; positions counted inside the cache are not offered.
 """
 from __future__ import annotations
 
@@ -53,6 +57,11 @@ def window_attention(
     as they were in a given ``out`` and are zeros in the returned tensor
     otherwise.  A NaN or infinity in a value row reaches the queries that see it,
     and may reach others of the same sequence and call.
+
+    Where ``min(max_seqlen_q, T)`` times the heads of a kv head is at most 32,
+    probabilities meet V as two bf16 numbers each (2^-16 of them is lost), else as
+    one (2^-8).  The bound decides for the whole call: a single token beside a long
+    prompt is computed as the prompt is, and faster in a call of its own.
 
     Caches: bf16; e4m3fn with static per-head scales; e4m3fn or int8 with the
     per-token scales of ``quant_kv_write`` and ``rope_kv_append``.  ``d`` is a
